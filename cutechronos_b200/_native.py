@@ -22,7 +22,8 @@ EXPORTED = (
     "cc2_stack_series", "cc2_select_quantiles", "cc2_set_attention_variant",
     "cc2_set_attention_trace", "cc2_set_gemm_trace", "cc2_kv_quant", "cc2_model_set_kv_quant",
     "cc2_set_launch_overlap", "cc2_test_starve_gemm", "cc2_group_attention_tc", "cc2_set_layer_chain",
-    "cc2_test_starve_layer_barrier", "cc2_set_layer_trace",
+    "cc2_test_starve_layer_barrier", "cc2_set_layer_trace", "cc2_kv4_page_bytes", "cc2_kv4_append", "cc2_kv4_read",
+    "cc2_kv4_attention_workspace_bytes", "cc2_kv4_attention",
 )
 KIND_NAMES = {1: "preprocess", 2: "gemm_tc", 3: "attn_time", 4: "attn_group", 5: "rmsnorm", 6: "output_transform",
               7: "gemm_qkv", 8: "gemm_o", 9: "gemm_group", 10: "gemm_ffn_up", 11: "gemm_ffn_down", 12: "gemm_io",
@@ -66,6 +67,20 @@ class Epilogue(C.Structure):
         ("rope_cs", _VP), ("rope_period", C.c_int), ("rope_cols", C.c_int),
         ("lo_out", _VP), ("resid_lo", _VP), ("ld_lo", C.c_int),
     ]
+
+
+class KV4Quant(C.Structure):
+    """Mirror of ``cc2_kv4_quant``."""
+
+    _fields_ = [("levels", C.c_float * 8), ("bounds", C.c_float * 7), ("signs", C.c_uint64), ("perm", C.c_uint8 * 64)]
+
+
+class KV4Cache(C.Structure):
+    """Mirror of ``cc2_kv4_cache``."""
+
+    _fields_ = [("pages", _VP), ("num_pages", C.c_int), ("page_size", C.c_int), ("heads", C.c_int),
+                ("norm_dtype", C.c_int), ("rope_cs", _VP), ("rope_len", C.c_int), ("key", KV4Quant),
+                ("value", KV4Quant)]
 
 
 class NativeError(RuntimeError):
@@ -114,6 +129,12 @@ def load(path: Path | str | None = None) -> C.CDLL:
     lib.cc2_test_starve_layer_barrier.argtypes = [i]
     lib.cc2_set_layer_trace.argtypes = [v]
     lib.cc2_group_attention_tc.argtypes = [v, i, i, i, i, v, i, v, i, i, i, i, v]
+    i64, kv4 = C.c_int64, C.POINTER(KV4Cache)
+    lib.cc2_kv4_page_bytes.argtypes = [i, i, C.POINTER(sz)]
+    lib.cc2_kv4_append.argtypes = [kv4, i, v, i64, i64, v, i64, i64, i, v, v, v, v, i, i, v]
+    lib.cc2_kv4_read.argtypes = [kv4, i, v, v, i, v, v, v, i, i, v]
+    lib.cc2_kv4_attention_workspace_bytes.argtypes = [kv4, i, i, i, i, i, i, C.POINTER(sz)]
+    lib.cc2_kv4_attention.argtypes = [kv4, i, v, i64, i64, v, i64, i64, i, i, i, v, i, v, i, v, i, i, f, i, v, v, sz, v]
     lib.cc2_forward_noalloc.argtypes = [v, v, v, i, i, i, v, v, v, v, v]
     lib.cc2_profile_read.argtypes = [v, v, v, v, i, C.POINTER(i)]
     lib.cc2_stack_series.argtypes = [v, v, i, i, v, v]

@@ -1,0 +1,738 @@
+// Attention over the paged 4-bit K/V cache (layout: kv4.cuh, definition: cc2.h).
+//
+// With K^ = n_k R^T c_k and V^ = n_v R'^T c_v (R the quantiser's rotation, c the
+// codes' levels) the cache is never rotated back:
+//   q . K^ = n_k (R q) . c_k,     sum p V^ = R'^T sum (p n_v) c_v,
+// so a row is rotated once going in and once coming out, and the products run
+// on the levels themselves, as fp16 on the tensor cores with fp32 sums.
+//
+// Rows are the queries of one sequence that share a head of keys: row r is
+// query token r / group, head r % group.  A block takes one head of keys of one
+// sequence, up to 8 NB rows and a chunk of the keys; its four warps take
+// 64-key stages in turn, each with a ring of its own that bulk copies fill, and
+// an online softmax of its own, joined at the end.
+//   S^T (16 keys x 8 rows) = K (decoded in registers, the A operand) . Q^T
+//   O^T (16 coordinates x 8 rows) += V^T (A, decoded) . P^T
+// Keys and coordinates as the long axis of the product: one token's query
+// fills 1 of 8 columns and not 1 of 16 rows.  P^T comes from S^T by one matrix
+// move a register pair.  What must not leave the type's range is scaled by
+// powers of two, which are exact: a row of Q to below 2^8, P n_v to below 2^14
+// against the largest norm met so far.
+// Rounding: Q and P n_v to fp16 (2^-12 of each, next to the output's bf16 with
+// 2^-9), levels to fp16.  fp32 calls split all three into two fp16 parts and
+// sum three products, which leaves about 2^-22.
+#include <algorithm>
+#include <cmath>
+
+#include "kv4.cuh"
+#include "tc_attn.cuh"
+
+namespace cc2 {
+
+int attention_error_word(int** p);
+
+namespace kv4 {
+
+Levels make_levels(const cc2_kv4_quant& q) {
+  Levels r{};
+  for (int i = 0; i < 8; ++i) {
+    const float c = 64.0f * q.levels[i];
+    const __half h = __float2half_rn(c);
+    const __half l = __float2half_rn(c - __half2float(h));
+    const uint16_t hb = __half_as_ushort(h), lb = __half_as_ushort(l);
+    const int w = i >> 2, s = 8 * (i & 3);
+    r.lo[w] |= (uint32_t)(hb & 255) << s;
+    r.hi[w] |= (uint32_t)(hb >> 8) << s;
+    r.rlo[w] |= (uint32_t)(lb & 255) << s;
+    r.rhi[w] |= (uint32_t)(lb >> 8) << s;
+  }
+  return r;
+}
+
+namespace {
+
+using namespace tcx;
+
+constexpr int kWarps = 4;
+constexpr int kStageKeys = 64;
+constexpr int kStageBytes = kStageKeys / kBlockTokens * kBlockBytes;  // 4352
+constexpr int kStages = 3;
+constexpr int kQPitch = 72;  // halves
+constexpr int kOPitch = 66;  // floats
+
+struct Rotation {
+  uint32_t signs[2];
+  uint8_t perm[64];  // going in: coordinate perm[i] becomes i; coming out: the inverse
+};
+
+struct Args {
+  Pool pool;
+  const void* q;
+  void* out;
+  float* lse;
+  long long q_ld, q_hs, o_ld, o_hs;
+  const int* cu;
+  const int* lens;
+  const int* table;
+  const float2* rope;
+  float* part;       // [unit][split][row][64]
+  float2* part_ml;   // [unit][split][row] (max, sum)
+  int* wait_err;
+  int* range_err;
+  int table_ld, rope_len, max_len;
+  int num_seqs, total_q, max_q, group;
+  int chunk, splits, row_tiles;
+  int causal, rotate;
+  float qscale;  // scale * log2(e)
+  Rotation rk, rv;
+  Levels lk, lv;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"((uint64_t)__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half(uint32_t x) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint16_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+
+// A vector spread over a warp, coordinates lane and lane + 32.
+__device__ __forceinline__ float spread_get(float lo, float hi, int i) {
+  const float a = __shfl_sync(0xffffffffu, lo, i & 31), b = __shfl_sync(0xffffffffu, hi, i & 31);
+  return i < 32 ? a : b;
+}
+__device__ __forceinline__ void spread_walsh(float& lo, float& hi, int lane) {
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) {
+    const float a = __shfl_xor_sync(0xffffffffu, lo, w), b = __shfl_xor_sync(0xffffffffu, hi, w);
+    lo = (lane & w) ? a - lo : lo + a;
+    hi = (lane & w) ? b - hi : hi + b;
+  }
+  const float a = lo;
+  lo = a + hi;
+  hi = a - hi;
+}
+__device__ __forceinline__ float flip(float x, const uint32_t signs[2], int half, int lane) {
+  return (signs[half] >> lane) & 1u ? -x : x;
+}
+
+// What a block or a row tile works on.
+struct Span {
+  int row0, rows;      // first row of the tile, rows of the sequence
+  int q_start, n;      // first query token, query tokens
+  int len;             // cached tokens
+  int keys;            // the tile's rows see none from here on
+};
+
+__device__ __forceinline__ Span span_of(const Args& a, int seq, int row_tile, int tile_rows, bool report) {
+  Span s;
+  int q0 = seq * a.max_q, q1 = q0 + a.max_q;
+  if (a.cu != nullptr) {
+    q0 = a.cu[seq];
+    q1 = a.cu[seq + 1];
+  }
+  const int len = a.lens[seq];
+  const long long room = (long long)a.table_ld << a.pool.page_shift;
+  const int most = (int)min((long long)a.max_len, room);
+  const bool bad = q0 < 0 || q1 < q0 || q1 > a.total_q || q1 - q0 > a.max_q || len < 0 || len > most;
+  if (bad && report) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+  s.q_start = min(max(q0, 0), a.total_q);
+  s.n = min(min(max(q1, s.q_start), a.total_q) - s.q_start, a.max_q);
+  s.len = min(max(len, 0), most);
+  s.row0 = row_tile * tile_rows;
+  s.rows = s.n * a.group;
+  const int last = (min(s.row0 + tile_rows, s.rows) - 1) / a.group;  // the tile's last query token
+  s.keys = a.causal ? min(max(s.len - s.n + last + 1, 0), s.len) : s.len;
+  return s;
+}
+
+// Number of chunks that hold keys of the tile.
+__device__ __forceinline__ int chunks_of(const Args& a, const Span& s) { return (s.keys + a.chunk - 1) / a.chunk; }
+
+// One row's sums -> output and log-sum-exp: lane holds coordinates lane and lane + 32 of the rotated sum.
+template <typename T>
+__device__ __forceinline__ void finish_row(const Args& a, const Span& s, int head, int row, float o0, float o1, float m,
+                                           float l, int lane) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  spread_walsh(o0, o1, lane);
+  o0 = flip(o0 * (0.125f * inv), a.rv.signs, 0, lane);
+  o1 = flip(o1 * (0.125f * inv), a.rv.signs, 1, lane);
+  const float x0 = spread_get(o0, o1, a.rv.perm[lane]);
+  const float x1 = spread_get(o0, o1, a.rv.perm[lane + 32]);
+  const int tok = s.q_start + row / a.group, qh = head * a.group + row % a.group;
+  T* out = (T*)a.out + (long long)tok * a.o_ld + (long long)qh * a.o_hs;
+  out[lane] = fromf<T>(x0);
+  out[lane + 32] = fromf<T>(x1);
+  if (a.lse != nullptr && lane == 0)
+    a.lse[(long long)tok * (a.pool.heads * a.group) + qh] =
+        l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <int NB, bool F32>
+struct Shared {
+  static constexpr int kRows = 8 * NB;
+  alignas(128) uint8_t ring[kWarps][kStages][kStageBytes];
+  alignas(16) __half q[F32 ? 2 : 1][kRows][kQPitch];
+  float rs[kRows];
+  float m[kWarps][kRows], l[kWarps][kRows];
+  uint64_t full[kWarps][kStages];
+  int abort_flag;
+  static_assert(kWarps * kRows * kOPitch * 4 <= kWarps * kStages * kStageBytes, "the joined sums reuse the ring");
+};
+
+template <int NB, bool F32>
+__global__ void __launch_bounds__(kWarps * 32)
+attend_kernel(const __grid_constant__ Args a) {
+  using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
+  using S = Shared<NB, F32>;
+  constexpr int kRows = S::kRows;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  S& sm = *reinterpret_cast<S*>(smem_raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  pdl_launch_dependents();
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(&sm.full[warp][i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid == 0) sm.abort_flag = 0;
+  pdl_wait();
+
+  unsigned idx = blockIdx.x;
+  const int row_tile = (int)(idx % a.row_tiles);
+  idx /= a.row_tiles;
+  const int split = (int)(idx % a.splits);
+  idx /= a.splits;
+  const int head = (int)(idx % a.pool.heads), seq = (int)(idx / a.pool.heads);
+  const Span s = span_of(a, seq, row_tile, kRows, split == 0 && row_tile == 0 && head == 0 && tid == 0);
+  if (s.row0 >= s.rows) return;
+  const int chunks = chunks_of(a, s);
+  if (split >= max(chunks, 1)) return;
+  const int c0 = split * a.chunk, c1 = min(s.keys, c0 + a.chunk);
+  const int stages = c1 > c0 ? (c1 - c0 + kStageKeys - 1) / kStageKeys : 0;
+  const int mine = stages > warp ? (stages - 1 - warp) / kWarps + 1 : 0;
+  __syncthreads();
+
+  // a stage's blocks of 16 keys, page by page (a page of 64 tokens or more holds
+  // a whole stage)
+  const int run = min((1 << a.pool.page_shift) / kBlockTokens, 4);  // blocks of a copy
+  const int* table = a.table + (long long)seq * a.table_ld;
+  auto issue = [&](int i) {
+    const int key0 = c0 + (warp + kWarps * i) * kStageKeys;
+    const int blocks = min((c1 - key0 + kBlockTokens - 1) / kBlockTokens, 4);
+    const uint32_t bar = smem_u32(&sm.full[warp][i % kStages]);
+    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)blocks * kBlockBytes);
+    __syncwarp();
+    const int first = lane * run;
+    if (first < blocks) {
+      const int key = key0 + first * kBlockTokens;
+      int page = table[key >> a.pool.page_shift];
+      if ((unsigned)page >= (unsigned)a.pool.num_pages) {
+        atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+        page = 0;  // in bounds; the rows are unspecified
+      }
+      const uint8_t* src =
+          a.pool.pages + block_offset(a.pool, page, head, key & ((1 << a.pool.page_shift) - 1));
+      bulk_load(smem_u32(sm.ring[warp][i % kStages]) + (uint32_t)first * kBlockBytes, src,
+                (uint32_t)min(run, blocks - first) * kBlockBytes, bar);
+    }
+  };
+  for (int i = 0; i < min(mine, kStages); ++i) issue(i);
+
+  // the rows: rotated to their positions, then as the keys' codes are, scaled
+  for (int r = warp; r < kRows; r += kWarps) {
+    const int row = s.row0 + r;
+    float x0 = 0.0f, x1 = 0.0f;
+    if (row < s.rows) {
+      const int i = row / a.group;
+      const T* q = (const T*)a.q + (long long)(s.q_start + i) * a.q_ld +
+                   (long long)(head * a.group + row % a.group) * a.q_hs;
+      x0 = tof<T>(q[lane]);
+      x1 = tof<T>(q[lane + 32]);
+      const int pos = s.len - s.n + i;
+      if (a.rotate && pos >= 0) {
+        if (pos >= a.rope_len) {
+          if (lane == 0) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+        } else {
+          const float2 cs = a.rope[(long long)pos * 32 + lane];
+          const float u = x0;
+          x0 = u * cs.x - x1 * cs.y;
+          x1 = x1 * cs.x + u * cs.y;
+        }
+      }
+    }
+    float y0 = flip(spread_get(x0, x1, a.rk.perm[lane]), a.rk.signs, 0, lane);
+    float y1 = flip(spread_get(x0, x1, a.rk.perm[lane + 32]), a.rk.signs, 1, lane);
+    spread_walsh(y0, y1, lane);
+    y0 *= 0.125f * a.qscale;
+    y1 *= 0.125f * a.qscale;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(y0), fabsf(y1))));
+    const int e = min(max((int)(top >> 23), 30), 254);
+    const float up = __int_as_float((261 - e) << 23);  // 2^(134 - e)
+    y0 *= up;
+    y1 *= up;
+    const __half h0 = __float2half_rn(y0), h1 = __float2half_rn(y1);
+    sm.q[0][r][lane] = h0;
+    sm.q[0][r][lane + 32] = h1;
+    if (F32) {
+      sm.q[F32 ? 1 : 0][r][lane] = __float2half_rn(y0 - __half2float(h0));
+      sm.q[F32 ? 1 : 0][r][lane + 32] = __float2half_rn(y1 - __half2float(h1));
+    }
+    if (lane == 0) sm.rs[r] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64: undoes both scalings
+  }
+  __syncthreads();
+
+  uint32_t qf[NB][F32 ? 16 : 8];
+  float rs[NB][2];
+  int limit[NB][2];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int p = 0; p < (F32 ? 2 : 1); ++p) {
+      const uint4* src = reinterpret_cast<const uint4*>(&sm.q[p][8 * b + g][16 * t]);
+      const uint4 u = src[0], v = src[1];
+      uint32_t* d = &qf[b][8 * p];
+      d[0] = u.x, d[1] = u.y, d[2] = u.z, d[3] = u.w, d[4] = v.x, d[5] = v.y, d[6] = v.z, d[7] = v.w;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = 8 * b + 2 * t + c;
+      rs[b][c] = sm.rs[r];
+      limit[b][c] = a.causal ? min(s.len - s.n + (s.row0 + r) / a.group + 1, s.len) : s.len;
+    }
+  }
+  // every row sees all keys below `clear`
+  const int clear = a.causal ? s.len - s.n + s.row0 / a.group + 1 : s.len;
+
+  float m[NB][2], l[NB][2], acc[4][NB][4];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    m[b][0] = m[b][1] = -INFINITY;
+    l[b][0] = l[b][1] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i][b][0] = acc[i][b][1] = acc[i][b][2] = acc[i][b][3] = 0.0f;
+  }
+  int ve = 20;  // exponent of the largest V norm met
+  const int krow = (g >> 1) + 4 * (g & 1);  // key of S^T rows g and (+ 8) g + 8 in a block of 16
+
+  for (int i = 0; i < mine; ++i) {
+    const int key0 = c0 + (warp + kWarps * i) * kStageKeys;
+    const uint32_t stage = smem_u32(sm.ring[warp][i % kStages]);
+    // the lanes leave together: one may see the block's abort flag where another saw its stage
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.full[warp][i % kStages]), (uint32_t)(i / kStages) & 1u,
+                                           &sm.abort_flag, a.wait_err)))
+      break;
+    float x[4][NB][4];
+    float nv[4][2];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t blk = stage + j * kBlockBytes;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) x[j][b][0] = x[j][b][1] = x[j][b][2] = x[j][b][3] = 0.0f;
+      const uint2 w0 = lds64(blk + krow * 32 + t * 8), w1 = lds64(blk + (krow + 8) * 32 + t * 8);
+      const uint32_t wa[2] = {w0.x, w0.y}, wb[2] = {w1.x, w1.y};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t da[4], db[4];
+        decode_k(wa[h], a.lk.lo, a.lk.hi, da);
+        decode_k(wb[h], a.lk.lo, a.lk.hi, db);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const uint32_t f[4] = {da[2 * p], db[2 * p], da[2 * p + 1], db[2 * p + 1]};
+          const int k = 2 * (2 * h + p);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            if (F32) mma(x[j][b], f, qf[b][8 + k], qf[b][8 + k + 1]);
+            mma(x[j][b], f, qf[b][k], qf[b][k + 1]);
+          }
+        }
+        if (F32) {
+          decode_k(wa[h], a.lk.rlo, a.lk.rhi, da);
+          decode_k(wb[h], a.lk.rlo, a.lk.rhi, db);
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const uint32_t f[4] = {da[2 * p], db[2 * p], da[2 * p + 1], db[2 * p + 1]};
+            const int k = 2 * (2 * h + p);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) mma(x[j][b], f, qf[b][k], qf[b][k + 1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint16_t kb = lds16(blk + kKNorms + (krow + 8 * c) * 2), vb = lds16(blk + kVNorms + (krow + 8 * c) * 2);
+        const bool seen = !(kb & 0x8000u) && key0 + 16 * j + krow + 8 * c < c1;
+        const float nk = norm_value(kb, a.pool.norm_bf16);
+        nv[j][c] = seen ? norm_value(vb, a.pool.norm_bf16) : 0.0f;
+        if (nv[j][c] <= 3.402823466e38f) top = max(top, __float_as_uint(nv[j][c]));
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          x[j][b][2 * c] = seen ? x[j][b][2 * c] * nk : -INFINITY;
+          x[j][b][2 * c + 1] = seen ? x[j][b][2 * c + 1] * nk : -INFINITY;
+        }
+      }
+    }
+    const bool edge = key0 + kStageKeys > clear;
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (key0 + 16 * j + krow + 8 * (c >> 1) >= limit[b][c & 1]) x[j][b][c] = -INFINITY;
+    }
+
+    // running maximum and largest norm; sums so far follow when one moves
+    const int ve_new = max(ve, (int)(__reduce_max_sync(0xffffffffu, top) >> 23));
+    float mn[NB][2];
+    bool moved = ve_new != ve;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float v = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v = max3(v, x[j][b][c], x[j][b][c + 2]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        mn[b][c] = fmaxf(m[b][c], v);
+        moved = moved || mn[b][c] != m[b][c];
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+      const float fv = __int_as_float((127 + max(ve - ve_new, -126)) << 23);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float f = m[b][c] == -INFINITY ? 0.0f : ex2((m[b][c] - mn[b][c]) * rs[b][c]);
+          m[b][c] = mn[b][c];
+          l[b][c] *= f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            acc[k][b][c] *= f * fv;
+            acc[k][b][c + 2] *= f * fv;
+          }
+        }
+      ve = ve_new;
+    }
+    const float vs = __int_as_float((267 - ve) << 23);  // 2^(140 - ve): norms below 2^14
+    float neg[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) neg[b][c] = m[b][c] == -INFINITY ? 0.0f : -m[b][c] * rs[b][c];
+
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t blk = stage + j * kBlockBytes + kVCodes + g * 4;
+      uint32_t pf[NB][F32 ? 4 : 2];
+      const float n0 = nv[j][0] * vs, n1 = nv[j][1] * vs;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float p[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          p[c] = ex2(fmaf(x[j][b][c], rs[b][c & 1], neg[b][c & 1]));
+          l[b][c & 1] += p[c];
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float n = c < 2 ? n0 : n1;
+          // a key that a row does not see adds nothing, whatever its norm
+          p[c] = edge && x[j][b][c] == -INFINITY ? 0.0f : p[c] * n;
+        }
+        const uint32_t h0 = pack_half(p[0], p[1]), h1 = pack_half(p[2], p[3]);
+        pf[b][0] = transpose8(h0);
+        pf[b][1] = transpose8(h1);
+        if (F32) {
+          const float2 f0 = unpack_half(h0), f1 = unpack_half(h1);
+          pf[b][F32 ? 2 : 0] = transpose8(pack_half(p[0] - f0.x, p[1] - f0.y));
+          pf[b][F32 ? 3 : 1] = transpose8(pack_half(p[2] - f1.x, p[3] - f1.y));
+        }
+      }
+      const ZipV z0 = zip_v(lds32(blk + t * 32), lds32(blk + (t + 4) * 32));
+      const ZipV z1 = zip_v(lds32(blk + (t + 8) * 32), lds32(blk + (t + 12) * 32));
+      uint32_t d0[8], d1[8];
+      if (F32) {
+        decode_v(z0, a.lv.rlo, a.lv.rhi, d0);
+        decode_v(z1, a.lv.rlo, a.lv.rhi, d1);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t f[4] = {d0[2 * k], d0[2 * k + 1], d1[2 * k], d1[2 * k + 1]};
+#pragma unroll
+          for (int b = 0; b < NB; ++b) mma(acc[k][b], f, pf[b][0], pf[b][1]);
+        }
+      }
+      decode_v(z0, a.lv.lo, a.lv.hi, d0);
+      decode_v(z1, a.lv.lo, a.lv.hi, d1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t f[4] = {d0[2 * k], d0[2 * k + 1], d1[2 * k], d1[2 * k + 1]};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          if (F32) mma(acc[k][b], f, pf[b][F32 ? 2 : 0], pf[b][F32 ? 3 : 1]);
+          mma(acc[k][b], f, pf[b][0], pf[b][1]);
+        }
+      }
+    }
+    __syncwarp();  // the stage is in registers
+    if (i + kStages < mine) issue(i + kStages);
+  }
+  if (sm.abort_flag) {  // a wait ran out: nothing may still be landing when the block ends
+    const unsigned long long t0 = globaltimer_ns();
+    for (int i = max(0, mine - kStages); i < mine; ++i)
+      while (!mbar_try(smem_u32(&sm.full[warp][i % kStages]), (uint32_t)(i / kStages) & 1u) &&
+             globaltimer_ns() - t0 < kWaitLimitNs) {
+      }
+  }
+  __syncthreads();  // all warps are done with the ring
+
+  float(*osum)[kRows][kOPitch] = reinterpret_cast<float(*)[kRows][kOPitch]>(&sm.ring[0][0][0]);
+  const float down = __int_as_float((ve - 19) << 23);  // 2^(ve - 140) / 64
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float v = l[b][c];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      const int r = 8 * b + 2 * t + c;
+      if (g == 0) {
+        sm.m[warp][r] = m[b][c] * rs[b][c];
+        sm.l[warp][r] = v;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<float2*>(&osum[warp][r][8 * g + 2 * k]) =
+            make_float2(acc[k][b][c] * down, acc[k][b][c + 2] * down);
+    }
+  __syncthreads();
+  for (int r = warp; r < kRows && s.row0 + r < s.rows; r += kWarps) {
+    float top = sm.m[0][r];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.m[w][r]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2(sm.m[w][r] - base);
+      sum += sm.l[w][r] * f;
+      o0 += osum[w][r][lane] * f;
+      o1 += osum[w][r][lane + 32] * f;
+    }
+    if (chunks <= 1) {
+      finish_row<T>(a, s, head, s.row0 + r, o0, o1, top, sum, lane);
+    } else {
+      const long long at =
+          ((((long long)seq * a.pool.heads + head) * a.splits + split) * a.row_tiles + row_tile) * kRows + r;
+      a.part[at * 64 + lane] = o0;
+      a.part[at * 64 + lane + 32] = o1;
+      if (lane == 0) a.part_ml[at] = make_float2(top, sum);
+    }
+  }
+}
+
+// Joins the chunks of the rows that have more than one: a warp a row.
+template <int NB, bool F32>
+__global__ void __launch_bounds__(128)
+join_kernel(const __grid_constant__ Args a) {
+  using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
+  constexpr int kRows = 8 * NB;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int r = (int)(w % kRows);
+  w /= kRows;
+  const int row_tile = (int)(w % a.row_tiles);
+  w /= a.row_tiles;
+  const int head = (int)(w % a.pool.heads);
+  const long long seq = w / a.pool.heads;
+  if (seq >= a.num_seqs) return;
+  const Span s = span_of(a, (int)seq, row_tile, kRows, false);
+  if (s.row0 + r >= s.rows) return;
+  const int chunks = chunks_of(a, s);
+  if (chunks <= 1) return;
+  const long long first = ((seq * a.pool.heads + head) * a.splits * a.row_tiles + row_tile) * kRows + r;
+  const long long step = (long long)a.row_tiles * kRows;
+  float top = -INFINITY;
+  for (int c = lane; c < chunks; c += 32) top = fmaxf(top, a.part_ml[first + c * step].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll 4
+  for (int c = 0; c < chunks; ++c) {
+    const float2 ml = a.part_ml[first + c * step];
+    const float* o = a.part + (first + c * step) * 64;
+    const float f = ex2(ml.x - base);
+    sum += ml.y * f;
+    o0 += o[lane] * f;
+    o1 += o[lane + 32] * f;
+  }
+  finish_row<T>(a, s, head, s.row0 + r, o0, o1, top, sum, lane);
+}
+
+struct Plan {
+  int nb, row_tiles, chunk, splits;
+  long long units;
+  size_t bytes;
+};
+
+int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, int max_q, int max_len, Plan& p) {
+  CC2_REQUIRE(dtype == CC2_BF16 || dtype == CC2_F32, "kv4_attention: unsupported dtype %d", dtype);
+  CC2_REQUIRE(q_heads > 0 && q_heads % pool.heads == 0,
+              "kv4_attention: %d query heads are no multiple of the cache's %d", q_heads, pool.heads);
+  CC2_REQUIRE(num_seqs > 0 && total_q >= 0 && max_q >= 0 && max_len >= 0, "kv4_attention: negative sizes or no sequence");
+  CC2_REQUIRE(max_len <= 1 << 30, "kv4_attention: max_len %d is above 2^30", max_len);
+  CC2_REQUIRE(max_q <= 0x7fffffff / 64 / q_heads, "kv4_attention: max_q %d is too large", max_q);
+  const int rows = std::max(1, max_q * (q_heads / pool.heads));
+  p.nb = rows <= 8 ? 1 : rows <= 16 || dtype == CC2_F32 ? 2 : 4;
+  p.row_tiles = (rows + 8 * p.nb - 1) / (8 * p.nb);
+  const long long tiles = (long long)num_seqs * pool.heads * p.row_tiles;
+  const int most = std::max(1, (max_len + 511) / 512);
+  const long long want = (8LL * num_sms() + tiles - 1) / tiles;
+  const int splits = (int)std::min<long long>(most, std::max<long long>(1, want));
+  p.chunk = ((std::max(1, max_len) + splits - 1) / splits + 255) / 256 * 256;
+  p.splits = std::max(1, (max_len + p.chunk - 1) / p.chunk);
+  p.units = tiles * p.splits;
+  CC2_REQUIRE(p.units <= 0x7fffffffLL, "kv4_attention: too many rows and keys for one call");
+  p.bytes = p.splits > 1 ? (size_t)p.units * 8 * p.nb * (64 * sizeof(float) + sizeof(float2)) : 0;
+  return CC2_OK;
+}
+
+template <int NB, bool F32>
+int launch(const Args& a, const Plan& p, cudaStream_t st) {
+  const size_t smem = sizeof(Shared<NB, F32>);
+  static unsigned long long attr_done = 0;  // one bit per device
+  int dev = 0;
+  CC2_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !((attr_done >> dev) & 1ull)) {
+    CC2_CUDA(cudaFuncSetAttribute(attend_kernel<NB, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (dev < 64) attr_done |= 1ull << dev;
+  }
+  CC2_CUDA(launch_k(attend_kernel<NB, F32>, (unsigned)p.units, kWarps * 32, smem, st, a));
+  if (p.splits > 1) {
+    const long long rows = p.units / p.splits * 8 * NB;
+    CC2_CUDA(launch_k(join_kernel<NB, F32>, (unsigned)((rows + 3) / 4), 128, 0, st, a));
+  }
+  CC2_CHECK_LAUNCH();
+  return CC2_OK;
+}
+
+bool row_aligned(int dtype, const void* p, int64_t ld, int64_t hs) {
+  const int64_t e = dtype == CC2_BF16 ? 8 : 4;
+  return ((uintptr_t)p & 15u) == 0 && ld % e == 0 && hs % e == 0;
+}
+
+}  // namespace
+}  // namespace kv4
+
+int kv4_attention_workspace(const cc2_kv4_cache* cache, int dtype, int q_heads, int num_seqs, int total_q, int max_q,
+                            int max_len, size_t* bytes) {
+  kv4::Pool pool;
+  CC2_TRY(kv4::check_cache(cache, "kv4_attention", pool));
+  CC2_REQUIRE(bytes != nullptr, "kv4_attention: bytes is null");
+  kv4::Plan p;
+  CC2_TRY(kv4::plan(pool, dtype, q_heads, num_seqs, total_q, max_q, max_len, p));
+  *bytes = p.bytes;
+  return CC2_OK;
+}
+
+int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, int64_t q_ld, int64_t q_hs, void* out,
+                         int64_t o_ld, int64_t o_hs, int q_heads, int num_seqs, int total_q, const int32_t* cu_q,
+                         int max_q, const int32_t* seq_lens, int max_len, const int32_t* table, int table_ld,
+                         int causal, float scale, int rotate_q, float* lse, void* ws, size_t ws_bytes,
+                         cudaStream_t st) {
+  using namespace kv4;
+  Args a{};
+  CC2_TRY(check_cache(cache, "kv4_attention", a.pool));
+  Plan p;
+  CC2_TRY(plan(a.pool, dtype, q_heads, num_seqs, total_q, max_q, max_len, p));
+  if (total_q == 0 || max_q == 0) return CC2_OK;
+  CC2_REQUIRE(q && out && seq_lens && table && table_ld > 0, "kv4_attention: null operand");
+  CC2_REQUIRE(cu_q != nullptr || (long long)num_seqs * max_q == total_q,
+              "kv4_attention: without cu_q the rows must be num_seqs * max_q, got %d", total_q);
+  CC2_REQUIRE(row_aligned(dtype, q, q_ld, q_hs) && row_aligned(dtype, out, o_ld, o_hs),
+              "kv4_attention: rows must start on 16 bytes, as must their strides");
+  CC2_REQUIRE(!rotate_q || cache->rope_cs, "kv4_attention: the cache has no table to rotate queries with");
+  CC2_REQUIRE(std::isfinite(scale), "kv4_attention: scale must be finite");
+  if (ws_bytes < p.bytes || (p.bytes > 0 && (ws == nullptr || ((uintptr_t)ws & 15u) != 0))) {
+    set_error("kv4_attention: workspace of %zu bytes (16-byte aligned) needed, got %zu", p.bytes, ws_bytes);
+    return CC2_E_WORKSPACE;
+  }
+  a.q = q;
+  a.out = out;
+  a.lse = lse;
+  a.q_ld = q_ld;
+  a.q_hs = q_hs;
+  a.o_ld = o_ld;
+  a.o_hs = o_hs;
+  a.cu = cu_q;
+  a.lens = seq_lens;
+  a.table = table;
+  a.rope = (const float2*)cache->rope_cs;
+  a.part = (float*)ws;
+  a.part_ml = (float2*)((char*)ws + (size_t)p.units * 8 * p.nb * 64 * sizeof(float));
+  CC2_TRY(attention_error_word(&a.wait_err));
+  CC2_TRY(error_word(&a.range_err));
+  a.table_ld = table_ld;
+  a.rope_len = cache->rope_len;
+  a.max_len = max_len;
+  a.num_seqs = num_seqs;
+  a.total_q = total_q;
+  a.max_q = max_q;
+  a.group = q_heads / a.pool.heads;
+  a.chunk = p.chunk;
+  a.splits = p.splits;
+  a.row_tiles = p.row_tiles;
+  a.causal = causal != 0;
+  a.rotate = rotate_q != 0;
+  a.qscale = scale * 1.4426950408889634f;
+  const Quant qk = make_quant(cache->key), qv = make_quant(cache->value);
+  for (int i = 0; i < 2; ++i) {
+    a.rk.signs[i] = qk.signs[i];
+    a.rv.signs[i] = qv.signs[i];
+  }
+  for (int i = 0; i < 64; ++i) {
+    a.rk.perm[i] = qk.perm[i];
+    a.rv.perm[qv.perm[i]] = (uint8_t)i;
+  }
+  a.lk = make_levels(cache->key);
+  a.lv = make_levels(cache->value);
+  if (dtype == CC2_F32) return p.nb == 1 ? launch<1, true>(a, p, st) : launch<2, true>(a, p, st);
+  return p.nb == 1 ? launch<1, false>(a, p, st) : p.nb == 2 ? launch<2, false>(a, p, st) : launch<4, false>(a, p, st);
+}
+
+}  // namespace cc2

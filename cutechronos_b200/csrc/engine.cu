@@ -90,6 +90,19 @@ int set_gemm_starve(int on);
 int set_chain_starve(int on);
 int set_chain_trace(void* buf);
 size_t gemm_f32_splitk_floats();
+int read_kv4_error(int clear, int* value);
+int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs, const void* v,
+                      int64_t v_ld, int64_t v_hs, int T, const int32_t* seq, const int32_t* pos, const uint8_t* mask,
+                      const int32_t* table, int table_ld, int num_seqs, cudaStream_t st);
+int launch_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_out, int T, const int32_t* seq,
+                    const int32_t* pos, const int32_t* table, int table_ld, int num_seqs, cudaStream_t st);
+int kv4_attention_workspace(const cc2_kv4_cache* cache, int dtype, int q_heads, int num_seqs, int total_q, int max_q,
+                            int max_len, size_t* bytes);
+int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, int64_t q_ld, int64_t q_hs, void* out,
+                         int64_t o_ld, int64_t o_hs, int q_heads, int num_seqs, int total_q, const int32_t* cu_q,
+                         int max_q, const int32_t* seq_lens, int max_len, const int32_t* table, int table_ld,
+                         int causal, float scale, int rotate_q, float* lse, void* ws, size_t ws_bytes,
+                         cudaStream_t st);
 int launch_kv_quant(int dtype, void* qkv, int ld, int rows, int q_col, int k_col, int v_col, int heads,
                     const cc2_kvq* key, const cc2_kvq* value, const float* rope_cs, int rope_period, float* stats,
                     cudaStream_t st);
@@ -457,7 +470,9 @@ int cc2_device_status(int clear) {
   int v = 0, a = 0;
   CC2_TRY(read_device_error(clear, &v));
   CC2_TRY(read_attention_error(clear, &a));
-  return v | (a ? DEV_ERR_ATTN_TIMEOUT : 0);
+  int r = 0;
+  CC2_TRY(read_kv4_error(clear, &r));
+  return v | (a ? DEV_ERR_ATTN_TIMEOUT : 0) | r;
 }
 
 int cc2_model_pack_bytes(const cc2_config* cfg, int dtype, size_t* bytes) {
@@ -957,6 +972,38 @@ int cc2_model_set_kv_quant(cc2_model* m, int layer, const cc2_kvq* key, const cc
   q.stats = stats;
   m->kvq[layer] = q;
   return CC2_OK;
+}
+
+int cc2_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs, const void* v,
+                   int64_t v_ld, int64_t v_hs, int T, const int32_t* seq, const int32_t* pos,
+                   const uint8_t* token_mask, const int32_t* block_table, int table_ld, int num_seqs, void* stream) {
+  clear_error();
+  return launch_kv4_append(cache, dtype, k, k_ld, k_hs, v, v_ld, v_hs, T, seq, pos, token_mask, block_table, table_ld,
+                           num_seqs, (cudaStream_t)stream);
+}
+
+int cc2_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_out, int T, const int32_t* seq,
+                 const int32_t* pos, const int32_t* block_table, int table_ld, int num_seqs, void* stream) {
+  clear_error();
+  return launch_kv4_read(cache, dtype, k_out, v_out, T, seq, pos, block_table, table_ld, num_seqs,
+                         (cudaStream_t)stream);
+}
+
+int cc2_kv4_attention_workspace_bytes(const cc2_kv4_cache* cache, int dtype, int q_heads, int num_seqs, int total_q,
+                                      int max_q, int max_len, size_t* bytes) {
+  clear_error();
+  return kv4_attention_workspace(cache, dtype, q_heads, num_seqs, total_q, max_q, max_len, bytes);
+}
+
+int cc2_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, int64_t q_ld, int64_t q_hs, void* out,
+                      int64_t o_ld, int64_t o_hs, int q_heads, int num_seqs, int total_q, const int32_t* cu_q,
+                      int max_q, const int32_t* seq_lens, int max_len, const int32_t* block_table, int table_ld,
+                      int causal, float scale, int rotate_q, float* lse, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  clear_error();
+  return launch_kv4_attention(cache, dtype, q, q_ld, q_hs, out, o_ld, o_hs, q_heads, num_seqs, total_q, cu_q, max_q,
+                              seq_lens, max_len, block_table, table_ld, causal, scale, rotate_q, lse, workspace,
+                              workspace_bytes, (cudaStream_t)stream);
 }
 
 int cc2_set_gemm_trace(void* device_buffer) {

@@ -1,0 +1,258 @@
+"""A paged K/V cache held in 4 bits: what ``CuteChronos2Model.enable_turboquant_kv`` simulates, stored.
+
+The TurboQuant hook quantises K and V and restores them in place; this cache keeps the codes.  Vectors of 64 values are
+rotated (signs, permutation, Hadamard), each coordinate held as one of 16 Lloyd-Max levels and the norm in 16 bits: 34
+bytes a vector where bf16 takes 128.  Tokens live in pages that a block table names per sequence; appending rotates the
+keys to their positions on the way (rotate-half, like the model's attention), and attention works on the codes: it
+rotates a query into the codes' frame and the result back out, never the cache.
+
+Every method enqueues work on the current stream of the cache's device and returns; lengths, positions and tables stay on
+the device.  A sequence, position, page or length out of range sets bit 8 of ``cc2_device_status`` (see
+:meth:`PagedKV4Cache.check`).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from contextlib import nullcontext
+
+import numpy as np
+import torch
+
+from . import _native as nat
+from .turboquant import TurboQuantParams
+
+DIM = 64
+NORMS = {"float16": 0, "bfloat16": 1}
+DEV_CACHE_RANGE = 8
+_CODES = {torch.bfloat16: nat.CC2_BF16, torch.float32: nat.CC2_F32}
+
+
+def rope_rows(positions: int, theta: float, device) -> torch.Tensor:
+    """(positions, 32, 2) float32 (cos, sin) of the fp32 angles position / theta^(2i/64), the model's rotation."""
+    inv = 1.0 / theta ** (torch.arange(0, DIM, 2, dtype=torch.int64).float() / DIM)
+    ang = torch.arange(positions, dtype=torch.float32, device=device)[:, None] * inv.to(device)[None]
+    return torch.stack([ang.double().cos(), ang.double().sin()], -1).float()
+
+
+def _quant(p: TurboQuantParams, which: str) -> nat.KV4Quant:
+    if p.mode != "mse" or p.bits != 4 or p.rotation != "hadamard" or p.dim != DIM:
+        raise ValueError(f"the {which} quantiser must be mode 'mse', 4 bits, rotation 'hadamard', dim {DIM}; got "
+                         f"{p.mode!r}, {p.bits}, {p.rotation!r}, {p.dim}")
+    if p.norm_dtype not in NORMS:
+        raise ValueError(f"the cache holds norms in 16 bits (float16 or bfloat16), got {p.norm_dtype}")
+    t = {k: p.tensors[k].cpu().numpy() for k in ("signs", "perm", "codebook", "boundaries")}
+    # sign and magnitude: the upper levels and their mirror image (the Lloyd-Max iteration leaves the two halves apart
+    # by 6e-5 of the norm at most; the cache keeps their mean)
+    half = np.float32(0.5)
+    levels = half * (t["codebook"][8:] - t["codebook"][7::-1])
+    bounds = half * (t["boundaries"][8:] - t["boundaries"][6::-1])
+    if np.abs(t["codebook"][8:] - levels).max() > 1e-3:
+        raise ValueError(f"the {which} quantiser's codebook is not symmetric")
+    if not (np.diff(levels) > 0).all() or not (np.diff(bounds) > 0).all() or levels[0] < 0 or levels[-1] > 512:
+        raise ValueError(f"the {which} quantiser's levels must ascend from 0 to at most 512")
+    if sorted(t["perm"].tolist()) != list(range(DIM)):
+        raise ValueError(f"the {which} quantiser's permutation is none")
+    signs = sum(1 << i for i in range(DIM) if t["signs"][i] < 0)
+    return nat.KV4Quant((C.c_float * 8)(*levels), (C.c_float * 7)(*bounds), signs,
+                        (C.c_uint8 * DIM)(*(int(i) for i in t["perm"])))
+
+
+def _aligned(t: torch.Tensor) -> bool:
+    per = 16 // t.element_size()
+    return (t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t (rows, heads, 64) as the kernels read it: last axis dense, rows and heads on 16-byte boundaries (copied where
+    they are not)."""
+    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+class PagedKV4Cache:
+    """``num_pages`` pages of ``page_size`` (16, 32, 64, 128, 256) tokens for ``num_heads`` key / value heads of 64.
+
+    ``key`` and ``value`` are the quantisers (:class:`TurboQuantParams`, 4 bits, "mse", "hadamard"; default seeds 0 and
+    1).  ``rope_theta`` None appends keys as they come; otherwise positions up to ``max_positions`` can be rotated to.
+    ``pages`` is the storage (uint8, ``(num_pages, bytes of a page)``); pages can be copied or shared between sequences.
+    """
+
+    def __init__(self, num_pages: int, num_heads: int, *, page_size: int = 64, key: TurboQuantParams | None = None,
+                 value: TurboQuantParams | None = None, rope_theta: float | None = 10000.0, max_positions: int = 8192,
+                 device="cuda"):
+        lib = nat.load()
+        key = key or TurboQuantParams.build(DIM, 4, mode="mse", seed=0, device="cpu")
+        value = value or TurboQuantParams.build(DIM, 4, mode="mse", seed=1, device="cpu")
+        if key.norm_dtype != value.norm_dtype:
+            raise ValueError("keys and values must hold their norms in the same type")
+        if num_pages < 1 or num_pages > 2**31 - 1:
+            raise ValueError(f"num_pages must be positive, got {num_pages}")
+        if rope_theta is not None and max_positions < 1:
+            raise ValueError(f"max_positions must be positive, got {max_positions}")
+        quants = _quant(key, "key"), _quant(value, "value")
+        nbytes = C.c_size_t()
+        if lib.cc2_kv4_page_bytes(page_size, num_heads, C.byref(nbytes)) != 0:
+            raise ValueError(lib.cc2_last_error().decode())
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError("cutechronos_b200 kernels take CUDA tensors only (no CPU path)")
+        self.pages = torch.zeros(num_pages, nbytes.value, dtype=torch.uint8, device=device)
+        self.device = self.pages.device
+        self.num_pages, self.num_heads, self.page_size = num_pages, num_heads, page_size
+        self.rope = rope_rows(max_positions, rope_theta, self.device) if rope_theta is not None else None
+        self._c = nat.KV4Cache(self.pages.data_ptr(), num_pages, page_size, num_heads, NORMS[key.norm_dtype],
+                               self.rope.data_ptr() if self.rope is not None else None,
+                               max_positions if self.rope is not None else 0, *quants)
+        self._ref = C.byref(self._c)
+        self._lib = lib
+        self._plan = (None, 0)  # sizes of the last attention call, bytes of its workspace
+
+    # -- arguments ---------------------------------------------------------------------------
+    def _guard(self):
+        return nullcontext() if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
+
+    def _index(self, t: torch.Tensor, what: str, dim: int = 1) -> torch.Tensor:
+        if t.device != self.device:
+            raise RuntimeError(f"{what} must be on {self.device}, got {t.device}")
+        if t.dim() != dim:
+            raise ValueError(f"{what} must have {dim} axis(es), got shape {tuple(t.shape)}")
+        if t.dtype != torch.int32:
+            if t.dtype != torch.int64:
+                raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+            t = t.to(torch.int32)
+        return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+    def _values(self, t: torch.Tensor, what: str) -> int:
+        if t.device != self.device:
+            raise RuntimeError(f"{what} must be on {self.device}, got {t.device} (no CPU path)")
+        if t.dim() != 3 or t.shape[2] != DIM:
+            raise ValueError(f"{what} must be (tokens, heads, {DIM}), got {tuple(t.shape)}")
+        if t.dtype not in _CODES:
+            raise TypeError(f"{what}: dtype {t.dtype} not supported (bfloat16 / float32)")
+        return _CODES[t.dtype]
+
+    def _table(self, block_table: torch.Tensor):
+        t = self._index(block_table, "block_table", 2)
+        if t.shape[0] < 1 or t.shape[1] < 1:
+            raise ValueError(f"block_table is empty: {tuple(t.shape)}")
+        return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    def _places(self, seq_ids, positions, block_table, tokens: int | None):
+        seq, pos = self._index(seq_ids, "seq_ids"), self._index(positions, "positions")
+        if seq.shape != pos.shape or (tokens is not None and seq.shape[0] != tokens):
+            raise ValueError(f"seq_ids and positions must name one place for each token, got {seq.shape[0]} and "
+                             f"{pos.shape[0]}" + ("" if tokens is None else f" for {tokens}"))
+        table, ld = self._table(block_table)
+        if ld < table.shape[1] and table.shape[0] > 1:
+            table, ld = table.contiguous(), table.shape[1]
+        return seq, pos, table, ld
+
+    # -- operators ---------------------------------------------------------------------------
+    def append(self, k: torch.Tensor, v: torch.Tensor, seq_ids: torch.Tensor, positions: torch.Tensor,
+               block_table: torch.Tensor, *, token_mask: torch.Tensor | None = None) -> None:
+        """Put k and v (tokens, heads, 64; bfloat16 or float32, any strides) at entries ``positions`` of sequences
+        ``seq_ids``: page ``block_table[seq, pos // page_size]``, place ``pos % page_size``.  Keys are rotated to their
+        positions.  ``token_mask`` 0 / False: attention will not see the token.  A negative sequence or position skips
+        the token; no two tokens of a call may have the same place."""
+        code = self._values(k, "k")
+        if self._values(v, "v") != code or v.shape != k.shape or k.shape[1] != self.num_heads:
+            raise ValueError(f"k and v must both be (tokens, {self.num_heads}, {DIM}) of one type, got "
+                             f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+        seq, pos, table, ld = self._places(seq_ids, positions, block_table, k.shape[0])
+        mask = None
+        if token_mask is not None:
+            if token_mask.shape != seq.shape or token_mask.device != self.device:
+                raise ValueError("token_mask must have one entry for each token, on the cache's device")
+            mask = token_mask.view(torch.uint8) if token_mask.dtype == torch.bool else token_mask
+            mask = (mask if mask.dtype == torch.uint8 else (mask != 0).view(torch.uint8)).contiguous()
+        k, v = _rows(k), _rows(v)
+        with self._guard():
+            nat.check(self._lib.cc2_kv4_append(
+                self._ref, code, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                k.shape[0], seq.data_ptr(), pos.data_ptr(), mask.data_ptr() if mask is not None else None,
+                table.data_ptr(), ld, table.shape[0], torch.cuda.current_stream().cuda_stream), "cc2_kv4_append")
+
+    def read(self, seq_ids: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor, *,
+             dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """What the entries stand for, dense: (k, v), each (tokens, heads, 64), keys as they were rotated.  Masked
+        tokens read like others; skipped ones give zeros."""
+        if dtype not in _CODES:
+            raise TypeError(f"dtype {dtype} not supported (bfloat16 / float32)")
+        seq, pos, table, ld = self._places(seq_ids, positions, block_table, None)
+        k = torch.empty(seq.shape[0], self.num_heads, DIM, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        with self._guard():
+            nat.check(self._lib.cc2_kv4_read(
+                self._ref, _CODES[dtype], k.data_ptr(), v.data_ptr(), k.shape[0], seq.data_ptr(), pos.data_ptr(),
+                table.data_ptr(), ld, table.shape[0], torch.cuda.current_stream().cuda_stream), "cc2_kv4_read")
+        return k, v
+
+    def attention(self, q: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, *,
+                  cu_q: torch.Tensor | None = None, max_q: int | None = None, max_len: int | None = None,
+                  causal: bool = True, scale: float = 1.0, rotate_q: bool = False, return_lse: bool = False,
+                  out: torch.Tensor | None = None):
+        """Attention of q (tokens, query heads, 64; bfloat16 or float32) over the cache -> the same shape and type.
+
+        ``seq_lens`` counts each sequence's cached tokens, the queries' own among them.  Sequence s has the rows
+        ``cu_q[s] : cu_q[s + 1]`` (at most ``max_q``; default: one equal share each), standing at its last positions;
+        ``causal`` lets a row see the entries up to its own.  Query head h reads key head h // (query heads / heads).
+        ``scale`` multiplies the scores (1, as in the model's attention); ``rotate_q`` rotates the queries to their
+        positions.  ``max_len`` bounds seq_lens (default: what the block table has room for); a tighter bound splits the
+        work better.  A row that sees no token gives 0.  With ``return_lse`` also the (tokens, query heads) float32
+        logarithm of each row's sum of exponentials (-inf for such a row), to join it with attention over other keys."""
+        code = self._values(q, "q")
+        lens = self._index(seq_lens, "seq_lens")
+        table, ld = self._table(block_table)
+        seqs, total, heads = lens.shape[0], q.shape[0], q.shape[1]
+        if table.shape[0] != seqs:
+            raise ValueError(f"block_table has {table.shape[0]} rows for {seqs} sequences")
+        if heads == 0 or heads % self.num_heads:
+            raise ValueError(f"{heads} query heads are no multiple of the cache's {self.num_heads}")
+        if cu_q is None:
+            if total % seqs or (max_q is not None and max_q != total // seqs):
+                raise ValueError(f"{total} query rows are no equal shares of {seqs} sequences: give cu_q")
+            max_q = total // seqs
+        else:
+            cu_q = self._index(cu_q, "cu_q")
+            if cu_q.shape[0] != seqs + 1:
+                raise ValueError(f"cu_q must have {seqs + 1} entries, got {cu_q.shape[0]}")
+            max_q = total if max_q is None else min(int(max_q), total)
+        room = table.shape[1] * self.page_size
+        max_len = room if max_len is None else min(int(max_len), room)
+        if max_q < 0 or max_len < 0:
+            raise ValueError("max_q and max_len must not be negative")
+        if rotate_q and self.rope is None:
+            raise ValueError("the cache was made without a rotation (rope_theta None)")
+        q = _rows(q)
+        if out is None:
+            out = torch.empty(total, heads, DIM, dtype=q.dtype, device=self.device)
+        elif (out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not _aligned(out)
+              or any(n > 1 and st < DIM for n, st in zip(out.shape[:2], out.stride()))):
+            raise ValueError("out must have q's shape, type and device, its rows apart, dense and on 16-byte boundaries")
+        lse = torch.empty(total, heads, dtype=torch.float32, device=self.device) if return_lse else None
+        with self._guard():
+            sizes = (code, heads, seqs, total, max_q, max_len)
+            if self._plan[0] != sizes:
+                nbytes = C.c_size_t()
+                nat.check(self._lib.cc2_kv4_attention_workspace_bytes(self._ref, *sizes, C.byref(nbytes)),
+                          "cc2_kv4_attention_workspace_bytes")
+                self._plan = (sizes, nbytes.value)
+            need = self._plan[1]
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            nat.check(self._lib.cc2_kv4_attention(
+                self._ref, code, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                heads, seqs, total, cu_q.data_ptr() if cu_q is not None else None, max_q, lens.data_ptr(), max_len,
+                table.data_ptr(), ld, int(causal), float(scale), int(rotate_q),
+                lse.data_ptr() if lse is not None else None, ws.data_ptr() if ws is not None else None, need,
+                torch.cuda.current_stream().cuda_stream), "cc2_kv4_attention")
+        return (out, lse) if return_lse else out
+
+    def check(self) -> None:
+        """Wait for the device and raise if a kernel of this library reported an error: for the cache, a sequence,
+        position, page or length out of range."""
+        with self._guard():
+            status = self._lib.cc2_device_status(1)
+        if status:
+            raise nat.NativeError(f"device status {status}" + (
+                ": a sequence, position, page or length of a cache call was out of range"
+                if status > 0 and status & DEV_CACHE_RANGE else ""))

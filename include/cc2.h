@@ -65,7 +65,10 @@ CC2_API const char* cc2_version(void);
  * incomplete while the launching call has already returned CC2_OK, so callers
  * that need to know poll this after synchronising (the native bridge and
  * CuteChronos2Model.set_device_checks(True) do). */
-enum { CC2_DEV_GEMM_TIMEOUT = 1, CC2_DEV_ATTN_TIMEOUT = 2, CC2_DEV_LAYER_TIMEOUT = 4 };
+enum {
+  CC2_DEV_GEMM_TIMEOUT = 1, CC2_DEV_ATTN_TIMEOUT = 2, CC2_DEV_LAYER_TIMEOUT = 4,
+  CC2_DEV_CACHE_RANGE = 8  /* a 4-bit cache call met a sequence, position, page or length out of range */
+};
 CC2_API int cc2_device_status(int clear);
 
 /* ------------------------------------------------------------------------ */
@@ -413,6 +416,91 @@ CC2_API int cc2_kv_quant(int dtype, void* qkv, int ld, int rows, int q_col, int 
  * time attention, accumulating into stats (dev float32[4] or NULL). */
 CC2_API int cc2_model_set_kv_quant(cc2_model* m, int layer, const cc2_kvq* key, const cc2_kvq* value,
                                    float* stats);
+
+/* ------------------------------------------------------------------------ */
+/* Paged K/V cache held in 4 bits (no counterpart in the reference, whose     */
+/* TurboQuant hook simulates the storage: it quantises and restores in place). */
+/* ------------------------------------------------------------------------ */
+/* A 64-value vector x of norm n is rotated, y = H (signs * x[perm]) with the
+ * 64 x 64 Walsh-Hadamard matrix H (entries +-1); coordinate i is held as the
+ * sign of y_i and the number of bounds b_j with |y_i| > b_j * 8n, n in 16 bits.
+ * It stands for x[perm[i]] = signs_i * (H c)_i * n / 8, c_i = +-levels[.].
+ * n is the square root of the squares added in halves (32 + 32, 16 + 16, ...)
+ * in fp32, y the fp32 butterflies of width 1, 2, ..., 32: a cache's content
+ * does not depend on how a call was split.  A finite n above fp16's largest
+ * value is held as that value, one that is not finite as NaN (the vector
+ * reads back as NaN). */
+typedef struct {
+  float levels[8];     /* magnitudes, ascending; the negative half mirrors them */
+  float bounds[7];     /* between them, ascending */
+  uint64_t signs;      /* bit i: signs_i = -1 */
+  uint8_t perm[64];
+} cc2_kv4_quant;
+
+/* A cache (host struct, read by each call; the caller owns the memory it
+ * points to).  Token `pos` of sequence s lies in page
+ * block_table[s * table_ld + pos / page_size], a page holds page_size tokens
+ * of all heads. */
+typedef struct {
+  void* pages;            /* (dev) num_pages * cc2_kv4_page_bytes, 16-byte aligned */
+  int num_pages;
+  int page_size;          /* 16, 32, 64, 128 or 256 tokens */
+  int heads;              /* key / value heads, 64 values each */
+  int norm_dtype;         /* 0 float16, 1 bfloat16 */
+  const float* rope_cs;   /* (dev) float2 (cos, sin) [rope_len][32], or NULL: keys are not rotated */
+  int rope_len;
+  cc2_kv4_quant key, value;
+} cc2_kv4_cache;
+
+/* Bytes of one page. */
+CC2_API int cc2_kv4_page_bytes(int page_size, int heads, size_t* bytes);
+
+/* Append T tokens: k and v (dev, dtype; token t's head h at t * ld + h * hs,
+ * 64 consecutive elements, 16-byte aligned), seq and pos (dev, int32, T):
+ * token t becomes entry pos[t] of sequence seq[t].  k is rotated to its
+ * position (rotate-half, as everywhere in this library) in fp32, then both are
+ * quantised.  token_mask (dev, uint8, T, or NULL): 0 = attention does not see
+ * the token.  seq[t] < 0 or pos[t] < 0 skips a token; a sequence, position or
+ * page out of range skips it too and raises CC2_DEV_CACHE_RANGE.  No two
+ * tokens of a call may have the same place. */
+CC2_API int cc2_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs,
+                           const void* v, int64_t v_ld, int64_t v_hs, int T, const int32_t* seq,
+                           const int32_t* pos, const uint8_t* token_mask, const int32_t* block_table,
+                           int table_ld, int num_seqs, void* stream);
+
+/* What T entries of the cache stand for, as dense rows k_out, v_out (dev,
+ * dtype, (T, heads, 64); either may be NULL): keys as they were rotated.
+ * Skipped tokens (see cc2_kv4_append) give zeros. */
+CC2_API int cc2_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_out, int T,
+                         const int32_t* seq, const int32_t* pos, const int32_t* block_table, int table_ld,
+                         int num_seqs, void* stream);
+
+/* Attention of total_q query rows over the cache.
+ *   q, out     (dev, dtype) row i, head h at i * ld + h * hs (64 consecutive
+ *              elements, 16-byte aligned); q_heads is a multiple of the
+ *              cache's heads, and q head h reads cache head h / (q_heads / heads)
+ *   cu_q       (dev, int32, num_seqs + 1) rows cu_q[s] .. cu_q[s + 1] belong
+ *              to sequence s (at most max_q of them), or NULL: max_q rows for
+ *              every sequence
+ *   seq_lens   (dev, int32) cached tokens of each sequence, the rows' own among
+ *              them; max_len is a host-side bound on them
+ *   causal     row i of n sees entries 0 .. len - n + i, else 0 .. len - 1
+ *   scale      factor of the scores (the model's attention uses 1)
+ *   rotate_q   rotate row i of n to position len - n + i first (cache->rope_cs)
+ *   lse        (dev, float32 (total_q, q_heads)) natural logarithm of each
+ *              row's sum of exponentials, or NULL
+ * Masked tokens are not seen; a row that sees nothing gives 0 and a
+ * log-sum-exp of -inf.  A length or page out of range raises
+ * CC2_DEV_CACHE_RANGE; that sequence's rows are then unspecified.
+ * workspace (dev, 16-byte aligned) >= cc2_kv4_attention_workspace_bytes, which
+ * may be 0. */
+CC2_API int cc2_kv4_attention_workspace_bytes(const cc2_kv4_cache* cache, int dtype, int q_heads, int num_seqs,
+                                              int total_q, int max_q, int max_len, size_t* bytes);
+CC2_API int cc2_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, int64_t q_ld, int64_t q_hs,
+                              void* out, int64_t o_ld, int64_t o_hs, int q_heads, int num_seqs, int total_q,
+                              const int32_t* cu_q, int max_q, const int32_t* seq_lens, int max_len,
+                              const int32_t* block_table, int table_ld, int causal, float scale, int rotate_q,
+                              float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Pipeline steps on the device (pipeline.py:221-322, 24-58).                 */
