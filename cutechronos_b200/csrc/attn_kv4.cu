@@ -24,8 +24,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "kv4.cuh"
-#include "tc_attn.cuh"
+#include "kv4_attn.cuh"
 
 namespace cc2 {
 
@@ -57,42 +56,10 @@ constexpr int kWarps = 4;
 constexpr int kStageKeys = 64;
 constexpr int kStageBytes = kStageKeys / kBlockTokens * kBlockBytes;  // 4352
 constexpr int kStages = 3;
+constexpr int kTcMoreThan = 32;  // bf16 rows of a sequence and head from which the tcgen05 kernel takes over
 constexpr int kQPitch = 72;  // halves
 constexpr int kOPitch = 66;  // floats
 
-struct Rotation {
-  uint32_t signs[2];
-  uint8_t perm[64];  // going in: coordinate perm[i] becomes i; coming out: the inverse
-};
-
-struct Args {
-  Pool pool;
-  const void* q;
-  void* out;
-  float* lse;
-  long long q_ld, q_hs, o_ld, o_hs;
-  const int* cu;
-  const int* lens;
-  const int* table;
-  const float2* rope;
-  float* part;       // [unit][split][row][64]
-  float2* part_ml;   // [unit][split][row] (max, sum)
-  int* wait_err;
-  int* range_err;
-  int table_ld, rope_len, max_len;
-  int num_seqs, total_q, max_q, group;
-  int chunk, splits, row_tiles;
-  int causal, rotate;
-  float qscale;  // scale * log2(e)
-  Rotation rk, rv;
-  Levels lk, lv;
-};
-
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"((uint64_t)__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
-               : "memory");
-}
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -123,78 +90,6 @@ __device__ __forceinline__ uint16_t lds16(uint32_t a) {
   uint16_t v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
   return v;
-}
-
-// A vector spread over a warp, coordinates lane and lane + 32.
-__device__ __forceinline__ float spread_get(float lo, float hi, int i) {
-  const float a = __shfl_sync(0xffffffffu, lo, i & 31), b = __shfl_sync(0xffffffffu, hi, i & 31);
-  return i < 32 ? a : b;
-}
-__device__ __forceinline__ void spread_walsh(float& lo, float& hi, int lane) {
-#pragma unroll
-  for (int w = 1; w < 32; w <<= 1) {
-    const float a = __shfl_xor_sync(0xffffffffu, lo, w), b = __shfl_xor_sync(0xffffffffu, hi, w);
-    lo = (lane & w) ? a - lo : lo + a;
-    hi = (lane & w) ? b - hi : hi + b;
-  }
-  const float a = lo;
-  lo = a + hi;
-  hi = a - hi;
-}
-__device__ __forceinline__ float flip(float x, const uint32_t signs[2], int half, int lane) {
-  return (signs[half] >> lane) & 1u ? -x : x;
-}
-
-// What a block or a row tile works on.
-struct Span {
-  int row0, rows;      // first row of the tile, rows of the sequence
-  int q_start, n;      // first query token, query tokens
-  int len;             // cached tokens
-  int keys;            // the tile's rows see none from here on
-};
-
-__device__ __forceinline__ Span span_of(const Args& a, int seq, int row_tile, int tile_rows, bool report) {
-  Span s;
-  int q0 = seq * a.max_q, q1 = q0 + a.max_q;
-  if (a.cu != nullptr) {
-    q0 = a.cu[seq];
-    q1 = a.cu[seq + 1];
-  }
-  const int len = a.lens[seq];
-  const long long room = (long long)a.table_ld << a.pool.page_shift;
-  const int most = (int)min((long long)a.max_len, room);
-  const bool bad = q0 < 0 || q1 < q0 || q1 > a.total_q || q1 - q0 > a.max_q || len < 0 || len > most;
-  if (bad && report) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
-  s.q_start = min(max(q0, 0), a.total_q);
-  s.n = min(min(max(q1, s.q_start), a.total_q) - s.q_start, a.max_q);
-  s.len = min(max(len, 0), most);
-  s.row0 = row_tile * tile_rows;
-  s.rows = s.n * a.group;
-  const int last = (min(s.row0 + tile_rows, s.rows) - 1) / a.group;  // the tile's last query token
-  s.keys = a.causal ? min(max(s.len - s.n + last + 1, 0), s.len) : s.len;
-  return s;
-}
-
-// Number of chunks that hold keys of the tile.
-__device__ __forceinline__ int chunks_of(const Args& a, const Span& s) { return (s.keys + a.chunk - 1) / a.chunk; }
-
-// One row's sums -> output and log-sum-exp: lane holds coordinates lane and lane + 32 of the rotated sum.
-template <typename T>
-__device__ __forceinline__ void finish_row(const Args& a, const Span& s, int head, int row, float o0, float o1, float m,
-                                           float l, int lane) {
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  spread_walsh(o0, o1, lane);
-  o0 = flip(o0 * (0.125f * inv), a.rv.signs, 0, lane);
-  o1 = flip(o1 * (0.125f * inv), a.rv.signs, 1, lane);
-  const float x0 = spread_get(o0, o1, a.rv.perm[lane]);
-  const float x1 = spread_get(o0, o1, a.rv.perm[lane + 32]);
-  const int tok = s.q_start + row / a.group, qh = head * a.group + row % a.group;
-  T* out = (T*)a.out + (long long)tok * a.o_ld + (long long)qh * a.o_hs;
-  out[lane] = fromf<T>(x0);
-  out[lane + 32] = fromf<T>(x1);
-  if (a.lse != nullptr && lane == 0)
-    a.lse[(long long)tok * (a.pool.heads * a.group) + qh] =
-        l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 template <int NB, bool F32>
@@ -233,7 +128,7 @@ attend_kernel(const __grid_constant__ Args a) {
   const int split = (int)(idx % a.splits);
   idx /= a.splits;
   const int head = (int)(idx % a.pool.heads), seq = (int)(idx / a.pool.heads);
-  const Span s = span_of(a, seq, row_tile, kRows, split == 0 && row_tile == 0 && head == 0 && tid == 0);
+  const Span s = span_of(a, seq, row_tile, split == 0 && row_tile == 0 && head == 0 && tid == 0);
   if (s.row0 >= s.rows) return;
   const int chunks = chunks_of(a, s);
   if (split >= max(chunks, 1)) return;
@@ -364,8 +259,8 @@ attend_kernel(const __grid_constant__ Args a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t da[4], db[4];
-        decode_k(wa[h], a.lk.lo, a.lk.hi, da);
-        decode_k(wb[h], a.lk.lo, a.lk.hi, db);
+        decode_pairs(wa[h], a.lk.lo, a.lk.hi, da);
+        decode_pairs(wb[h], a.lk.lo, a.lk.hi, db);
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const uint32_t f[4] = {da[2 * p], db[2 * p], da[2 * p + 1], db[2 * p + 1]};
@@ -377,8 +272,8 @@ attend_kernel(const __grid_constant__ Args a) {
           }
         }
         if (F32) {
-          decode_k(wa[h], a.lk.rlo, a.lk.rhi, da);
-          decode_k(wb[h], a.lk.rlo, a.lk.rhi, db);
+          decode_pairs(wa[h], a.lk.rlo, a.lk.rhi, da);
+          decode_pairs(wb[h], a.lk.rlo, a.lk.rhi, db);
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
             const uint32_t f[4] = {da[2 * p], db[2 * p], da[2 * p + 1], db[2 * p + 1]};
@@ -481,12 +376,12 @@ attend_kernel(const __grid_constant__ Args a) {
           pf[b][F32 ? 3 : 1] = transpose8(pack_half(p[2] - f1.x, p[3] - f1.y));
         }
       }
-      const ZipV z0 = zip_v(lds32(blk + t * 32), lds32(blk + (t + 4) * 32));
-      const ZipV z1 = zip_v(lds32(blk + (t + 8) * 32), lds32(blk + (t + 12) * 32));
+      const Zip z0 = zip(lds32(blk + t * 32), lds32(blk + (t + 4) * 32));
+      const Zip z1 = zip(lds32(blk + (t + 8) * 32), lds32(blk + (t + 12) * 32));
       uint32_t d0[8], d1[8];
       if (F32) {
-        decode_v(z0, a.lv.rlo, a.lv.rhi, d0);
-        decode_v(z1, a.lv.rlo, a.lv.rhi, d1);
+        decode_zip(z0, a.lv.rlo, a.lv.rhi, d0);
+        decode_zip(z1, a.lv.rlo, a.lv.rhi, d1);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t f[4] = {d0[2 * k], d0[2 * k + 1], d1[2 * k], d1[2 * k + 1]};
@@ -494,8 +389,8 @@ attend_kernel(const __grid_constant__ Args a) {
           for (int b = 0; b < NB; ++b) mma(acc[k][b], f, pf[b][0], pf[b][1]);
         }
       }
-      decode_v(z0, a.lv.lo, a.lv.hi, d0);
-      decode_v(z1, a.lv.lo, a.lv.hi, d1);
+      decode_zip(z0, a.lv.lo, a.lv.hi, d0);
+      decode_zip(z1, a.lv.lo, a.lv.hi, d1);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t f[4] = {d0[2 * k], d0[2 * k + 1], d1[2 * k], d1[2 * k + 1]};
@@ -554,8 +449,7 @@ attend_kernel(const __grid_constant__ Args a) {
     if (chunks <= 1) {
       finish_row<T>(a, s, head, s.row0 + r, o0, o1, top, sum, lane);
     } else {
-      const long long at =
-          ((((long long)seq * a.pool.heads + head) * a.splits + split) * a.row_tiles + row_tile) * kRows + r;
+      const long long at = part_at(a, s, head, split, s.row0 + r);
       a.part[at * 64 + lane] = o0;
       a.part[at * 64 + lane + 32] = o1;
       if (lane == 0) a.part_ml[at] = make_float2(top, sum);
@@ -564,28 +458,32 @@ attend_kernel(const __grid_constant__ Args a) {
 }
 
 // Joins the chunks of the rows that have more than one: a warp a row.
-template <int NB, bool F32>
+template <typename T>
 __global__ void __launch_bounds__(128)
 join_kernel(const __grid_constant__ Args a) {
-  using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
-  constexpr int kRows = 8 * NB;
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int r = (int)(w % kRows);
-  w /= kRows;
-  const int row_tile = (int)(w % a.row_tiles);
-  w /= a.row_tiles;
-  const int head = (int)(w % a.pool.heads);
-  const long long seq = w / a.pool.heads;
-  if (seq >= a.num_seqs) return;
-  const Span s = span_of(a, (int)seq, row_tile, kRows, false);
-  if (s.row0 + r >= s.rows) return;
+  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int rows = a.total_q * a.group;
+  const int head = (int)(w / rows), call_row = (int)(w % rows), tok = call_row / a.group;
+  if (head >= a.pool.heads) return;
+  int seq = 0;  // the last sequence that starts at or before the row's token
+  if (a.cu == nullptr) {
+    seq = tok / a.max_q;
+  } else {
+    for (int i = lane; i - lane < a.num_seqs; i += 32)
+      seq += __popc(__ballot_sync(0xffffffffu, i < a.num_seqs && a.cu[i] <= tok));
+    --seq;
+  }
+  if (seq < 0) return;
+  const int q0 = a.cu == nullptr ? seq * a.max_q : a.cu[seq];
+  const int row = (tok - q0) * a.group + call_row % a.group;
+  const Span s = span_of(a, seq, row / a.tile_rows, false);
+  if (row >= s.rows) return;
   const int chunks = chunks_of(a, s);
   if (chunks <= 1) return;
-  const long long first = ((seq * a.pool.heads + head) * a.splits * a.row_tiles + row_tile) * kRows + r;
-  const long long step = (long long)a.row_tiles * kRows;
+  const long long first = part_at(a, s, head, 0, row), step = (long long)a.pool.heads * rows;
   float top = -INFINITY;
   for (int c = lane; c < chunks; c += 32) top = fmaxf(top, a.part_ml[first + c * step].x);
 #pragma unroll
@@ -601,13 +499,15 @@ join_kernel(const __grid_constant__ Args a) {
     o0 += o[lane] * f;
     o1 += o[lane + 32] * f;
   }
-  finish_row<T>(a, s, head, s.row0 + r, o0, o1, top, sum, lane);
+  finish_row<T>(a, s, head, row, o0, o1, top, sum, lane);
 }
 
 struct Plan {
-  int nb, row_tiles, chunk, splits;
-  long long units;
-  size_t bytes;
+  bool tc;  // attn_kv4_tc.cu's kernel
+  int nb, row_tiles, tile_rows, chunk, splits;
+  long long units, tiles;
+  size_t part_bytes, ml_bytes, q_bytes, scale_bytes;
+  size_t bytes() const { return part_bytes + ml_bytes + q_bytes + scale_bytes; }
 };
 
 int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, int max_q, int max_len, Plan& p) {
@@ -616,19 +516,33 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
               "kv4_attention: %d query heads are no multiple of the cache's %d", q_heads, pool.heads);
   CC2_REQUIRE(num_seqs > 0 && total_q >= 0 && max_q >= 0 && max_len >= 0, "kv4_attention: negative sizes or no sequence");
   CC2_REQUIRE(max_len <= 1 << 30, "kv4_attention: max_len %d is above 2^30", max_len);
-  CC2_REQUIRE(max_q <= 0x7fffffff / 64 / q_heads, "kv4_attention: max_q %d is too large", max_q);
+  CC2_REQUIRE(std::max(max_q, total_q) <= 0x7fffffff / 64 / q_heads, "kv4_attention: %d query rows are too many",
+              std::max(max_q, total_q));
   const int rows = std::max(1, max_q * (q_heads / pool.heads));
+  p = Plan{};
+  p.tc = dtype == CC2_BF16 && rows > kTcMoreThan;
   p.nb = rows <= 8 ? 1 : rows <= 16 || dtype == CC2_F32 ? 2 : 4;
-  p.row_tiles = (rows + 8 * p.nb - 1) / (8 * p.nb);
+  p.tile_rows = p.tc ? kTcRows : 8 * p.nb;
+  p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const long long tiles = (long long)num_seqs * pool.heads * p.row_tiles;
-  const int most = std::max(1, (max_len + 511) / 512);
+  const int least = p.tc ? 1024 : 512;  // keys below which a chunk's own cost shows
+  const int most = std::max(1, (max_len + least - 1) / least);
   const long long want = (8LL * num_sms() + tiles - 1) / tiles;
   const int splits = (int)std::min<long long>(most, std::max<long long>(1, want));
   p.chunk = ((std::max(1, max_len) + splits - 1) / splits + 255) / 256 * 256;
   p.splits = std::max(1, (max_len + p.chunk - 1) / p.chunk);
   p.units = tiles * p.splits;
   CC2_REQUIRE(p.units <= 0x7fffffffLL, "kv4_attention: too many rows and keys for one call");
-  p.bytes = p.splits > 1 ? (size_t)p.units * 8 * p.nb * (64 * sizeof(float) + sizeof(float2)) : 0;
+  if (p.splits > 1) {
+    const size_t n = (size_t)p.splits * total_q * q_heads;
+    p.part_bytes = n * 64 * sizeof(float);
+    p.ml_bytes = align_up(n * sizeof(float2), 128);
+  }
+  if (p.tc) {
+    p.tiles = query_tiles((long long)total_q * (q_heads / pool.heads), num_seqs) * pool.heads;
+    p.q_bytes = (size_t)p.tiles * 128 * 128;
+    p.scale_bytes = (size_t)p.tiles * 128 * sizeof(float);
+  }
   return CC2_OK;
 }
 
@@ -643,10 +557,15 @@ int launch(const Args& a, const Plan& p, cudaStream_t st) {
     if (dev < 64) attr_done |= 1ull << dev;
   }
   CC2_CUDA(launch_k(attend_kernel<NB, F32>, (unsigned)p.units, kWarps * 32, smem, st, a));
-  if (p.splits > 1) {
-    const long long rows = p.units / p.splits * 8 * NB;
-    CC2_CUDA(launch_k(join_kernel<NB, F32>, (unsigned)((rows + 3) / 4), 128, 0, st, a));
-  }
+  CC2_CHECK_LAUNCH();
+  return CC2_OK;
+}
+
+int join(const Args& a, int dtype, cudaStream_t st) {
+  if (a.splits <= 1) return CC2_OK;
+  const unsigned grid = (unsigned)(((long long)a.total_q * a.group * a.pool.heads + 3) / 4);
+  if (dtype == CC2_F32) CC2_CUDA(launch_k(join_kernel<float>, grid, 128, 0, st, a));
+  else CC2_CUDA(launch_k(join_kernel<__nv_bfloat16>, grid, 128, 0, st, a));
   CC2_CHECK_LAUNCH();
   return CC2_OK;
 }
@@ -666,7 +585,7 @@ int kv4_attention_workspace(const cc2_kv4_cache* cache, int dtype, int q_heads, 
   CC2_REQUIRE(bytes != nullptr, "kv4_attention: bytes is null");
   kv4::Plan p;
   CC2_TRY(kv4::plan(pool, dtype, q_heads, num_seqs, total_q, max_q, max_len, p));
-  *bytes = p.bytes;
+  *bytes = p.bytes();
   return CC2_OK;
 }
 
@@ -688,8 +607,8 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
               "kv4_attention: rows must start on 16 bytes, as must their strides");
   CC2_REQUIRE(!rotate_q || cache->rope_cs, "kv4_attention: the cache has no table to rotate queries with");
   CC2_REQUIRE(std::isfinite(scale), "kv4_attention: scale must be finite");
-  if (ws_bytes < p.bytes || (p.bytes > 0 && (ws == nullptr || ((uintptr_t)ws & 15u) != 0))) {
-    set_error("kv4_attention: workspace of %zu bytes (16-byte aligned) needed, got %zu", p.bytes, ws_bytes);
+  if (ws_bytes < p.bytes() || (p.bytes() > 0 && (ws == nullptr || ((uintptr_t)ws & 15u) != 0))) {
+    set_error("kv4_attention: workspace of %zu bytes (16-byte aligned) needed, got %zu", p.bytes(), ws_bytes);
     return CC2_E_WORKSPACE;
   }
   a.q = q;
@@ -703,8 +622,10 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   a.lens = seq_lens;
   a.table = table;
   a.rope = (const float2*)cache->rope_cs;
-  a.part = (float*)ws;
-  a.part_ml = (float2*)((char*)ws + (size_t)p.units * 8 * p.nb * 64 * sizeof(float));
+  a.qt = (uint8_t*)ws;
+  a.part = (float*)(a.qt + p.q_bytes);
+  a.part_ml = (float2*)((char*)a.part + p.part_bytes);
+  a.q_scale = (float*)((char*)a.part_ml + p.ml_bytes);
   CC2_TRY(attention_error_word(&a.wait_err));
   CC2_TRY(error_word(&a.range_err));
   a.table_ld = table_ld;
@@ -717,6 +638,7 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   a.chunk = p.chunk;
   a.splits = p.splits;
   a.row_tiles = p.row_tiles;
+  a.tile_rows = p.tile_rows;
   a.causal = causal != 0;
   a.rotate = rotate_q != 0;
   a.qscale = scale * 1.4426950408889634f;
@@ -726,13 +648,15 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
     a.rv.signs[i] = qv.signs[i];
   }
   for (int i = 0; i < 64; ++i) {
-    a.rk.perm[i] = qk.perm[i];
-    a.rv.perm[qv.perm[i]] = (uint8_t)i;
+    a.rk.inv[a.rk.perm[i] = qk.perm[i]] = (uint8_t)i;
+    a.rv.inv[a.rv.perm[i] = qv.perm[i]] = (uint8_t)i;
   }
   a.lk = make_levels(cache->key);
   a.lv = make_levels(cache->value);
-  if (dtype == CC2_F32) return p.nb == 1 ? launch<1, true>(a, p, st) : launch<2, true>(a, p, st);
-  return p.nb == 1 ? launch<1, false>(a, p, st) : p.nb == 2 ? launch<2, false>(a, p, st) : launch<4, false>(a, p, st);
+  if (p.tc) CC2_TRY(launch_attend_tc(a, st));
+  else if (dtype == CC2_F32) CC2_TRY(p.nb == 1 ? (launch<1, true>(a, p, st)) : (launch<2, true>(a, p, st)));
+  else CC2_TRY(p.nb == 1 ? (launch<1, false>(a, p, st)) : p.nb == 2 ? (launch<2, false>(a, p, st)) : (launch<4, false>(a, p, st)));
+  return join(a, dtype, st);
 }
 
 }  // namespace cc2

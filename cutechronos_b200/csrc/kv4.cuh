@@ -9,9 +9,12 @@
 //
 // A vector's 64 codes are 8 words; nibble p of word w holds the 3-bit magnitude
 // index of coordinate 8w + p in its low bits.  The nibbles' top bits hold the
-// signs, but not each its own nibble's: they stand where the decoder can merge
-// them with one operation for four coordinates (kv4_sign_bit).  A key norm's
-// sign bit marks a masked token.
+// signs, but not each its own nibble's: bits 7, 15, 23, 31 are coordinates
+// 0..3's and bits 3, 11, 19, 27 coordinates 4..7's, so that a decoder merges
+// four signs with four looked-up bytes in one operation, whether it makes
+// pairs of neighbouring coordinates of one token (decode_pairs) or of one
+// coordinate of two tokens (decode_zip).  A key norm's sign bit marks a
+// masked token.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -54,13 +57,7 @@ struct Levels {
 };
 
 // Bit of a word of codes that holds the sign of coordinate p (0..7) of it.
-// K: bits 7, 15, 23, 31 are coordinates 0..3, bits 3, 11, 19, 27 coordinates
-// 4..7 (the decoder makes pairs of neighbouring coordinates of one token).
-// V: nibble 2j's sign is in nibble 2j + 1 and the other way round (the
-// decoder makes pairs of one coordinate of two tokens).
-__host__ __device__ constexpr int sign_bit(bool value, int p) {
-  return value ? ((p & 1) ? 4 * (p - 1) + 3 : 4 * (p + 1) + 3) : (p < 4 ? 8 * p + 7 : 8 * (p - 4) + 3);
-}
+__host__ __device__ constexpr int sign_bit(int p) { return p < 4 ? 8 * p + 7 : 8 * (p - 4) + 3; }
 
 __device__ __forceinline__ float norm_value(uint16_t bits, int norm_bf16) {
   const uint16_t b = bits & 0x7fffu;
@@ -85,8 +82,8 @@ __device__ __forceinline__ long long block_offset(const Pool& p, int page, int h
 // A byte permute looks four 3-bit indices up in a table of 8 bytes at once.
 __device__ __forceinline__ uint32_t look(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
-// K: the 8 coordinates of a word as four fp16 pairs (0 1) (2 3) (4 5) (6 7).
-__device__ __forceinline__ void decode_k(uint32_t w, const uint32_t lo[2], const uint32_t hi[2], uint32_t out[4]) {
+// The 8 coordinates of a word as four fp16 pairs (0 1) (2 3) (4 5) (6 7).
+__device__ __forceinline__ void decode_pairs(uint32_t w, const uint32_t lo[2], const uint32_t hi[2], uint32_t out[4]) {
   const uint32_t s = w & 0x77777777u, s2 = s >> 16;
   const uint32_t l0 = look(lo[0], lo[1], s), l1 = look(lo[0], lo[1], s2);
   const uint32_t h0 = look(hi[0], hi[1], s) ^ (w & 0x80808080u);
@@ -97,23 +94,23 @@ __device__ __forceinline__ void decode_k(uint32_t w, const uint32_t lo[2], const
   out[3] = __byte_perm(l1, h1, 0x7362);
 }
 
-// V: coordinate p of tokens a and b as the fp16 pair out[p], p = 0..7.
-struct ZipV {
-  uint32_t u, v, su, sv, tu, tv;  // selectors of even / odd coordinates, their signs (low, high half)
+// Coordinate p of tokens a and b as the fp16 pair out[p], p = 0..7.
+struct Zip {
+  uint32_t u, v, su, sv, tu, tv;  // selectors of even / odd coordinates; their signs (low, high half)
 };
-__device__ __forceinline__ ZipV zip_v(uint32_t a, uint32_t b) {
+__device__ __forceinline__ Zip zip(uint32_t a, uint32_t b) {
   constexpr uint32_t m = 0x0f0f0f0fu;
-  ZipV z;
+  Zip z;
   z.u = ((a & m) | ((b << 4) & ~m)) & 0x77777777u;
   z.v = (((a >> 4) & m) | (b & ~m)) & 0x77777777u;
-  const uint32_t s0 = __byte_perm(a, b, 0x5140), s1 = __byte_perm(a, b, 0x7362);
+  const uint32_t s0 = __byte_perm(a, b, 0x6240), s1 = __byte_perm(a, b, 0x7351);
   z.su = s0 & 0x80808080u;
-  z.tu = s1 & 0x80808080u;
-  z.sv = (s0 << 4) & 0x80808080u;
+  z.tu = (s0 << 4) & 0x80808080u;
+  z.sv = s1 & 0x80808080u;
   z.tv = (s1 << 4) & 0x80808080u;
   return z;
 }
-__device__ __forceinline__ void decode_v(const ZipV& z, const uint32_t lo[2], const uint32_t hi[2], uint32_t out[8]) {
+__device__ __forceinline__ void decode_zip(const Zip& z, const uint32_t lo[2], const uint32_t hi[2], uint32_t out[8]) {
   uint32_t l, h;
   l = look(lo[0], lo[1], z.u);
   h = look(hi[0], hi[1], z.u) ^ z.su;

@@ -1,0 +1,143 @@
+// Shared by the kernels of attention over the 4-bit cache: their arguments,
+// what rows and keys a block has, the rotation of a row spread over a warp.
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "kv4.cuh"
+#include "tc_attn.cuh"
+
+namespace cc2 {
+namespace kv4 {
+
+using tcx::ex2;
+
+struct Rotation {
+  uint32_t signs[2];
+  uint8_t perm[64];  // coordinate perm[i] of a vector is i of the rotated one
+  uint8_t inv[64];
+};
+
+struct Args {
+  Pool pool;
+  const void* q;
+  void* out;
+  float* lse;
+  long long q_ld, q_hs, o_ld, o_hs;
+  const int* cu;
+  const int* lens;
+  const int* table;
+  const float2* rope;
+  float* part;       // [split][head][row of the call][64]: a chunk's sums, rotated
+  float2* part_ml;   // the same places: maximum (log2) and sum of exponentials
+  const uint8_t* qt;  // rotated queries as fp16 tiles (attn_kv4_tc.cu) and their rows' scales
+  const float* q_scale;
+  int* wait_err;
+  int* range_err;
+  int table_ld, rope_len, max_len;
+  int num_seqs, total_q, max_q, group;
+  int chunk, splits, row_tiles, tile_rows;
+  int causal, rotate;
+  float qscale;  // scale * log2(e)
+  Rotation rk, rv;
+  Levels lk, lv;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"((uint64_t)__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+// A vector spread over a warp, coordinates lane and lane + 32.
+__device__ __forceinline__ float spread_get(float lo, float hi, int i) {
+  const float a = __shfl_sync(0xffffffffu, lo, i & 31), b = __shfl_sync(0xffffffffu, hi, i & 31);
+  return i < 32 ? a : b;
+}
+__device__ __forceinline__ void spread_walsh(float& lo, float& hi, int lane) {
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) {
+    const float a = __shfl_xor_sync(0xffffffffu, lo, w), b = __shfl_xor_sync(0xffffffffu, hi, w);
+    lo = (lane & w) ? a - lo : lo + a;
+    hi = (lane & w) ? b - hi : hi + b;
+  }
+  const float a = lo;
+  lo = a + hi;
+  hi = a - hi;
+}
+__device__ __forceinline__ float flip(float x, const uint32_t signs[2], int half, int lane) {
+  return (signs[half] >> lane) & 1u ? -x : x;
+}
+
+// What a block or a row tile works on.
+struct Span {
+  int row0, rows;      // first row of the tile, rows of the sequence
+  int q_start, n;      // first query token, query tokens
+  int len;             // cached tokens
+  int keys;            // the tile's rows see none from here on
+};
+
+__device__ __forceinline__ Span span_of(const Args& a, int seq, int row_tile, bool report) {
+  Span s;
+  int q0 = seq * a.max_q, q1 = q0 + a.max_q;
+  if (a.cu != nullptr) {
+    q0 = a.cu[seq];
+    q1 = a.cu[seq + 1];
+  }
+  const int len = a.lens[seq];
+  const long long room = (long long)a.table_ld << a.pool.page_shift;
+  const int most = (int)min((long long)a.max_len, room);
+  const bool bad = q0 < 0 || q1 < q0 || q1 > a.total_q || q1 - q0 > a.max_q || len < 0 || len > most;
+  if (bad && report) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+  s.q_start = min(max(q0, 0), a.total_q);
+  s.n = min(min(max(q1, s.q_start), a.total_q) - s.q_start, a.max_q);
+  s.len = min(max(len, 0), most);
+  s.row0 = row_tile * a.tile_rows;
+  s.rows = s.n * a.group;
+  const int last = (min(s.row0 + a.tile_rows, s.rows) - 1) / a.group;  // the tile's last query token
+  s.keys = a.causal ? min(max(s.len - s.n + last + 1, 0), s.len) : s.len;
+  return s;
+}
+
+// Place of a row's sums among the parts.
+__device__ __forceinline__ long long part_at(const Args& a, const Span& s, int head, int split, int row) {
+  return ((long long)split * a.pool.heads + head) * ((long long)a.total_q * a.group) +
+         (long long)s.q_start * a.group + row;
+}
+
+// Number of chunks that hold keys of the tile.
+__device__ __forceinline__ int chunks_of(const Args& a, const Span& s) { return (s.keys + a.chunk - 1) / a.chunk; }
+
+// One row's sums -> output and log-sum-exp: lane holds coordinates lane and lane + 32 of the rotated sum.
+template <typename T>
+__device__ __forceinline__ void finish_row(const Args& a, const Span& s, int head, int row, float o0, float o1, float m,
+                                           float l, int lane) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  spread_walsh(o0, o1, lane);
+  o0 = flip(o0 * (0.125f * inv), a.rv.signs, 0, lane);
+  o1 = flip(o1 * (0.125f * inv), a.rv.signs, 1, lane);
+  const float x0 = spread_get(o0, o1, a.rv.inv[lane]);
+  const float x1 = spread_get(o0, o1, a.rv.inv[lane + 32]);
+  const int tok = s.q_start + row / a.group, qh = head * a.group + row % a.group;
+  T* out = (T*)a.out + (long long)tok * a.o_ld + (long long)qh * a.o_hs;
+  out[lane] = fromf<T>(x0);
+  out[lane + 32] = fromf<T>(x1);
+  if (a.lse != nullptr && lane == 0)
+    a.lse[(long long)tok * (a.pool.heads * a.group) + qh] =
+        l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+
+// attn_kv4_tc.cu: tiles of 256 rows on tcgen05 (bf16 calls).  Rotated queries in the workspace: tiles of 128 rows for
+// each head, sequence s from tile floor(q_start * group / 128) + s on.
+constexpr int kTcRows = 256;
+__host__ __device__ inline long long query_tiles(long long total_rows, int num_seqs) {
+  return total_rows / 128 + num_seqs;
+}
+__device__ __forceinline__ long long first_query_tile(const Args& a, int seq, int q_start) {
+  return (long long)q_start * a.group / 128 + seq;
+}
+int launch_attend_tc(const Args& a, cudaStream_t st);
+
+}  // namespace kv4
+}  // namespace cc2

@@ -138,7 +138,6 @@ __device__ __forceinline__ void walsh(float (&y)[64]) {
   }
 }
 
-template <bool V>
 __device__ __forceinline__ void encode(const float (&y)[64], float n8, const Quant& q, uint32_t (&word)[8]) {
   float t[7];
 #pragma unroll
@@ -153,7 +152,7 @@ __device__ __forceinline__ void encode(const float (&y)[64], float n8, const Qua
       const bool m = a > (h ? t[5] : t[1]);
       const bool l = a > (m ? (h ? t[6] : t[2]) : (h ? t[4] : t[0]));
       c |= (h ? 4u << (4 * p) : 0u) | (m ? 2u << (4 * p) : 0u) | (l ? 1u << (4 * p) : 0u);
-      c |= v < 0.0f ? 1u << sign_bit(V, p) : 0u;
+      c |= v < 0.0f ? 1u << sign_bit(p) : 0u;
     }
     word[w] = c;
   }
@@ -248,7 +247,7 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant q
   }
   walsh(y);
   uint32_t word[8];
-  if (is_v) encode<true>(y, n8, q, word); else encode<false>(y, n8, q, word);
+  encode(y, n8, q, word);
   uint8_t* block = pool.pages + at_block;
   const int slot = off & (kBlockTokens - 1);
   uint4* codes = reinterpret_cast<uint4*>(block + (is_v ? kVCodes : 0) + slot * 32);
@@ -295,8 +294,7 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant qk,
       for (int i = 0; i < 64; ++i) {
         const uint32_t w = word[i >> 3];
         const float c = lv[(w >> (4 * (i & 7))) & 7u];
-        const uint32_t s = is_v ? w << (31 - sign_bit(true, i & 7)) : w << (31 - sign_bit(false, i & 7));
-        y[i] = __uint_as_float(__float_as_uint(c) ^ (s & 0x80000000u));
+        y[i] = __uint_as_float(__float_as_uint(c) ^ ((w << (31 - sign_bit(i & 7))) & 0x80000000u));
       }
       walsh(y);
 #pragma unroll

@@ -39,8 +39,7 @@ def unpack(cache, which: int):
     codes = b[..., 512 * which:512 * which + 512].reshape(cache.num_pages, h, ps, 8, 4).long()
     word = codes[..., 0] | codes[..., 1] << 8 | codes[..., 2] << 16 | codes[..., 3] << 24
     at = torch.arange(8)
-    bit = torch.where(at % 2 == 0, 4 * (at + 1) + 3, 4 * (at - 1) + 3) if which else \
-        torch.where(at < 4, 8 * at + 7, 8 * (at - 4) + 3)
+    bit = torch.where(at < 4, 8 * at + 7, 8 * (at - 4) + 3)
     mag = (word[..., None] >> (4 * at)) & 7
     sign = 1 - 2 * ((word[..., None] >> bit) & 1)
     raw = b[..., 1024 + 32 * which:1056 + 32 * which].reshape(cache.num_pages, h, ps, 2).contiguous()
