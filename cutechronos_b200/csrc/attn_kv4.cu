@@ -527,7 +527,7 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
   const long long tiles = (long long)num_seqs * pool.heads * p.row_tiles;
   const int least = p.tc ? 1024 : 512;  // keys below which a chunk's own cost shows
   const int most = std::max(1, (max_len + least - 1) / least);
-  const long long want = (8LL * num_sms() + tiles - 1) / tiles;
+  const long long want = ((p.tc ? 4LL : 8LL) * num_sms() + tiles - 1) / tiles;
   const int splits = (int)std::min<long long>(most, std::max<long long>(1, want));
   p.chunk = ((std::max(1, max_len) + splits - 1) / splits + 255) / 256 * 256;
   p.splits = std::max(1, (max_len + p.chunk - 1) / p.chunk);
@@ -541,7 +541,7 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
   if (p.tc) {
     p.tiles = query_tiles((long long)total_q * (q_heads / pool.heads), num_seqs) * pool.heads;
     p.q_bytes = (size_t)p.tiles * 128 * 128;
-    p.scale_bytes = (size_t)p.tiles * 128 * sizeof(float);
+    p.scale_bytes = (size_t)p.tiles * 128 * sizeof(float) + 128;  // and the items' counter
   }
   return CC2_OK;
 }
@@ -625,7 +625,8 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   a.qt = (uint8_t*)ws;
   a.part = (float*)(a.qt + p.q_bytes);
   a.part_ml = (float2*)((char*)a.part + p.part_bytes);
-  a.q_scale = (float*)((char*)a.part_ml + p.ml_bytes);
+  a.counter = (int*)((char*)a.part_ml + p.ml_bytes);
+  a.q_scale = (float*)((char*)a.counter + 128);
   CC2_TRY(attention_error_word(&a.wait_err));
   CC2_TRY(error_word(&a.range_err));
   a.table_ld = table_ld;

@@ -7,16 +7,20 @@
 // the workspace as fp16 tiles in the tensor core's shared-memory order, each
 // row scaled to below 2^8.  Then persistent blocks, one an SM, walk items
 // (sequence, head, 256 rows, chunk of keys):
-//   warp 0        loader: finds the items, brings raw key blocks and query
-//                 tiles by bulk copies
-//   warps 12-15   decoders, a key a thread: K^ and V^ tiles as fp16, norms
+//   warp 0        loader: finds the items, brings raw key blocks by bulk copies
+//   warp 3        the same for the items' query tiles
+//   warps 20-23   decoders, a key a thread: K^ and V^ tiles as fp16, norms
 //                 multiplied in after scaling them by a power of two a block
-//   warps 1, 2    MMA issuers of the two pipelines (128 rows each):
-//                 S_j = Q K_j^T, O += P_j V_j, P in TMEM
-//   warps 4-11    softmax, a row a thread: running maximum (moved only past
-//                 2^8), exponentials partly as a polynomial on the FMA pipe,
-//                 P as fp16; at the end O back out of the codes' frame (64
-//                 registers of butterflies) and to memory
+//   warps 1, 2    MMA issuers of the two tiles of 128 rows
+//   warps 4-19    softmax, a row a thread: four chains, each a tile and every
+//                 other step of 64 keys
+//   warps 24-27   output: joins the two chains of a tile, turns the sums out of
+//                 the codes' frame (64 registers of butterflies), writes rows
+// A chain is S_j = Q K_j^T -> running maximum (moved only past 2^8), P_j =
+// 2^(S_j - m) as fp16 over S_j's place in TMEM -> O += P_j V_j -> S_{j+2}, with a
+// maximum, sum and O of its own.  One warp alone leaves its scheduler idle most
+// of the time (each of the steps waits for the one before it); four warps a
+// scheduler, none of which waits for another, fill it.
 // Exponents: K^ of a block is scaled by 2^-eK with eK from its largest norm,
 // which goes into the scores' factor; V^ by 2^-eV, which goes into P's exponent
 // against the largest eV so far.  Neither costs an operation a score.
@@ -33,20 +37,21 @@ namespace {
 
 using namespace tcx;
 
-constexpr int kThreads = 512;
-// 128 x (40 + 72) + 256 x 200 = 65536 registers, what the block is launched with (512 x 128)
-constexpr int kRegsControl = 40, kRegsDecode = 72, kRegsSoftmax = 200;
+constexpr int kThreads = 896;
+constexpr int kSoftmaxWarp = 4, kDecodeWarp = 20, kOutWarp = 24;
 constexpr int kTile = 128;                      // rows of a pipeline, keys of a block
 constexpr uint32_t kTileBytes = 128 * 128;      // 128 rows of 64 fp16
 constexpr uint32_t kRawBytes = 8 * kBlockBytes;
 constexpr int kKvStages = 3, kRawStages = 3, kItems = 4;
-constexpr int kOutPitch = 132;                  // bytes a staged output row
+constexpr int kSumPitch = 65 * 4, kOutPitch = 132;  // bytes of a row's staged sums, of its staged output
 constexpr uint32_t kQAt = 0, kKvAt = 2 * kTileBytes, kRawAt = kKvAt + kKvStages * 2 * kTileBytes,
-                   kOutAt = kRawAt + kRawStages * kRawBytes, kSmem = kOutAt + 2 * 128 * kOutPitch;
+                   kSumAt = kRawAt + kRawStages * kRawBytes, kOutAt = kSumAt + 128 * kSumPitch,
+                   kSmem = kOutAt + 128 * kOutPitch;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kSCol = 0, kPCol = 256, kOCol = 384;  // + 128 G, 64 G, 64 G for pipeline G
+constexpr int kStep = 64;                       // keys of a step of the softmax
+// TMEM columns of tile g, chain c: S (and P over it) at 128 g + 64 c, O at 256 + 128 g + 64 c
+constexpr uint32_t kSCol = 0, kOCol = 256;
 constexpr float kRescaleLog2 = 8.0f;
-constexpr uint32_t kPolyPairs = (1u << 2) | (1u << 5) | (1u << 7) | (1u << 10) | (1u << 13) | (1u << 15);
 
 __device__ __forceinline__ uint32_t idesc_f16(int M, int N, bool b_mn_major) {
   return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
@@ -68,16 +73,24 @@ struct Item {
   long long q_tile;
 };
 
+struct Note {  // on half a block of keys: bit k of the words is key k
+  uint32_t seen[2];    // the key counts
+  uint32_t poison[2];  // its K or V is not finite
+};
+
 struct Control {
   uint64_t item_full[kItems], item_empty[kItems];
   uint64_t raw_full[kRawStages], raw_empty[kRawStages];
   uint64_t kv_full[kKvStages], kv_empty[kKvStages];
-  uint64_t q_full[2], q_empty[2], s_full[2], s_free[2], p_full[2], p_free[2], o_full[2], mma_done[2];
+  uint64_t q_full[2], q_empty[2], o_full[2], o_free[2], mma_done[2];
+  uint64_t s_full[2][2], p_full[2][2];  // [tile][chain]
   Item items[kItems];
-  uint32_t seen[kKvStages][4];    // bit k: key k of the block counts
-  uint32_t poison[kKvStages][4];  // bit k: its K or V is not finite
-  int e_k[kKvStages], e_v[kKvStages];
+  alignas(16) Note notes[kKvStages][2];
+  int2 exps[kKvStages];                 // eK, eV
+  float m[2][2][2][128], l[2][2][2][128];  // [turn][tile][chain][row]
+  int ve[2][2][2];
   uint32_t top[2][4];
+  uint32_t turn_out[64];                // byte offset in an output row of rotated coordinate i, its sign in bit 31
   uint32_t tmem;
   int abort_flag;
 };
@@ -92,78 +105,161 @@ struct Ring {
   }
 };
 
-// A warp's bounded wait: its lanes go on together or leave together.
-__device__ __forceinline__ bool wait(uint64_t& bar, uint32_t parity, Control& c, int* err) {
-  return __all_sync(0xffffffffu, mbar_wait_inl(smem_u32(&bar), parity, &c.abort_flag, err));
+// A warp's bounded wait: its lanes go on together or leave together.  The try
+// suspends the warp for up to `kSuspendNs`, so that a role that waits does not
+// take issue slots from the softmax and decoder warps of its scheduler.
+constexpr uint32_t kSuspendNs = 4000;
+__device__ __forceinline__ bool try_suspended(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(kSuspendNs)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int* flag, int* err) {
+  const unsigned long long t0 = globaltimer_ns();
+  for (;;) {
+    if (__all_sync(0xffffffffu, try_suspended(bar, parity))) return true;
+    const bool late = globaltimer_ns() - t0 > kWaitLimitNs;
+    if (late && *flag == 0) {
+      *flag = 1;
+      atomicOr(err, 1);
+    }
+    if (__any_sync(0xffffffffu, late || *flag)) return false;
+  }
+}
+__device__ __forceinline__ bool wait(uint64_t& bar_, uint32_t parity, Control& c, int* err) {
+  const uint32_t bar = smem_u32(&bar_);
+  return __all_sync(0xffffffffu, try_suspended(bar, parity)) || wait_long(bar, parity, &c.abort_flag, err);
 }
 
-// Butterflies of a row of 64 in registers.
+// Of 32 keys that count, those below the row's limit.
+__device__ __forceinline__ uint32_t visible(uint32_t seen, int limit) {
+  return limit >= 32 ? seen : limit <= 0 ? 0u : seen & ((1u << limit) - 1u);
+}
+// Scores of keys that the row does not see.
+__device__ __forceinline__ void hide(uint32_t (&v)[32], uint32_t vis) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (!((vis >> i) & 1u)) v[i] = 0xff800000u;
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Butterflies of a row of 64 in registers: width 1 within a pair of neighbours,
+// widths 2..32 two at a time.
 __device__ __forceinline__ void walsh(float* y) {
+  uint64_t p[32];
 #pragma unroll
-  for (int w = 1; w < 64; w <<= 1)
+  for (int i = 0; i < 32; ++i) p[i] = f2_pack(y[2 * i] + y[2 * i + 1], y[2 * i] - y[2 * i + 1]);
+  const uint64_t minus = f2_pack(-1.0f, -1.0f);
 #pragma unroll
-    for (int i = 0; i < 64; ++i)
+  for (int w = 1; w < 32; w <<= 1)
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
       if (!(i & w)) {
-        const float a = y[i], b = y[i + w];
-        y[i] = a + b;
-        y[i + w] = a - b;
+        const uint64_t a = p[i], b = p[i + w];
+        p[i] = f2_add(a, b);
+        p[i + w] = f2_fma(b, minus, a);
       }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f2_unpack(p[i], y[2 * i], y[2 * i + 1]);
 }
-
 // ------------------------------------------------------------------ queries --
-// A block rotates a tile of 128 rows of one head: a thread a row, as in
-// kv4_cache.cu.
+// A block rotates 128 rows of the call for one head, whatever sequences they
+// belong to: a thread a row, as in kv4_cache.cu.  Rows come in by four threads
+// each through shared memory and leave as 16-byte pieces of their tile.
 constexpr int kQThreads = 128, kQPitch = 65;
 
+struct QueryRow {
+  int seq, q_start;  // -1: no sequence has it
+};
+__device__ __forceinline__ QueryRow find_row(const Args& a, int tok, int lane) {
+  QueryRow r;
+  if (a.cu == nullptr) {
+    r.seq = tok / a.max_q;
+    r.q_start = r.seq * a.max_q;
+    return r;
+  }
+  r.seq = -1;  // the last sequence that starts at or before the token
+  for (int i = lane; i - lane < a.num_seqs; i += 32)
+    r.seq += __popc(__ballot_sync(0xffffffffu, i < a.num_seqs && a.cu[i] <= tok));
+  r.q_start = r.seq >= 0 ? a.cu[r.seq] : 0;
+  return r;
+}
+
 __global__ void __launch_bounds__(kQThreads)
-rotate_queries_kernel(const __grid_constant__ Args a) {
+rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles) {
   pdl_launch_dependents();
   pdl_wait();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.counter = 0;  // for the kernel after this one
   __shared__ float rows[128 * kQPitch];
   const int tid = threadIdx.x, lane = tid & 31;
-  const int head = blockIdx.y;
-  const long long tile = blockIdx.x;
-  // the last sequence whose tiles start at or before this one
-  int seq = -1;
-  for (int i = lane; i - lane < a.num_seqs; i += 32) {
-    const bool in = i < a.num_seqs &&
-                    first_query_tile(a, i, a.cu != nullptr ? min(max(a.cu[i], 0), a.total_q) : i * a.max_q) <= tile;
-    seq += __popc(__ballot_sync(0xffffffffu, in));
+  const int head = blockIdx.y, base = blockIdx.x * 128, all = a.total_q * a.group;
+  __shared__ const __nv_bfloat16* row_at[128];
+  __shared__ int row_pos[128];
+  __shared__ uint32_t turn_in[64];  // rotated coordinate i: byte offset of the one it comes from, its sign in bit 31
+  if (tid < 64) turn_in[tid] = 4u * a.rk.perm[tid] | ((a.rk.signs[tid >> 5] >> (tid & 31)) & 1u) << 31;
+  // this thread's row: a block's rows mostly belong to one sequence, the others follow it
+  const QueryRow at = find_row(a, base / a.group, lane);
+  const int row = base + tid;
+  const __nv_bfloat16* from = nullptr;
+  int pos = -1, in_seq = 0;
+  long long to = -1;
+  if (row < all) {
+    const int tok = row / a.group;
+    int seq = at.seq;
+    if (a.cu == nullptr) seq = tok / a.max_q;
+    else
+      while (seq + 1 < a.num_seqs && a.cu[seq + 1] <= tok) ++seq;
+    if (seq >= 0) {
+      const Span s = span_of(a, seq, 0, false);
+      in_seq = row - s.q_start * a.group;
+      if (in_seq < s.rows) {
+        from = (const __nv_bfloat16*)a.q + (long long)tok * a.q_ld + (long long)(head * a.group + row % a.group) * a.q_hs;
+        to = (long long)head * q_tiles + first_query_tile(a, seq, s.q_start) + in_seq / 128;
+        if (a.rotate) pos = s.len - s.n + (tok - s.q_start);
+        if (pos >= a.rope_len) {
+          if (a.rotate) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+          pos = -1;
+        }
+      }
+    }
   }
-  if (seq < 0) return;
-  Span s = span_of(a, seq, 0, tile == 0 && head == 0 && tid == 0);
-  const int row0 = (int)(tile - first_query_tile(a, seq, s.q_start)) * 128;
-  if (row0 >= s.rows) return;
+  row_at[tid] = from;
+  row_pos[tid] = pos;
+  __syncthreads();
 #pragma unroll
   for (int it = 0; it < 4; ++it) {
-    const int r = it * 32 + (tid >> 2), c = tid & 3, row = row0 + r;
+    const int r = it * 32 + (tid >> 2), c = tid & 3, p = row_pos[r];
+    const __nv_bfloat16* q = row_at[r];
     float x[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) x[j] = 0.0f;
-    if (row < s.rows) {
-      const int i = row / a.group;
-      const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (long long)(s.q_start + i) * a.q_ld +
-                               (long long)(head * a.group + row % a.group) * a.q_hs + 8 * c;
-      const uint4 u = *reinterpret_cast<const uint4*>(q), v = *reinterpret_cast<const uint4*>(q + 32);
+    if (q != nullptr) {
+      const uint4 u = *reinterpret_cast<const uint4*>(q + 8 * c), v = *reinterpret_cast<const uint4*>(q + 8 * c + 32);
       const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[2 * j] = __uint_as_float(w[j] << 16);
         x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
       }
-      const int pos = s.len - s.n + i;
-      if (a.rotate && pos >= 0) {
-        if (pos >= a.rope_len) {
-          atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
-        } else {
-          const float2* cs = a.rope + (long long)pos * 32 + 8 * c;
+      if (p >= 0) {
+        const float4* cs = reinterpret_cast<const float4*>(a.rope + (long long)p * 32 + 8 * c);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float2 f = cs[j];
-            const float p = x[j], q1 = x[8 + j];
-            x[j] = p * f.x - q1 * f.y;
-            x[8 + j] = q1 * f.x + p * f.y;
-          }
+        for (int j = 0; j < 4; ++j) {
+          const float4 f = cs[j];
+          const float p0 = x[2 * j], q0 = x[8 + 2 * j], p1 = x[2 * j + 1], q1 = x[9 + 2 * j];
+          x[2 * j] = p0 * f.x - q0 * f.y;
+          x[8 + 2 * j] = q0 * f.x + p0 * f.y;
+          x[2 * j + 1] = p1 * f.z - q1 * f.w;
+          x[9 + 2 * j] = q1 * f.z + p1 * f.w;
         }
       }
     }
@@ -174,23 +270,23 @@ rotate_queries_kernel(const __grid_constant__ Args a) {
     }
   }
   __syncthreads();
+  if (to < 0) return;
   float y[64];
 #pragma unroll
   for (int i = 0; i < 64; ++i) {
-    const float x = rows[tid * kQPitch + a.rk.perm[i]];
-    y[i] = (a.rk.signs[i >> 5] >> (i & 31)) & 1u ? -x : x;
+    const uint32_t t = turn_in[i];
+    const uint32_t x = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(rows + tid * kQPitch) + (t & 0xffu));
+    y[i] = __uint_as_float(x ^ (t & 0x80000000u));
   }
   walsh(y);
   float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 64; ++i) {
-    y[i] *= 0.125f * a.qscale;
-    top = fmaxf(top, fabsf(y[i]));
-  }
-  const int e = min(max((int)(__float_as_uint(top) >> 23), 30), 254);
-  const float up = __int_as_float((261 - e) << 23);  // 2^(134 - e): the row below 2^8
-  const long long at = (long long)head * gridDim.x + tile;
-  uint8_t* dst = const_cast<uint8_t*>(a.qt) + at * kTileBytes + tid * 128;
+  for (int i = 0; i < 64; ++i) top = fmaxf(top, fabsf(y[i]));
+  const float by = 0.125f * a.qscale;
+  const int e = min(max((int)(__float_as_uint(top * fabsf(by)) >> 23), 30), 254);
+  const float up = by * __int_as_float((261 - e) << 23);  // 2^(134 - e): the row below 2^8
+  const int r = in_seq & 127;
+  uint8_t* dst = const_cast<uint8_t*>(a.qt) + to * kTileBytes + r * 128;
 #pragma unroll
   for (int c = 0; c < 8; ++c) {  // 16-byte pieces, exchanged within 8 rows as the tensor core reads them
     uint4 w;
@@ -198,9 +294,9 @@ rotate_queries_kernel(const __grid_constant__ Args a) {
     w.y = pack_half(y[8 * c + 2] * up, y[8 * c + 3] * up);
     w.z = pack_half(y[8 * c + 4] * up, y[8 * c + 5] * up);
     w.w = pack_half(y[8 * c + 6] * up, y[8 * c + 7] * up);
-    *reinterpret_cast<uint4*>(dst + ((c ^ (tid & 7)) << 4)) = w;
+    *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) = w;
   }
-  const_cast<float*>(a.q_scale)[at * 128 + tid] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64
+  const_cast<float*>(a.q_scale)[to * 128 + r] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64
 }
 
 // ---------------------------------------------------------------- attention --
@@ -208,28 +304,31 @@ __global__ void __launch_bounds__(kThreads, 1)
 attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const int total_items) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ Control ctl;
-  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  const uint32_t smem = smem_u32(smem_raw) + pad;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* const err = a.wait_err;
   pdl_launch_dependents();
 
   if (tid == 0) {
-    for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&ctl.item_full[i]), 1), mbar_init(smem_u32(&ctl.item_empty[i]), 14);
+    for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&ctl.item_full[i]), 1), mbar_init(smem_u32(&ctl.item_empty[i]), 27);
     for (int i = 0; i < kRawStages; ++i) mbar_init(smem_u32(&ctl.raw_full[i]), 1), mbar_init(smem_u32(&ctl.raw_empty[i]), 4);
-    for (int i = 0; i < kKvStages; ++i) mbar_init(smem_u32(&ctl.kv_full[i]), 4), mbar_init(smem_u32(&ctl.kv_empty[i]), 2 + 8);
+    for (int i = 0; i < kKvStages; ++i) mbar_init(smem_u32(&ctl.kv_full[i]), 4), mbar_init(smem_u32(&ctl.kv_empty[i]), 2 + 16);
     for (int g = 0; g < 2; ++g) {
       mbar_init(smem_u32(&ctl.q_full[g]), 1);
       mbar_init(smem_u32(&ctl.q_empty[g]), 1);
-      mbar_init(smem_u32(&ctl.s_full[g]), 1);
-      mbar_init(smem_u32(&ctl.s_free[g]), 4);
-      mbar_init(smem_u32(&ctl.p_full[g]), 4);
-      mbar_init(smem_u32(&ctl.p_free[g]), 1);
-      mbar_init(smem_u32(&ctl.o_full[g]), 1);
+      mbar_init(smem_u32(&ctl.o_full[g]), 2);
+      mbar_init(smem_u32(&ctl.o_free[g]), 4);
       mbar_init(smem_u32(&ctl.mma_done[g]), 1);
+      for (int c = 0; c < 2; ++c) {
+        mbar_init(smem_u32(&ctl.s_full[g][c]), 1);
+        mbar_init(smem_u32(&ctl.p_full[g][c]), 4);
+      }
     }
     ctl.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid < 64) ctl.turn_out[tid] = 2u * a.rv.perm[tid] | ((a.rv.signs[tid >> 5] >> (tid & 31)) & 1u) << 31;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)),
                  "r"(kTmemCols)
@@ -242,34 +341,35 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
   pdl_wait();
   const uint32_t tmem = ctl.tmem;
 
-  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
-  else if (warp >= 12) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsDecode));
-  else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-
   if (warp == 0) {
     // ---------------- loader ----------------
     Ring<kItems> it;
     Ring<kRawStages> raw;
     long long n_items = 0, n_raw = 0;
-    uint32_t nq[2] = {0, 0};
     const int mask = (1 << a.pool.page_shift) - 1;
     const int run = min((mask + 1) / kBlockTokens, 8);  // blocks of 16 keys a copy brings
     bool ok = true;
-    for (long long base = blockIdx.x; ok; base += 32LL * gridDim.x) {
-      // each lane looks at one item
-      const long long mine = base + (long long)lane * gridDim.x;
+    // Items are taken as blocks get to them (their costs differ by the rows' and
+    // sequences' lengths): a few at a time where there are many, since many of
+    // them may turn out to have no rows or no keys.
+    const int batch = min(max(total_items / (8 * (int)gridDim.x), 1), 32);
+    while (ok) {
+      int base = 0;
+      if (lane == 0) base = atomicAdd(a.counter, batch);
+      base = __shfl_sync(0xffffffffu, base, 0);
       const bool any_left = base < total_items;
+      const int mine = lane < batch ? base + lane : total_items;  // each lane looks at one item
       Item d;
       d.seq = -1;
       if (mine < total_items) {
         unsigned idx = (unsigned)mine;
-        const int tile = (int)(idx % a.row_tiles);
+        const int tile = a.row_tiles - 1 - (int)(idx % a.row_tiles);  // causal rows with the most keys first
         idx /= a.row_tiles;
         d.split = (int)(idx % a.splits);
         idx /= a.splits;
         d.head = (int)(idx % a.pool.heads);
         const int seq = (int)(idx / a.pool.heads);
-        const Span s = span_of(a, seq, tile, false);
+        const Span s = span_of(a, seq, tile, d.split == 0 && d.head == 0 && tile == 0);
         d.chunks = chunks_of(a, s);
         if (s.row0 < s.rows && d.split < max(d.chunks, 1)) {
           d.seq = seq;
@@ -304,9 +404,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         }
         __syncwarp();
         const Item& e = ctl.items[it.i];
-        const int seq = e.seq, c0 = e.c0, c1 = e.c1, head = e.head, rows = e.rows - e.row0;
-        const int blocks[2] = {e.blocks[0], e.blocks[1]};
-        const long long q_tile = e.q_tile;
+        const int seq = e.seq, c0 = e.c0, c1 = e.c1, head = e.head, nb = max(e.blocks[0], e.blocks[1]);
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctl.item_full[it.i]));
         it.next();
@@ -315,21 +413,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
           ok = false;
           break;
         }
-        for (int g = 0; g < 2 && ok; ++g) {
-          if (blocks[g] == 0) continue;
-          if (nq[g] > 0 && !wait(ctl.q_empty[g], (nq[g] - 1) & 1u, ctl, err)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) {  // the tile's rows, in groups of 8
-            const uint32_t bytes = (uint32_t)min((rows - kTile * g + 7) / 8, kTile / 8) * 1024u;
-            mbar_arrive_expect_tx(smem_u32(&ctl.q_full[g]), bytes);
-            bulk_load(smem + kQAt + g * kTileBytes, a.qt + (q_tile + g) * kTileBytes, bytes, smem_u32(&ctl.q_full[g]));
-          }
-          ++nq[g];
-        }
         const int* table = a.table + (long long)seq * a.table_ld;
-        const int nb = max(blocks[0], blocks[1]);
         const int first = lane * run;  // this lane's first block of 16 keys
         int page = -1;
         if (nb > 0 && lane < 8 && c0 + first * kBlockTokens < c1 && first < 8)
@@ -370,6 +454,39 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
                globaltimer_ns() - t0 < kWaitLimitNs) {
         }
       }
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ---------------- query loader ----------------
+    Ring<kItems> it;
+    uint32_t nq[2] = {0, 0};
+    bool ok = true;
+    while (ok) {
+      if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
+      const Item& e = ctl.items[it.i];
+      const int seq = e.seq, rows = e.rows - e.row0, blocks[2] = {e.blocks[0], e.blocks[1]};
+      const long long q_tile = e.q_tile;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
+      it.next();
+      if (seq < 0) break;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (blocks[g] == 0 || !ok) continue;
+        if (nq[g] > 0) ok = wait(ctl.q_empty[g], (nq[g] - 1) & 1u, ctl, err);
+        if (!ok) break;
+        if (lane == 0) {  // the tile's rows, in groups of 8
+          const uint32_t bytes = (uint32_t)min((rows - kTile * g + 7) / 8, kTile / 8) * 1024u;
+          mbar_arrive_expect_tx(smem_u32(&ctl.q_full[g]), bytes);
+          bulk_load(smem + kQAt + g * kTileBytes, a.qt + (q_tile + g) * kTileBytes, bytes, smem_u32(&ctl.q_full[g]));
+        }
+        __syncwarp();
+        ++nq[g];
+      }
+    }
+    if (lane == 0) {  // as above
+      const unsigned long long t0 = globaltimer_ns();
+#pragma unroll
       for (int g = 0; g < 2; ++g)
         if (nq[g] > 0)
           while (!mbar_try(smem_u32(&ctl.q_full[g]), (nq[g] - 1) & 1u) && globaltimer_ns() - t0 < kWaitLimitNs) {
@@ -377,92 +494,99 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
     }
     __syncwarp();
   } else if (warp < 3) {
-    // ---------------- MMA issuer of pipeline g ----------------
+    // ---------------- MMA issuer of tile g ----------------
+    // The warp stays converged and what it branches on is broadcast, so that
+    // descriptors stay in uniform registers; one elected lane issues.  The tensor
+    // core runs its products in order: S_{j+2} may follow P_j V_j, whose P it
+    // overwrites, at once, and its completion says that P_j V_j is done too.
     const int g = warp - 1;
     Ring<kItems> it;
     Ring<kKvStages> kv_s, kv_p;  // stage of the next S, of the next P V
-    uint32_t ns = 0, np = 0, nt = 0;
-    const uint32_t t_s = tmem + kSCol + 128u * g, t_p = tmem + kPCol + 64u * g, t_o = tmem + kOCol + 64u * g;
-    const uint64_t dq = sw128_desc(smem + kQAt + g * kTileBytes);
-    bool ok = true, any = false;
+    uint32_t nt = 0, np0 = 0, np1 = 0;  // items with keys, steps of the two chains
+    const uint32_t t_s = tmem + kSCol + 128u * g, t_o = tmem + kOCol + 128u * g;
+    const uint64_t dq = sw128_desc(smem + kQAt + g * kTileBytes), dk0 = sw128_desc(smem + kKvAt),
+                   dv0 = sw128_desc(smem + kKvAt + kTileBytes);
+    const uint32_t id_o = idesc_f16(128, 64, true);
+    constexpr uint64_t kStage = 2 * kTileBytes >> 4, kHalf = kTileBytes / 2 >> 4;  // descriptor steps
+    bool ok = true;
     while (ok) {
       if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
       const Item& e = ctl.items[it.i];
-      const int seq = e.seq, c0 = e.c0, blocks = e.blocks[g], key_end = e.key_end[g];
-      const int all = max(e.blocks[0], e.blocks[1]);
-      __syncwarp();
+      const int seq = __shfl_sync(0xffffffffu, e.seq, 0), blocks = __shfl_sync(0xffffffffu, e.blocks[g], 0),
+                keys = __shfl_sync(0xffffffffu, e.key_end[g] - e.c0, 0),
+                all = __shfl_sync(0xffffffffu, max(e.blocks[0], e.blocks[1]), 0);
       if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
+      __syncwarp();
       it.next();
       if (seq < 0) break;
-      auto issue_s = [&](int j) -> bool {
-        if (!wait(ctl.kv_full[kv_s.i], kv_s.phase, ctl, err)) return false;
-        if (ns > 0 && !wait(ctl.s_free[g], (ns - 1) & 1u, ctl, err)) return false;
-        tc_fence_after();
-        if (lane == 0) {
-          const int cols = min((key_end - c0 - j * kTile + 15) / 16 * 16, kTile);
-          const uint32_t id = idesc_f16(128, cols, false);
-          const uint64_t dk = sw128_desc(smem + kKvAt + kv_s.i * 2 * kTileBytes);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_bf16(t_s, dq + 2u * k, dk + 2u * k, id, k > 0);
-          mma_commit(smem_u32(&ctl.s_full[g]));
-          if (j == blocks - 1) mma_commit(smem_u32(&ctl.q_empty[g]));
-        }
-        __syncwarp();
-        any = true;
-        kv_s.next();
-        ++ns;
-        return true;
-      };
-      if (blocks > 0) {
-        if (!wait(ctl.q_full[g], nt & 1u, ctl, err)) break;
-        ++nt;
-        ok = issue_s(0);
-        for (int j = 0; j < blocks && ok; ++j) {
-          if (j + 1 < blocks) ok = issue_s(j + 1);
-          if (!ok || !wait(ctl.p_full[g], np & 1u, ctl, err)) {
-            ok = false;
-            break;
-          }
+      const int steps = blocks > 0 ? (keys + kStep - 1) / kStep : 0;
+      if (steps > 0) ok = wait(ctl.q_full[g], nt & 1u, ctl, err);
+      for (int j = -2; j < steps && ok; ++j) {  // P_j V_j, then S_{j+2}
+        if (j >= 0) {
+          const int n = min((keys - j * kStep + 15) >> 4, kStep / 16);
+          const uint32_t c = j & 1, parity = (c ? np1++ : np0++) & 1u;
+          const uint64_t dv = dv0 + kv_p.i * kStage + c * kHalf;
+          const bool last = j == steps - 1, done = c == 1 || last;
+          // the first product of an item waits until the item before has been read out
+          ok = (j > 0 || nt == 0 || wait(ctl.o_free[g], (nt - 1) & 1u, ctl, err)) &&
+               wait(ctl.p_full[g][c], parity, ctl, err);
+          if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
-            const int steps = min((key_end - c0 - j * kTile + 15) / 16, kTile / 16);
-            const uint32_t id = idesc_f16(128, 64, true);
-            const uint64_t dv = sw128_desc(smem + kKvAt + kv_p.i * 2 * kTileBytes + kTileBytes);
-            for (int k = 0; k < steps; ++k) mma_bf16_ts(t_o, t_p + 8u * k, dv + 128u * k, id, (j > 0 || k > 0) ? 1u : 0u);
-            mma_commit(smem_u32(&ctl.p_free[g]));
-            mma_commit(smem_u32(&ctl.kv_empty[kv_p.i]));
-            if (j == blocks - 1) mma_commit(smem_u32(&ctl.o_full[g]));
+          if (elect_one()) {
+            const uint32_t tp = t_s + 64u * c, to = t_o + 64u * c, acc = j > 1 ? 1u : 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (k < n) mma_bf16_ts(to, tp + 8u * k, dv + 128u * k, id_o, k > 0 ? 1u : acc);
+            if (done) mma_commit(smem_u32(&ctl.kv_empty[kv_p.i]));
+            if (last) {
+              mma_commit(smem_u32(&ctl.o_full[g]));
+              mbar_arrive(smem_u32(&ctl.o_full[g]));  // hands on the maxima and sums that came with P
+            }
           }
           __syncwarp();
-          kv_p.next();
-          ++np;
+          if (done) kv_p.next();
+        }
+        const int i = j + 2;
+        if (i < steps) {
+          const uint32_t id = idesc_f16(128, min((keys - i * kStep + 15) & ~15, kStep), false), c = i & 1;
+          if (c == 0) ok = wait(ctl.kv_full[kv_s.i], kv_s.phase, ctl, err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t dk = dk0 + kv_s.i * kStage + c * kHalf;
+          const bool last = i == steps - 1;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_bf16(t_s + 64u * c, dq + 2u * k, dk + 2u * k, id, k > 0);
+            mma_commit(smem_u32(&ctl.s_full[g][c]));
+            if (last) mma_commit(smem_u32(&ctl.q_empty[g]));
+          }
+          __syncwarp();
+          if (c == 1 || last) kv_s.next();
         }
       }
-      for (int j = blocks; j < all && ok; ++j) {  // blocks that only the other pipeline's rows see
-        if (!wait(ctl.kv_full[kv_p.i], kv_p.phase, ctl, err)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) mbar_arrive(smem_u32(&ctl.kv_empty[kv_p.i]));
+      if (steps > 0) ++nt;
+      for (int j = blocks; j < all && ok; ++j) {  // blocks that only the other tile's rows see
+        ok = wait(ctl.kv_full[kv_p.i], kv_p.phase, ctl, err);
+        if (ok && lane == 0) mbar_arrive(smem_u32(&ctl.kv_empty[kv_p.i]));
         __syncwarp();
         kv_p.next();
         kv_s.next();
       }
     }
-    if (any && lane == 0) {  // every MMA has completed before TMEM is released
+    if (nt > 0 && elect_one()) {  // every MMA has completed before TMEM is released
       mma_commit(smem_u32(&ctl.mma_done[g]));
       const unsigned long long t0 = globaltimer_ns();
       while (!mbar_try(smem_u32(&ctl.mma_done[g]), 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
       }
     }
     __syncwarp();
-  } else if (warp >= 12) {
+  } else if (warp >= kDecodeWarp && warp < kOutWarp) {
     // ---------------- decoders ----------------
     Ring<kItems> it;
     Ring<kRawStages> raw;
     Ring<kKvStages> kv;
     long long n_kv = 0;
-    const int k = tid - 12 * 32, w = warp - 12;  // key of the block, warp
+    const int k = tid - kDecodeWarp * 32, w = warp - kDecodeWarp;  // key of the block, warp
     uint32_t flip = 0;
     bool ok = true;
     while (ok) {
@@ -505,16 +629,18 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         }
         flip ^= 1u;
         if (lane == 0) {
-          ctl.seen[kv.i][w] = sb;
-          ctl.poison[kv.i][w] = pb;
-          if (w == 0) ctl.e_k[kv.i] = (int)ek, ctl.e_v[kv.i] = (int)ev;
+          ctl.notes[kv.i][w >> 1].seen[w & 1] = sb;
+          ctl.notes[kv.i][w >> 1].poison[w & 1] = pb;
+          if (w == 0) ctl.exps[kv.i] = make_int2((int)ek, (int)ev);
         }
         // norms below 1: 2^(126 - e)
         const __half2 hk = __float2half2_rn(nk * __int_as_float((253 - (int)ek) << 23));
         const __half2 hv = __float2half2_rn(nv * __int_as_float((253 - (int)ev) << 23));
         const uint32_t dst = smem + kKvAt + kv.i * 2 * kTileBytes + k * 128;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        // warps past the last key's group of 16 have nothing that an MMA reads
+        const bool used = 32 * w < c1 - (c0 + j * kTile);
+#pragma unroll 1
+        for (int m = 0; m < 2 && used; ++m) {
           const Levels& lv = m ? a.lv : a.lk;
           const __half2 n = m ? hv : hk;
 #pragma unroll
@@ -547,241 +673,303 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         ++n_kv;
       }
     }
-  } else if (warp >= 4) {
-    // ---------------- softmax and output of pipeline g ----------------
-    const int g = warp >= 8 ? 1 : 0, quarter = warp & 3, r = 32 * quarter + lane;
+  } else if (warp < kDecodeWarp) {
+    // ---------------- softmax: chain c of tile g ----------------
+    const int g = (warp - kSoftmaxWarp) >> 3, c = ((warp - kSoftmaxWarp) >> 2) & 1, quarter = warp & 3,
+              r = 32 * quarter + lane;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
-    const uint32_t t_s = t_lane + kSCol + 128u * g, t_p = t_lane + kPCol + 64u * g, t_o = t_lane + kOCol + 64u * g;
+    const uint32_t t_s = t_lane + kSCol + 128u * g + 64u * c, t_o = t_lane + kOCol + 128u * g;
     Ring<kItems> it;
     Ring<kKvStages> kv;
-    uint32_t ns = 0, np = 0, nt = 0;
+    uint32_t n = 0, nt = 0;  // steps of this chain, items with keys
+    bool ok = true;
+    while (ok) {
+      if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
+      const Item& in = ctl.items[it.i];
+      const int seq = in.seq, c0 = in.c0, blocks = in.blocks[g], all = max(in.blocks[0], in.blocks[1]);
+      const int row = in.row0 + kTile * g + r;
+      const bool warp_rows = row - lane < in.rows;
+      const int limit = a.causal ? min(in.len - in.n + row / a.group + 1, in.len) : in.len;  // keys the row sees
+      const int clear = a.causal ? in.len - in.n + (in.row0 + kTile * g) / a.group + 1 : in.len;
+      const int keys = in.key_end[g] - c0, steps = blocks > 0 ? (keys + kStep - 1) / kStep : 0;
+      const float* q_scale = a.q_scale + (in.q_tile + g) * 128 + r;
+      const bool valid = row < in.rows && blocks > 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
+      it.next();
+      if (seq < 0) break;
+      const float rs = valid ? *q_scale : 0.0f;
+      float m = -INFINITY, l = 0.0f;
+      int ve = 20;
+      for (int t = 0; t < all; ++t) {
+        // the decoders' notes on the block, then the scores
+        if (!wait(ctl.kv_full[kv.i], kv.phase, ctl, err)) {
+          ok = false;
+          break;
+        }
+        const int j = 2 * t + c;
+        const Note note = ctl.notes[kv.i][c];
+        const int2 ex = ctl.exps[kv.i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.kv_empty[kv.i]));
+        kv.next();
+        if (j >= steps) continue;
+        const int key0 = c0 + j * kStep;
+        const float sc = rs * __int_as_float((ex.x + 1) << 23);  // rs 2^(eK - 126)
+        const bool clean = key0 + kStep <= clear && (note.seen[0] & note.seen[1]) == 0xffffffffu &&
+                           (note.poison[0] | note.poison[1]) == 0;
+        const int cols = min(keys - j * kStep, kStep);
+        if (!wait(ctl.s_full[g][c], n & 1u, ctl, err)) {
+          ok = false;
+          break;
+        }
+        ++n;
+        tc_fence_after();
+        float scale = 1.0f;
+        bool rescale = false;
+        if (warp_rows) {
+          // two passes over S, 32 scores in registers at a time: 64 would spill
+          const bool two = cols > 32;
+          float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !two) break;
+            uint32_t v[32];
+            tmem_ld32(t_s + 32u * h, v);
+            tmem_ld_wait();
+            if (!clean) {
+              const uint32_t vis = visible(h ? note.seen[1] : note.seen[0], limit - key0 - 32 * h);
+              if ((h ? note.poison[1] : note.poison[0]) & vis) l = __int_as_float(0x7fffffff);
+              hide(v, vis);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              b0 = max3(b0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+              b1 = max3(b1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+              b2 = max3(b2, __uint_as_float(v[i + 4]), __uint_as_float(v[i + 5]));
+              b3 = max3(b3, __uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
+            }
+          }
+          const float bm = fmaxf(max3(b0, b1, b2), b3) * sc;
+          if (bm > m + kRescaleLog2 || (m == -INFINITY && bm > m)) {
+            scale = m == -INFINITY ? 0.0f : ex2(m - bm);
+            l *= scale;
+            m = bm;
+            rescale = true;
+          }
+          if (ex.y > ve) {
+            scale *= __int_as_float((127 - min(ex.y - ve, 126)) << 23);
+            ve = ex.y;
+            rescale = true;
+          }
+          // P = 2^(x - m) times 2^(eV - largest eV), the latter taken back out of the row's sum
+          const float dv = (float)max(ex.y - ve, -60);
+          const float off = (m == -INFINITY ? 0.0f : -m) + dv;
+          const uint64_t sc2 = f2_pack(sc, sc), off2 = f2_pack(off, off);
+          uint64_t la = f2_pack(0.0f, 0.0f), lb = la;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !two) break;
+            uint32_t v[32];
+            tmem_ld32(t_s + 32u * h, v);
+            tmem_ld_wait();
+            if (!clean) hide(v, visible(h ? note.seen[1] : note.seen[0], limit - key0 - 32 * h));
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), sc2, off2);
+              float x0, x1;
+              f2_unpack(x2, x0, x1);
+              x0 = ex2(x0);
+              x1 = ex2(x1);
+              if (k & 1) lb = f2_add(lb, f2_pack(x0, x1)); else la = f2_add(la, f2_pack(x0, x1));
+              v[k] = pack_half(x0, x1);
+            }
+            tmem_st16(t_s + 16u * h, v);  // over scores that both passes have read
+          }
+          float l0, l1;
+          f2_unpack(f2_add(la, lb), l0, l1);
+          l += (l0 + l1) * __int_as_float((127 - (int)dv) << 23);
+        }
+        if (t > 0 && __any_sync(0xffffffffu, rescale)) {  // S_j's completion said that O stands still
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            uint32_t o[16];
+            tmem_ld16(t_o + 64u * c + 16u * i, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * scale);
+            tmem_st16(t_o + 64u * c + 16u * i, o);
+          }
+        }
+        if (j + 2 >= steps) {  // the chain's last step: its maximum and sum, once the item before has been read out
+          if (nt > 0 && !wait(ctl.o_free[g], (nt - 1) & 1u, ctl, err)) {
+            ok = false;
+            break;
+          }
+          const int turn = (int)(nt & 1u);
+          ctl.m[turn][g][c][r] = m;
+          ctl.l[turn][g][c][r] = l;
+          if (r == 0) ctl.ve[turn][g][c] = ve;
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[g][c]));
+      }
+      if (!ok) break;
+
+      if (steps > 0) ++nt;
+    }
+  } else {
+    // ---------------- output ----------------
+    const int quarter = warp & 3, r = 32 * quarter + lane;
+    const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
+    Ring<kItems> it;
+    uint32_t nt[2] = {0, 0};  // a tile's items with keys
     bool ok = true;
     while (ok) {
       if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
       const Item& in = ctl.items[it.i];
       struct {
-        int seq, head, row0, rows, q_start, split, chunks, c0, key_end;
-      } e = {in.seq, in.head, in.row0, in.rows, in.q_start, in.split, in.chunks, in.c0, in.key_end[g]};
-      const int blocks = in.blocks[g], all = max(in.blocks[0], in.blocks[1]);
-      const int row = e.row0 + kTile * g + r;
-      const bool valid = row < e.rows;
-      const bool warp_rows = e.row0 + kTile * g + 32 * quarter < e.rows;
-      const int tok = row / a.group;
-      const int limit = a.causal ? min(in.len - in.n + tok + 1, in.len) : in.len;  // keys the row sees
-      const int clear = a.causal ? in.len - in.n + (e.row0 + kTile * g) / a.group + 1 : in.len;
-      const long long q_tile = in.q_tile;
+        int seq, head, row0, rows, q_start, split, chunks, keys[2];
+      } e = {in.seq, in.head, in.row0, in.rows, in.q_start, in.split, in.chunks, {in.key_end[0] - in.c0, in.key_end[1] - in.c0}};
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
       it.next();
       if (e.seq < 0) break;
-      const float rs = valid && blocks > 0 ? a.q_scale[(q_tile + g) * 128 + r] : 0.0f;
-      float m = -INFINITY, l = 0.0f;
-      int ve = 0;
-      for (int j = 0; j < blocks; ++j) {
-        // the decoders' notes on the block, then the scores
-        if (!wait(ctl.kv_full[kv.i], kv.phase, ctl, err) || !wait(ctl.s_full[g], ns & 1u, ctl, err)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const int key0 = e.c0 + j * kTile;
-        uint32_t sw[4], pw = 0;
-        bool clean = key0 + kTile <= clear;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sw[i] = ctl.seen[kv.i][i];
-          pw |= ctl.poison[kv.i][i];
-          clean = clean && sw[i] == 0xffffffffu;
-        }
-        clean = clean && pw == 0;
-        const float sc = rs * __int_as_float((ctl.e_k[kv.i] + 1) << 23);  // rs 2^(eK - 126)
-        const int ev = ctl.e_v[kv.i];
-        const int cols = min(e.key_end - key0, kTile);
-        uint32_t v[128];
-        if (warp_rows) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (32 * c < cols) tmem_ld32(t_s + 32u * c, v + 32 * c);
-          tmem_ld_wait();
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ctl.s_free[g]));
-        ++ns;
-        float scale = 1.0f;
-        bool rescale = false;
-        if (warp_rows) {
-          if (!clean) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (32 * c < cols) {
-                const int rel = limit - key0 - 32 * c;
-                const uint32_t vis = rel >= 32 ? sw[c] : rel <= 0 ? 0u : sw[c] & ((1u << rel) - 1u);
-                if (ctl.poison[kv.i][c] & vis) l = __int_as_float(0x7fffffff);
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (!((vis >> i) & 1u)) v[32 * c + i] = 0xff800000u;
-              }
-            }
-          }
-          float b0 = -INFINITY, b1 = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (32 * c < cols) {
-#pragma unroll
-              for (int i = 32 * c; i < 32 * c + 32; i += 4) {
-                b0 = max3(b0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-                b1 = max3(b1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-              }
-            }
-          const float bm = fmaxf(b0, b1) * sc;
-          if (j == 0) {
-            m = bm;
-            ve = ev;
-          } else {
-            if (bm > m + kRescaleLog2 || (m == -INFINITY && bm > m)) {
-              scale = m == -INFINITY ? 0.0f : ex2(m - bm);
-              l *= scale;
-              m = bm;
-              rescale = true;
-            }
-            if (ev > ve) {
-              scale *= __int_as_float((127 - min(ev - ve, 126)) << 23);
-              ve = ev;
-              rescale = true;
-            }
-          }
-        }
-        if (np > 0 && !wait(ctl.p_free[g], (np - 1) & 1u, ctl, err)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (warp_rows) {
-          // P = 2^(x - m) times 2^(eV - largest eV), the latter taken back out of the row's sum
-          const float dv = (float)max(ev - ve, -60);
-          const float off = (m == -INFINITY ? 0.0f : -m) + dv;
-          const uint64_t sc2 = f2_pack(sc, sc), off2 = f2_pack(off, off);
-          uint64_t l2 = f2_pack(0.0f, 0.0f);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (32 * c < cols) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const uint64_t x2 =
-                    f2_fma(f2_pack(__uint_as_float(v[32 * c + 2 * k]), __uint_as_float(v[32 * c + 2 * k + 1])), sc2, off2);
-                uint64_t p2;
-                if ((kPolyPairs >> k) & 1u) {
-                  p2 = f2_exp2_poly(x2);
-                } else {
-                  float x0, x1;
-                  f2_unpack(x2, x0, x1);
-                  p2 = f2_pack(ex2(x0), ex2(x1));
-                }
-                l2 = f2_add(l2, p2);
-                float p0, p1;
-                f2_unpack(p2, p0, p1);
-                pk[k] = pack_half(p0, p1);
-              }
-              tmem_st16(t_p + 16u * c, pk);
-            }
-          }
-          float l0, l1;
-          f2_unpack(l2, l0, l1);
-          l += (l0 + l1) * __int_as_float((127 - (int)dv) << 23);
-        }
-        if (j > 0 && __any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t o[32];
-            tmem_ld32(t_o + 32u * c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
-            tmem_st32(t_o + 32u * c, o);
+      for (int g = 0; g < 2; ++g) {
+        const int row = e.row0 + kTile * g + r;
+        const bool valid = row < e.rows, warp_rows = row - lane < e.rows;
+        const int keys = g ? e.keys[1] : e.keys[0];
+        const bool some = keys > 0, two = keys > kStep;
+        const uint32_t turn = (g ? nt[1] : nt[0]) & 1u;
+        float m = -INFINITY, l = 0.0f, fa = 0.0f, fb = 0.0f;
+        if (some) {
+          if (!wait(ctl.o_full[g], turn, ctl, err)) {
+            ok = false;
+            break;
+          }
+          if (g) ++nt[1]; else ++nt[0];
+          tc_fence_after();
+          const float ma = ctl.m[turn][g][0][r], mb = two ? ctl.m[turn][g][1][r] : -INFINITY;
+          m = fmaxf(ma, mb);
+          const float wa = ma == -INFINITY ? 0.0f : ex2(ma - m), wb = mb == -INFINITY ? 0.0f : ex2(mb - m);
+          l = ctl.l[turn][g][0][r] * wa;
+          // 2^(eV - 126) / 64 takes the scales of V and of the levels back out
+          fa = wa * __int_as_float((ctl.ve[turn][g][0] - 5) << 23);
+          if (two) {
+            l += ctl.l[turn][g][1][r] * wb;
+            fb = wb * __int_as_float((ctl.ve[turn][g][1] - 5) << 23);
           }
         }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(smem_u32(&ctl.p_full[g]));
-          mbar_arrive(smem_u32(&ctl.kv_empty[kv.i]));
+        const bool part = e.chunks > 1;
+        if (!part) {
+          const float inv = l == 0.0f ? 0.0f : __fdividef(0.125f, l);
+          fa *= inv;
+          fb *= inv;
         }
-        ++np;
-        kv.next();
-      }
-      if (!ok) break;
-      for (int j = blocks; j < all; ++j) {
-        if (!wait(ctl.kv_full[kv.i], kv.phase, ctl, err)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) mbar_arrive(smem_u32(&ctl.kv_empty[kv.i]));
-        kv.next();
-      }
-      if (!ok) break;
-      float o[64];
-#pragma unroll
-      for (int i = 0; i < 64; ++i) o[i] = 0.0f;
-      if (blocks > 0) {
-        if (!wait(ctl.o_full[g], nt & 1u, ctl, err)) {
-          ok = false;
-          break;
-        }
-        ++nt;
-        tc_fence_after();
-        if (warp_rows) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) tmem_ld32(t_o + 32u * c, reinterpret_cast<uint32_t*>(o) + 32 * c);
-          tmem_ld_wait();
-        }
-        tc_fence_before();
-      }
-      if (!warp_rows) continue;
-      if (m == -INFINITY && l == l) l = 0.0f;
-      const float down = blocks > 0 ? __int_as_float((ve - 5) << 23) : 0.0f;  // 2^(eV - 126) / 64
-      if (e.chunks > 1) {
-        if (valid) {
+        // 16 coordinates at a time: the chains joined, and butterflies of width 1..8
+        float* sums = reinterpret_cast<float*>(smem_raw + pad + kSumAt + r * kSumPitch);
+        const uint32_t t_o = t_lane + kOCol + 128u * g;
+        long long at = 0;
+        if (part) {
           Span s;
           s.q_start = e.q_start;
-          const long long at = part_at(a, s, e.head, e.split, row);
-          float4* dst = reinterpret_cast<float4*>(a.part + at * 64);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            dst[i] = make_float4(o[4 * i] * down, o[4 * i + 1] * down, o[4 * i + 2] * down, o[4 * i + 3] * down);
-          a.part_ml[at] = make_float2(m, l);
+          at = part_at(a, s, e.head, e.split, row);
         }
-        continue;
-      }
-      const float inv = l == 0.0f ? 0.0f : down * 0.125f / l;
+        if (warp_rows) {
+#pragma unroll 1
+          for (int h = 0; h < 4; ++h) {
+            uint32_t x[16], y[16];
+            if (some) tmem_ld16(t_o + 16u * h, x);
+            if (two) tmem_ld16(t_o + 64u + 16u * h, y);
+            tmem_ld_wait();
+            float o[16];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) o[i] *= inv;
-      walsh(o);
-      // out through shared memory: the permutation, then whole rows
-      const uint32_t stage = smem + kOutAt + g * 128 * kOutPitch + 32 * quarter * kOutPitch;
-      const uint32_t my = stage + lane * kOutPitch;
+            for (int i = 0; i < 16; ++i) {  // a chain without a step has no O
+              o[i] = some ? __uint_as_float(x[i]) * fa : 0.0f;
+              if (two) o[i] = fmaf(__uint_as_float(y[i]), fb, o[i]);
+            }
+            if (part) {
+              if (valid) {
+                float4* dst = reinterpret_cast<float4*>(a.part + at * 64 + 16 * h);
 #pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        const uint16_t b = __bfloat16_as_ushort(__float2bfloat16_rn((a.rv.signs[i >> 5] >> (i & 31)) & 1u ? -o[i] : o[i]));
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(my + 2u * a.rv.perm[i]), "h"(b) : "memory");
+                for (int i = 0; i < 4; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              }
+              continue;
+            }
+#pragma unroll
+            for (int w = 1; w < 16; w <<= 1)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (!(i & w)) {
+                  const float u = o[i], v = o[i + w];
+                  o[i] = u + v;
+                  o[i + w] = u - v;
+                }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[16 * h + i] = o[i];
+          }
+        }
+        if (some) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ctl.o_free[g]));
+        }
+        if (part && valid) a.part_ml[at] = make_float2(m, l);
+        if (part || !warp_rows) continue;
+        // widths 16 and 32, signs and permutation; whole rows leave through shared memory
+        uint8_t* stage = smem_raw + pad + kOutAt + 32 * quarter * kOutPitch;
+        uint8_t* my = stage + lane * kOutPitch;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 16; i0 += 4) {
+          float z[4][4];
+          uint32_t to[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              z[i][k] = sums[i0 + i + 16 * k];
+              to[i][k] = ctl.turn_out[i0 + i + 16 * k];
+            }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = z[i][0] + z[i][1], q = z[i][0] - z[i][1], u = z[i][2] + z[i][3], v = z[i][2] - z[i][3];
+            z[i][0] = p + u, z[i][1] = q + v, z[i][2] = p - u, z[i][3] = q - v;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint16_t*>(my + (to[i][k] & 0xffu)) = __bfloat16_as_ushort(
+                  __float2bfloat16_rn(__uint_as_float(__float_as_uint(z[i][k]) ^ (to[i][k] & 0x80000000u))));
+        }
+        __syncwarp();
+        const int tok = row / a.group, qh = e.head * a.group + row % a.group;
+        const unsigned long long mine =
+            (unsigned long long)((__nv_bfloat16*)a.out + (long long)(e.q_start + tok) * a.o_ld + (long long)qh * a.o_hs);
+        const int n_rows = min(32, e.rows - (row - lane));
+#pragma unroll 1
+        for (int i = 0; i < n_rows; i += 16) {  // eight lanes a row, 16 bytes each
+          uint8_t* dst[4];
+          uint4 x[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int k = i + 4 * w + (lane >> 3);
+            dst[w] = (uint8_t*)__shfl_sync(0xffffffffu, mine, k);
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(stage + k * kOutPitch + 16 * (lane & 7));
+            x[w] = make_uint4(src[0], src[1], src[2], src[3]);
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            if (i + 4 * w + (lane >> 3) < n_rows) *reinterpret_cast<uint4*>(dst[w] + 16 * (lane & 7)) = x[w];
+        }
+        __syncwarp();
+        if (a.lse != nullptr && valid)
+          a.lse[(long long)(e.q_start + tok) * (a.pool.heads * a.group) + qh] =
+              l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       }
-      __syncwarp();
-      const int qh = e.head * a.group + row % a.group;
-      const unsigned long long mine =
-          (unsigned long long)((__nv_bfloat16*)a.out + (long long)(e.q_start + tok) * a.o_ld + (long long)qh * a.o_hs);
-      const int n_rows = min(32, e.rows - (e.row0 + kTile * g + 32 * quarter));
-      for (int i = 0; i < n_rows; ++i) {
-        uint32_t* dst = (uint32_t*)__shfl_sync(0xffffffffu, mine, i);
-        uint32_t x;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(stage + i * kOutPitch + 4 * lane));
-        dst[lane] = x;
-      }
-      __syncwarp();
-      if (a.lse != nullptr && valid)
-        a.lse[(long long)(e.q_start + tok) * (a.pool.heads * a.group) + qh] =
-            l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
     }
   }
 
@@ -805,7 +993,8 @@ int launch_attend_tc(const Args& a, cudaStream_t st) {
     CC2_CUDA(cudaFuncSetAttribute(attend_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem + 1024));
     if (dev < 64) attr_done |= 1ull << dev;
   }
-  CC2_CUDA(launch_k(rotate_queries_kernel, dim3((unsigned)q_tiles, (unsigned)a.pool.heads), kQThreads, 0, st, a));
+  const unsigned q_blocks = (unsigned)(((long long)a.total_q * a.group + 127) / 128);
+  CC2_CUDA(launch_k(rotate_queries_kernel, dim3(q_blocks, (unsigned)a.pool.heads), kQThreads, 0, st, a, q_tiles));
   const unsigned grid = (unsigned)std::min<long long>(items, num_sms());
   CC2_CUDA(launch_k(attend_tc_kernel, grid, kThreads, kSmem + 1024, st, a, q_tiles, (int)items));
   CC2_CHECK_LAUNCH();

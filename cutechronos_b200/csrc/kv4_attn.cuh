@@ -33,6 +33,7 @@ struct Args {
   float2* part_ml;   // the same places: maximum (log2) and sum of exponentials
   const uint8_t* qt;  // rotated queries as fp16 tiles (attn_kv4_tc.cu) and their rows' scales
   const float* q_scale;
+  int* counter;       // items that the tcgen05 kernel's blocks have taken
   int* wait_err;
   int* range_err;
   int table_ld, rope_len, max_len;
