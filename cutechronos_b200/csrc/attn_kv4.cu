@@ -643,14 +643,13 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   a.causal = causal != 0;
   a.rotate = rotate_q != 0;
   a.qscale = scale * 1.4426950408889634f;
-  const Quant qk = make_quant(cache->key), qv = make_quant(cache->value);
-  for (int i = 0; i < 2; ++i) {
-    a.rk.signs[i] = qk.signs[i];
-    a.rv.signs[i] = qv.signs[i];
-  }
-  for (int i = 0; i < 64; ++i) {
-    a.rk.inv[a.rk.perm[i] = qk.perm[i]] = (uint8_t)i;
-    a.rv.inv[a.rv.perm[i] = qv.perm[i]] = (uint8_t)i;
+  const cc2_kv4_quant* quant[2] = {&cache->key, &cache->value};
+  Rotation* rotation[2] = {&a.rk, &a.rv};
+  for (int k = 0; k < 2; ++k) {
+    Rotation& r = *rotation[k];
+    r.signs[0] = (uint32_t)quant[k]->signs;
+    r.signs[1] = (uint32_t)(quant[k]->signs >> 32);
+    for (int i = 0; i < 64; ++i) r.inv[r.perm[i] = quant[k]->perm[i] & 63] = (uint8_t)i;
   }
   a.lk = make_levels(cache->key);
   a.lv = make_levels(cache->value);

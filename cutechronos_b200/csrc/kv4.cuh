@@ -39,11 +39,17 @@ struct Pool {
   int norm_bf16;   // norms are bf16 (else fp16)
 };
 
-// One quantiser for the kernels that quantise (by value: constant bank).
+// One quantiser for the kernels that quantise and restore (by value).
 struct Quant {
-  float levels[8], bounds[7];
-  uint32_t signs[2];  // bit i: coordinate i of the permuted vector is negated
-  uint8_t perm[64];
+  float levels[8];
+  // Element e of a vector is rotated coordinate go[e] & 63, negated if bit 7 is set.
+  uint8_t go[64];
+  // The magnitude by one comparison: r = round(512 |y| / 8n) is in 0..512 (|y| <= 8n), and of the bounds at most one,
+  // `bound`, can lie among the |y| of r / 8's cell; `below` bounds lie under it.
+  struct Cell {
+    float bound;  // +inf: none
+    uint32_t below;
+  } cells[65];
 };
 
 // Level tables of the fp16 decoder: 64 c_i split into its fp16 value and, for
@@ -132,7 +138,7 @@ __device__ __forceinline__ void decode_zip(const Zip& z, const uint32_t lo[2], c
 
 // --- host side --------------------------------------------------------------
 int check_cache(const cc2_kv4_cache* c, const char* what, Pool& pool);
-Quant make_quant(const cc2_kv4_quant& q);
+int make_quant(const cc2_kv4_quant& q, const char* what, Quant& r);
 Levels make_levels(const cc2_kv4_quant& q);
 // Device error word of the cache's kernels (DEV_ERR_CACHE_RANGE).
 int error_word(int** p);

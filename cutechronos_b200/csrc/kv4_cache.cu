@@ -1,20 +1,26 @@
 // Appending to and reading from the paged 4-bit K/V cache (layout: kv4.cuh,
 // definition: cc2.h).
 //
-// Append: y = H (s * x[perm]) / (8 n) of every K (rotated to its position
-// first) and V vector, each coordinate to a sign and one of 8 magnitudes, the
-// norm to 16 bits.  Bound by the arithmetic next to the memory: a token's head
-// moves 324 bytes (bf16), about 5e-11 s of the card's copy rate, and takes some
-// 2,300 operations, about 6e-11 s of its fp32 lanes.
-// So one thread owns a whole vector: the butterflies are 64 register adds a
-// width with no shuffles, sign and permutation are the same for all threads of
-// a warp, and the permutation costs nothing beyond the shared-memory read that
-// brings the vector in.  Rows of 64 floats at a pitch of 65 make that read and
-// the write before it free of bank conflicts.  Codes leave as two 16-byte
-// stores a thread.
+// Append: y = H (s * x[perm]) of every K (rotated to its position first) and V
+// vector, each coordinate to a sign and one of 8 magnitudes, the norm to 16
+// bits.  Read: the other way.  The memory's share is small (324 bytes a token
+// and head in bf16), so both are bound by the instructions a vector takes, and
+// everything here is laid out to save them:
+//  - four threads bring a vector in (or out), one thread then owns it whole: its
+//    butterflies are register adds, two at a time, with no shuffles;
+//  - sign and permutation are applied where four threads scatter (gather) a row
+//    in shared memory, from 16 places that each thread keeps in registers, so
+//    that the owner reads (writes) its row straight, 16 bytes at a time; a row
+//    pitch of 68 floats keeps that free of bank conflicts;
+//  - a magnitude takes one lookup and one comparison (kv4.cuh, Quant): three
+//    comparisons of a binary search and their selects ran on the half-rate
+//    integer pipe and were its limit;
+//  - places in the cache, pointers and positions are worked out once a vector.
 #include <algorithm>
+#include <cmath>
 
 #include "kv4.cuh"
+#include "tc_attn.cuh"
 
 namespace cc2 {
 namespace kv4 {
@@ -53,21 +59,37 @@ int check_cache(const cc2_kv4_cache* c, const char* what, Pool& pool) {
   return CC2_OK;
 }
 
-Quant make_quant(const cc2_kv4_quant& q) {
-  Quant r;
+int make_quant(const cc2_kv4_quant& q, const char* what, Quant& r) {
+  uint64_t met = 0;
+  for (int i = 0; i < 64; ++i) {
+    const int e = q.perm[i] & 63;
+    met |= 1ull << e;
+    r.go[e] = (uint8_t)(i | (((q.signs >> i) & 1) << 7));
+  }
+  CC2_REQUIRE(met == ~0ull, "%s: a quantiser's perm is no permutation", what);
   for (int i = 0; i < 8; ++i) r.levels[i] = q.levels[i];
-  for (int i = 0; i < 7; ++i) r.bounds[i] = q.bounds[i];
-  r.signs[0] = (uint32_t)q.signs;
-  r.signs[1] = (uint32_t)(q.signs >> 32);
-  for (int i = 0; i < 64; ++i) r.perm[i] = q.perm[i] & 63;
-  return r;
+  for (int c = 0; c < 65; ++c) {
+    // |y| / 8n of r = 8c .. 8c + 7, with room for the rounding of r itself
+    const float lo = (8 * c - 0.52f) / 512.0f, hi = (8 * c + 7.52f) / 512.0f;
+    r.cells[c].bound = INFINITY;
+    r.cells[c].below = 0;
+    for (int j = 0; j < 7; ++j) {
+      CC2_REQUIRE(q.bounds[j] > (j ? q.bounds[j - 1] : 0.0f), "%s: a quantiser's bounds must ascend from above 0", what);
+      if (q.bounds[j] <= lo) ++r.cells[c].below;
+      else if (q.bounds[j] <= hi) {
+        CC2_REQUIRE(r.cells[c].bound == INFINITY, "%s: a quantiser's bounds must be more than 1/60 apart", what);
+        r.cells[c].bound = q.bounds[j];
+      }
+    }
+  }
+  return CC2_OK;
 }
 
 namespace {
 
 constexpr int kThreads = 128;
 constexpr int kUnits = 64;   // (token, head) pairs a block handles: a thread for each K and each V
-constexpr int kPitch = 65;
+constexpr int kPitch = 68;
 
 struct Places {
   const int32_t* seq;
@@ -95,20 +117,30 @@ __device__ __forceinline__ long long place(const Pool& pool, const Places& at, i
   return block_offset(pool, page, head, *off);
 }
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float* x);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float* x) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float* x) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+// Eight neighbouring values as they lie in memory, and as floats.
+template <typename T> struct Raw;
+template <> struct Raw<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
   }
-}
+  __device__ __forceinline__ void get(float* x) const {
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  }
+};
+template <> struct Raw<__nv_bfloat16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float* x) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
 template <typename T> __device__ __forceinline__ void store8(T* p, const float* x);
 template <> __device__ __forceinline__ void store8<float>(float* p, const float* x) {
   reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -124,137 +156,187 @@ template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16*
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Butterflies of width 1, 2, ..., 32 over 64 registers.
+// Butterflies of width 1, 2, ..., 32 over 64 registers, each sum and difference rounded once: width 1 within pairs of
+// neighbours, the others two at a time (a - b as a + b * -1, the product exact).
 __device__ __forceinline__ void walsh(float (&y)[64]) {
+  using namespace tcx;
+  uint64_t p[32];
 #pragma unroll
-  for (int w = 1; w < 64; w <<= 1) {
+  for (int i = 0; i < 32; ++i) p[i] = f2_pack(__fadd_rn(y[2 * i], y[2 * i + 1]), __fsub_rn(y[2 * i], y[2 * i + 1]));
+  const uint64_t minus = f2_pack(-1.0f, -1.0f);
 #pragma unroll
-    for (int i = 0; i < 64; ++i) {
-      if (i & w) continue;
-      const float a = y[i], b = y[i + w];
-      y[i] = __fadd_rn(a, b);
-      y[i + w] = __fsub_rn(a, b);
+  for (int w = 1; w < 32; w <<= 1)
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (!(i & w)) {
+        const uint64_t a = p[i], b = p[i + w];
+        p[i] = f2_add(a, b);
+        p[i + w] = f2_fma(b, minus, a);
+      }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f2_unpack(p[i], y[2 * i], y[2 * i + 1]);
+}
+
+// The 16 places of a thread's elements 8c .. 8c + 7 and 32 + 8c .. in a rotated row: byte offsets, signs in bit 31.
+__device__ __forceinline__ void my_places(const Quant& q, int c, uint32_t (&to)[16]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint2 w = *reinterpret_cast<const uint2*>(q.go + 32 * h + 8 * c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t b = ((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu;
+      to[8 * h + j] = (b & 63u) * 4u | (b & 128u) << 24;
     }
   }
 }
-
-__device__ __forceinline__ void encode(const float (&y)[64], float n8, const Quant& q, uint32_t (&word)[8]) {
-  float t[7];
-#pragma unroll
-  for (int j = 0; j < 7; ++j) t[j] = __fmul_rn(q.bounds[j], n8);
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    uint32_t c = 0;
-#pragma unroll
-    for (int p = 0; p < 8; ++p) {  // three comparisons find the magnitude: 4, 2, 1
-      const float v = y[8 * w + p], a = fabsf(v);
-      const bool h = a > t[3];
-      const bool m = a > (h ? t[5] : t[1]);
-      const bool l = a > (m ? (h ? t[6] : t[2]) : (h ? t[4] : t[0]));
-      c |= (h ? 4u << (4 * p) : 0u) | (m ? 2u << (4 * p) : 0u) | (l ? 1u << (4 * p) : 0u);
-      c |= v < 0.0f ? 1u << sign_bit(p) : 0u;
-    }
-    word[w] = c;
-  }
+__device__ __forceinline__ float flip(float x, uint32_t to) {
+  return __uint_as_float(__float_as_uint(x) ^ (to & 0x80000000u));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
+// What a block knows of its units.
+struct Unit {
+  long long block;   // byte offset of the unit's block of 16 tokens, -1: skip
+  int pos;           // to rotate to
+  int slot;          // place in the block of 16; bit 8: masked
+};
+
+template <typename T, bool kRope>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4)
 append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant qk, const __grid_constant__ Quant qv,
               const T* __restrict__ k, long long k_ld, long long k_hs, const T* __restrict__ v, long long v_ld,
               long long v_hs, int tokens, Places at, const uint8_t* __restrict__ mask,
               const float2* __restrict__ rope, int rope_len, int* __restrict__ err) {
   pdl_launch_dependents();
-  pdl_wait();
-  __shared__ float rows[2 * kUnits * kPitch];
+  __shared__ __align__(16) float rows[2 * kUnits * kPitch];
   __shared__ float norm[2 * kUnits];
+  __shared__ Quant::Cell cells[2][128];  // 65 used; a NaN may point at any
+  __shared__ Unit units[kUnits];
+  constexpr int kIts = kUnits * 4 / kThreads;
   const int tid = threadIdx.x;
-  const long long units = (long long)tokens * pool.heads;
+  cells[0][tid] = qk.cells[min(tid, 64)];
+  cells[1][tid] = qv.cells[min(tid, 64)];
+  pdl_wait();
+  const long long total = (long long)tokens * pool.heads;
   const long long u0 = (long long)blockIdx.x * kUnits;
-  const int pos_limit = rope != nullptr ? rope_len : 0x7fffffff;
+  const int t0 = (int)(u0 / pool.heads), h0 = (int)(u0 % pool.heads);
+  const int last = (int)min(total - u0, (long long)kUnits) - 1;  // units past it read the last one's rows
 
   // four threads bring a vector in: thread c its values 8c .. 8c+7 and 32 + 8c ..
+  const int c = tid & 3;
+  Raw<T> raw[2][kIts][2];
 #pragma unroll
-  for (int it = 0; it < 2 * kUnits * 4 / kThreads; ++it) {
-    const int task = it * kThreads + tid, r = task >> 2, c = task & 3;
-    const bool is_v = r >= kUnits;
-    const long long u = u0 + (r & (kUnits - 1));
-    float a[8], b[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.0f;
-    if (u < units) {
-      const int t = (int)(u / pool.heads), h = (int)(u % pool.heads);
-      const T* x = is_v ? v + (long long)t * v_ld + (long long)h * v_hs : k + (long long)t * k_ld + (long long)h * k_hs;
-      load8(x + 8 * c, a);
-      load8(x + 32 + 8 * c, b);
-      if (!is_v && rope != nullptr) {
-        const int pos = at.pos[t];
-        if (pos >= 0 && pos < rope_len) {
-          const float4* cs = reinterpret_cast<const float4*>(rope + (long long)pos * 32 + 8 * c);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 f = cs[j];
-            const float a0 = a[2 * j], b0 = b[2 * j], a1 = a[2 * j + 1], b1 = b[2 * j + 1];
-            a[2 * j] = __fsub_rn(__fmul_rn(a0, f.x), __fmul_rn(b0, f.y));
-            b[2 * j] = __fadd_rn(__fmul_rn(b0, f.x), __fmul_rn(a0, f.y));
-            a[2 * j + 1] = __fsub_rn(__fmul_rn(a1, f.z), __fmul_rn(b1, f.w));
-            b[2 * j + 1] = __fadd_rn(__fmul_rn(b1, f.z), __fmul_rn(a1, f.w));
-          }
-        }
-      }
+  for (int it = 0; it < kIts; ++it) {
+    const unsigned x = (unsigned)(h0 + min(it * (kThreads / 4) + (tid >> 2), last));
+    const unsigned dt = x / (unsigned)pool.heads, h = x - dt * (unsigned)pool.heads;
+    const T* from = k + (long long)(t0 + dt) * k_ld + (long long)h * k_hs + 8 * c;
+    raw[0][it][0].load(from);
+    raw[0][it][1].load(from + 32);
+    from = v + (long long)(t0 + dt) * v_ld + (long long)h * v_hs + 8 * c;
+    raw[1][it][0].load(from);
+    raw[1][it][1].load(from + 32);
+  }
+  if (tid < kUnits) {
+    Unit u;
+    u.block = -1;
+    u.pos = 0;
+    u.slot = 0;
+    if (tid <= last) {
+      const unsigned x = (unsigned)(h0 + tid), dt = x / (unsigned)pool.heads, h = x - dt * (unsigned)pool.heads;
+      const int t = t0 + (int)dt;
+      int off = 0;
+      u.block = place(pool, at, t, (int)h, kRope ? rope_len : 0x7fffffff, &off, err);
+      u.slot = (off & (kBlockTokens - 1)) | (mask != nullptr && mask[t] == 0 ? 256 : 0);
+      if (kRope && u.block >= 0) u.pos = at.pos[t];
     }
-    // squares added in halves: i and i + 32, then 16 and 8 apart (the threads of
-    // a vector), then 4, 2, 1 apart
-    float s[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = __fadd_rn(__fmul_rn(a[j], a[j]), __fmul_rn(b[j], b[j]));
-#pragma unroll
-    for (int o = 2; o > 0; o >>= 1) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = __fadd_rn(s[j], __shfl_xor_sync(0xffffffffu, s[j], o));
-    }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-#pragma unroll
-      for (int j = 0; j < o; ++j) s[j] = __fadd_rn(s[j], s[j + o]);
-    }
-    float* row = rows + r * kPitch;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      row[8 * c + j] = a[j];
-      row[32 + 8 * c + j] = b[j];
-    }
-    if (c == 0) norm[r] = __fsqrt_rn(s[0]);
+    units[tid] = u;
   }
   __syncthreads();
 
-  const bool is_v = tid >= kUnits;  // whole warps
-  const long long u = u0 + (tid & (kUnits - 1));
-  if (u >= units) return;
-  const int t = (int)(u / pool.heads), h = (int)(u % pool.heads);
-  int off = 0;
-  const long long at_block = place(pool, at, t, h, pos_limit, &off, err);
-  if (at_block < 0) return;
-  const float* row = rows + tid * kPitch;
-  const float n = norm[tid];
-  const float n8 = __fmul_rn(n, 8.0f);
-  const Quant& q = is_v ? qv : qk;
+#pragma unroll
+  for (int is_v = 1; is_v >= 0; --is_v) {
+    uint32_t to[16];
+    my_places(is_v ? qv : qk, c, to);
+#pragma unroll
+    for (int it = 0; it < kIts; ++it) {
+      const int r = it * (kThreads / 4) + (tid >> 2);
+      float a[8], b[8];
+      raw[is_v][it][0].get(a);
+      raw[is_v][it][1].get(b);
+      if (kRope && !is_v) {
+        const float4* cs = reinterpret_cast<const float4*>(rope + (long long)units[r].pos * 32 + 8 * c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4 f = cs[j];
+          const float a0 = a[2 * j], b0 = b[2 * j], a1 = a[2 * j + 1], b1 = b[2 * j + 1];
+          a[2 * j] = __fsub_rn(__fmul_rn(a0, f.x), __fmul_rn(b0, f.y));
+          b[2 * j] = __fadd_rn(__fmul_rn(b0, f.x), __fmul_rn(a0, f.y));
+          a[2 * j + 1] = __fsub_rn(__fmul_rn(a1, f.z), __fmul_rn(b1, f.w));
+          b[2 * j + 1] = __fadd_rn(__fmul_rn(b1, f.z), __fmul_rn(a1, f.w));
+        }
+      }
+      // squares added in halves: i and i + 32, then 16 and 8 apart (the threads of
+      // a vector), then 4, 2, 1 apart
+      float s[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = __fadd_rn(__fmul_rn(a[j], a[j]), __fmul_rn(b[j], b[j]));
+#pragma unroll
+      for (int o = 2; o > 0; o >>= 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = __fadd_rn(s[j], __shfl_xor_sync(0xffffffffu, s[j], o));
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+#pragma unroll
+        for (int j = 0; j < o; ++j) s[j] = __fadd_rn(s[j], s[j + o]);
+      }
+      uint8_t* row = reinterpret_cast<uint8_t*>(rows + (is_v * kUnits + r) * kPitch);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        *reinterpret_cast<float*>(row + (to[j] & 0xffu)) = flip(a[j], to[j]);
+        *reinterpret_cast<float*>(row + (to[8 + j] & 0xffu)) = flip(b[j], to[8 + j]);
+      }
+      if (c == 0) norm[is_v * kUnits + r] = __fsqrt_rn(s[0]);
+    }
+  }
+  __syncthreads();
+
+  const int is_v = tid >= kUnits;  // whole warps
+  const Unit& u = units[tid & (kUnits - 1)];
+  if (u.block < 0) return;
   float y[64];
 #pragma unroll
-  for (int i = 0; i < 64; ++i) {
-    const float x = row[q.perm[i]];
-    y[i] = (q.signs[i >> 5] >> (i & 31)) & 1u ? -x : x;
+  for (int i = 0; i < 16; ++i) {
+    const float4 f = *reinterpret_cast<const float4*>(rows + tid * kPitch + 4 * i);
+    y[4 * i] = f.x, y[4 * i + 1] = f.y, y[4 * i + 2] = f.z, y[4 * i + 3] = f.w;
   }
   walsh(y);
+  const float n = norm[tid];
+  const float n8 = __fmul_rn(n, 8.0f);
+  const float fine = n8 > 0.0f ? __fdividef(512.0f, n8) : 0.0f;  // its error is within the cells' room
+  const uint8_t* table = reinterpret_cast<const uint8_t*>(cells[is_v]);
   uint32_t word[8];
-  encode(y, n8, q, word);
-  uint8_t* block = pool.pages + at_block;
-  const int slot = off & (kBlockTokens - 1);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    uint32_t code = 0;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const float x = y[8 * w + p], a = fabsf(x);
+      // r in the low bits of 2^23 + r; its cell's entry
+      const uint32_t r = __float_as_uint(fmaf(a, fine, 8388608.0f)) & 0x3f8u;
+      const Quant::Cell cell = *reinterpret_cast<const Quant::Cell*>(table + r);
+      code += cell.below * (1u << (4 * p));
+      if (a > __fmul_rn(cell.bound, n8)) code += 1u << (4 * p);
+      if (x < 0.0f) code |= 1u << sign_bit(p);
+    }
+    word[w] = code;
+  }
+  uint8_t* block = pool.pages + u.block;
+  const int slot = u.slot & 255;
   uint4* codes = reinterpret_cast<uint4*>(block + (is_v ? kVCodes : 0) + slot * 32);
   codes[0] = make_uint4(word[0], word[1], word[2], word[3]);
   codes[1] = make_uint4(word[4], word[5], word[6], word[7]);
   uint16_t nb = norm_bits(n, pool.norm_bf16);
-  if (!is_v && mask != nullptr && mask[t] == 0) nb |= 0x8000u;
+  if (!is_v && (u.slot & 256)) nb |= 0x8000u;
   reinterpret_cast<uint16_t*>(block + (is_v ? kVNorms : kKNorms))[slot] = nb;
 }
 
@@ -264,10 +346,11 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant qk,
             T* __restrict__ k_out, T* __restrict__ v_out, int tokens, Places at, int* __restrict__ err) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float rows[2 * kUnits * kPitch];
+  __shared__ __align__(16) float rows[2 * kUnits * kPitch];
+  __shared__ float scale[2 * kUnits];
   __shared__ float level[2][8];
   const int tid = threadIdx.x;
-  const long long units = (long long)tokens * pool.heads;
+  const long long total = (long long)tokens * pool.heads;
   const long long u0 = (long long)blockIdx.x * kUnits;
   if (tid < 16) level[tid >> 3][tid & 7] = (tid >> 3 ? qv : qk).levels[tid & 7];
   __syncthreads();
@@ -276,54 +359,59 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant qk,
     const long long u = u0 + (tid & (kUnits - 1));
     int off = 0;
     long long at_block = -1;
-    if (u < units && (is_v ? v_out : k_out) != nullptr)
+    if (u < total && (is_v ? v_out : k_out) != nullptr)
       at_block = place(pool, at, (int)(u / pool.heads), (int)(u % pool.heads), 0x7fffffff, &off, err);
-    const Quant& q = is_v ? qv : qk;
-    float* row = rows + tid * kPitch;
+    float4* row = reinterpret_cast<float4*>(rows + tid * kPitch);
+    float f = 0.0f;
+    float y[64];
+#pragma unroll
+    for (int i = 0; i < 64; ++i) y[i] = 0.0f;
     if (at_block >= 0) {
       const uint8_t* block = pool.pages + at_block;
       const int slot = off & (kBlockTokens - 1);
       const uint4* codes = reinterpret_cast<const uint4*>(block + (is_v ? kVCodes : 0) + slot * 32);
       const uint4 w0 = codes[0], w1 = codes[1];
       const uint32_t word[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-      const float f = 0.125f * norm_value(reinterpret_cast<const uint16_t*>(block + (is_v ? kVNorms : kKNorms))[slot],
-                                          pool.norm_bf16);
-      const float* lv = level[is_v];
-      float y[64];
+      f = 0.125f * norm_value(reinterpret_cast<const uint16_t*>(block + (is_v ? kVNorms : kKNorms))[slot], pool.norm_bf16);
+      const uint8_t* lv = reinterpret_cast<const uint8_t*>(level[is_v]);
 #pragma unroll
       for (int i = 0; i < 64; ++i) {
         const uint32_t w = word[i >> 3];
-        const float c = lv[(w >> (4 * (i & 7))) & 7u];
-        y[i] = __uint_as_float(__float_as_uint(c) ^ ((w << (31 - sign_bit(i & 7))) & 0x80000000u));
+        constexpr int kByte = 2;  // log2 of a level's bytes
+        const int p = i & 7;
+        const uint32_t sel = (p ? w >> (4 * p - kByte) : w << kByte) & (7u << kByte);
+        const float x = *reinterpret_cast<const float*>(lv + sel);
+        y[i] = __uint_as_float(__float_as_uint(x) ^ ((w << (31 - sign_bit(p))) & 0x80000000u));
       }
       walsh(y);
-#pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        const float x = __fmul_rn(y[i], f);
-        row[q.perm[i]] = (q.signs[i >> 5] >> (i & 31)) & 1u ? -x : x;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 64; ++i) row[i] = 0.0f;
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) row[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+    scale[tid] = f;
   }
   __syncthreads();
+  const int c = tid & 3;
 #pragma unroll
-  for (int it = 0; it < 2 * kUnits * 4 / kThreads; ++it) {
-    const int task = it * kThreads + tid, r = task >> 2, c = task & 3;
-    const bool is_v = r >= kUnits;
-    const long long u = u0 + (r & (kUnits - 1));
+  for (int is_v = 0; is_v < 2; ++is_v) {
     T* out = is_v ? v_out : k_out;
-    if (u >= units || out == nullptr) continue;
-    const float* row = rows + r * kPitch;
-    float a[8], b[8];
+    if (out == nullptr) continue;
+    uint32_t from[16];
+    my_places(is_v ? qv : qk, c, from);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      a[j] = row[8 * c + j];
-      b[j] = row[32 + 8 * c + j];
+    for (int it = 0; it < kUnits * 4 / kThreads; ++it) {
+      const int r = it * (kThreads / 4) + (tid >> 2);
+      if (u0 + r >= total) continue;
+      const uint8_t* row = reinterpret_cast<const uint8_t*>(rows + (is_v * kUnits + r) * kPitch);
+      const float f = scale[is_v * kUnits + r];
+      float a[8], b[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        a[j] = flip(__fmul_rn(*reinterpret_cast<const float*>(row + (from[j] & 0xffu)), f), from[j]);
+        b[j] = flip(__fmul_rn(*reinterpret_cast<const float*>(row + (from[8 + j] & 0xffu)), f), from[8 + j]);
+      }
+      store8(out + (u0 + r) * 64 + 8 * c, a);
+      store8(out + (u0 + r) * 64 + 32 + 8 * c, b);
     }
-    store8(out + u * 64 + 8 * c, a);
-    store8(out + u * 64 + 32 + 8 * c, b);
   }
 }
 
@@ -373,18 +461,21 @@ int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int6
   int grid = 0, *err = nullptr;
   CC2_TRY(grid_of(T, pool.heads, &grid));
   CC2_TRY(error_word(&err));
-  const Quant qk = make_quant(cache->key), qv = make_quant(cache->value);
+  Quant qk, qv;
+  CC2_TRY(make_quant(cache->key, "kv4_append", qk));
+  CC2_TRY(make_quant(cache->value, "kv4_append", qv));
   const Places at{seq, pos, table, table_ld, num_seqs};
   const float2* rope = (const float2*)cache->rope_cs;
+#define CC2_APPEND(TT, ROPE)                                                                                        \
+  CC2_CUDA(launch_k(append_kernel<TT, ROPE>, grid, kThreads, 0, st, pool, qk, qv, (const TT*)k, (long long)k_ld,    \
+                    (long long)k_hs, (const TT*)v, (long long)v_ld, (long long)v_hs, T, at, mask, rope,             \
+                    cache->rope_len, err))
   if (dtype == CC2_BF16) {
-    CC2_CUDA(launch_k(append_kernel<__nv_bfloat16>, grid, kThreads, 0, st, pool, qk, qv, (const __nv_bfloat16*)k,
-                      (long long)k_ld, (long long)k_hs, (const __nv_bfloat16*)v, (long long)v_ld, (long long)v_hs, T, at,
-                      mask, rope, cache->rope_len, err));
+    if (rope != nullptr) CC2_APPEND(__nv_bfloat16, true); else CC2_APPEND(__nv_bfloat16, false);
   } else {
-    CC2_CUDA(launch_k(append_kernel<float>, grid, kThreads, 0, st, pool, qk, qv, (const float*)k, (long long)k_ld,
-                      (long long)k_hs, (const float*)v, (long long)v_ld, (long long)v_hs, T, at, mask, rope,
-                      cache->rope_len, err));
+    if (rope != nullptr) CC2_APPEND(float, true); else CC2_APPEND(float, false);
   }
+#undef CC2_APPEND
   CC2_CHECK_LAUNCH();
   return CC2_OK;
 }
@@ -401,7 +492,9 @@ int launch_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_
   int grid = 0, *err = nullptr;
   CC2_TRY(grid_of(T, pool.heads, &grid));
   CC2_TRY(error_word(&err));
-  const Quant qk = make_quant(cache->key), qv = make_quant(cache->value);
+  Quant qk, qv;
+  CC2_TRY(make_quant(cache->key, "kv4_read", qk));
+  CC2_TRY(make_quant(cache->value, "kv4_read", qv));
   const Places at{seq, pos, table, table_ld, num_seqs};
   if (dtype == CC2_BF16) {
     CC2_CUDA(launch_k(read_kernel<__nv_bfloat16>, grid, kThreads, 0, st, pool, qk, qv, (__nv_bfloat16*)k_out,

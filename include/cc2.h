@@ -432,7 +432,7 @@ CC2_API int cc2_model_set_kv_quant(cc2_model* m, int layer, const cc2_kvq* key, 
  * reads back as NaN). */
 typedef struct {
   float levels[8];     /* magnitudes, ascending; the negative half mirrors them */
-  float bounds[7];     /* between them, ascending */
+  float bounds[7];     /* between them, ascending from above 0, more than 1/60 apart */
   uint64_t signs;      /* bit i: signs_i = -1 */
   uint8_t perm[64];
 } cc2_kv4_quant;
