@@ -55,7 +55,6 @@ using namespace tcx;
 constexpr int kWarps = 4;
 constexpr int kStageKeys = 64;
 constexpr int kStageBytes = kStageKeys / kBlockTokens * kBlockBytes;  // 4352
-constexpr int kStages = 3;
 constexpr int kTcMoreThan = 32;  // bf16 rows of a sequence and head from which the tcgen05 kernel takes over
 constexpr int kQPitch = 72;  // halves
 constexpr int kOPitch = 66;  // floats
@@ -86,30 +85,31 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
-__device__ __forceinline__ uint16_t lds16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
-}
-
 template <int NB, bool F32>
 struct Shared {
   static constexpr int kRows = 8 * NB;
+  static constexpr int kStages = 2;  // keeps some 170 KB in flight an SM
   alignas(128) uint8_t ring[kWarps][kStages][kStageBytes];
   alignas(16) __half q[F32 ? 2 : 1][kRows][kQPitch];
   float rs[kRows];
   float m[kWarps][kRows], l[kWarps][kRows];
   uint64_t full[kWarps][kStages];
+  Turns turns;
   int abort_flag;
   static_assert(kWarps * kRows * kOPitch * 4 <= kWarps * kStages * kStageBytes, "the joined sums reuse the ring");
 };
 
-template <int NB, bool F32>
-__global__ void __launch_bounds__(kWarps * 32)
+template <bool kBf16> __device__ __forceinline__ float norm_of(uint32_t bits) { return norm_value((uint16_t)bits, kBf16); }
+
+// Blocks an SM the registers are held down to: as many as the rings leave room for.
+template <int NB, bool F32> constexpr int blocks_per_sm() { return NB == 1 ? (F32 ? 4 : 5) : NB == 2 ? (F32 ? 2 : 3) : 2; }
+
+template <int NB, bool F32, bool NormBf16>
+__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<NB, F32>())
 attend_kernel(const __grid_constant__ Args a) {
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
   using S = Shared<NB, F32>;
-  constexpr int kRows = S::kRows;
+  constexpr int kRows = S::kRows, kStages = S::kStages;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -120,6 +120,7 @@ attend_kernel(const __grid_constant__ Args a) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid == 0) sm.abort_flag = 0;
+  load_turns(sm.turns, a, tid);
   pdl_wait();
 
   unsigned idx = blockIdx.x;
@@ -166,27 +167,28 @@ attend_kernel(const __grid_constant__ Args a) {
   // the rows: rotated to their positions, then as the keys' codes are, scaled
   for (int r = warp; r < kRows; r += kWarps) {
     const int row = s.row0 + r;
-    float x0 = 0.0f, x1 = 0.0f;
-    if (row < s.rows) {
-      const int i = row / a.group;
-      const T* q = (const T*)a.q + (long long)(s.q_start + i) * a.q_ld +
-                   (long long)(head * a.group + row % a.group) * a.q_hs;
-      x0 = tof<T>(q[lane]);
-      x1 = tof<T>(q[lane + 32]);
-      const int pos = s.len - s.n + i;
-      if (a.rotate && pos >= 0) {
-        if (pos >= a.rope_len) {
-          if (lane == 0) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
-        } else {
-          const float2 cs = a.rope[(long long)pos * 32 + lane];
-          const float u = x0;
-          x0 = u * cs.x - x1 * cs.y;
-          x1 = x1 * cs.x + u * cs.y;
-        }
+    if (row >= s.rows) {  // a column of zeros
+#pragma unroll
+      for (int p = 0; p < (F32 ? 2 : 1); ++p) sm.q[p][r][lane] = sm.q[p][r][lane + 32] = __float2half_rn(0.0f);
+      if (lane == 0) sm.rs[r] = 1.0f;
+      continue;
+    }
+    const int i = row / a.group;
+    const T* q = (const T*)a.q + (long long)(s.q_start + i) * a.q_ld + (long long)(head * a.group + row % a.group) * a.q_hs;
+    float x0 = tof<T>(q[lane]), x1 = tof<T>(q[lane + 32]);
+    const int pos = s.len - s.n + i;
+    if (a.rotate && pos >= 0) {
+      if (pos >= a.rope_len) {
+        if (lane == 0) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+      } else {
+        const float2 cs = a.rope[(long long)pos * 32 + lane];
+        const float u = x0;
+        x0 = u * cs.x - x1 * cs.y;
+        x1 = x1 * cs.x + u * cs.y;
       }
     }
-    float y0 = flip(spread_get(x0, x1, a.rk.perm[lane]), a.rk.signs, 0, lane);
-    float y1 = flip(spread_get(x0, x1, a.rk.perm[lane + 32]), a.rk.signs, 1, lane);
+    float y0 = flip(spread_get(x0, x1, sm.turns.k_perm[lane]), a.rk.signs, 0, lane);
+    float y1 = flip(spread_get(x0, x1, sm.turns.k_perm[lane + 32]), a.rk.signs, 1, lane);
     spread_walsh(y0, y1, lane);
     y0 *= 0.125f * a.qscale;
     y1 *= 0.125f * a.qscale;
@@ -195,12 +197,12 @@ attend_kernel(const __grid_constant__ Args a) {
     const float up = __int_as_float((261 - e) << 23);  // 2^(134 - e)
     y0 *= up;
     y1 *= up;
-    const __half h0 = __float2half_rn(y0), h1 = __float2half_rn(y1);
-    sm.q[0][r][lane] = h0;
-    sm.q[0][r][lane + 32] = h1;
+    const __half g0 = __float2half_rn(y0), g1 = __float2half_rn(y1);
+    sm.q[0][r][lane] = g0;
+    sm.q[0][r][lane + 32] = g1;
     if (F32) {
-      sm.q[F32 ? 1 : 0][r][lane] = __float2half_rn(y0 - __half2float(h0));
-      sm.q[F32 ? 1 : 0][r][lane + 32] = __float2half_rn(y1 - __half2float(h1));
+      sm.q[F32 ? 1 : 0][r][lane] = __float2half_rn(y0 - __half2float(g0));
+      sm.q[F32 ? 1 : 0][r][lane + 32] = __float2half_rn(y1 - __half2float(g1));
     }
     if (lane == 0) sm.rs[r] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64: undoes both scalings
   }
@@ -228,10 +230,11 @@ attend_kernel(const __grid_constant__ Args a) {
   // every row sees all keys below `clear`
   const int clear = a.causal ? s.len - s.n + s.row0 / a.group + 1 : s.len;
 
-  float m[NB][2], l[NB][2], acc[4][NB][4];
+  float m[NB][2], lift[NB][2], neg[NB][2], l[NB][2], acc[4][NB][4];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    m[b][0] = m[b][1] = -INFINITY;
+    m[b][0] = m[b][1] = lift[b][0] = lift[b][1] = -INFINITY;
+    neg[b][0] = neg[b][1] = 0.0f;
     l[b][0] = l[b][1] = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i][b][0] = acc[i][b][1] = acc[i][b][2] = acc[i][b][3] = 0.0f;
@@ -239,13 +242,9 @@ attend_kernel(const __grid_constant__ Args a) {
   int ve = 20;  // exponent of the largest V norm met
   const int krow = (g >> 1) + 4 * (g & 1);  // key of S^T rows g and (+ 8) g + 8 in a block of 16
 
-  for (int i = 0; i < mine; ++i) {
-    const int key0 = c0 + (warp + kWarps * i) * kStageKeys;
-    const uint32_t stage = smem_u32(sm.ring[warp][i % kStages]);
-    // the lanes leave together: one may see the block's abort flag where another saw its stage
-    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.full[warp][i % kStages]), (uint32_t)(i / kStages) & 1u,
-                                           &sm.abort_flag, a.wait_err)))
-      break;
+  // One stage of 64 keys.  kEdge: some key is past the end, masked, or not for every row.
+  auto attend_stage = [&](auto edge_, uint32_t stage, int key0, const uint32_t (&nb)[4][2]) {
+    constexpr bool kEdge = decltype(edge_)::value;
     float x[4][NB][4];
     float nv[4][2];
     uint32_t top = 0;
@@ -285,32 +284,32 @@ attend_kernel(const __grid_constant__ Args a) {
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const uint16_t kb = lds16(blk + kKNorms + (krow + 8 * c) * 2), vb = lds16(blk + kVNorms + (krow + 8 * c) * 2);
-        const bool seen = !(kb & 0x8000u) && key0 + 16 * j + krow + 8 * c < c1;
-        const float nk = norm_value(kb, a.pool.norm_bf16);
-        nv[j][c] = seen ? norm_value(vb, a.pool.norm_bf16) : 0.0f;
-        if (nv[j][c] <= 3.402823466e38f) top = max(top, __float_as_uint(nv[j][c]));
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          x[j][b][2 * c] = seen ? x[j][b][2 * c] * nk : -INFINITY;
-          x[j][b][2 * c + 1] = seen ? x[j][b][2 * c + 1] * nk : -INFINITY;
+        const float nk = norm_of<NormBf16>(nb[j][c]);
+        nv[j][c] = norm_of<NormBf16>(nb[j][c] >> 16);
+        bool seen = true;
+        if (kEdge) {
+          seen = !(nb[j][c] & 0x8000u) && key0 + 16 * j + krow + 8 * c < c1;
+          if (!seen) nv[j][c] = 0.0f;
+          // where not every row sees a V that is not finite, it must not set the scale for the others
+          if (nv[j][c] <= 3.402823466e38f) top = max(top, __float_as_uint(nv[j][c]));
+        } else {
+          top = max(top, __float_as_uint(nv[j][c]));
         }
-      }
-    }
-    const bool edge = key0 + kStageKeys > clear;
-    if (edge) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (key0 + 16 * j + krow + 8 * (c >> 1) >= limit[b][c & 1]) x[j][b][c] = -INFINITY;
+          for (int i = 0; i < 2; ++i) {
+            float& v = x[j][b][2 * c + i];
+            v *= nk;
+            if (kEdge && (!seen || key0 + 16 * j + krow + 8 * c >= limit[b][i])) v = -INFINITY;
+          }
+      }
     }
 
-    // running maximum and largest norm; sums so far follow when one moves
+    // The running maximum moves only when a score is more than 2^8 above it, the
+    // largest norm when a larger one comes; then the sums so far follow.
     const int ve_new = max(ve, (int)(__reduce_max_sync(0xffffffffu, top) >> 23));
-    float mn[NB][2];
+    float mx[NB][2];
     bool moved = ve_new != ve;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -319,10 +318,8 @@ attend_kernel(const __grid_constant__ Args a) {
         float v = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v = max3(v, x[j][b][c], x[j][b][c + 2]);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-        mn[b][c] = fmaxf(m[b][c], v);
-        moved = moved || mn[b][c] != m[b][c];
+        mx[b][c] = v;
+        moved = moved || v > lift[b][c];
       }
     if (__any_sync(0xffffffffu, moved)) {
       const float fv = __int_as_float((127 + max(ve - ve_new, -126)) << 23);
@@ -330,8 +327,14 @@ attend_kernel(const __grid_constant__ Args a) {
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float f = m[b][c] == -INFINITY ? 0.0f : ex2((m[b][c] - mn[b][c]) * rs[b][c]);
-          m[b][c] = mn[b][c];
+          float v = mx[b][c];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+          v = fmaxf(m[b][c], v);
+          const float f = m[b][c] == -INFINITY ? 0.0f : ex2((m[b][c] - v) * rs[b][c]);
+          m[b][c] = v;
+          neg[b][c] = v == -INFINITY ? 0.0f : -v * rs[b][c];
+          lift[b][c] = v + 8.0f / rs[b][c];  // -inf until a key is seen
           l[b][c] *= f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -341,31 +344,30 @@ attend_kernel(const __grid_constant__ Args a) {
         }
       ve = ve_new;
     }
-    const float vs = __int_as_float((267 - ve) << 23);  // 2^(140 - ve): norms below 2^14
-    float neg[NB][2];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) neg[b][c] = m[b][c] == -INFINITY ? 0.0f : -m[b][c] * rs[b][c];
+    const float vs = __int_as_float((259 - ve) << 23);  // 2^(132 - ve): norms below 2^6, P n_v below 2^14
 
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t blk = stage + j * kBlockBytes + kVCodes + g * 4;
       uint32_t pf[NB][F32 ? 4 : 2];
-      const float n0 = nv[j][0] * vs, n1 = nv[j][1] * vs;
+      const uint64_t n0 = f2_pack(nv[j][0] * vs, nv[j][0] * vs), n1 = f2_pack(nv[j][1] * vs, nv[j][1] * vs);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
+        const uint64_t r2 = f2_pack(rs[b][0], rs[b][1]), g2 = f2_pack(neg[b][0], neg[b][1]);
         float p[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          p[c] = ex2(fmaf(x[j][b][c], rs[b][c & 1], neg[b][c & 1]));
-          l[b][c & 1] += p[c];
+        for (int c = 0; c < 4; c += 2) {
+          f2_unpack(f2_fma(f2_pack(x[j][b][c], x[j][b][c + 1]), r2, g2), p[c], p[c + 1]);
+          p[c] = ex2(p[c]);
+          p[c + 1] = ex2(p[c + 1]);
         }
+        f2_unpack(f2_add(f2_add(f2_pack(l[b][0], l[b][1]), f2_pack(p[0], p[1])), f2_pack(p[2], p[3])), l[b][0], l[b][1]);
+        if (kEdge) {  // a key that a row does not see adds nothing, whatever its norm
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float n = c < 2 ? n0 : n1;
-          // a key that a row does not see adds nothing, whatever its norm
-          p[c] = edge && x[j][b][c] == -INFINITY ? 0.0f : p[c] * n;
+          for (int c = 0; c < 4; ++c) p[c] = x[j][b][c] == -INFINITY ? 0.0f : p[c] * (c < 2 ? nv[j][0] : nv[j][1]) * vs;
+        } else {
+          f2_unpack(f2_mul(f2_pack(p[0], p[1]), n0), p[0], p[1]);
+          f2_unpack(f2_mul(f2_pack(p[2], p[3]), n1), p[2], p[3]);
         }
         const uint32_t h0 = pack_half(p[0], p[1]), h1 = pack_half(p[2], p[3]);
         pf[b][0] = transpose8(h0);
@@ -401,6 +403,28 @@ attend_kernel(const __grid_constant__ Args a) {
         }
       }
     }
+  };
+
+  for (int i = 0; i < mine; ++i) {
+    const int key0 = c0 + (warp + kWarps * i) * kStageKeys;
+    const uint32_t stage = smem_u32(sm.ring[warp][i % kStages]);
+    // the lanes leave together: one may see the block's abort flag where another saw its stage
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.full[warp][i % kStages]), (uint32_t)(i / kStages) & 1u,
+                                           &sm.abort_flag, a.wait_err)))
+      break;
+    uint32_t nb[4][2], any = 0;  // norms of this lane's keys: K low, V high
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        nb[j][c] = lds32(stage + j * kBlockBytes + kNorms + (krow + 8 * c) * 4);
+        any |= nb[j][c];
+      }
+    // (past the end the norms may be anything)
+    if (key0 + kStageKeys > min(clear, c1) || __any_sync(0xffffffffu, any & 0x8000u))
+      attend_stage(std::true_type{}, stage, key0, nb);
+    else
+      attend_stage(std::false_type{}, stage, key0, nb);
     __syncwarp();  // the stage is in registers
     if (i + kStages < mine) issue(i + kStages);
   }
@@ -414,7 +438,7 @@ attend_kernel(const __grid_constant__ Args a) {
   __syncthreads();  // all warps are done with the ring
 
   float(*osum)[kRows][kOPitch] = reinterpret_cast<float(*)[kRows][kOPitch]>(&sm.ring[0][0][0]);
-  const float down = __int_as_float((ve - 19) << 23);  // 2^(ve - 140) / 64
+  const float down = __int_as_float((ve - 11) << 23);  // 2^(ve - 132) / 64
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -447,7 +471,7 @@ attend_kernel(const __grid_constant__ Args a) {
       o1 += osum[w][r][lane + 32] * f;
     }
     if (chunks <= 1) {
-      finish_row<T>(a, s, head, s.row0 + r, o0, o1, top, sum, lane);
+      finish_row<T>(a, sm.turns, s, head, s.row0 + r, o0, o1, top, sum, lane);
     } else {
       const long long at = part_at(a, s, head, split, s.row0 + r);
       a.part[at * 64 + lane] = o0;
@@ -457,14 +481,19 @@ attend_kernel(const __grid_constant__ Args a) {
   }
 }
 
-// Joins the chunks of the rows that have more than one: a warp a row.
-template <typename T>
+// Joins the chunks of the rows that have more than one: kRowWarps warps a row,
+// each a share of the chunks.
+template <typename T, int kRowWarps>
 __global__ void __launch_bounds__(128)
 join_kernel(const __grid_constant__ Args a) {
+  __shared__ Turns turns;
+  __shared__ float share[4][66];
   pdl_launch_dependents();
+  load_turns(turns, a, threadIdx.x);
+  __syncthreads();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kRowWarps;
+  const long long w = (long long)blockIdx.x * (4 / kRowWarps) + warp / kRowWarps;
   const int rows = a.total_q * a.group;
   const int head = (int)(w / rows), call_row = (int)(w % rows), tok = call_row / a.group;
   if (head >= a.pool.heads) return;
@@ -490,16 +519,30 @@ join_kernel(const __grid_constant__ Args a) {
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float base = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-#pragma unroll 4
-  for (int c = 0; c < chunks; ++c) {
+#pragma unroll 8
+  for (int c = part; c < chunks; c += kRowWarps) {
     const float2 ml = a.part_ml[first + c * step];
-    const float* o = a.part + (first + c * step) * 64;
+    const float2 o = *reinterpret_cast<const float2*>(a.part + (first + c * step) * 64 + 2 * lane);
     const float f = ex2(ml.x - base);
     sum += ml.y * f;
-    o0 += o[lane] * f;
-    o1 += o[lane + 32] * f;
+    o0 += o.x * f;
+    o1 += o.y * f;
   }
-  finish_row<T>(a, s, head, row, o0, o1, top, sum, lane);
+  // through shared memory: coordinates 2 lane, 2 lane + 1 to lane, lane + 32
+  share[warp][2 * lane] = o0;
+  share[warp][2 * lane + 1] = o1;
+  if (lane == 0) share[warp][64] = sum;
+  if (kRowWarps > 1) __syncthreads();  // a block has one row then
+  else __syncwarp();
+  if (part != 0) return;
+  o0 = o1 = sum = 0.0f;
+#pragma unroll
+  for (int p = 0; p < kRowWarps; ++p) {
+    o0 += share[warp + p][lane];
+    o1 += share[warp + p][lane + 32];
+    sum += share[warp + p][64];
+  }
+  finish_row<T>(a, turns, s, head, row, o0, o1, top, sum, lane);
 }
 
 struct Plan {
@@ -525,11 +568,25 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
   p.tile_rows = p.tc ? kTcRows : 8 * p.nb;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const long long tiles = (long long)num_seqs * pool.heads * p.row_tiles;
-  const int least = p.tc ? 1024 : 512;  // keys below which a chunk's own cost shows
-  const int most = std::max(1, (max_len + least - 1) / least);
-  const long long want = ((p.tc ? 4LL : 8LL) * num_sms() + tiles - 1) / tiles;
-  const int splits = (int)std::min<long long>(most, std::max<long long>(1, want));
-  p.chunk = ((std::max(1, max_len) + splits - 1) / splits + 255) / 256 * 256;
+  if (p.tc) {
+    // blocks take items as they get to them: about four an SM even them out; a chunk's own cost is some 1000 keys
+    const long long want = (4LL * num_sms() + tiles - 1) / tiles;
+    const int splits = (int)std::min<long long>(std::max(1, (max_len + 1023) / 1024), std::max<long long>(1, want));
+    p.chunk = ((std::max(1, max_len) + splits - 1) / splits + 255) / 256 * 256;
+  } else {
+    // the chunk for which the waves of blocks, each of the chunk's keys and of 512 more for its start and its
+    // join, take the least; it is worth looking where the blocks just fill one to eight waves
+    const long long slots = (long long)num_sms() * (p.nb == 1 ? 5 : p.nb == 2 ? 3 : 2);
+    const int len = std::max(1, max_len);
+    long long best = -1;
+    for (int w = 0; w <= 8; ++w) {
+      const long long splits = std::min<long long>(std::max(1LL, w * slots / tiles), (len + 511) / 512);
+      const int chunk = (int)(((len + splits - 1) / splits + 255) / 256 * 256);
+      const long long waves = (tiles * ((len + chunk - 1) / chunk) + slots - 1) / slots;
+      const long long cost = waves * (chunk + 512);
+      if (best < 0 || cost < best) best = cost, p.chunk = chunk;
+    }
+  }
   p.splits = std::max(1, (max_len + p.chunk - 1) / p.chunk);
   p.units = tiles * p.splits;
   CC2_REQUIRE(p.units <= 0x7fffffffLL, "kv4_attention: too many rows and keys for one call");
@@ -546,26 +603,38 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
   return CC2_OK;
 }
 
-template <int NB, bool F32>
+template <int NB, bool F32, bool NormBf16>
 int launch(const Args& a, const Plan& p, cudaStream_t st) {
   const size_t smem = sizeof(Shared<NB, F32>);
   static unsigned long long attr_done = 0;  // one bit per device
   int dev = 0;
   CC2_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !((attr_done >> dev) & 1ull)) {
-    CC2_CUDA(cudaFuncSetAttribute(attend_kernel<NB, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CC2_CUDA(cudaFuncSetAttribute(attend_kernel<NB, F32, NormBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (dev < 64) attr_done |= 1ull << dev;
   }
-  CC2_CUDA(launch_k(attend_kernel<NB, F32>, (unsigned)p.units, kWarps * 32, smem, st, a));
+  CC2_CUDA(launch_k(attend_kernel<NB, F32, NormBf16>, (unsigned)p.units, kWarps * 32, smem, st, a));
   CC2_CHECK_LAUNCH();
   return CC2_OK;
+}
+template <int NB, bool F32>
+int launch(const Args& a, const Plan& p, cudaStream_t st) {
+  return a.pool.norm_bf16 ? launch<NB, F32, true>(a, p, st) : launch<NB, F32, false>(a, p, st);
 }
 
 int join(const Args& a, int dtype, cudaStream_t st) {
   if (a.splits <= 1) return CC2_OK;
-  const unsigned grid = (unsigned)(((long long)a.total_q * a.group * a.pool.heads + 3) / 4);
-  if (dtype == CC2_F32) CC2_CUDA(launch_k(join_kernel<float>, grid, 128, 0, st, a));
-  else CC2_CUDA(launch_k(join_kernel<__nv_bfloat16>, grid, 128, 0, st, a));
+  const long long rows = (long long)a.total_q * a.group * a.pool.heads;
+  // many chunks mean few rows: four warps then share a row's
+  const bool four = a.splits > 8;
+  const unsigned grid = (unsigned)(four ? rows : (rows + 3) / 4);
+  if (dtype == CC2_F32) {
+    if (four) CC2_CUDA(launch_k(join_kernel<float, 4>, grid, 128, 0, st, a));
+    else CC2_CUDA(launch_k(join_kernel<float, 1>, grid, 128, 0, st, a));
+  } else {
+    if (four) CC2_CUDA(launch_k(join_kernel<__nv_bfloat16, 4>, grid, 128, 0, st, a));
+    else CC2_CUDA(launch_k(join_kernel<__nv_bfloat16, 1>, grid, 128, 0, st, a));
+  }
   CC2_CHECK_LAUNCH();
   return CC2_OK;
 }

@@ -604,10 +604,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         const uint32_t src = smem + kRawAt + raw.i * kRawBytes + (k >> 4) * kBlockBytes;
         uint32_t nbits = 0;
         if (ok) {
-          uint16_t kb, vb;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(kb) : "r"(src + kKNorms + (k & 15) * 2));
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(vb) : "r"(src + kVNorms + (k & 15) * 2));
-          nbits = kb | (uint32_t)vb << 16;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(nbits) : "r"(src + kNorms + (k & 15) * 4));
         }
         const bool seen = !(nbits & 0x8000u) && c0 + j * kTile + k < c1;
         float nk = seen ? norm_value((uint16_t)nbits, a.pool.norm_bf16) : 0.0f;

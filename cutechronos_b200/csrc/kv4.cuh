@@ -3,7 +3,7 @@
 //
 // Pool: page-major.  A page holds, for each head, page_size / 16 blocks of 16
 // tokens, and a block is 1088 consecutive bytes
-//     [16 x 32 bytes K codes | 16 x 32 bytes V codes | 16 K norms | 16 V norms]
+//     [16 x 32 bytes K codes | 16 x 32 bytes V codes | 16 x (K norm, V norm)]
 // so that everything attention needs of 16 tokens of a head is one aligned
 // run of memory, and of a page one longer run: one bulk copy brings it.
 //
@@ -26,7 +26,7 @@ namespace kv4 {
 
 constexpr int kBlockTokens = 16;
 constexpr int kBlockBytes = 1088;
-constexpr int kVCodes = 512, kKNorms = 1024, kVNorms = 1056;  // offsets in a block
+constexpr int kVCodes = 512, kNorms = 1024;  // offsets in a block
 
 // Where a page and a head's blocks of it start.
 struct Pool {

@@ -15,9 +15,21 @@ using tcx::ex2;
 
 struct Rotation {
   uint32_t signs[2];
-  uint8_t perm[64];  // coordinate perm[i] of a vector is i of the rotated one
-  uint8_t inv[64];
+  alignas(4) uint8_t perm[64];  // coordinate perm[i] of a vector is i of the rotated one
+  alignas(4) uint8_t inv[64];
 };
+
+// Keys' permutation going in and values' coming out, in shared memory: lanes
+// that index the kernel's arguments apart are served one by one.
+struct Turns {
+  alignas(4) uint8_t k_perm[64];
+  alignas(4) uint8_t v_inv[64];
+};
+template <typename A>
+__device__ __forceinline__ void load_turns(Turns& t, const A& a, int tid) {
+  if (tid < 16) reinterpret_cast<uint32_t*>(t.k_perm)[tid] = reinterpret_cast<const uint32_t*>(a.rk.perm)[tid];
+  else if (tid < 32) reinterpret_cast<uint32_t*>(t.v_inv)[tid - 16] = reinterpret_cast<const uint32_t*>(a.rv.inv)[tid - 16];
+}
 
 struct Args {
   Pool pool;
@@ -49,6 +61,11 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"((uint64_t)__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
                : "memory");
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 // A vector spread over a warp, coordinates lane and lane + 32.
 __device__ __forceinline__ float spread_get(float lo, float hi, int i) {
@@ -111,14 +128,14 @@ __device__ __forceinline__ int chunks_of(const Args& a, const Span& s) { return 
 
 // One row's sums -> output and log-sum-exp: lane holds coordinates lane and lane + 32 of the rotated sum.
 template <typename T>
-__device__ __forceinline__ void finish_row(const Args& a, const Span& s, int head, int row, float o0, float o1, float m,
+__device__ __forceinline__ void finish_row(const Args& a, const Turns& turns, const Span& s, int head, int row, float o0, float o1, float m,
                                            float l, int lane) {
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   spread_walsh(o0, o1, lane);
   o0 = flip(o0 * (0.125f * inv), a.rv.signs, 0, lane);
   o1 = flip(o1 * (0.125f * inv), a.rv.signs, 1, lane);
-  const float x0 = spread_get(o0, o1, a.rv.inv[lane]);
-  const float x1 = spread_get(o0, o1, a.rv.inv[lane + 32]);
+  const float x0 = spread_get(o0, o1, turns.v_inv[lane]);
+  const float x1 = spread_get(o0, o1, turns.v_inv[lane + 32]);
   const int tok = s.q_start + row / a.group, qh = head * a.group + row % a.group;
   T* out = (T*)a.out + (long long)tok * a.o_ld + (long long)qh * a.o_hs;
   out[lane] = fromf<T>(x0);

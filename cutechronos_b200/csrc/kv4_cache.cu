@@ -337,7 +337,7 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant q
   codes[1] = make_uint4(word[4], word[5], word[6], word[7]);
   uint16_t nb = norm_bits(n, pool.norm_bf16);
   if (!is_v && (u.slot & 256)) nb |= 0x8000u;
-  reinterpret_cast<uint16_t*>(block + (is_v ? kVNorms : kKNorms))[slot] = nb;
+  reinterpret_cast<uint16_t*>(block + kNorms)[2 * slot + is_v] = nb;
 }
 
 template <typename T>
@@ -372,7 +372,7 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant qk,
       const uint4* codes = reinterpret_cast<const uint4*>(block + (is_v ? kVCodes : 0) + slot * 32);
       const uint4 w0 = codes[0], w1 = codes[1];
       const uint32_t word[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-      f = 0.125f * norm_value(reinterpret_cast<const uint16_t*>(block + (is_v ? kVNorms : kKNorms))[slot], pool.norm_bf16);
+      f = 0.125f * norm_value(reinterpret_cast<const uint16_t*>(block + kNorms)[2 * slot + is_v], pool.norm_bf16);
       const uint8_t* lv = reinterpret_cast<const uint8_t*>(level[is_v]);
 #pragma unroll
       for (int i = 0; i < 64; ++i) {

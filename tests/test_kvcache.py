@@ -42,8 +42,7 @@ def unpack(cache, which: int):
     bit = torch.where(at < 4, 8 * at + 7, 8 * (at - 4) + 3)
     mag = (word[..., None] >> (4 * at)) & 7
     sign = 1 - 2 * ((word[..., None] >> bit) & 1)
-    raw = b[..., 1024 + 32 * which:1056 + 32 * which].reshape(cache.num_pages, h, ps, 2).contiguous()
-    raw = raw.view(torch.int16).squeeze(-1)
+    raw = b[..., 1024:].reshape(cache.num_pages, h, ps, 2, 2)[..., which, :].contiguous().view(torch.int16).squeeze(-1)
     kind = torch.bfloat16 if cache._c.norm_dtype else torch.float16
     norm = (raw & 0x7FFF).view(kind).double()
     flat = lambda t: t.reshape(cache.num_pages, h, ps, D).transpose(1, 2)  # noqa: E731
