@@ -72,15 +72,15 @@ class Epilogue(C.Structure):
 class KV4Quant(C.Structure):
     """Mirror of ``cc2_kv4_quant``."""
 
-    _fields_ = [("levels", C.c_float * 8), ("bounds", C.c_float * 7), ("signs", C.c_uint64), ("perm", C.c_uint8 * 64)]
+    _fields_ = [("signs", C.c_uint64), ("perm", C.c_uint8 * 64)]
 
 
 class KV4Cache(C.Structure):
     """Mirror of ``cc2_kv4_cache``."""
 
     _fields_ = [("pages", _VP), ("num_pages", C.c_int), ("page_size", C.c_int), ("heads", C.c_int),
-                ("norm_dtype", C.c_int), ("rope_cs", _VP), ("rope_len", C.c_int), ("key", KV4Quant),
-                ("value", KV4Quant)]
+                ("norm_dtype", C.c_int), ("rope_cs", _VP), ("rope_len", C.c_int),
+                ("levels", C.c_float * 8), ("bounds", C.c_float * 7), ("key", KV4Quant), ("value", KV4Quant)]
 
 
 class NativeError(RuntimeError):

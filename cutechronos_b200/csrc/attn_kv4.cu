@@ -7,17 +7,28 @@
 // on the levels themselves, as fp16 on the tensor cores with fp32 sums.
 //
 // Rows are the queries of one sequence that share a head of keys: row r is
-// query token r / group, head r % group.  A block takes one head of keys of one
-// sequence, up to 8 NB rows and a chunk of the keys; its four warps take
-// 64-key stages in turn, each with a ring of its own that bulk copies fill, and
-// an online softmax of its own, joined at the end.
-//   S^T (16 keys x 8 rows) = K (decoded in registers, the A operand) . Q^T
+// query token r / group, head r % group.  A unit of work is one head of keys of
+// one sequence, up to 8 NB rows and a chunk of the keys; persistent blocks walk
+// the units, one for each of their teams of warps; a team's warps take 64-key
+// stages of its unit in turn, each with a ring of its own that bulk copies fill,
+// and an online softmax of its own, joined at the end of the unit while the next
+// one's first stage is on its way.
+//   S^T (16 keys x 8 rows) = K (the A operand, decoded in registers) . Q^T
 //   O^T (16 coordinates x 8 rows) += V^T (A, decoded) . P^T
 // Keys and coordinates as the long axis of the product: one token's query
 // fills 1 of 8 columns and not 1 of 16 rows.  P^T comes from S^T by one matrix
-// move a register pair.  What must not leave the type's range is scaled by
-// powers of two, which are exact: a row of Q to below 2^8, P n_v to below 2^14
-// against the largest norm met so far.
+// move a register pair.
+// Decoding: a byte of codes is an fp16 pair (K: neighbouring coordinates; V: one
+// coordinate of two tokens, their words zipped first), looked up in a table of
+// 256 pairs in shared memory that every lane has its own bank's copy of, so no
+// lookup waits for another: one byte permute makes the address of two values
+// (the code byte above the lane's place, hence 256 bytes an entry) and one load
+// brings them.  One block an SM, for one table.  Byte permutes of the levels' bytes took 1.6 (K) and 2.1 (V)
+// operations a value on the half-rate integer pipe and were what bound the kernel
+// (208 us instead of see below for the 484 MB of 64 sequences of up to 16384 tokens).
+// What must not leave the type's range is scaled by powers of two, which are
+// exact: a row of Q to below 2^8, P n_v to below 2^14 against the largest norm
+// met so far.
 // Rounding: Q and P n_v to fp16 (2^-12 of each, next to the output's bf16 with
 // 2^-9), levels to fp16.  fp32 calls split all three into two fp16 parts and
 // sum three products, which leaves about 2^-22.
@@ -32,18 +43,15 @@ int attention_error_word(int** p);
 
 namespace kv4 {
 
-Levels make_levels(const cc2_kv4_quant& q) {
+Levels make_levels(const cc2_kv4_cache& cache) {
   Levels r{};
   for (int i = 0; i < 8; ++i) {
-    const float c = 64.0f * q.levels[i];
+    const float c = 64.0f * cache.levels[i];
     const __half h = __float2half_rn(c);
-    const __half l = __float2half_rn(c - __half2float(h));
-    const uint16_t hb = __half_as_ushort(h), lb = __half_as_ushort(l);
-    const int w = i >> 2, s = 8 * (i & 3);
-    r.lo[w] |= (uint32_t)(hb & 255) << s;
-    r.hi[w] |= (uint32_t)(hb >> 8) << s;
-    r.rlo[w] |= (uint32_t)(lb & 255) << s;
-    r.rhi[w] |= (uint32_t)(lb >> 8) << s;
+    r.value[i] = __half_as_ushort(h);
+    r.rest[i] = __half_as_ushort(__float2half_rn(c - __half2float(h)));
+    r.lo[i >> 2] |= (uint32_t)(r.value[i] & 255) << 8 * (i & 3);
+    r.hi[i >> 2] |= (uint32_t)(r.value[i] >> 8) << 8 * (i & 3);
   }
   return r;
 }
@@ -52,7 +60,6 @@ namespace {
 
 using namespace tcx;
 
-constexpr int kWarps = 4;
 constexpr int kStageKeys = 64;
 constexpr int kStageBytes = kStageKeys / kBlockTokens * kBlockBytes;  // 4352
 constexpr int kTcMoreThan = 32;  // bf16 rows of a sequence and head from which the tcgen05 kernel takes over
@@ -85,405 +92,510 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
+// Teams of a block and their warps: what registers and shared memory leave room for.
+template <int NB, bool F32> constexpr int teams_of() { return NB == 2 && !F32 ? 3 : 2; }
+template <int NB, bool F32> constexpr int warps_of() { return NB == 1 && !F32 ? 8 : 4; }
+
 template <int NB, bool F32>
 struct Shared {
-  static constexpr int kRows = 8 * NB;
-  static constexpr int kStages = 2;  // keeps some 170 KB in flight an SM
-  alignas(128) uint8_t ring[kWarps][kStages][kStageBytes];
-  alignas(16) __half q[F32 ? 2 : 1][kRows][kQPitch];
-  float rs[kRows];
-  float m[kWarps][kRows], l[kWarps][kRows];
-  uint64_t full[kWarps][kStages];
+  static constexpr int kTeams = teams_of<NB, F32>(), kWarps = warps_of<NB, F32>(), kRows = 8 * NB;
+  struct Team {
+    alignas(128) uint8_t ring[kWarps][2][kStageBytes];
+    alignas(16) __half q[F32 ? 2 : 1][kRows][kQPitch];
+    float rs[kRows];
+    float m[kWarps][kRows], l[kWarps][kRows];
+    uint64_t full[kWarps][2];
+    const float* sums[kWarps];  // a warp's joined sums: in its ring, beside the slot that the next unit's first stage takes
+  };
+  alignas(256) uint8_t pairs[256][256];  // every lane's copy of the pair of codes (low nibble, high nibble); fp32: and its rest
+  Team team[kTeams];
   Turns turns;
   int abort_flag;
-  static_assert(kWarps * kRows * kOPitch * 4 <= kWarps * kStages * kStageBytes, "the joined sums reuse the ring");
+  static_assert(kRows * kOPitch * 4 <= 2 * kStageBytes, "a warp's sums fit its ring");
 };
+// Whether a warp's sums leave one slot of its ring free.
+template <int NB> constexpr bool sums_in_a_slot() { return 8 * NB * kOPitch * 4 <= kStageBytes; }
 
 template <bool kBf16> __device__ __forceinline__ float norm_of(uint32_t bits) { return norm_value((uint16_t)bits, kBf16); }
 
-// Blocks an SM the registers are held down to: as many as the rings leave room for.
-template <int NB, bool F32> constexpr int blocks_per_sm() { return NB == 1 ? (F32 ? 4 : 5) : NB == 2 ? (F32 ? 2 : 3) : 2; }
+// Walks a team's rounds unit by unit; every warp of the team does so for itself,
+// its lanes holding 32 sequences' places on the line.
+struct Walk {
+  long long at, end;         // the team's rounds
+  int window;                // first of the 32 sequences
+  SeqCost mine;              // of sequence window + lane
+  long long cost_at, unit_at;  // where that sequence starts
+  long long window_end, window_units;
+  // what next() found
+  int seq, head, tile, r0, r1;
+  long long unit;
+  bool whole;
+
+  __device__ __forceinline__ void load(const Args& a, int lane, long long cost0, long long units0) {
+    mine = SeqCost{0, 0, 0, 0};
+    if (window + lane < a.num_seqs) mine = cost_of(a, window + lane);
+    long long c = mine.cost, u = mine.units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long pc = __shfl_up_sync(0xffffffffu, c, o), pu = __shfl_up_sync(0xffffffffu, u, o);
+      if (lane >= o) c += pc, u += pu;
+    }
+    window_end = cost0 + __shfl_sync(0xffffffffu, c, 31);
+    window_units = units0 + __shfl_sync(0xffffffffu, u, 31);
+    cost_at = cost0 + c - mine.cost;
+    unit_at = units0 + u - mine.units;
+  }
+  __device__ __forceinline__ void start(const Args& a, int team, int lane) {
+    long long total = 0;
+    if (a.num_seqs <= 32) {
+      window = 0;
+      load(a, lane, 0, 0);
+      total = window_end;
+    } else {
+      for (int i = lane; i < a.num_seqs; i += 32) total += cost_of(a, i).cost;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      window = 0;
+      load(a, lane, 0, 0);
+    }
+    at = team_start(total, team, a.teams);
+    end = team_start(total, team + 1, a.teams);
+  }
+  __device__ __forceinline__ bool next(const Args& a, int lane) {
+    while (at < end) {
+      while (at >= window_end) {
+        window += 32;
+        load(a, lane, window_end, window_units);
+      }
+      const unsigned before = __ballot_sync(0xffffffffu, mine.cost > 0 && cost_at <= at);
+      const int src = 31 - __clz(before);
+      seq = window + src;
+      const int tiles = __shfl_sync(0xffffffffu, mine.tiles, src), rounds = __shfl_sync(0xffffffffu, mine.rounds, src);
+      const long long rest = at - __shfl_sync(0xffffffffu, cost_at, src);
+      const long long k = rest / (rounds + 1);
+      r0 = (int)(rest - k * (rounds + 1));
+      unit = __shfl_sync(0xffffffffu, unit_at, src) + k;
+      head = (int)(k / tiles);
+      tile = (int)(k % tiles);
+      r1 = (int)min((long long)rounds, r0 + (end - at));
+      whole = r0 == 0 && r1 == rounds;
+      at += rounds + 1 - r0;
+      if (r0 < r1) return true;
+    }
+    return false;
+  }
+};
 
 template <int NB, bool F32, bool NormBf16>
-__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<NB, F32>())
+__global__ void __launch_bounds__(32 * warps_of<NB, F32>() * teams_of<NB, F32>(), 1)
 attend_kernel(const __grid_constant__ Args a) {
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
   using S = Shared<NB, F32>;
-  constexpr int kRows = S::kRows, kStages = S::kStages;
+  constexpr int kRows = S::kRows, kWarps = S::kWarps;
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  S& sm = *reinterpret_cast<S*>(smem_raw);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  S& all = *reinterpret_cast<S*>(smem_raw);
+  const int tid = threadIdx.x, lane = tid & 31, team = (tid >> 5) / kWarps, warp = (tid >> 5) % kWarps;
+  typename S::Team& sm = all.team[team];
   const int g = lane >> 2, t = lane & 3;
   pdl_launch_dependents();
   if (lane == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(&sm.full[warp][i]), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.full[warp][i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (tid == 0) sm.abort_flag = 0;
-  load_turns(sm.turns, a, tid);
+  if (tid == 0) all.abort_flag = 0;
+  load_turns(all.turns, a, tid);
+  for (int e = tid >> 5; e < 256; e += kWarps * S::kTeams) {  // the table; an entry's 32 copies by one store
+    const uint32_t i = e & 7, j = (e >> 4) & 7, sign = (uint32_t)(e & 8) << 12 | (uint32_t)(e & 128) << 24;
+    const uint32_t v = ((uint32_t)a.levels.value[i] | (uint32_t)a.levels.value[j] << 16) ^ sign;
+    if (F32) {
+      const uint32_t r = ((uint32_t)a.levels.rest[i] | (uint32_t)a.levels.rest[j] << 16) ^ sign;
+      reinterpret_cast<uint2*>(all.pairs[e])[lane] = make_uint2(v, r);
+    } else {
+      reinterpret_cast<uint32_t*>(all.pairs[e])[lane] = v;
+    }
+  }
   pdl_wait();
-
-  unsigned idx = blockIdx.x;
-  const int row_tile = (int)(idx % a.row_tiles);
-  idx /= a.row_tiles;
-  const int split = (int)(idx % a.splits);
-  idx /= a.splits;
-  const int head = (int)(idx % a.pool.heads), seq = (int)(idx / a.pool.heads);
-  const Span s = span_of(a, seq, row_tile, split == 0 && row_tile == 0 && head == 0 && tid == 0);
-  if (s.row0 >= s.rows) return;
-  const int chunks = chunks_of(a, s);
-  if (split >= max(chunks, 1)) return;
-  const int c0 = split * a.chunk, c1 = min(s.keys, c0 + a.chunk);
-  const int stages = c1 > c0 ? (c1 - c0 + kStageKeys - 1) / kStageKeys : 0;
-  const int mine = stages > warp ? (stages - 1 - warp) / kWarps + 1 : 0;
   __syncthreads();
+  // every lane of the team's warps, and whether all say yes
+  auto meet = [&](bool yes) { return barrier_and(1u + (uint32_t)team, 32u * kWarps, yes); };
+
+  // the pairs of a word's four bytes
+  const uint32_t mine_at = (uint32_t)lane * (F32 ? 8u : 4u);
+  auto look = [&](uint32_t w, uint32_t (&v)[4], uint32_t (&r)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = __byte_perm(w, mine_at, 0x6604 | i << 4);  // byte 0 the lane's place, byte 1 the codes
+      if (F32) {
+        const uint2 x = *reinterpret_cast<const uint2*>(smem_raw + at);
+        v[i] = x.x, r[i] = x.y;
+      } else {
+        v[i] = *reinterpret_cast<const uint32_t*>(smem_raw + at);
+      }
+    }
+  };
 
   // a stage's blocks of 16 keys, page by page (a page of 64 tokens or more holds
-  // a whole stage)
+  // a whole stage), into the slot of the warp's stage number n
   const int run = min((1 << a.pool.page_shift) / kBlockTokens, 4);  // blocks of a copy
-  const int* table = a.table + (long long)seq * a.table_ld;
-  auto issue = [&](int i) {
-    const int key0 = c0 + (warp + kWarps * i) * kStageKeys;
+  struct Unit {
+    Span s;
+    int seq, head, c0, c1, stages;  // its keys, this warp's stages of them
+    long long piece;
+    bool whole;
+  };
+  auto issue = [&](const Unit& u, int i, uint32_t n) {
+    const int c1 = u.c1, key0 = u.c0 + (warp + kWarps * i) * kStageKeys;
     const int blocks = min((c1 - key0 + kBlockTokens - 1) / kBlockTokens, 4);
-    const uint32_t bar = smem_u32(&sm.full[warp][i % kStages]);
+    const uint32_t bar = smem_u32(&sm.full[warp][n & 1u]);
     if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)blocks * kBlockBytes);
     __syncwarp();
     const int first = lane * run;
     if (first < blocks) {
       const int key = key0 + first * kBlockTokens;
-      int page = table[key >> a.pool.page_shift];
+      int page = a.table[(long long)u.seq * a.table_ld + (key >> a.pool.page_shift)];
       if ((unsigned)page >= (unsigned)a.pool.num_pages) {
         atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
         page = 0;  // in bounds; the rows are unspecified
       }
-      const uint8_t* src =
-          a.pool.pages + block_offset(a.pool, page, head, key & ((1 << a.pool.page_shift) - 1));
-      bulk_load(smem_u32(sm.ring[warp][i % kStages]) + (uint32_t)first * kBlockBytes, src,
+      const uint8_t* src = a.pool.pages + block_offset(a.pool, page, u.head, key & ((1 << a.pool.page_shift) - 1));
+      bulk_load(smem_u32(sm.ring[warp][n & 1u]) + (uint32_t)first * kBlockBytes, src,
                 (uint32_t)min(run, blocks - first) * kBlockBytes, bar);
     }
   };
-  for (int i = 0; i < min(mine, kStages); ++i) issue(i);
+  Walk walk;
+  const int team_at = (int)blockIdx.x * S::kTeams + team;
+  walk.start(a, team_at, lane);
+  auto next = [&](Unit& u) {
+    if (!walk.next(a, lane)) return false;
+    u.s = span_of(a, walk.seq, walk.tile, warp == 0 && walk.head == 0 && walk.tile == 0 && walk.r0 == 0);
+    u.seq = walk.seq;
+    u.head = walk.head;
+    u.c0 = walk.r0 * (kWarps * kStageKeys);
+    u.c1 = min(u.s.keys, walk.r1 * (kWarps * kStageKeys));
+    const int stages = u.c1 > u.c0 ? (u.c1 - u.c0 + kStageKeys - 1) / kStageKeys : 0;
+    u.stages = stages > warp ? (stages - 1 - warp) / kWarps + 1 : 0;
+    u.piece = walk.unit + team_at;
+    u.whole = walk.whole;
+    return true;
+  };
+  Unit coming;
+  bool more = next(coming);
+  uint32_t n = 0;      // stages that this warp has taken
+  int ahead = 0;       // of the unit's stages, those under way
+  bool broken = false;
+  while (more) {
+    const Unit u = coming;
+    const Span& s = u.s;
+    const int c0 = u.c0, c1 = u.c1, mine = u.stages;
+    for (; ahead < min(mine, 2); ++ahead) issue(u, ahead, n + (uint32_t)ahead);
 
-  // the rows: rotated to their positions, then as the keys' codes are, scaled
-  for (int r = warp; r < kRows; r += kWarps) {
-    const int row = s.row0 + r;
-    if (row >= s.rows) {  // a column of zeros
+    // the rows: rotated to their positions, then as the keys' codes are, scaled
+    for (int r = warp; r < kRows; r += kWarps) {
+      const int row = s.row0 + r;
+      if (row >= s.rows) {  // a column of zeros
 #pragma unroll
-      for (int p = 0; p < (F32 ? 2 : 1); ++p) sm.q[p][r][lane] = sm.q[p][r][lane + 32] = __float2half_rn(0.0f);
-      if (lane == 0) sm.rs[r] = 1.0f;
-      continue;
+        for (int p = 0; p < (F32 ? 2 : 1); ++p) sm.q[p][r][lane] = sm.q[p][r][lane + 32] = __float2half_rn(0.0f);
+        if (lane == 0) sm.rs[r] = 1.0f;
+        continue;
+      }
+      const int i = row / a.group;
+      const T* q = (const T*)a.q + (long long)(s.q_start + i) * a.q_ld +
+                   (long long)(u.head * a.group + row % a.group) * a.q_hs;
+      float x0 = tof<T>(q[lane]), x1 = tof<T>(q[lane + 32]);
+      const int pos = s.len - s.n + i;
+      if (a.rotate && pos >= 0) {
+        if (pos >= a.rope_len) {
+          if (lane == 0) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+        } else {
+          const float2 cs = a.rope[(long long)pos * 32 + lane];
+          const float x = x0;
+          x0 = x * cs.x - x1 * cs.y;
+          x1 = x1 * cs.x + x * cs.y;
+        }
+      }
+      float y0 = flip(spread_get(x0, x1, all.turns.k_perm[lane]), a.rk.signs, 0, lane);
+      float y1 = flip(spread_get(x0, x1, all.turns.k_perm[lane + 32]), a.rk.signs, 1, lane);
+      spread_walsh(y0, y1, lane);
+      y0 *= 0.125f * a.qscale;
+      y1 *= 0.125f * a.qscale;
+      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(y0), fabsf(y1))));
+      const int e = min(max((int)(top >> 23), 30), 254);
+      const float up = __int_as_float((261 - e) << 23);  // 2^(134 - e)
+      y0 *= up;
+      y1 *= up;
+      const __half g0 = __float2half_rn(y0), g1 = __float2half_rn(y1);
+      sm.q[0][r][lane] = g0;
+      sm.q[0][r][lane + 32] = g1;
+      if (F32) {
+        sm.q[F32 ? 1 : 0][r][lane] = __float2half_rn(y0 - __half2float(g0));
+        sm.q[F32 ? 1 : 0][r][lane + 32] = __float2half_rn(y1 - __half2float(g1));
+      }
+      if (lane == 0) sm.rs[r] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64: undoes both scalings
     }
-    const int i = row / a.group;
-    const T* q = (const T*)a.q + (long long)(s.q_start + i) * a.q_ld + (long long)(head * a.group + row % a.group) * a.q_hs;
-    float x0 = tof<T>(q[lane]), x1 = tof<T>(q[lane + 32]);
-    const int pos = s.len - s.n + i;
-    if (a.rotate && pos >= 0) {
-      if (pos >= a.rope_len) {
-        if (lane == 0) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
-      } else {
-        const float2 cs = a.rope[(long long)pos * 32 + lane];
-        const float u = x0;
-        x0 = u * cs.x - x1 * cs.y;
-        x1 = x1 * cs.x + u * cs.y;
+    meet(true);
+
+    uint32_t qf[NB][F32 ? 16 : 8];
+    float rs[NB][2];
+    int limit[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int p = 0; p < (F32 ? 2 : 1); ++p) {
+        const uint4* src = reinterpret_cast<const uint4*>(&sm.q[p][8 * b + g][16 * t]);
+        const uint4 x = src[0], y = src[1];
+        uint32_t* d = &qf[b][8 * p];
+        d[0] = x.x, d[1] = x.y, d[2] = x.z, d[3] = x.w, d[4] = y.x, d[5] = y.y, d[6] = y.z, d[7] = y.w;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = 8 * b + 2 * t + c;
+        rs[b][c] = sm.rs[r];
+        limit[b][c] = a.causal ? min(s.len - s.n + (s.row0 + r) / a.group + 1, s.len) : s.len;
       }
     }
-    float y0 = flip(spread_get(x0, x1, sm.turns.k_perm[lane]), a.rk.signs, 0, lane);
-    float y1 = flip(spread_get(x0, x1, sm.turns.k_perm[lane + 32]), a.rk.signs, 1, lane);
-    spread_walsh(y0, y1, lane);
-    y0 *= 0.125f * a.qscale;
-    y1 *= 0.125f * a.qscale;
-    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(y0), fabsf(y1))));
-    const int e = min(max((int)(top >> 23), 30), 254);
-    const float up = __int_as_float((261 - e) << 23);  // 2^(134 - e)
-    y0 *= up;
-    y1 *= up;
-    const __half g0 = __float2half_rn(y0), g1 = __float2half_rn(y1);
-    sm.q[0][r][lane] = g0;
-    sm.q[0][r][lane + 32] = g1;
-    if (F32) {
-      sm.q[F32 ? 1 : 0][r][lane] = __float2half_rn(y0 - __half2float(g0));
-      sm.q[F32 ? 1 : 0][r][lane + 32] = __float2half_rn(y1 - __half2float(g1));
-    }
-    if (lane == 0) sm.rs[r] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64: undoes both scalings
-  }
-  __syncthreads();
+    // every row sees all keys below `clear`
+    const int clear = a.causal ? s.len - s.n + s.row0 / a.group + 1 : s.len;
 
-  uint32_t qf[NB][F32 ? 16 : 8];
-  float rs[NB][2];
-  int limit[NB][2];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-#pragma unroll
-    for (int p = 0; p < (F32 ? 2 : 1); ++p) {
-      const uint4* src = reinterpret_cast<const uint4*>(&sm.q[p][8 * b + g][16 * t]);
-      const uint4 u = src[0], v = src[1];
-      uint32_t* d = &qf[b][8 * p];
-      d[0] = u.x, d[1] = u.y, d[2] = u.z, d[3] = u.w, d[4] = v.x, d[5] = v.y, d[6] = v.z, d[7] = v.w;
+    float m[NB][2], lift[NB][2], neg[NB][2], l[NB][2], acc[4][NB][4];
+  #pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      m[b][0] = m[b][1] = lift[b][0] = lift[b][1] = -INFINITY;
+      neg[b][0] = neg[b][1] = 0.0f;
+      l[b][0] = l[b][1] = 0.0f;
+  #pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i][b][0] = acc[i][b][1] = acc[i][b][2] = acc[i][b][3] = 0.0f;
     }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int r = 8 * b + 2 * t + c;
-      rs[b][c] = sm.rs[r];
-      limit[b][c] = a.causal ? min(s.len - s.n + (s.row0 + r) / a.group + 1, s.len) : s.len;
-    }
-  }
-  // every row sees all keys below `clear`
-  const int clear = a.causal ? s.len - s.n + s.row0 / a.group + 1 : s.len;
+    int ve = 20;  // exponent of the largest V norm met
+    const int krow = (g >> 1) + 4 * (g & 1);  // key of S^T rows g and (+ 8) g + 8 in a block of 16
 
-  float m[NB][2], lift[NB][2], neg[NB][2], l[NB][2], acc[4][NB][4];
+    // One stage of 64 keys.  kEdge: some key is past the end or not for every row.
+    auto attend_stage = [&](auto edge_, uint32_t stage, int key0, const uint32_t (&nb)[4][2]) {
+      constexpr bool kEdge = decltype(edge_)::value;
+      float x[4][NB][4];
+      float nv[4][2];
+      uint32_t top = 0;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    m[b][0] = m[b][1] = lift[b][0] = lift[b][1] = -INFINITY;
-    neg[b][0] = neg[b][1] = 0.0f;
-    l[b][0] = l[b][1] = 0.0f;
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t blk = stage + j * kBlockBytes;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i][b][0] = acc[i][b][1] = acc[i][b][2] = acc[i][b][3] = 0.0f;
-  }
-  int ve = 20;  // exponent of the largest V norm met
-  const int krow = (g >> 1) + 4 * (g & 1);  // key of S^T rows g and (+ 8) g + 8 in a block of 16
-
-  // One stage of 64 keys.  kEdge: some key is past the end, masked, or not for every row.
-  auto attend_stage = [&](auto edge_, uint32_t stage, int key0, const uint32_t (&nb)[4][2]) {
-    constexpr bool kEdge = decltype(edge_)::value;
-    float x[4][NB][4];
-    float nv[4][2];
-    uint32_t top = 0;
+        for (int b = 0; b < NB; ++b) x[j][b][0] = x[j][b][1] = x[j][b][2] = x[j][b][3] = 0.0f;
+        const uint2 w0 = lds64(blk + krow * 32 + t * 8), w1 = lds64(blk + (krow + 8) * 32 + t * 8);
+        const uint32_t wa[2] = {w0.x, w0.y}, wb[2] = {w1.x, w1.y};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t blk = stage + j * kBlockBytes;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) x[j][b][0] = x[j][b][1] = x[j][b][2] = x[j][b][3] = 0.0f;
-      const uint2 w0 = lds64(blk + krow * 32 + t * 8), w1 = lds64(blk + (krow + 8) * 32 + t * 8);
-      const uint32_t wa[2] = {w0.x, w0.y}, wb[2] = {w1.x, w1.y};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t da[4], db[4];
-        decode_pairs(wa[h], a.lk.lo, a.lk.hi, da);
-        decode_pairs(wb[h], a.lk.lo, a.lk.hi, db);
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const uint32_t f[4] = {da[2 * p], db[2 * p], da[2 * p + 1], db[2 * p + 1]};
-          const int k = 2 * (2 * h + p);
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            if (F32) mma(x[j][b], f, qf[b][8 + k], qf[b][8 + k + 1]);
-            mma(x[j][b], f, qf[b][k], qf[b][k + 1]);
-          }
-        }
-        if (F32) {
-          decode_pairs(wa[h], a.lk.rlo, a.lk.rhi, da);
-          decode_pairs(wb[h], a.lk.rlo, a.lk.rhi, db);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t da[4], db[4], ra[4], rb[4];
+          look(wa[h], da, ra);
+          look(wb[h], db, rb);
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
             const uint32_t f[4] = {da[2 * p], db[2 * p], da[2 * p + 1], db[2 * p + 1]};
             const int k = 2 * (2 * h + p);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) mma(x[j][b], f, qf[b][k], qf[b][k + 1]);
+            for (int b = 0; b < NB; ++b) {
+              if (F32) {
+                const uint32_t e[4] = {ra[2 * p], rb[2 * p], ra[2 * p + 1], rb[2 * p + 1]};
+                mma(x[j][b], e, qf[b][k], qf[b][k + 1]);
+                mma(x[j][b], f, qf[b][F32 ? 8 + k : k], qf[b][F32 ? 9 + k : k + 1]);
+              }
+              mma(x[j][b], f, qf[b][k], qf[b][k + 1]);
+            }
           }
         }
-      }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float nk = norm_of<NormBf16>(nb[j][c]);
-        nv[j][c] = norm_of<NormBf16>(nb[j][c] >> 16);
-        bool seen = true;
-        if (kEdge) {
-          seen = !(nb[j][c] & 0x8000u) && key0 + 16 * j + krow + 8 * c < c1;
-          if (!seen) nv[j][c] = 0.0f;
+        for (int c = 0; c < 2; ++c) {
+          float nk = norm_of<NormBf16>(nb[j][c]);
+          nv[j][c] = norm_of<NormBf16>(nb[j][c] >> 16);
+          const bool seen = !(nb[j][c] & 0x8000u) && (!kEdge || key0 + 16 * j + krow + 8 * c < c1);
+          if (!seen) nk = nv[j][c] = 0.0f;
           // where not every row sees a V that is not finite, it must not set the scale for the others
-          if (nv[j][c] <= 3.402823466e38f) top = max(top, __float_as_uint(nv[j][c]));
-        } else {
-          top = max(top, __float_as_uint(nv[j][c]));
+          if (!kEdge || nv[j][c] <= 3.402823466e38f) top = max(top, __float_as_uint(nv[j][c]));
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float& v = x[j][b][2 * c + i];
+              v *= nk;
+              if (!seen || (kEdge && key0 + 16 * j + krow + 8 * c >= limit[b][i])) v = -INFINITY;
+            }
         }
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float& v = x[j][b][2 * c + i];
-            v *= nk;
-            if (kEdge && (!seen || key0 + 16 * j + krow + 8 * c >= limit[b][i])) v = -INFINITY;
-          }
       }
-    }
 
-    // The running maximum moves only when a score is more than 2^8 above it, the
-    // largest norm when a larger one comes; then the sums so far follow.
-    const int ve_new = max(ve, (int)(__reduce_max_sync(0xffffffffu, top) >> 23));
-    float mx[NB][2];
-    bool moved = ve_new != ve;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float v = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v = max3(v, x[j][b][c], x[j][b][c + 2]);
-        mx[b][c] = v;
-        moved = moved || v > lift[b][c];
-      }
-    if (__any_sync(0xffffffffu, moved)) {
-      const float fv = __int_as_float((127 + max(ve - ve_new, -126)) << 23);
+      // The running maximum moves only when a score is more than 2^8 above it, the
+      // largest norm when a larger one comes; then the sums so far follow.
+      const int ve_new = max(ve, (int)(__reduce_max_sync(0xffffffffu, top) >> 23));
+      float mx[NB][2];
+      bool moved = ve_new != ve;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float v = mx[b][c];
+          float v = -INFINITY;
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-          v = fmaxf(m[b][c], v);
-          const float f = m[b][c] == -INFINITY ? 0.0f : ex2((m[b][c] - v) * rs[b][c]);
-          m[b][c] = v;
-          neg[b][c] = v == -INFINITY ? 0.0f : -v * rs[b][c];
-          lift[b][c] = v + 8.0f / rs[b][c];  // -inf until a key is seen
-          l[b][c] *= f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            acc[k][b][c] *= f * fv;
-            acc[k][b][c + 2] *= f * fv;
-          }
+          for (int j = 0; j < 4; ++j) v = max3(v, x[j][b][c], x[j][b][c + 2]);
+          mx[b][c] = v;
+          moved = moved || v > lift[b][c];
         }
-      ve = ve_new;
-    }
-    const float vs = __int_as_float((259 - ve) << 23);  // 2^(132 - ve): norms below 2^6, P n_v below 2^14
+      if (__any_sync(0xffffffffu, moved)) {
+        const float fv = __int_as_float((127 + max(ve - ve_new, -126)) << 23);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float v = mx[b][c];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+            v = fmaxf(m[b][c], v);
+            const float f = m[b][c] == -INFINITY ? 0.0f : ex2((m[b][c] - v) * rs[b][c]);
+            m[b][c] = v;
+            neg[b][c] = v == -INFINITY ? 0.0f : -v * rs[b][c];
+            lift[b][c] = v + 8.0f / rs[b][c];  // -inf until a key is seen
+            l[b][c] *= f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              acc[k][b][c] *= f * fv;
+              acc[k][b][c + 2] *= f * fv;
+            }
+          }
+        ve = ve_new;
+      }
+      const float vs = __int_as_float((259 - ve) << 23);  // 2^(132 - ve): norms below 2^6, P n_v below 2^14
 
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t blk = stage + j * kBlockBytes + kVCodes + g * 4;
-      uint32_t pf[NB][F32 ? 4 : 2];
-      const uint64_t n0 = f2_pack(nv[j][0] * vs, nv[j][0] * vs), n1 = f2_pack(nv[j][1] * vs, nv[j][1] * vs);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const uint64_t r2 = f2_pack(rs[b][0], rs[b][1]), g2 = f2_pack(neg[b][0], neg[b][1]);
-        float p[4];
-#pragma unroll
-        for (int c = 0; c < 4; c += 2) {
-          f2_unpack(f2_fma(f2_pack(x[j][b][c], x[j][b][c + 1]), r2, g2), p[c], p[c + 1]);
-          p[c] = ex2(p[c]);
-          p[c + 1] = ex2(p[c + 1]);
-        }
-        f2_unpack(f2_add(f2_add(f2_pack(l[b][0], l[b][1]), f2_pack(p[0], p[1])), f2_pack(p[2], p[3])), l[b][0], l[b][1]);
-        if (kEdge) {  // a key that a row does not see adds nothing, whatever its norm
-#pragma unroll
-          for (int c = 0; c < 4; ++c) p[c] = x[j][b][c] == -INFINITY ? 0.0f : p[c] * (c < 2 ? nv[j][0] : nv[j][1]) * vs;
-        } else {
-          f2_unpack(f2_mul(f2_pack(p[0], p[1]), n0), p[0], p[1]);
-          f2_unpack(f2_mul(f2_pack(p[2], p[3]), n1), p[2], p[3]);
-        }
-        const uint32_t h0 = pack_half(p[0], p[1]), h1 = pack_half(p[2], p[3]);
-        pf[b][0] = transpose8(h0);
-        pf[b][1] = transpose8(h1);
-        if (F32) {
-          const float2 f0 = unpack_half(h0), f1 = unpack_half(h1);
-          pf[b][F32 ? 2 : 0] = transpose8(pack_half(p[0] - f0.x, p[1] - f0.y));
-          pf[b][F32 ? 3 : 1] = transpose8(pack_half(p[2] - f1.x, p[3] - f1.y));
-        }
-      }
-      const Zip z0 = zip(lds32(blk + t * 32), lds32(blk + (t + 4) * 32));
-      const Zip z1 = zip(lds32(blk + (t + 8) * 32), lds32(blk + (t + 12) * 32));
-      uint32_t d0[8], d1[8];
-      if (F32) {
-        decode_zip(z0, a.lv.rlo, a.lv.rhi, d0);
-        decode_zip(z1, a.lv.rlo, a.lv.rhi, d1);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t f[4] = {d0[2 * k], d0[2 * k + 1], d1[2 * k], d1[2 * k + 1]};
-#pragma unroll
-          for (int b = 0; b < NB; ++b) mma(acc[k][b], f, pf[b][0], pf[b][1]);
-        }
-      }
-      decode_zip(z0, a.lv.lo, a.lv.hi, d0);
-      decode_zip(z1, a.lv.lo, a.lv.hi, d1);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t f[4] = {d0[2 * k], d0[2 * k + 1], d1[2 * k], d1[2 * k + 1]};
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t blk = stage + j * kBlockBytes + kVCodes + g * 4;
+        uint32_t pf[NB][F32 ? 4 : 2];
+        const uint64_t n0 = f2_pack(nv[j][0] * vs, nv[j][0] * vs), n1 = f2_pack(nv[j][1] * vs, nv[j][1] * vs);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          if (F32) mma(acc[k][b], f, pf[b][F32 ? 2 : 0], pf[b][F32 ? 3 : 1]);
-          mma(acc[k][b], f, pf[b][0], pf[b][1]);
+          const uint64_t r2 = f2_pack(rs[b][0], rs[b][1]), g2 = f2_pack(neg[b][0], neg[b][1]);
+          float p[4];
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            f2_unpack(f2_fma(f2_pack(x[j][b][c], x[j][b][c + 1]), r2, g2), p[c], p[c + 1]);
+            p[c] = ex2(p[c]);
+            p[c + 1] = ex2(p[c + 1]);
+          }
+          f2_unpack(f2_add(f2_add(f2_pack(l[b][0], l[b][1]), f2_pack(p[0], p[1])), f2_pack(p[2], p[3])), l[b][0], l[b][1]);
+          if (kEdge) {  // a key that a row does not see adds nothing, whatever its norm
+#pragma unroll
+            for (int c = 0; c < 4; ++c) p[c] = x[j][b][c] == -INFINITY ? 0.0f : p[c] * (c < 2 ? nv[j][0] : nv[j][1]) * vs;
+          } else {
+            f2_unpack(f2_mul(f2_pack(p[0], p[1]), n0), p[0], p[1]);
+            f2_unpack(f2_mul(f2_pack(p[2], p[3]), n1), p[2], p[3]);
+          }
+          const uint32_t h0 = pack_half(p[0], p[1]), h1 = pack_half(p[2], p[3]);
+          pf[b][0] = transpose8(h0);
+          pf[b][1] = transpose8(h1);
+          if (F32) {
+            const float2 f0 = unpack_half(h0), f1 = unpack_half(h1);
+            pf[b][F32 ? 2 : 0] = transpose8(pack_half(p[0] - f0.x, p[1] - f0.y));
+            pf[b][F32 ? 3 : 1] = transpose8(pack_half(p[2] - f1.x, p[3] - f1.y));
+          }
+        }
+        uint32_t u0, v0, u1, v1;  // even and odd coordinates of tokens t, t + 4 and t + 8, t + 12
+        zip(lds32(blk + t * 32), lds32(blk + (t + 4) * 32), u0, v0);
+        zip(lds32(blk + (t + 8) * 32), lds32(blk + (t + 12) * 32), u1, v1);
+        uint32_t d[4][4], r[4][4];
+        look(u0, d[0], r[0]);
+        look(v0, d[1], r[1]);
+        look(u1, d[2], r[2]);
+        look(v1, d[3], r[3]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t f[4] = {d[0][k], d[1][k], d[2][k], d[3][k]};
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            if (F32) {
+              const uint32_t e[4] = {r[0][k], r[1][k], r[2][k], r[3][k]};
+              mma(acc[k][b], e, pf[b][0], pf[b][1]);
+              mma(acc[k][b], f, pf[b][F32 ? 2 : 0], pf[b][F32 ? 3 : 1]);
+            }
+            mma(acc[k][b], f, pf[b][0], pf[b][1]);
+          }
         }
       }
-    }
-  };
+    };
 
-  for (int i = 0; i < mine; ++i) {
-    const int key0 = c0 + (warp + kWarps * i) * kStageKeys;
-    const uint32_t stage = smem_u32(sm.ring[warp][i % kStages]);
-    // the lanes leave together: one may see the block's abort flag where another saw its stage
-    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.full[warp][i % kStages]), (uint32_t)(i / kStages) & 1u,
-                                           &sm.abort_flag, a.wait_err)))
-      break;
-    uint32_t nb[4][2], any = 0;  // norms of this lane's keys: K low, V high
+    for (int i = 0; i < mine; ++i, ++n) {
+      const int key0 = c0 + (warp + kWarps * i) * kStageKeys;
+      const uint32_t stage = smem_u32(sm.ring[warp][n & 1u]);
+      // the lanes leave together: one may see the block's abort flag where another saw its stage
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.full[warp][n & 1u]), (n >> 1) & 1u, &all.abort_flag, a.wait_err))) {
+        broken = true;
+        break;
+      }
+      uint32_t nb[4][2];  // norms of this lane's keys: K low, V high
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) nb[j][c] = lds32(stage + j * kBlockBytes + kNorms + (krow + 8 * c) * 4);
+      if (key0 + kStageKeys > min(clear, c1)) attend_stage(std::true_type{}, stage, key0, nb);
+      else attend_stage(std::false_type{}, stage, key0, nb);
+      __syncwarp();  // the stage is in registers
+      if (ahead < mine) issue(u, ahead, n + 2u), ++ahead;
+    }
+
+    // the next unit's first stage sets out before this one is joined
+    ahead = 0;
+    more = next(coming);
+    if (sums_in_a_slot<NB>() && more && !broken && coming.stages > 0) issue(coming, 0, n), ahead = 1;
+    float* mine_sums = reinterpret_cast<float*>(sm.ring[warp][sums_in_a_slot<NB>() ? (n + 1u) & 1u : 0]);
+    const float down = __int_as_float((ve - 11) << 23);  // 2^(ve - 132) / 64
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        nb[j][c] = lds32(stage + j * kBlockBytes + kNorms + (krow + 8 * c) * 4);
-        any |= nb[j][c];
+        float v = l[b][c];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        const int r = 8 * b + 2 * t + c;
+        if (g == 0) {
+          sm.m[warp][r] = m[b][c] * rs[b][c];
+          sm.l[warp][r] = v;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<float2*>(mine_sums + r * kOPitch + 8 * g + 2 * k) =
+              make_float2(acc[k][b][c] * down, acc[k][b][c + 2] * down);
       }
-    // (past the end the norms may be anything)
-    if (key0 + kStageKeys > min(clear, c1) || __any_sync(0xffffffffu, any & 0x8000u))
-      attend_stage(std::true_type{}, stage, key0, nb);
-    else
-      attend_stage(std::false_type{}, stage, key0, nb);
-    __syncwarp();  // the stage is in registers
-    if (i + kStages < mine) issue(i + kStages);
+    if (lane == 0) sm.sums[warp] = mine_sums;
+    if (!meet(!broken)) break;
+    for (int r = warp; r < kRows && s.row0 + r < s.rows; r += kWarps) {
+      float top = sm.m[0][r];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.m[w][r]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = ex2(sm.m[w][r] - base);
+        sum += sm.l[w][r] * f;
+        o0 += sm.sums[w][r * kOPitch + lane] * f;
+        o1 += sm.sums[w][r * kOPitch + lane + 32] * f;
+      }
+      if (u.whole) {
+        finish_row<T>(a, all.turns, s, u.head, s.row0 + r, o0, o1, top, sum, lane);
+      } else {
+        const long long at = u.piece * kRows + r;
+        a.part[at * 64 + lane] = o0;
+        a.part[at * 64 + lane + 32] = o1;
+        if (lane == 0) a.part_ml[at] = make_float2(top, sum);
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the sums' places go back to the copies
+    meet(true);
   }
-  if (sm.abort_flag) {  // a wait ran out: nothing may still be landing when the block ends
+  if (broken || all.abort_flag) {  // a wait ran out: nothing may still be landing when the block ends
     const unsigned long long t0 = globaltimer_ns();
-    for (int i = max(0, mine - kStages); i < mine; ++i)
-      while (!mbar_try(smem_u32(&sm.full[warp][i % kStages]), (uint32_t)(i / kStages) & 1u) &&
-             globaltimer_ns() - t0 < kWaitLimitNs) {
+    for (uint32_t i = n; i < n + 2u; ++i)
+      while (!mbar_try(smem_u32(&sm.full[warp][i & 1u]), (i >> 1) & 1u) && globaltimer_ns() - t0 < kWaitLimitNs) {
       }
-  }
-  __syncthreads();  // all warps are done with the ring
-
-  float(*osum)[kRows][kOPitch] = reinterpret_cast<float(*)[kRows][kOPitch]>(&sm.ring[0][0][0]);
-  const float down = __int_as_float((ve - 11) << 23);  // 2^(ve - 132) / 64
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float v = l[b][c];
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      const int r = 8 * b + 2 * t + c;
-      if (g == 0) {
-        sm.m[warp][r] = m[b][c] * rs[b][c];
-        sm.l[warp][r] = v;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        *reinterpret_cast<float2*>(&osum[warp][r][8 * g + 2 * k]) =
-            make_float2(acc[k][b][c] * down, acc[k][b][c + 2] * down);
-    }
-  __syncthreads();
-  for (int r = warp; r < kRows && s.row0 + r < s.rows; r += kWarps) {
-    float top = sm.m[0][r];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.m[w][r]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2(sm.m[w][r] - base);
-      sum += sm.l[w][r] * f;
-      o0 += osum[w][r][lane] * f;
-      o1 += osum[w][r][lane + 32] * f;
-    }
-    if (chunks <= 1) {
-      finish_row<T>(a, sm.turns, s, head, s.row0 + r, o0, o1, top, sum, lane);
-    } else {
-      const long long at = part_at(a, s, head, split, s.row0 + r);
-      a.part[at * 64 + lane] = o0;
-      a.part[at * 64 + lane + 32] = o1;
-      if (lane == 0) a.part_ml[at] = make_float2(top, sum);
-    }
   }
 }
 
-// Joins the chunks of the rows that have more than one: kRowWarps warps a row,
-// each a share of the chunks.
-template <typename T, int kRowWarps>
+// Joins the chunks (tcgen05) or pieces of the rows that have more than one:
+// kRowWarps warps a row, each a share of them.
+template <typename T, int kRowWarps, bool kPieces>
 __global__ void __launch_bounds__(128)
 join_kernel(const __grid_constant__ Args a) {
   __shared__ Turns turns;
@@ -510,9 +622,29 @@ join_kernel(const __grid_constant__ Args a) {
   const int row = (tok - q0) * a.group + call_row % a.group;
   const Span s = span_of(a, seq, row / a.tile_rows, false);
   if (row >= s.rows) return;
-  const int chunks = chunks_of(a, s);
+  int chunks = chunks_of(a, s);
+  long long first = part_at(a, s, head, 0, row), step = (long long)a.pool.heads * rows;
+  if (kPieces) {
+    long long cost = 0, units = 0, total = 0;  // up to the sequence; of all
+    for (int i = lane; i < a.num_seqs; i += 32) {
+      const SeqCost c = cost_of(a, i);
+      total += c.cost;
+      if (i < seq) cost += c.cost, units += c.units;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      cost += __shfl_xor_sync(0xffffffffu, cost, o);
+      units += __shfl_xor_sync(0xffffffffu, units, o);
+    }
+    const SeqCost c = cost_of(a, seq);
+    const long long k = (long long)head * c.tiles + row / a.tile_rows, at = cost + k * (c.rounds + 1);
+    const int t0 = team_of(total, at, a.teams);
+    chunks = team_of(total, at + c.rounds - 1, a.teams) - t0 + 1;
+    first = (units + k + t0) * a.tile_rows + row % a.tile_rows;
+    step = a.tile_rows;
+  }
   if (chunks <= 1) return;
-  const long long first = part_at(a, s, head, 0, row), step = (long long)a.pool.heads * rows;
   float top = -INFINITY;
   for (int c = lane; c < chunks; c += 32) top = fmaxf(top, a.part_ml[first + c * step].x);
 #pragma unroll
@@ -547,8 +679,11 @@ join_kernel(const __grid_constant__ Args a) {
 
 struct Plan {
   bool tc;  // attn_kv4_tc.cu's kernel
-  int nb, row_tiles, tile_rows, chunk, splits;
-  long long units, tiles;
+  bool joined;
+  int nb, row_tiles, tile_rows;
+  int chunk, splits;               // tcgen05
+  int round_keys, blocks, teams;   // else
+  long long tiles;
   size_t part_bytes, ml_bytes, q_bytes, scale_bytes;
   size_t bytes() const { return part_bytes + ml_bytes + q_bytes + scale_bytes; }
 };
@@ -573,33 +708,35 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
     const long long want = (4LL * num_sms() + tiles - 1) / tiles;
     const int splits = (int)std::min<long long>(std::max(1, (max_len + 1023) / 1024), std::max<long long>(1, want));
     p.chunk = ((std::max(1, max_len) + splits - 1) / splits + 255) / 256 * 256;
-  } else {
-    // the chunk for which the waves of blocks, each of the chunk's keys and of 512 more for its start and its
-    // join, take the least; it is worth looking where the blocks just fill one to eight waves
-    const long long slots = (long long)num_sms() * (p.nb == 1 ? 5 : p.nb == 2 ? 3 : 2);
-    const int len = std::max(1, max_len);
-    long long best = -1;
-    for (int w = 0; w <= 8; ++w) {
-      const long long splits = std::min<long long>(std::max(1LL, w * slots / tiles), (len + 511) / 512);
-      const int chunk = (int)(((len + splits - 1) / splits + 255) / 256 * 256);
-      const long long waves = (tiles * ((len + chunk - 1) / chunk) + slots - 1) / slots;
-      const long long cost = waves * (chunk + 512);
-      if (best < 0 || cost < best) best = cost, p.chunk = chunk;
-    }
-  }
-  p.splits = std::max(1, (max_len + p.chunk - 1) / p.chunk);
-  p.units = tiles * p.splits;
-  CC2_REQUIRE(p.units <= 0x7fffffffLL, "kv4_attention: too many rows and keys for one call");
-  if (p.splits > 1) {
-    const size_t n = (size_t)p.splits * total_q * q_heads;
+    p.splits = std::max(1, (max_len + p.chunk - 1) / p.chunk);
+    CC2_REQUIRE(tiles * p.splits <= 0x7f000000LL, "kv4_attention: too many rows and keys for one call");
+    const size_t n = p.splits > 1 ? (size_t)p.splits * total_q * q_heads : 0;
     p.part_bytes = n * 64 * sizeof(float);
     p.ml_bytes = align_up(n * sizeof(float2), 128);
-  }
-  if (p.tc) {
     p.tiles = query_tiles((long long)total_q * (q_heads / pool.heads), num_seqs) * pool.heads;
     p.q_bytes = (size_t)p.tiles * 128 * 128;
     p.scale_bytes = (size_t)p.tiles * 128 * sizeof(float) + 128;  // and the items' counter
+  } else {
+    const bool f32 = dtype == CC2_F32;
+    const int warps = p.nb == 1 && !f32 ? warps_of<1, false>() : 4, a_block = p.nb == 2 && !f32 ? teams_of<2, false>() : 2;
+    static_assert(warps_of<2, false>() == 4 && warps_of<4, false>() == 4 && warps_of<1, true>() == 4 &&
+                      warps_of<2, true>() == 4 && teams_of<1, false>() == 2 && teams_of<4, false>() == 2 &&
+                      teams_of<1, true>() == 2 && teams_of<2, true>() == 2,
+                  "as assumed above");
+    p.round_keys = warps * kStageKeys;
+    // no more blocks than there are rounds
+    const long long rounds = (long long)num_seqs * pool.heads * p.row_tiles * std::max(1, (max_len + p.round_keys - 1) / p.round_keys);
+    p.blocks = (int)std::min<long long>((rounds + a_block - 1) / a_block, num_sms());
+    p.teams = p.blocks * a_block;
+    p.joined = max_len > p.round_keys;
+    if (p.joined) {
+      const long long units = ((long long)total_q * (q_heads / pool.heads) / p.tile_rows + num_seqs) * pool.heads;
+      const size_t n = (size_t)(units + p.teams) * p.tile_rows;
+      p.part_bytes = n * 64 * sizeof(float);
+      p.ml_bytes = align_up(n * sizeof(float2), 128);
+    }
   }
+  p.joined = p.tc ? p.splits > 1 : p.joined;
   return CC2_OK;
 }
 
@@ -613,7 +750,8 @@ int launch(const Args& a, const Plan& p, cudaStream_t st) {
     CC2_CUDA(cudaFuncSetAttribute(attend_kernel<NB, F32, NormBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (dev < 64) attr_done |= 1ull << dev;
   }
-  CC2_CUDA(launch_k(attend_kernel<NB, F32, NormBf16>, (unsigned)p.units, kWarps * 32, smem, st, a));
+  CC2_CUDA(launch_k(attend_kernel<NB, F32, NormBf16>, (unsigned)p.blocks, 32 * teams_of<NB, F32>() * warps_of<NB, F32>(),
+                    smem, st, a));
   CC2_CHECK_LAUNCH();
   return CC2_OK;
 }
@@ -622,18 +760,19 @@ int launch(const Args& a, const Plan& p, cudaStream_t st) {
   return a.pool.norm_bf16 ? launch<NB, F32, true>(a, p, st) : launch<NB, F32, false>(a, p, st);
 }
 
-int join(const Args& a, int dtype, cudaStream_t st) {
-  if (a.splits <= 1) return CC2_OK;
+template <typename T>
+int join(const Args& a, const Plan& p, cudaStream_t st) {
+  if (!p.joined) return CC2_OK;
   const long long rows = (long long)a.total_q * a.group * a.pool.heads;
-  // many chunks mean few rows: four warps then share a row's
-  const bool four = a.splits > 8;
+  // where there are fewer rows than warps on the card, four share one: a row then has many parts
+  const bool four = rows <= 16LL * num_sms();
   const unsigned grid = (unsigned)(four ? rows : (rows + 3) / 4);
-  if (dtype == CC2_F32) {
-    if (four) CC2_CUDA(launch_k(join_kernel<float, 4>, grid, 128, 0, st, a));
-    else CC2_CUDA(launch_k(join_kernel<float, 1>, grid, 128, 0, st, a));
+  if (p.tc) {
+    if (four) CC2_CUDA(launch_k(join_kernel<T, 4, false>, grid, 128, 0, st, a));
+    else CC2_CUDA(launch_k(join_kernel<T, 1, false>, grid, 128, 0, st, a));
   } else {
-    if (four) CC2_CUDA(launch_k(join_kernel<__nv_bfloat16, 4>, grid, 128, 0, st, a));
-    else CC2_CUDA(launch_k(join_kernel<__nv_bfloat16, 1>, grid, 128, 0, st, a));
+    if (four) CC2_CUDA(launch_k(join_kernel<T, 4, true>, grid, 128, 0, st, a));
+    else CC2_CUDA(launch_k(join_kernel<T, 1, true>, grid, 128, 0, st, a));
   }
   CC2_CHECK_LAUNCH();
   return CC2_OK;
@@ -709,6 +848,8 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   a.splits = p.splits;
   a.row_tiles = p.row_tiles;
   a.tile_rows = p.tile_rows;
+  a.teams = p.teams;
+  a.round_keys = p.round_keys;
   a.causal = causal != 0;
   a.rotate = rotate_q != 0;
   a.qscale = scale * 1.4426950408889634f;
@@ -720,12 +861,11 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
     r.signs[1] = (uint32_t)(quant[k]->signs >> 32);
     for (int i = 0; i < 64; ++i) r.inv[r.perm[i] = quant[k]->perm[i] & 63] = (uint8_t)i;
   }
-  a.lk = make_levels(cache->key);
-  a.lv = make_levels(cache->value);
+  a.levels = make_levels(*cache);
   if (p.tc) CC2_TRY(launch_attend_tc(a, st));
   else if (dtype == CC2_F32) CC2_TRY(p.nb == 1 ? (launch<1, true>(a, p, st)) : (launch<2, true>(a, p, st)));
   else CC2_TRY(p.nb == 1 ? (launch<1, false>(a, p, st)) : p.nb == 2 ? (launch<2, false>(a, p, st)) : (launch<4, false>(a, p, st)));
-  return join(a, dtype, st);
+  return dtype == CC2_F32 ? join<float>(a, p, st) : join<__nv_bfloat16>(a, p, st);
 }
 
 }  // namespace cc2

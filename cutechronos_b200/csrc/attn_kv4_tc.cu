@@ -638,7 +638,6 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         const bool used = 32 * w < c1 - (c0 + j * kTile);
 #pragma unroll 1
         for (int m = 0; m < 2 && used; ++m) {
-          const Levels& lv = m ? a.lv : a.lk;
           const __half2 n = m ? hv : hk;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -649,7 +648,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t o[4];
-              decode_pairs(c[i], lv.lo, lv.hi, o);
+              decode_pairs(c[i], a.levels.lo, a.levels.hi, o);
 #pragma unroll
               for (int p = 0; p < 4; ++p) {
                 const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&o[p]), n);

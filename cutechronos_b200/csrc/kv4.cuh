@@ -7,14 +7,11 @@
 // so that everything attention needs of 16 tokens of a head is one aligned
 // run of memory, and of a page one longer run: one bulk copy brings it.
 //
-// A vector's 64 codes are 8 words; nibble p of word w holds the 3-bit magnitude
-// index of coordinate 8w + p in its low bits.  The nibbles' top bits hold the
-// signs, but not each its own nibble's: bits 7, 15, 23, 31 are coordinates
-// 0..3's and bits 3, 11, 19, 27 coordinates 4..7's, so that a decoder merges
-// four signs with four looked-up bytes in one operation, whether it makes
-// pairs of neighbouring coordinates of one token (decode_pairs) or of one
-// coordinate of two tokens (decode_zip).  A key norm's sign bit marks a
-// masked token.
+// A vector's 64 codes are 8 words; nibble p of word w is coordinate 8w + p: the
+// magnitude's index in its low three bits, the sign in its top bit.  A byte is
+// two codes, of neighbouring coordinates of a token or, once two tokens' words
+// are zipped, of one coordinate of both: one of 256 fp16 pairs either way.  A
+// key norm's sign bit marks a masked token.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -52,18 +49,18 @@ struct Quant {
   } cells[65];
 };
 
-// Level tables of the fp16 decoder: 64 c_i split into its fp16 value and, for
-// fp32 calls, what that leaves over, each as four words: bytes 0 and 1 of the
-// eight values (8 low bytes, 8 high bytes).  The factor 64 keeps the rest of
+// The levels as the fp16 decoders take them: 64 c_i split into its fp16 value
+// and, for fp32 calls, what that leaves over.  The factor 64 keeps the rest of
 // the split out of fp16's subnormal range; it is exact and taken out again at
-// the end.
+// the end.  `lo` and `hi` are the low and the high bytes of the eight fp16
+// values, for byte permutes.
 struct Levels {
-  uint32_t lo[2], hi[2];    // fp16(64 c)
-  uint32_t rlo[2], rhi[2];  // fp16(64 c - fp16(64 c))
+  uint16_t value[8], rest[8];
+  uint32_t lo[2], hi[2];
 };
 
 // Bit of a word of codes that holds the sign of coordinate p (0..7) of it.
-__host__ __device__ constexpr int sign_bit(int p) { return p < 4 ? 8 * p + 7 : 8 * (p - 4) + 3; }
+__host__ __device__ constexpr int sign_bit(int p) { return 4 * p + 3; }
 
 __device__ __forceinline__ float norm_value(uint16_t bits, int norm_bf16) {
   const uint16_t b = bits & 0x7fffu;
@@ -86,60 +83,30 @@ __device__ __forceinline__ long long block_offset(const Pool& p, int page, int h
 
 // --- decoding to fp16 -------------------------------------------------------
 // A byte permute looks four 3-bit indices up in a table of 8 bytes at once.
-__device__ __forceinline__ uint32_t look(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
-
 // The 8 coordinates of a word as four fp16 pairs (0 1) (2 3) (4 5) (6 7).
 __device__ __forceinline__ void decode_pairs(uint32_t w, const uint32_t lo[2], const uint32_t hi[2], uint32_t out[4]) {
-  const uint32_t s = w & 0x77777777u, s2 = s >> 16;
-  const uint32_t l0 = look(lo[0], lo[1], s), l1 = look(lo[0], lo[1], s2);
-  const uint32_t h0 = look(hi[0], hi[1], s) ^ (w & 0x80808080u);
-  const uint32_t h1 = look(hi[0], hi[1], s2) ^ ((w << 4) & 0x80808080u);
+  const uint32_t s = w & 0x77777777u, s2 = s >> 16, x = w << 4;
+  // the signs of four coordinates as the top bits of four bytes
+  const uint32_t n0 = __byte_perm(x, w, 0x5140), n1 = __byte_perm(x, w, 0x7362);
+  const uint32_t l0 = __byte_perm(lo[0], lo[1], s), l1 = __byte_perm(lo[0], lo[1], s2);
+  const uint32_t h0 = __byte_perm(hi[0], hi[1], s) ^ (n0 & 0x80808080u);
+  const uint32_t h1 = __byte_perm(hi[0], hi[1], s2) ^ (n1 & 0x80808080u);
   out[0] = __byte_perm(l0, h0, 0x5140);
   out[1] = __byte_perm(l0, h0, 0x7362);
   out[2] = __byte_perm(l1, h1, 0x5140);
   out[3] = __byte_perm(l1, h1, 0x7362);
 }
-
-// Coordinate p of tokens a and b as the fp16 pair out[p], p = 0..7.
-struct Zip {
-  uint32_t u, v, su, sv, tu, tv;  // selectors of even / odd coordinates; their signs (low, high half)
-};
-__device__ __forceinline__ Zip zip(uint32_t a, uint32_t b) {
+// Codes of tokens a and b zipped: byte i of u is coordinate 2i of both, of v 2i + 1.
+__device__ __forceinline__ void zip(uint32_t a, uint32_t b, uint32_t& u, uint32_t& v) {
   constexpr uint32_t m = 0x0f0f0f0fu;
-  Zip z;
-  z.u = ((a & m) | ((b << 4) & ~m)) & 0x77777777u;
-  z.v = (((a >> 4) & m) | (b & ~m)) & 0x77777777u;
-  const uint32_t s0 = __byte_perm(a, b, 0x6240), s1 = __byte_perm(a, b, 0x7351);
-  z.su = s0 & 0x80808080u;
-  z.tu = (s0 << 4) & 0x80808080u;
-  z.sv = s1 & 0x80808080u;
-  z.tv = (s1 << 4) & 0x80808080u;
-  return z;
-}
-__device__ __forceinline__ void decode_zip(const Zip& z, const uint32_t lo[2], const uint32_t hi[2], uint32_t out[8]) {
-  uint32_t l, h;
-  l = look(lo[0], lo[1], z.u);
-  h = look(hi[0], hi[1], z.u) ^ z.su;
-  out[0] = __byte_perm(l, h, 0x5140);
-  out[2] = __byte_perm(l, h, 0x7362);
-  l = look(lo[0], lo[1], z.u >> 16);
-  h = look(hi[0], hi[1], z.u >> 16) ^ z.tu;
-  out[4] = __byte_perm(l, h, 0x5140);
-  out[6] = __byte_perm(l, h, 0x7362);
-  l = look(lo[0], lo[1], z.v);
-  h = look(hi[0], hi[1], z.v) ^ z.sv;
-  out[1] = __byte_perm(l, h, 0x5140);
-  out[3] = __byte_perm(l, h, 0x7362);
-  l = look(lo[0], lo[1], z.v >> 16);
-  h = look(hi[0], hi[1], z.v >> 16) ^ z.tv;
-  out[5] = __byte_perm(l, h, 0x5140);
-  out[7] = __byte_perm(l, h, 0x7362);
+  u = (a & m) | ((b << 4) & ~m);
+  v = ((a >> 4) & m) | (b & ~m);
 }
 
 // --- host side --------------------------------------------------------------
 int check_cache(const cc2_kv4_cache* c, const char* what, Pool& pool);
-int make_quant(const cc2_kv4_quant& q, const char* what, Quant& r);
-Levels make_levels(const cc2_kv4_quant& q);
+int make_quant(const cc2_kv4_cache& c, const cc2_kv4_quant& q, const char* what, Quant& r);
+Levels make_levels(const cc2_kv4_cache& c);
 // Device error word of the cache's kernels (DEV_ERR_CACHE_RANGE).
 int error_word(int** p);
 

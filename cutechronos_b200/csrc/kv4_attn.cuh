@@ -41,7 +41,7 @@ struct Args {
   const int* lens;
   const int* table;
   const float2* rope;
-  float* part;       // [split][head][row of the call][64]: a chunk's sums, rotated
+  float* part;       // tcgen05: [split][head][row of the call][64], else [piece][row][64]: a part's sums, rotated
   float2* part_ml;   // the same places: maximum (log2) and sum of exponentials
   const uint8_t* qt;  // rotated queries as fp16 tiles (attn_kv4_tc.cu) and their rows' scales
   const float* q_scale;
@@ -51,10 +51,11 @@ struct Args {
   int table_ld, rope_len, max_len;
   int num_seqs, total_q, max_q, group;
   int chunk, splits, row_tiles, tile_rows;
+  int teams, round_keys;  // else: teams of warps on the card, keys that one takes in a round of its warps
   int causal, rotate;
   float qscale;  // scale * log2(e)
   Rotation rk, rv;
-  Levels lk, lv;
+  Levels levels;
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -115,6 +116,36 @@ __device__ __forceinline__ Span span_of(const Args& a, int seq, int row_tile, bo
   const int last = (min(s.row0 + a.tile_rows, s.rows) - 1) / a.group;  // the tile's last query token
   s.keys = a.causal ? min(max(s.len - s.n + last + 1, 0), s.len) : s.len;
   return s;
+}
+
+// The work of a call without tcgen05, as one line of rounds: sequence after
+// sequence, head after head, row tile after row tile, each of as many rounds of
+// a team's warps as its keys take (one at least) and one more for what a unit
+// costs by itself.  Team t of N gets the rounds from floor(t W / N) on, so all
+// take the same time whatever the sequences' lengths; a unit that crosses a
+// border is joined from its pieces.  Pieces are numbered unit + team, which
+// grows along the line.
+struct SeqCost {
+  int tiles;       // of a head's rows
+  int rounds;      // of a unit's keys
+  long long units, cost;
+};
+__device__ __forceinline__ SeqCost cost_of(const Args& a, int seq) {
+  const Span s = span_of(a, seq, 0, false);
+  SeqCost c;
+  c.tiles = (s.rows + a.tile_rows - 1) / a.tile_rows;
+  c.rounds = max((s.len + a.round_keys - 1) / a.round_keys, 1);
+  c.units = (long long)c.tiles * a.pool.heads;
+  c.cost = c.units * (c.rounds + 1);
+  return c;
+}
+// No more teams than rounds take part: none of them is without one.
+__device__ __forceinline__ long long team_start(long long total, int team, int teams) {
+  teams = (int)min((long long)teams, max(total, 1LL));
+  return total * min(team, teams) / teams;
+}
+__device__ __forceinline__ int team_of(long long total, long long round, int teams) {
+  return (int)(((round + 1) * min((long long)teams, total) - 1) / total);
 }
 
 // Place of a row's sums among the parts.

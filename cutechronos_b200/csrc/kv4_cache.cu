@@ -59,7 +59,7 @@ int check_cache(const cc2_kv4_cache* c, const char* what, Pool& pool) {
   return CC2_OK;
 }
 
-int make_quant(const cc2_kv4_quant& q, const char* what, Quant& r) {
+int make_quant(const cc2_kv4_cache& cache, const cc2_kv4_quant& q, const char* what, Quant& r) {
   uint64_t met = 0;
   for (int i = 0; i < 64; ++i) {
     const int e = q.perm[i] & 63;
@@ -67,18 +67,18 @@ int make_quant(const cc2_kv4_quant& q, const char* what, Quant& r) {
     r.go[e] = (uint8_t)(i | (((q.signs >> i) & 1) << 7));
   }
   CC2_REQUIRE(met == ~0ull, "%s: a quantiser's perm is no permutation", what);
-  for (int i = 0; i < 8; ++i) r.levels[i] = q.levels[i];
+  for (int i = 0; i < 8; ++i) r.levels[i] = cache.levels[i];
   for (int c = 0; c < 65; ++c) {
     // |y| / 8n of r = 8c .. 8c + 7, with room for the rounding of r itself
     const float lo = (8 * c - 0.52f) / 512.0f, hi = (8 * c + 7.52f) / 512.0f;
     r.cells[c].bound = INFINITY;
     r.cells[c].below = 0;
     for (int j = 0; j < 7; ++j) {
-      CC2_REQUIRE(q.bounds[j] > (j ? q.bounds[j - 1] : 0.0f), "%s: a quantiser's bounds must ascend from above 0", what);
-      if (q.bounds[j] <= lo) ++r.cells[c].below;
-      else if (q.bounds[j] <= hi) {
-        CC2_REQUIRE(r.cells[c].bound == INFINITY, "%s: a quantiser's bounds must be more than 1/60 apart", what);
-        r.cells[c].bound = q.bounds[j];
+      CC2_REQUIRE(cache.bounds[j] > (j ? cache.bounds[j - 1] : 0.0f), "%s: the bounds must ascend from above 0", what);
+      if (cache.bounds[j] <= lo) ++r.cells[c].below;
+      else if (cache.bounds[j] <= hi) {
+        CC2_REQUIRE(r.cells[c].bound == INFINITY, "%s: the bounds must be more than 1/60 apart", what);
+        r.cells[c].bound = cache.bounds[j];
       }
     }
   }
@@ -462,8 +462,8 @@ int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int6
   CC2_TRY(grid_of(T, pool.heads, &grid));
   CC2_TRY(error_word(&err));
   Quant qk, qv;
-  CC2_TRY(make_quant(cache->key, "kv4_append", qk));
-  CC2_TRY(make_quant(cache->value, "kv4_append", qv));
+  CC2_TRY(make_quant(*cache, cache->key, "kv4_append", qk));
+  CC2_TRY(make_quant(*cache, cache->value, "kv4_append", qv));
   const Places at{seq, pos, table, table_ld, num_seqs};
   const float2* rope = (const float2*)cache->rope_cs;
 #define CC2_APPEND(TT, ROPE)                                                                                        \
@@ -493,8 +493,8 @@ int launch_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_
   CC2_TRY(grid_of(T, pool.heads, &grid));
   CC2_TRY(error_word(&err));
   Quant qk, qv;
-  CC2_TRY(make_quant(cache->key, "kv4_read", qk));
-  CC2_TRY(make_quant(cache->value, "kv4_read", qv));
+  CC2_TRY(make_quant(*cache, cache->key, "kv4_read", qk));
+  CC2_TRY(make_quant(*cache, cache->value, "kv4_read", qv));
   const Places at{seq, pos, table, table_ld, num_seqs};
   if (dtype == CC2_BF16) {
     CC2_CUDA(launch_k(read_kernel<__nv_bfloat16>, grid, kThreads, 0, st, pool, qk, qv, (__nv_bfloat16*)k_out,

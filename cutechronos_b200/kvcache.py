@@ -35,7 +35,8 @@ def rope_rows(positions: int, theta: float, device) -> torch.Tensor:
     return torch.stack([ang.double().cos(), ang.double().sin()], -1).float()
 
 
-def _quant(p: TurboQuantParams, which: str) -> nat.KV4Quant:
+def _quant(p: TurboQuantParams, which: str) -> tuple[nat.KV4Quant, np.ndarray, np.ndarray]:
+    """-> the rotation, the upper half of the levels, the bounds between them"""
     if p.mode != "mse" or p.bits != 4 or p.rotation != "hadamard" or p.dim != DIM:
         raise ValueError(f"the {which} quantiser must be mode 'mse', 4 bits, rotation 'hadamard', dim {DIM}; got "
                          f"{p.mode!r}, {p.bits}, {p.rotation!r}, {p.dim}")
@@ -49,13 +50,12 @@ def _quant(p: TurboQuantParams, which: str) -> nat.KV4Quant:
     bounds = half * (t["boundaries"][8:] - t["boundaries"][6::-1])
     if np.abs(t["codebook"][8:] - levels).max() > 1e-3:
         raise ValueError(f"the {which} quantiser's codebook is not symmetric")
-    if not (np.diff(levels) > 0).all() or not (np.diff(bounds) > 0).all() or levels[0] < 0 or levels[-1] > 512:
-        raise ValueError(f"the {which} quantiser's levels must ascend from 0 to at most 512")
+    if not (np.diff(levels) > 0).all() or not (np.diff(bounds) > 0).all() or levels[0] < 0 or levels[-1] > 1:
+        raise ValueError(f"the {which} quantiser's levels must ascend between 0 and 1")
     if sorted(t["perm"].tolist()) != list(range(DIM)):
         raise ValueError(f"the {which} quantiser's permutation is none")
     signs = sum(1 << i for i in range(DIM) if t["signs"][i] < 0)
-    return nat.KV4Quant((C.c_float * 8)(*levels), (C.c_float * 7)(*bounds), signs,
-                        (C.c_uint8 * DIM)(*(int(i) for i in t["perm"])))
+    return nat.KV4Quant(signs, (C.c_uint8 * DIM)(*(int(i) for i in t["perm"]))), levels, bounds
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -89,7 +89,9 @@ class PagedKV4Cache:
             raise ValueError(f"num_pages must be positive, got {num_pages}")
         if rope_theta is not None and max_positions < 1:
             raise ValueError(f"max_positions must be positive, got {max_positions}")
-        quants = _quant(key, "key"), _quant(value, "value")
+        (kq, levels, bounds), (vq, *v_book) = _quant(key, "key"), _quant(value, "value")
+        if not (np.array_equal(levels, v_book[0]) and np.array_equal(bounds, v_book[1])):
+            raise ValueError("keys and values must share one codebook")
         nbytes = C.c_size_t()
         if lib.cc2_kv4_page_bytes(page_size, num_heads, C.byref(nbytes)) != 0:
             raise ValueError(lib.cc2_last_error().decode())
@@ -102,7 +104,8 @@ class PagedKV4Cache:
         self.rope = rope_rows(max_positions, rope_theta, self.device) if rope_theta is not None else None
         self._c = nat.KV4Cache(self.pages.data_ptr(), num_pages, page_size, num_heads, NORMS[key.norm_dtype],
                                self.rope.data_ptr() if self.rope is not None else None,
-                               max_positions if self.rope is not None else 0, *quants)
+                               max_positions if self.rope is not None else 0, (C.c_float * 8)(*levels),
+                               (C.c_float * 7)(*bounds), kq, vq)
         self._ref = C.byref(self._c)
         self._lib = lib
         self._plan = (None, 0)  # sizes of the last attention call, bytes of its workspace

@@ -431,8 +431,6 @@ CC2_API int cc2_model_set_kv_quant(cc2_model* m, int layer, const cc2_kvq* key, 
  * value is held as that value, one that is not finite as NaN (the vector
  * reads back as NaN). */
 typedef struct {
-  float levels[8];     /* magnitudes, ascending; the negative half mirrors them */
-  float bounds[7];     /* between them, ascending from above 0, more than 1/60 apart */
   uint64_t signs;      /* bit i: signs_i = -1 */
   uint8_t perm[64];
 } cc2_kv4_quant;
@@ -449,6 +447,8 @@ typedef struct {
   int norm_dtype;         /* 0 float16, 1 bfloat16 */
   const float* rope_cs;   /* (dev) float2 (cos, sin) [rope_len][32], or NULL: keys are not rotated */
   int rope_len;
+  float levels[8];        /* magnitudes, ascending; the negative half mirrors them */
+  float bounds[7];        /* between them, ascending from above 0, more than 1/60 apart */
   cc2_kv4_quant key, value;
 } cc2_kv4_cache;
 

@@ -39,9 +39,8 @@ def unpack(cache, which: int):
     codes = b[..., 512 * which:512 * which + 512].reshape(cache.num_pages, h, ps, 8, 4).long()
     word = codes[..., 0] | codes[..., 1] << 8 | codes[..., 2] << 16 | codes[..., 3] << 24
     at = torch.arange(8)
-    bit = torch.where(at < 4, 8 * at + 7, 8 * (at - 4) + 3)
     mag = (word[..., None] >> (4 * at)) & 7
-    sign = 1 - 2 * ((word[..., None] >> bit) & 1)
+    sign = 1 - 2 * ((word[..., None] >> (4 * at + 3)) & 1)
     raw = b[..., 1024:].reshape(cache.num_pages, h, ps, 2, 2)[..., which, :].contiguous().view(torch.int16).squeeze(-1)
     kind = torch.bfloat16 if cache._c.norm_dtype else torch.float16
     norm = (raw & 0x7FFF).view(kind).double()
@@ -201,6 +200,10 @@ def test_cache_refuses_other_quantisers():
     skew.tensors["codebook"] = skew.tensors["codebook"] + 0.01
     with pytest.raises(ValueError, match="symmetric"):
         PagedKV4Cache(4, 2, key=skew)
+    wide = b()
+    wide.tensors["codebook"], wide.tensors["boundaries"] = wide.tensors["codebook"] * 1.5, wide.tensors["boundaries"] * 1.5
+    with pytest.raises(ValueError, match="share one codebook"):
+        PagedKV4Cache(4, 2, key=wide)
     with pytest.raises(ValueError, match="page_size"):
         PagedKV4Cache(4, 2, page_size=48)
     with pytest.raises(ValueError, match="num_pages"):
