@@ -68,19 +68,18 @@ int make_quant(const cc2_kv4_cache& cache, const cc2_kv4_quant& q, const char* w
   }
   CC2_REQUIRE(met == ~0ull, "%s: a quantiser's perm is no permutation", what);
   for (int i = 0; i < 8; ++i) r.levels[i] = cache.levels[i];
+  for (int j = 0; j < 7; ++j)
+    CC2_REQUIRE(cache.bounds[j] > (j ? cache.bounds[j - 1] : 0.0f) && cache.bounds[j] < 1.0f,
+                "%s: the bounds must ascend between 0 and 1", what);
+  int j = 0;  // bounds below the cell
   for (int c = 0; c < 65; ++c) {
     // |y| / 8n of r = 8c .. 8c + 7, with room for the rounding of r itself
     const float lo = (8 * c - 0.52f) / 512.0f, hi = (8 * c + 7.52f) / 512.0f;
-    r.cells[c].bound = INFINITY;
-    r.cells[c].below = 0;
-    for (int j = 0; j < 7; ++j) {
-      CC2_REQUIRE(cache.bounds[j] > (j ? cache.bounds[j - 1] : 0.0f), "%s: the bounds must ascend from above 0", what);
-      if (cache.bounds[j] <= lo) ++r.cells[c].below;
-      else if (cache.bounds[j] <= hi) {
-        CC2_REQUIRE(r.cells[c].bound == INFINITY, "%s: the bounds must be more than 1/60 apart", what);
-        r.cells[c].bound = cache.bounds[j];
-      }
-    }
+    while (j < 7 && cache.bounds[j] <= lo) ++j;
+    const bool in = j < 7 && cache.bounds[j] <= hi;
+    CC2_REQUIRE(!in || j == 6 || cache.bounds[j + 1] > hi, "%s: the bounds must be more than 1/60 apart", what);
+    r.cells[c].bound = in ? cache.bounds[j] : INFINITY;
+    r.cells[c].below = (uint32_t)j;
   }
   return CC2_OK;
 }

@@ -14,7 +14,6 @@ the device.  A sequence, position, page or length out of range sets bit 8 of ``c
 from __future__ import annotations
 
 import ctypes as C
-from contextlib import nullcontext
 
 import numpy as np
 import torch
@@ -58,9 +57,13 @@ def _quant(p: TurboQuantParams, which: str) -> tuple[nat.KV4Quant, np.ndarray, n
     return nat.KV4Quant(signs, (C.c_uint8 * DIM)(*(int(i) for i in t["perm"]))), levels, bounds
 
 
+_PER = {torch.bfloat16: 7, torch.float32: 3}  # elements of 16 bytes, less one
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(i).cuda_stream in a fraction of its time
+
+
 def _aligned(t: torch.Tensor) -> bool:
-    per = 16 // t.element_size()
-    return (t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0)
+    rows, heads, last = t.stride()
+    return last == 1 and not (rows | heads) & _PER[t.dtype] and not t.data_ptr() & 15
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -111,8 +114,17 @@ class PagedKV4Cache:
         self._plan = (None, 0)  # sizes of the last attention call, bytes of its workspace
 
     # -- arguments ---------------------------------------------------------------------------
-    def _guard(self):
-        return nullcontext() if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
+    # Plain code on purpose: a single-token step's kernels take about as long as these checks.
+    def _call(self, fn, what: str, *args) -> None:
+        """fn(cache, *args, stream) on the cache's device and the caller's current stream."""
+        i = self.device.index
+        if torch._C._cuda_getDevice() == i:
+            status = fn(self._ref, *args, _raw_stream(i))
+        else:
+            with torch.cuda.device(i):
+                status = fn(self._ref, *args, _raw_stream(i))
+        if status:
+            nat.check(status, what)
 
     def _index(self, t: torch.Tensor, what: str, dim: int = 1) -> torch.Tensor:
         if t.device != self.device:
@@ -123,32 +135,36 @@ class PagedKV4Cache:
             if t.dtype != torch.int64:
                 raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
             t = t.to(torch.int32)
-        return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+        return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
 
     def _values(self, t: torch.Tensor, what: str) -> int:
         if t.device != self.device:
             raise RuntimeError(f"{what} must be on {self.device}, got {t.device} (no CPU path)")
         if t.dim() != 3 or t.shape[2] != DIM:
             raise ValueError(f"{what} must be (tokens, heads, {DIM}), got {tuple(t.shape)}")
-        if t.dtype not in _CODES:
+        code = _CODES.get(t.dtype)
+        if code is None:
             raise TypeError(f"{what}: dtype {t.dtype} not supported (bfloat16 / float32)")
-        return _CODES[t.dtype]
+        return code
 
-    def _table(self, block_table: torch.Tensor):
+    def _table(self, block_table: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+        """-> the table, its rows, its columns, elements from row to row"""
         t = self._index(block_table, "block_table", 2)
-        if t.shape[0] < 1 or t.shape[1] < 1:
-            raise ValueError(f"block_table is empty: {tuple(t.shape)}")
-        return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        rows, cols = t.shape
+        if rows < 1 or cols < 1:
+            raise ValueError(f"block_table is empty: {(rows, cols)}")
+        ld = t.stride(0) if rows > 1 else cols
+        if ld < cols:  # rows that overlap (an expanded row)
+            t, ld = t.contiguous(), cols
+        return t, rows, cols, ld
 
-    def _places(self, seq_ids, positions, block_table, tokens: int | None):
+    def _places(self, seq_ids, positions, tokens: int | None):
         seq, pos = self._index(seq_ids, "seq_ids"), self._index(positions, "positions")
-        if seq.shape != pos.shape or (tokens is not None and seq.shape[0] != tokens):
-            raise ValueError(f"seq_ids and positions must name one place for each token, got {seq.shape[0]} and "
-                             f"{pos.shape[0]}" + ("" if tokens is None else f" for {tokens}"))
-        table, ld = self._table(block_table)
-        if ld < table.shape[1] and table.shape[0] > 1:
-            table, ld = table.contiguous(), table.shape[1]
-        return seq, pos, table, ld
+        n = seq.shape[0]
+        if pos.shape[0] != n or (tokens is not None and n != tokens):
+            raise ValueError(f"seq_ids and positions must name one place for each token, got {n} and {pos.shape[0]}"
+                             + ("" if tokens is None else f" for {tokens}"))
+        return seq, pos, n
 
     # -- operators ---------------------------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor, seq_ids: torch.Tensor, positions: torch.Tensor,
@@ -161,7 +177,8 @@ class PagedKV4Cache:
         if self._values(v, "v") != code or v.shape != k.shape or k.shape[1] != self.num_heads:
             raise ValueError(f"k and v must both be (tokens, {self.num_heads}, {DIM}) of one type, got "
                              f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-        seq, pos, table, ld = self._places(seq_ids, positions, block_table, k.shape[0])
+        seq, pos, n = self._places(seq_ids, positions, k.shape[0])
+        table, seqs, _, ld = self._table(block_table)
         mask = None
         if token_mask is not None:
             if token_mask.shape != seq.shape or token_mask.device != self.device:
@@ -169,25 +186,23 @@ class PagedKV4Cache:
             mask = token_mask.view(torch.uint8) if token_mask.dtype == torch.bool else token_mask
             mask = (mask if mask.dtype == torch.uint8 else (mask != 0).view(torch.uint8)).contiguous()
         k, v = _rows(k), _rows(v)
-        with self._guard():
-            nat.check(self._lib.cc2_kv4_append(
-                self._ref, code, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                k.shape[0], seq.data_ptr(), pos.data_ptr(), mask.data_ptr() if mask is not None else None,
-                table.data_ptr(), ld, table.shape[0], torch.cuda.current_stream().cuda_stream), "cc2_kv4_append")
+        self._call(self._lib.cc2_kv4_append, "cc2_kv4_append", code, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                   v.stride(0), v.stride(1), n, seq.data_ptr(), pos.data_ptr(),
+                   None if mask is None else mask.data_ptr(), table.data_ptr(), ld, seqs)
 
     def read(self, seq_ids: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor, *,
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
         """What the entries stand for, dense: (k, v), each (tokens, heads, 64), keys as they were rotated.  Masked
         tokens read like others; skipped ones give zeros."""
-        if dtype not in _CODES:
+        code = _CODES.get(dtype)
+        if code is None:
             raise TypeError(f"dtype {dtype} not supported (bfloat16 / float32)")
-        seq, pos, table, ld = self._places(seq_ids, positions, block_table, None)
-        k = torch.empty(seq.shape[0], self.num_heads, DIM, dtype=dtype, device=self.device)
+        seq, pos, n = self._places(seq_ids, positions, None)
+        table, seqs, _, ld = self._table(block_table)
+        k = torch.empty((n, self.num_heads, DIM), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        with self._guard():
-            nat.check(self._lib.cc2_kv4_read(
-                self._ref, _CODES[dtype], k.data_ptr(), v.data_ptr(), k.shape[0], seq.data_ptr(), pos.data_ptr(),
-                table.data_ptr(), ld, table.shape[0], torch.cuda.current_stream().cuda_stream), "cc2_kv4_read")
+        self._call(self._lib.cc2_kv4_read, "cc2_kv4_read", code, k.data_ptr(), v.data_ptr(), n, seq.data_ptr(),
+                   pos.data_ptr(), table.data_ptr(), ld, seqs)
         return k, v
 
     def attention(self, q: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, *,
@@ -205,55 +220,53 @@ class PagedKV4Cache:
         logarithm of each row's sum of exponentials (-inf for such a row), to join it with attention over other keys."""
         code = self._values(q, "q")
         lens = self._index(seq_lens, "seq_lens")
-        table, ld = self._table(block_table)
-        seqs, total, heads = lens.shape[0], q.shape[0], q.shape[1]
-        if table.shape[0] != seqs:
-            raise ValueError(f"block_table has {table.shape[0]} rows for {seqs} sequences")
+        table, rows, cols, ld = self._table(block_table)
+        total, heads, _ = q.shape
+        seqs = lens.shape[0]
+        if rows != seqs:
+            raise ValueError(f"block_table has {rows} rows for {seqs} sequences")
         if heads == 0 or heads % self.num_heads:
             raise ValueError(f"{heads} query heads are no multiple of the cache's {self.num_heads}")
         if cu_q is None:
             if total % seqs or (max_q is not None and max_q != total // seqs):
                 raise ValueError(f"{total} query rows are no equal shares of {seqs} sequences: give cu_q")
-            max_q = total // seqs
+            max_q, cu = total // seqs, None
         else:
             cu_q = self._index(cu_q, "cu_q")
             if cu_q.shape[0] != seqs + 1:
                 raise ValueError(f"cu_q must have {seqs + 1} entries, got {cu_q.shape[0]}")
-            max_q = total if max_q is None else min(int(max_q), total)
-        room = table.shape[1] * self.page_size
-        max_len = room if max_len is None else min(int(max_len), room)
+            max_q, cu = total if max_q is None or max_q > total else int(max_q), cu_q.data_ptr()
+        room = cols * self.page_size
+        max_len = room if max_len is None or max_len > room else int(max_len)
         if max_q < 0 or max_len < 0:
             raise ValueError("max_q and max_len must not be negative")
         if rotate_q and self.rope is None:
             raise ValueError("the cache was made without a rotation (rope_theta None)")
         q = _rows(q)
         if out is None:
-            out = torch.empty(total, heads, DIM, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif (out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not _aligned(out)
               or any(n > 1 and st < DIM for n, st in zip(out.shape[:2], out.stride()))):
             raise ValueError("out must have q's shape, type and device, its rows apart, dense and on 16-byte boundaries")
-        lse = torch.empty(total, heads, dtype=torch.float32, device=self.device) if return_lse else None
-        with self._guard():
-            sizes = (code, heads, seqs, total, max_q, max_len)
-            if self._plan[0] != sizes:
-                nbytes = C.c_size_t()
-                nat.check(self._lib.cc2_kv4_attention_workspace_bytes(self._ref, *sizes, C.byref(nbytes)),
-                          "cc2_kv4_attention_workspace_bytes")
-                self._plan = (sizes, nbytes.value)
-            need = self._plan[1]
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            nat.check(self._lib.cc2_kv4_attention(
-                self._ref, code, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                heads, seqs, total, cu_q.data_ptr() if cu_q is not None else None, max_q, lens.data_ptr(), max_len,
-                table.data_ptr(), ld, int(causal), float(scale), int(rotate_q),
-                lse.data_ptr() if lse is not None else None, ws.data_ptr() if ws is not None else None, need,
-                torch.cuda.current_stream().cuda_stream), "cc2_kv4_attention")
+        lse = torch.empty((total, heads), dtype=torch.float32, device=self.device) if return_lse else None
+        sizes = (code, heads, seqs, total, max_q, max_len)
+        if self._plan[0] != sizes:
+            nbytes = C.c_size_t()
+            self._call(lambda ref, *a: self._lib.cc2_kv4_attention_workspace_bytes(ref, *a[:-1]),
+                       "cc2_kv4_attention_workspace_bytes", *sizes, C.byref(nbytes))
+            self._plan = (sizes, nbytes.value)
+        need = self._plan[1]
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._call(self._lib.cc2_kv4_attention, "cc2_kv4_attention", code, q.data_ptr(), q.stride(0), q.stride(1),
+                   out.data_ptr(), out.stride(0), out.stride(1), heads, seqs, total, cu, max_q, lens.data_ptr(), max_len,
+                   table.data_ptr(), ld, causal, scale, rotate_q, None if lse is None else lse.data_ptr(),
+                   None if ws is None else ws.data_ptr(), need)
         return (out, lse) if return_lse else out
 
     def check(self) -> None:
         """Wait for the device and raise if a kernel of this library reported an error: for the cache, a sequence,
         position, page or length out of range."""
-        with self._guard():
+        with torch.cuda.device(self.device):
             status = self._lib.cc2_device_status(1)
         if status:
             raise nat.NativeError(f"device status {status}" + (

@@ -466,6 +466,23 @@ class CuteChronos2Model(nn.Module):
         self._tq_state = (eng, layers, stats)
         return self._tq_state
 
+    def kv4_cache(self, num_pages: int, *, layer: int = 0, page_size: int = 64, max_positions: int | None = None,
+                  seed: int = 0, norm_dtype: str = "float16"):
+        """A paged 4-bit K/V cache (:class:`~cutechronos_b200.kvcache.PagedKV4Cache`) for a layer's time attention: its
+        heads and rotation, and the quantisers that ``enable_turboquant_kv(4, key_mode="mse", seed=seed)`` gives that
+        layer."""
+        from .kvcache import PagedKV4Cache
+        from .turboquant import TurboQuantParams
+        cfg = self.config
+        if not 0 <= layer < cfg.num_layers:
+            raise ValueError(f"layer {layer} out of range")
+        key, value = (TurboQuantParams.build(cfg.d_kv, 4, mode="mse", seed=seed + 2 * layer + i, norm_dtype=norm_dtype,
+                                             device="cpu") for i in range(2))
+        tokens = cfg.context_length // cfg.input_patch_size + int(cfg.use_reg_token) + cfg.max_output_patches
+        return PagedKV4Cache(num_pages, cfg.num_heads, page_size=page_size, key=key, value=value,
+                             rope_theta=cfg.rope_theta, max_positions=max_positions or tokens,
+                             device=self._param_device())
+
     def get_tubroquant_summary(self) -> dict[str, Any]:
         """Per-layer statistics of the last forward (model.py:669-688): raw and
         packed bytes of K and V, compression ratio, mean squared and max

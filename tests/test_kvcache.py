@@ -591,3 +591,29 @@ def test_out_of_range_is_skipped_and_reported():
             cache.check()
     cache.attention(q, torch.tensor([48, 16], **dev), table)
     cache.check()
+
+
+@pytest.mark.gpu
+def test_model_cache_and_streaming_example():
+    import importlib.util
+    from pathlib import Path
+
+    from conftest import small_config
+    spec = importlib.util.spec_from_file_location(
+        "streaming_attention", Path(__file__).resolve().parents[1] / "examples" / "streaming_attention.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got = example.main(series=3, context=500, steps=9, page_size=16, layer=1, config=small_config())
+    assert got["output"].shape == got["reference"].shape == (3, 32, 2, 64)
+    # 4 bits leave 0.1 of a vector's norm; averages over keys less, the first tokens' rows most of it
+    assert got["error"] < 0.12 and got["ratio"] > 3.7
+    assert torch.isfinite(got["update"].float()).all()
+
+
+def test_model_cache_refuses_bad_layers():
+    from conftest import small_config
+    from cutechronos_b200.model import CuteChronos2Model
+    with pytest.raises(ValueError, match="layer"):
+        CuteChronos2Model(small_config()).kv4_cache(4, layer=2)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        CuteChronos2Model(small_config()).kv4_cache(4)
