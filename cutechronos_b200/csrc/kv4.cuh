@@ -36,17 +36,21 @@ struct Pool {
   int norm_bf16;   // norms are bf16 (else fp16)
 };
 
-// One quantiser for the kernels that quantise and restore (by value).
-struct Quant {
-  float levels[8];
-  // Element e of a vector is rotated coordinate go[e] & 63, negated if bit 7 is set.
-  uint8_t go[64];
-  // The magnitude by one comparison: r = round(512 |y| / 8n) is in 0..512 (|y| <= 8n), and of the bounds at most one,
-  // `bound`, can lie among the |y| of r / 8's cell; `below` bounds lie under it.
+// One rotation for the kernels that quantise and restore (by value: its entries
+// are operands in constant memory).  Coordinate i of the rotated vector comes
+// from element place[i] / 4, times sign[i].
+struct Turn {
+  uint32_t place[64];
+  float sign[64];
+};
+
+// The magnitude of a coordinate by one comparison: r = round(511 |y| / 8n) is in 0..511 (|y| <= 8n), and of the
+// bounds at most one, `bound`, can lie among the |y| of r / 8's cell; `below` bounds lie under it.
+struct Cells {
   struct Cell {
     float bound;  // +inf: none
     uint32_t below;
-  } cells[65];
+  } of[64];
 };
 
 // The levels as the fp16 decoders take them: 64 c_i split into its fp16 value
@@ -105,7 +109,7 @@ __device__ __forceinline__ void zip(uint32_t a, uint32_t b, uint32_t& u, uint32_
 
 // --- host side --------------------------------------------------------------
 int check_cache(const cc2_kv4_cache* c, const char* what, Pool& pool);
-int make_quant(const cc2_kv4_cache& c, const cc2_kv4_quant& q, const char* what, Quant& r);
+int make_turn(const cc2_kv4_quant& q, const char* what, Turn& t);
 Levels make_levels(const cc2_kv4_cache& c);
 // Device error word of the cache's kernels (DEV_ERR_CACHE_RANGE).
 int error_word(int** p);

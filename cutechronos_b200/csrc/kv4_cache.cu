@@ -8,13 +8,13 @@
 // everything here is laid out to save them:
 //  - four threads bring a vector in (or out), one thread then owns it whole: its
 //    butterflies are register adds, two at a time, with no shuffles;
-//  - sign and permutation are applied where four threads scatter (gather) a row
-//    in shared memory, from 16 places that each thread keeps in registers, so
-//    that the owner reads (writes) its row straight, 16 bytes at a time; a row
-//    pitch of 68 floats keeps that free of bank conflicts;
-//  - a magnitude takes one lookup and one comparison (kv4.cuh, Quant): three
-//    comparisons of a binary search and their selects ran on the half-rate
-//    integer pipe and were its limit;
+//  - sign and permutation are applied by the owner, for whom they are constants
+//    of the launch: an element is one load at a constant place, times +-1 on
+//    the multiply pipe, and rows of 64 floats at a pitch of 65 keep these loads
+//    and the four threads' stores free of bank conflicts;
+//  - a magnitude takes one lookup and one comparison (Cells): three comparisons
+//    of a binary search and their selects ran on the half-rate integer pipe and
+//    were its limit;
 //  - places in the cache, pointers and positions are worked out once a vector.
 #include <algorithm>
 #include <cmath>
@@ -59,36 +59,44 @@ int check_cache(const cc2_kv4_cache* c, const char* what, Pool& pool) {
   return CC2_OK;
 }
 
-int make_quant(const cc2_kv4_cache& cache, const cc2_kv4_quant& q, const char* what, Quant& r) {
+int make_turn(const cc2_kv4_quant& q, const char* what, Turn& t) {
   uint64_t met = 0;
   for (int i = 0; i < 64; ++i) {
-    const int e = q.perm[i] & 63;
+    const uint32_t e = q.perm[i] & 63u;
     met |= 1ull << e;
-    r.go[e] = (uint8_t)(i | (((q.signs >> i) & 1) << 7));
+    t.place[i] = 4 * e;
+    t.sign[i] = (q.signs >> i) & 1 ? -1.0f : 1.0f;
   }
   CC2_REQUIRE(met == ~0ull, "%s: a quantiser's perm is no permutation", what);
-  for (int i = 0; i < 8; ++i) r.levels[i] = cache.levels[i];
-  for (int j = 0; j < 7; ++j)
-    CC2_REQUIRE(cache.bounds[j] > (j ? cache.bounds[j - 1] : 0.0f) && cache.bounds[j] < 1.0f,
-                "%s: the bounds must ascend between 0 and 1", what);
-  int j = 0;  // bounds below the cell
-  for (int c = 0; c < 65; ++c) {
-    // |y| / 8n of r = 8c .. 8c + 7, with room for the rounding of r itself
-    const float lo = (8 * c - 0.52f) / 512.0f, hi = (8 * c + 7.52f) / 512.0f;
-    while (j < 7 && cache.bounds[j] <= lo) ++j;
-    const bool in = j < 7 && cache.bounds[j] <= hi;
-    CC2_REQUIRE(!in || j == 6 || cache.bounds[j + 1] > hi, "%s: the bounds must be more than 1/60 apart", what);
-    r.cells[c].bound = in ? cache.bounds[j] : INFINITY;
-    r.cells[c].below = (uint32_t)j;
-  }
   return CC2_OK;
 }
 
 namespace {
 
+int make_cells(const cc2_kv4_cache& cache, const char* what, Cells& r) {
+  for (int j = 0; j < 7; ++j)
+    CC2_REQUIRE(cache.bounds[j] > (j ? cache.bounds[j - 1] : 0.0f) && cache.bounds[j] < 1.0f,
+                "%s: the bounds must ascend between 0 and 1", what);
+  int j = 0;  // bounds below the cell
+  for (int c = 0; c < 64; ++c) {
+    // |y| / 8n of r = 8c .. 8c + 7, with room for the rounding of r itself
+    const float lo = (8 * c - 0.52f) / 511.0f, hi = (8 * c + 7.52f) / 511.0f;
+    while (j < 7 && cache.bounds[j] <= lo) ++j;
+    const bool in = j < 7 && cache.bounds[j] <= hi;
+    CC2_REQUIRE(!in || j == 6 || cache.bounds[j + 1] > hi, "%s: the bounds must be more than 1/60 apart", what);
+    r.of[c].bound = in ? cache.bounds[j] : INFINITY;
+    r.of[c].below = (uint32_t)j;
+  }
+  return CC2_OK;
+}
+
+}  // namespace
+
+namespace {
+
 constexpr int kThreads = 128;
 constexpr int kUnits = 64;   // (token, head) pairs a block handles: a thread for each K and each V
-constexpr int kPitch = 68;
+constexpr int kPitch = 65;
 
 struct Places {
   const int32_t* seq;
@@ -176,22 +184,6 @@ __device__ __forceinline__ void walsh(float (&y)[64]) {
   for (int i = 0; i < 32; ++i) f2_unpack(p[i], y[2 * i], y[2 * i + 1]);
 }
 
-// The 16 places of a thread's elements 8c .. 8c + 7 and 32 + 8c .. in a rotated row: byte offsets, signs in bit 31.
-__device__ __forceinline__ void my_places(const Quant& q, int c, uint32_t (&to)[16]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint2 w = *reinterpret_cast<const uint2*>(q.go + 32 * h + 8 * c);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t b = ((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu;
-      to[8 * h + j] = (b & 63u) * 4u | (b & 128u) << 24;
-    }
-  }
-}
-__device__ __forceinline__ float flip(float x, uint32_t to) {
-  return __uint_as_float(__float_as_uint(x) ^ (to & 0x80000000u));
-}
-
 // What a block knows of its units.
 struct Unit {
   long long block;   // byte offset of the unit's block of 16 tokens, -1: skip
@@ -199,38 +191,59 @@ struct Unit {
   int slot;          // place in the block of 16; bit 8: masked
 };
 
+// A block's 64 units, neighbours in (token, head) order.
+struct Units {
+  int t0, h0, heads, last;  // last: the last unit that there is
+  __device__ __forceinline__ Units(int tokens, int heads_) : heads(heads_) {
+    const long long u0 = (long long)blockIdx.x * kUnits;
+    t0 = (int)(u0 / heads);
+    h0 = (int)(u0 % heads);
+    last = (int)min((long long)tokens * heads - u0, (long long)kUnits) - 1;
+  }
+  // token and head of unit r; false past the end (then the last one's)
+  __device__ __forceinline__ bool find(int r, int& t, int& h) const {
+    const unsigned x = (unsigned)(h0 + min(r, last)), dt = x / (unsigned)heads;
+    h = (int)(x - dt * (unsigned)heads);
+    t = t0 + (int)dt;
+    return r <= last;
+  }
+};
+
+// An owner's row: at constant places, times constant signs.
+__device__ __forceinline__ void take_row(const float* row, const Turn& turn, float (&y)[64]) {
+#pragma unroll
+  for (int i = 0; i < 64; ++i)
+    y[i] = __fmul_rn(*reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(row) + turn.place[i]), turn.sign[i]);
+}
+
 template <typename T, bool kRope>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4)
-append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant qk, const __grid_constant__ Quant qv,
-              const T* __restrict__ k, long long k_ld, long long k_hs, const T* __restrict__ v, long long v_ld,
-              long long v_hs, int tokens, Places at, const uint8_t* __restrict__ mask,
-              const float2* __restrict__ rope, int rope_len, int* __restrict__ err) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 5)
+append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn_k, const __grid_constant__ Turn turn_v,
+              const __grid_constant__ Cells table, const T* __restrict__ k, long long k_ld, long long k_hs,
+              const T* __restrict__ v, long long v_ld, long long v_hs, int tokens, Places at,
+              const uint8_t* __restrict__ mask, const float2* __restrict__ rope, int rope_len, int* __restrict__ err) {
   pdl_launch_dependents();
   __shared__ __align__(16) float rows[2 * kUnits * kPitch];
   __shared__ float norm[2 * kUnits];
-  __shared__ Quant::Cell cells[2][128];  // 65 used; a NaN may point at any
+  __shared__ Cells::Cell cells[64];
   __shared__ Unit units[kUnits];
   constexpr int kIts = kUnits * 4 / kThreads;
   const int tid = threadIdx.x;
-  cells[0][tid] = qk.cells[min(tid, 64)];
-  cells[1][tid] = qv.cells[min(tid, 64)];
+  if (tid < 64) cells[tid] = table.of[tid];
   pdl_wait();
-  const long long total = (long long)tokens * pool.heads;
-  const long long u0 = (long long)blockIdx.x * kUnits;
-  const int t0 = (int)(u0 / pool.heads), h0 = (int)(u0 % pool.heads);
-  const int last = (int)min(total - u0, (long long)kUnits) - 1;  // units past it read the last one's rows
+  const Units my(tokens, pool.heads);
 
   // four threads bring a vector in: thread c its values 8c .. 8c+7 and 32 + 8c ..
   const int c = tid & 3;
   Raw<T> raw[2][kIts][2];
 #pragma unroll
   for (int it = 0; it < kIts; ++it) {
-    const unsigned x = (unsigned)(h0 + min(it * (kThreads / 4) + (tid >> 2), last));
-    const unsigned dt = x / (unsigned)pool.heads, h = x - dt * (unsigned)pool.heads;
-    const T* from = k + (long long)(t0 + dt) * k_ld + (long long)h * k_hs + 8 * c;
+    int t, h;
+    my.find(it * (kThreads / 4) + (tid >> 2), t, h);
+    const T* from = k + (long long)t * k_ld + (long long)h * k_hs + 8 * c;
     raw[0][it][0].load(from);
     raw[0][it][1].load(from + 32);
-    from = v + (long long)(t0 + dt) * v_ld + (long long)h * v_hs + 8 * c;
+    from = v + (long long)t * v_ld + (long long)h * v_hs + 8 * c;
     raw[1][it][0].load(from);
     raw[1][it][1].load(from + 32);
   }
@@ -239,11 +252,10 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant q
     u.block = -1;
     u.pos = 0;
     u.slot = 0;
-    if (tid <= last) {
-      const unsigned x = (unsigned)(h0 + tid), dt = x / (unsigned)pool.heads, h = x - dt * (unsigned)pool.heads;
-      const int t = t0 + (int)dt;
+    int t, h;
+    if (my.find(tid, t, h)) {
       int off = 0;
-      u.block = place(pool, at, t, (int)h, kRope ? rope_len : 0x7fffffff, &off, err);
+      u.block = place(pool, at, t, h, kRope ? rope_len : 0x7fffffff, &off, err);
       u.slot = (off & (kBlockTokens - 1)) | (mask != nullptr && mask[t] == 0 ? 256 : 0);
       if (kRope && u.block >= 0) u.pos = at.pos[t];
     }
@@ -253,8 +265,6 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant q
 
 #pragma unroll
   for (int is_v = 1; is_v >= 0; --is_v) {
-    uint32_t to[16];
-    my_places(is_v ? qv : qk, c, to);
 #pragma unroll
     for (int it = 0; it < kIts; ++it) {
       const int r = it * (kThreads / 4) + (tid >> 2);
@@ -288,11 +298,11 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant q
 #pragma unroll
         for (int j = 0; j < o; ++j) s[j] = __fadd_rn(s[j], s[j + o]);
       }
-      uint8_t* row = reinterpret_cast<uint8_t*>(rows + (is_v * kUnits + r) * kPitch);
+      float* row = rows + (is_v * kUnits + r) * kPitch + 8 * c;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        *reinterpret_cast<float*>(row + (to[j] & 0xffu)) = flip(a[j], to[j]);
-        *reinterpret_cast<float*>(row + (to[8 + j] & 0xffu)) = flip(b[j], to[8 + j]);
+        row[j] = a[j];
+        row[32 + j] = b[j];
       }
       if (c == 0) norm[is_v * kUnits + r] = __fsqrt_rn(s[0]);
     }
@@ -303,16 +313,13 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant q
   const Unit& u = units[tid & (kUnits - 1)];
   if (u.block < 0) return;
   float y[64];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float4 f = *reinterpret_cast<const float4*>(rows + tid * kPitch + 4 * i);
-    y[4 * i] = f.x, y[4 * i + 1] = f.y, y[4 * i + 2] = f.z, y[4 * i + 3] = f.w;
-  }
+  if (is_v) take_row(rows + tid * kPitch, turn_v, y);  // two copies, each with its own constants
+  else take_row(rows + tid * kPitch, turn_k, y);
   walsh(y);
   const float n = norm[tid];
   const float n8 = __fmul_rn(n, 8.0f);
-  const float fine = n8 > 0.0f ? __fdividef(512.0f, n8) : 0.0f;  // its error is within the cells' room
-  const uint8_t* table = reinterpret_cast<const uint8_t*>(cells[is_v]);
+  const float fine = n8 > 0.0f ? __fdividef(511.0f, n8) : 0.0f;  // its error is within the cells' room
+  const uint8_t* entries = reinterpret_cast<const uint8_t*>(cells);
   uint32_t word[8];
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
@@ -320,9 +327,9 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant q
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       const float x = y[8 * w + p], a = fabsf(x);
-      // r in the low bits of 2^23 + r; its cell's entry
-      const uint32_t r = __float_as_uint(fmaf(a, fine, 8388608.0f)) & 0x3f8u;
-      const Quant::Cell cell = *reinterpret_cast<const Quant::Cell*>(table + r);
+      // r in the low bits of 2^23 + r: its cell's entry (a NaN points at one of them too)
+      const uint32_t r = __float_as_uint(fmaf(a, fine, 8388608.0f)) & 0x1f8u;
+      const Cells::Cell cell = *reinterpret_cast<const Cells::Cell*>(entries + r);
       code += cell.below * (1u << (4 * p));
       if (a > __fmul_rn(cell.bound, n8)) code += 1u << (4 * p);
       if (x < 0.0f) code |= 1u << sign_bit(p);
@@ -340,27 +347,27 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant q
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant qk, const __grid_constant__ Quant qv,
-            T* __restrict__ k_out, T* __restrict__ v_out, int tokens, Places at, int* __restrict__ err) {
+__global__ void __launch_bounds__(kThreads, 6)
+read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn_k, const __grid_constant__ Turn turn_v,
+            const float4 levels_lo, const float4 levels_hi, T* __restrict__ k_out, T* __restrict__ v_out, int tokens,
+            Places at, int* __restrict__ err) {
   pdl_launch_dependents();
-  pdl_wait();
   __shared__ __align__(16) float rows[2 * kUnits * kPitch];
-  __shared__ float scale[2 * kUnits];
-  __shared__ float level[2][8];
+  __shared__ __align__(16) float level[8];
   const int tid = threadIdx.x;
-  const long long total = (long long)tokens * pool.heads;
-  const long long u0 = (long long)blockIdx.x * kUnits;
-  if (tid < 16) level[tid >> 3][tid & 7] = (tid >> 3 ? qv : qk).levels[tid & 7];
+  if (tid == 0) {
+    reinterpret_cast<float4*>(level)[0] = levels_lo;
+    reinterpret_cast<float4*>(level)[1] = levels_hi;
+  }
+  pdl_wait();
   __syncthreads();
+  const Units my(tokens, pool.heads);
   {
     const bool is_v = tid >= kUnits;
-    const long long u = u0 + (tid & (kUnits - 1));
-    int off = 0;
+    int off = 0, t, h;
     long long at_block = -1;
-    if (u < total && (is_v ? v_out : k_out) != nullptr)
-      at_block = place(pool, at, (int)(u / pool.heads), (int)(u % pool.heads), 0x7fffffff, &off, err);
-    float4* row = reinterpret_cast<float4*>(rows + tid * kPitch);
+    if (my.find(tid & (kUnits - 1), t, h) && (is_v ? v_out : k_out) != nullptr)
+      at_block = place(pool, at, t, h, 0x7fffffff, &off, err);
     float f = 0.0f;
     float y[64];
 #pragma unroll
@@ -372,21 +379,26 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant qk,
       const uint4 w0 = codes[0], w1 = codes[1];
       const uint32_t word[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
       f = 0.125f * norm_value(reinterpret_cast<const uint16_t*>(block + kNorms)[2 * slot + is_v], pool.norm_bf16);
-      const uint8_t* lv = reinterpret_cast<const uint8_t*>(level[is_v]);
 #pragma unroll
       for (int i = 0; i < 64; ++i) {
         const uint32_t w = word[i >> 3];
-        constexpr int kByte = 2;  // log2 of a level's bytes
         const int p = i & 7;
-        const uint32_t sel = (p ? w >> (4 * p - kByte) : w << kByte) & (7u << kByte);
-        const float x = *reinterpret_cast<const float*>(lv + sel);
+        const uint32_t sel = (p ? w >> (4 * p - 2) : w << 2) & 28u;  // a level's byte offset
+        const float x = *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(level) + sel);
         y[i] = __uint_as_float(__float_as_uint(x) ^ ((w << (31 - sign_bit(p))) & 0x80000000u));
       }
       walsh(y);
     }
+    uint8_t* row = reinterpret_cast<uint8_t*>(rows + tid * kPitch);
+    if (is_v) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) row[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-    scale[tid] = f;
+      for (int i = 0; i < 64; ++i)
+        *reinterpret_cast<float*>(row + turn_v.place[i]) = __fmul_rn(__fmul_rn(y[i], f), turn_v.sign[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 64; ++i)
+        *reinterpret_cast<float*>(row + turn_k.place[i]) = __fmul_rn(__fmul_rn(y[i], f), turn_k.sign[i]);
+    }
   }
   __syncthreads();
   const int c = tid & 3;
@@ -394,22 +406,21 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Quant qk,
   for (int is_v = 0; is_v < 2; ++is_v) {
     T* out = is_v ? v_out : k_out;
     if (out == nullptr) continue;
-    uint32_t from[16];
-    my_places(is_v ? qv : qk, c, from);
 #pragma unroll
     for (int it = 0; it < kUnits * 4 / kThreads; ++it) {
       const int r = it * (kThreads / 4) + (tid >> 2);
-      if (u0 + r >= total) continue;
-      const uint8_t* row = reinterpret_cast<const uint8_t*>(rows + (is_v * kUnits + r) * kPitch);
-      const float f = scale[is_v * kUnits + r];
+      int t, h;
+      if (!my.find(r, t, h)) continue;
+      const float* row = rows + (is_v * kUnits + r) * kPitch + 8 * c;
       float a[8], b[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        a[j] = flip(__fmul_rn(*reinterpret_cast<const float*>(row + (from[j] & 0xffu)), f), from[j]);
-        b[j] = flip(__fmul_rn(*reinterpret_cast<const float*>(row + (from[8 + j] & 0xffu)), f), from[8 + j]);
+        a[j] = row[j];
+        b[j] = row[32 + j];
       }
-      store8(out + (u0 + r) * 64 + 8 * c, a);
-      store8(out + (u0 + r) * 64 + 32 + 8 * c, b);
+      T* to = out + ((long long)t * pool.heads + h) * 64 + 8 * c;
+      store8(to, a);
+      store8(to + 32, b);
     }
   }
 }
@@ -428,7 +439,7 @@ bool rows_ok(int dtype, const void* p, int64_t ld, int64_t hs) {
 
 int grid_of(int T, int heads, int* grid) {
   const long long blocks = ((long long)T * heads + kUnits - 1) / kUnits;
-  CC2_REQUIRE(blocks <= 0x7fffffffLL, "kv4: too many tokens for one call");
+  CC2_REQUIRE(blocks <= 0x1fffffffLL, "kv4: too many tokens for one call");
   *grid = (int)blocks;
   return CC2_OK;
 }
@@ -460,13 +471,15 @@ int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int6
   int grid = 0, *err = nullptr;
   CC2_TRY(grid_of(T, pool.heads, &grid));
   CC2_TRY(error_word(&err));
-  Quant qk, qv;
-  CC2_TRY(make_quant(*cache, cache->key, "kv4_append", qk));
-  CC2_TRY(make_quant(*cache, cache->value, "kv4_append", qv));
+  Turn turn_k, turn_v;
+  Cells cells;
+  CC2_TRY(make_turn(cache->key, "kv4_append", turn_k));
+  CC2_TRY(make_turn(cache->value, "kv4_append", turn_v));
+  CC2_TRY(make_cells(*cache, "kv4_append", cells));
   const Places at{seq, pos, table, table_ld, num_seqs};
   const float2* rope = (const float2*)cache->rope_cs;
 #define CC2_APPEND(TT, ROPE)                                                                                        \
-  CC2_CUDA(launch_k(append_kernel<TT, ROPE>, grid, kThreads, 0, st, pool, qk, qv, (const TT*)k, (long long)k_ld,    \
+  CC2_CUDA(launch_k(append_kernel<TT, ROPE>, grid, kThreads, 0, st, pool, turn_k, turn_v, cells, (const TT*)k, (long long)k_ld,    \
                     (long long)k_hs, (const TT*)v, (long long)v_ld, (long long)v_hs, T, at, mask, rope,             \
                     cache->rope_len, err))
   if (dtype == CC2_BF16) {
@@ -491,15 +504,18 @@ int launch_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_
   int grid = 0, *err = nullptr;
   CC2_TRY(grid_of(T, pool.heads, &grid));
   CC2_TRY(error_word(&err));
-  Quant qk, qv;
-  CC2_TRY(make_quant(*cache, cache->key, "kv4_read", qk));
-  CC2_TRY(make_quant(*cache, cache->value, "kv4_read", qv));
+  Turn turn_k, turn_v;
+  CC2_TRY(make_turn(cache->key, "kv4_read", turn_k));
+  CC2_TRY(make_turn(cache->value, "kv4_read", turn_v));
+  const float* lv = cache->levels;
+  const float4 lo = make_float4(lv[0], lv[1], lv[2], lv[3]), hi = make_float4(lv[4], lv[5], lv[6], lv[7]);
   const Places at{seq, pos, table, table_ld, num_seqs};
   if (dtype == CC2_BF16) {
-    CC2_CUDA(launch_k(read_kernel<__nv_bfloat16>, grid, kThreads, 0, st, pool, qk, qv, (__nv_bfloat16*)k_out,
-                      (__nv_bfloat16*)v_out, T, at, err));
+    CC2_CUDA(launch_k(read_kernel<__nv_bfloat16>, grid, kThreads, 0, st, pool, turn_k, turn_v, lo, hi,
+                      (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, T, at, err));
   } else {
-    CC2_CUDA(launch_k(read_kernel<float>, grid, kThreads, 0, st, pool, qk, qv, (float*)k_out, (float*)v_out, T, at, err));
+    CC2_CUDA(launch_k(read_kernel<float>, grid, kThreads, 0, st, pool, turn_k, turn_v, lo, hi, (float*)k_out,
+                      (float*)v_out, T, at, err));
   }
   CC2_CHECK_LAUNCH();
   return CC2_OK;
