@@ -37,16 +37,16 @@ namespace {
 
 using namespace tcx;
 
-constexpr int kThreads = 896;
+constexpr int kThreads = 1024;
 constexpr int kSoftmaxWarp = 4, kDecodeWarp = 20, kOutWarp = 24;
 constexpr int kTile = 128;                      // rows of a pipeline, keys of a block
 constexpr uint32_t kTileBytes = 128 * 128;      // 128 rows of 64 fp16
 constexpr uint32_t kRawBytes = 8 * kBlockBytes;
-constexpr int kKvStages = 3, kRawStages = 3, kItems = 4;
-constexpr int kSumPitch = 65 * 4, kOutPitch = 132;  // bytes of a row's staged sums, of its staged output
+constexpr int kKvStages = 3, kRawStages = 2, kItems = 4;
+constexpr int kSumPitch = 68 * 4;  // bytes of a row's staged sums
 constexpr uint32_t kQAt = 0, kKvAt = 2 * kTileBytes, kRawAt = kKvAt + kKvStages * 2 * kTileBytes,
-                   kSumAt = kRawAt + kRawStages * kRawBytes, kOutAt = kSumAt + 128 * kSumPitch,
-                   kSmem = kOutAt + 128 * kOutPitch;
+                   kSumAt = kRawAt + kRawStages * kRawBytes,
+                   kSmem = kSumAt + 256 * kSumPitch;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kStep = 64;                       // keys of a step of the softmax
 // TMEM columns of tile g, chain c: S (and P over it) at 128 g + 64 c, O at 256 + 128 g + 64 c
@@ -70,6 +70,7 @@ struct Item {
   int head, row0, rows, q_start, n, len, split, chunks;
   int c0, c1;    // keys of the chunk that some row of the item sees
   int blocks[2], key_end[2];
+  int lane0[2];  // TMEM lane of a tile's first row
   long long q_tile;
 };
 
@@ -90,7 +91,6 @@ struct Control {
   float m[2][2][2][128], l[2][2][2][128];  // [turn][tile][chain][row]
   int ve[2][2][2];
   uint32_t top[2][4];
-  uint32_t turn_out[64];                // byte offset in an output row of rotated coordinate i, its sign in bit 31
   uint32_t tmem;
   int abort_flag;
 };
@@ -140,9 +140,9 @@ __device__ __forceinline__ uint32_t visible(uint32_t seen, int limit) {
   return limit >= 32 ? seen : limit <= 0 ? 0u : seen & ((1u << limit) - 1u);
 }
 // Scores of keys that the row does not see.
-__device__ __forceinline__ void hide(uint32_t (&v)[32], uint32_t vis) {
+__device__ __forceinline__ void hide(uint32_t (&v)[16], uint32_t vis) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
+  for (int i = 0; i < 16; ++i)
     if (!((vis >> i) & 1u)) v[i] = 0xff800000u;
 }
 
@@ -195,17 +195,15 @@ __device__ __forceinline__ QueryRow find_row(const Args& a, int tok, int lane) {
 }
 
 __global__ void __launch_bounds__(kQThreads)
-rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles) {
+rotate_queries_kernel(const __grid_constant__ Args a, const __grid_constant__ Turn turn, const long long q_tiles) {
   pdl_launch_dependents();
   pdl_wait();
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.counter = 0;  // for the kernel after this one
-  __shared__ float rows[128 * kQPitch];
+  __shared__ __align__(16) float rows[128 * kQPitch];
   const int tid = threadIdx.x, lane = tid & 31;
   const int head = blockIdx.y, base = blockIdx.x * 128, all = a.total_q * a.group;
   __shared__ const __nv_bfloat16* row_at[128];
   __shared__ int row_pos[128];
-  __shared__ uint32_t turn_in[64];  // rotated coordinate i: byte offset of the one it comes from, its sign in bit 31
-  if (tid < 64) turn_in[tid] = 4u * a.rk.perm[tid] | ((a.rk.signs[tid >> 5] >> (tid & 31)) & 1u) << 31;
   // this thread's row: a block's rows mostly belong to one sequence, the others follow it
   const QueryRow at = find_row(a, base / a.group, lane);
   const int row = base + tid;
@@ -235,32 +233,37 @@ rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles) {
   row_at[tid] = from;
   row_pos[tid] = pos;
   __syncthreads();
+  const int c = tid & 3;
+  uint4 lo[4], hi[4];
 #pragma unroll
   for (int it = 0; it < 4; ++it) {
-    const int r = it * 32 + (tid >> 2), c = tid & 3, p = row_pos[r];
-    const __nv_bfloat16* q = row_at[r];
-    float x[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+    const __nv_bfloat16* q = row_at[it * 32 + (tid >> 2)];
+    lo[it] = hi[it] = make_uint4(0, 0, 0, 0);
     if (q != nullptr) {
-      const uint4 u = *reinterpret_cast<const uint4*>(q + 8 * c), v = *reinterpret_cast<const uint4*>(q + 8 * c + 32);
-      const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      lo[it] = *reinterpret_cast<const uint4*>(q + 8 * c);
+      hi[it] = *reinterpret_cast<const uint4*>(q + 8 * c + 32);
+    }
+  }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[2 * j] = __uint_as_float(w[j] << 16);
-        x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      }
-      if (p >= 0) {
-        const float4* cs = reinterpret_cast<const float4*>(a.rope + (long long)p * 32 + 8 * c);
+  for (int it = 0; it < 4; ++it) {
+    const int r = it * 32 + (tid >> 2), p = row_pos[r];
+    float x[16];
+    const uint32_t w[8] = {lo[it].x, lo[it].y, lo[it].z, lo[it].w, hi[it].x, hi[it].y, hi[it].z, hi[it].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 f = cs[j];
-          const float p0 = x[2 * j], q0 = x[8 + 2 * j], p1 = x[2 * j + 1], q1 = x[9 + 2 * j];
-          x[2 * j] = p0 * f.x - q0 * f.y;
-          x[8 + 2 * j] = q0 * f.x + p0 * f.y;
-          x[2 * j + 1] = p1 * f.z - q1 * f.w;
-          x[9 + 2 * j] = q1 * f.z + p1 * f.w;
-        }
+    for (int j = 0; j < 8; ++j) {
+      x[2 * j] = __uint_as_float(w[j] << 16);
+      x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+    if (p >= 0) {
+      const float4* cs = reinterpret_cast<const float4*>(a.rope + (long long)p * 32 + 8 * c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 f = cs[j];
+        const float p0 = x[2 * j], q0 = x[8 + 2 * j], p1 = x[2 * j + 1], q1 = x[9 + 2 * j];
+        x[2 * j] = p0 * f.x - q0 * f.y;
+        x[8 + 2 * j] = q0 * f.x + p0 * f.y;
+        x[2 * j + 1] = p1 * f.z - q1 * f.w;
+        x[9 + 2 * j] = q1 * f.z + p1 * f.w;
       }
     }
 #pragma unroll
@@ -270,13 +273,10 @@ rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles) {
     }
   }
   __syncthreads();
-  if (to < 0) return;
   float y[64];
 #pragma unroll
   for (int i = 0; i < 64; ++i) {
-    const uint32_t t = turn_in[i];
-    const uint32_t x = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(rows + tid * kQPitch) + (t & 0xffu));
-    y[i] = __uint_as_float(x ^ (t & 0x80000000u));
+    y[i] = turn.sign[i] * *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(rows + tid * kQPitch) + turn.place[i]);
   }
   walsh(y);
   float top = 0.0f;
@@ -286,17 +286,30 @@ rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles) {
   const int e = min(max((int)(__float_as_uint(top * fabsf(by)) >> 23), 30), 254);
   const float up = by * __int_as_float((261 - e) << 23);  // 2^(134 - e): the row below 2^8
   const int r = in_seq & 127;
-  uint8_t* dst = const_cast<uint8_t*>(a.qt) + to * kTileBytes + r * 128;
+  // a warp's rows go out as whole lines (a thread's 16-byte pieces of its own row would touch 32 lines each time):
+  // through the warp's part of `rows`, 144 bytes a row, pieces exchanged within 8 rows as the tensor core reads them
+  __syncwarp();
+  uint8_t* stage = reinterpret_cast<uint8_t*>(rows + (tid - lane) * kQPitch);
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {  // 16-byte pieces, exchanged within 8 rows as the tensor core reads them
+  for (int c = 0; c < 8; ++c) {
     uint4 w;
     w.x = pack_half(y[8 * c] * up, y[8 * c + 1] * up);
     w.y = pack_half(y[8 * c + 2] * up, y[8 * c + 3] * up);
     w.z = pack_half(y[8 * c + 4] * up, y[8 * c + 5] * up);
     w.w = pack_half(y[8 * c + 6] * up, y[8 * c + 7] * up);
-    *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) = w;
+    *reinterpret_cast<uint4*>(stage + lane * 144 + ((c ^ (r & 7)) << 4)) = w;
   }
-  const_cast<float*>(a.q_scale)[to * 128 + r] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64
+  if (to >= 0) const_cast<float*>(a.q_scale)[to * 128 + r] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64
+  const unsigned long long mine =
+      to < 0 ? 0ull : (unsigned long long)(const_cast<uint8_t*>(a.qt) + to * kTileBytes + r * 128);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int k = 4 * i + (lane >> 3);
+    uint8_t* dst = (uint8_t*)__shfl_sync(0xffffffffu, mine, k);
+    const uint4 w = *reinterpret_cast<const uint4*>(stage + k * 144 + 16 * (lane & 7));
+    if (dst != nullptr) *reinterpret_cast<uint4*>(dst + 16 * (lane & 7)) = w;
+  }
 }
 
 // ---------------------------------------------------------------- attention --
@@ -311,7 +324,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
   pdl_launch_dependents();
 
   if (tid == 0) {
-    for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&ctl.item_full[i]), 1), mbar_init(smem_u32(&ctl.item_empty[i]), 27);
+    for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&ctl.item_full[i]), 1), mbar_init(smem_u32(&ctl.item_empty[i]), 31);
     for (int i = 0; i < kRawStages; ++i) mbar_init(smem_u32(&ctl.raw_full[i]), 1), mbar_init(smem_u32(&ctl.raw_empty[i]), 4);
     for (int i = 0; i < kKvStages; ++i) mbar_init(smem_u32(&ctl.kv_full[i]), 4), mbar_init(smem_u32(&ctl.kv_empty[i]), 2 + 16);
     for (int g = 0; g < 2; ++g) {
@@ -328,7 +341,6 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
     ctl.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (tid < 64) ctl.turn_out[tid] = 2u * a.rv.perm[tid] | ((a.rv.signs[tid >> 5] >> (tid & 31)) & 1u) << 31;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)),
                  "r"(kTmemCols)
@@ -341,6 +353,8 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
   pdl_wait();
   const uint32_t tmem = ctl.tmem;
 
+  if (warp < kSoftmaxWarp) {
+    
   if (warp == 0) {
     // ---------------- loader ----------------
     Ring<kItems> it;
@@ -399,6 +413,13 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
           break;
         }
         if (lane == src) {
+          // A scheduler has one quarter of the lanes of both tiles: a tile that leaves quarters unused starts in
+          // another one each time, so that short tiles do not all fall to the first.
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int used = (min(d.rows - d.row0 - kTile * g, kTile) + 31) / 32, n = (int)n_items;
+            d.lane0[g] = used > 3 ? 0 : used == 3 ? 32 * (n & 1) : used == 2 ? 64 * (n & 1) : 32 * (n & 3);
+          }
           ctl.items[it.i] = d;
           if (!any_left) ctl.items[it.i].seq = -1;
         }
@@ -464,7 +485,8 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
     while (ok) {
       if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
       const Item& e = ctl.items[it.i];
-      const int seq = e.seq, rows = e.rows - e.row0, blocks[2] = {e.blocks[0], e.blocks[1]};
+      const int seq = e.seq, rows = e.rows - e.row0, blocks[2] = {e.blocks[0], e.blocks[1]},
+                lane0[2] = {e.lane0[0], e.lane0[1]};
       const long long q_tile = e.q_tile;
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
@@ -478,7 +500,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         if (lane == 0) {  // the tile's rows, in groups of 8
           const uint32_t bytes = (uint32_t)min((rows - kTile * g + 7) / 8, kTile / 8) * 1024u;
           mbar_arrive_expect_tx(smem_u32(&ctl.q_full[g]), bytes);
-          bulk_load(smem + kQAt + g * kTileBytes, a.qt + (q_tile + g) * kTileBytes, bytes, smem_u32(&ctl.q_full[g]));
+          bulk_load(smem + kQAt + g * kTileBytes + lane0[g] * 128, a.qt + (q_tile + g) * kTileBytes, bytes, smem_u32(&ctl.q_full[g]));
         }
         __syncwarp();
         ++nq[g];
@@ -580,7 +602,9 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
       }
     }
     __syncwarp();
+  }
   } else if (warp >= kDecodeWarp && warp < kOutWarp) {
+    
     // ---------------- decoders ----------------
     Ring<kItems> it;
     Ring<kRawStages> raw;
@@ -670,6 +694,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
       }
     }
   } else if (warp < kDecodeWarp) {
+    
     // ---------------- softmax: chain c of tile g ----------------
     const int g = (warp - kSoftmaxWarp) >> 3, c = ((warp - kSoftmaxWarp) >> 2) & 1, quarter = warp & 3,
               r = 32 * quarter + lane;
@@ -683,13 +708,13 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
       if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
       const Item& in = ctl.items[it.i];
       const int seq = in.seq, c0 = in.c0, blocks = in.blocks[g], all = max(in.blocks[0], in.blocks[1]);
-      const int row = in.row0 + kTile * g + r;
-      const bool warp_rows = row - lane < in.rows;
+      const int lane0 = in.lane0[g], at = r - lane0, row = in.row0 + kTile * g + at;
+      const bool warp_rows = 32 * quarter >= lane0 && row - lane < in.rows;
       const int limit = a.causal ? min(in.len - in.n + row / a.group + 1, in.len) : in.len;  // keys the row sees
       const int clear = a.causal ? in.len - in.n + (in.row0 + kTile * g) / a.group + 1 : in.len;
       const int keys = in.key_end[g] - c0, steps = blocks > 0 ? (keys + kStep - 1) / kStep : 0;
-      const float* q_scale = a.q_scale + (in.q_tile + g) * 128 + r;
-      const bool valid = row < in.rows && blocks > 0;
+      const float* q_scale = a.q_scale + (in.q_tile + g) * 128 + at;
+      const bool valid = at >= 0 && row < in.rows && blocks > 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
       it.next();
@@ -726,6 +751,23 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         if (warp_rows) {
           // two passes over S, 32 scores in registers at a time: 64 would spill
           const bool two = cols > 32;
+          if (!clean) {  // first the scores of keys that the row does not see, in place
+            uint32_t vis[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              vis[h] = visible(note.seen[h], limit - key0 - 32 * h);
+              if (note.poison[h] & vis[h]) l = __int_as_float(0x7fffffff);
+            }
+#pragma unroll 1
+            for (int i = 0; i < (two ? 4 : 2); ++i) {
+              uint32_t v[16];
+              tmem_ld16(t_s + 16u * i, v);
+              tmem_ld_wait();
+              hide(v, (i < 2 ? vis[0] : vis[1]) >> (16 * (i & 1)));
+              tmem_st16(t_s + 16u * i, v);
+            }
+            tmem_st_wait();
+          }
           float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -733,11 +775,6 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
             uint32_t v[32];
             tmem_ld32(t_s + 32u * h, v);
             tmem_ld_wait();
-            if (!clean) {
-              const uint32_t vis = visible(h ? note.seen[1] : note.seen[0], limit - key0 - 32 * h);
-              if ((h ? note.poison[1] : note.poison[0]) & vis) l = __int_as_float(0x7fffffff);
-              hide(v, vis);
-            }
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               b0 = max3(b0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
@@ -769,7 +806,6 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
             uint32_t v[32];
             tmem_ld32(t_s + 32u * h, v);
             tmem_ld_wait();
-            if (!clean) hide(v, visible(h ? note.seen[1] : note.seen[0], limit - key0 - 32 * h));
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), sc2, off2);
@@ -805,7 +841,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
           const int turn = (int)(nt & 1u);
           ctl.m[turn][g][c][r] = m;
           ctl.l[turn][g][c][r] = l;
-          if (r == 0) ctl.ve[turn][g][c] = ve;
+          if (at == 0) ctl.ve[turn][g][c] = ve;
         }
         tmem_st_wait();
         tc_fence_before();
@@ -818,83 +854,81 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
     }
   } else {
     // ---------------- output ----------------
-    const int quarter = warp & 3, r = 32 * quarter + lane;
-    const uint32_t t_lane = tmem + ((uint32_t)(32 * quarter) << 16);
+    const int g = (warp - kOutWarp) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
+    const uint32_t t_o = tmem + ((uint32_t)(32 * quarter) << 16) + kOCol + 128u * g;
+    uint8_t* const stage = smem_raw + pad + kSumAt + (128 * g + 32 * quarter) * kSumPitch;  // this warp's
     Ring<kItems> it;
-    uint32_t nt[2] = {0, 0};  // a tile's items with keys
+    uint32_t nt = 0;  // the tile's items with keys
+    // the places in a staged row of this lane's eight coordinates of an output row, and their signs
+    uint32_t from[4] = {0, 0, 0, 0}, flip[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const uint32_t i = a.rv.inv[8 * (lane & 7) + t];
+      from[t >> 1] |= (4u * (i & ~3u) + 2u * (i & 3u)) << (16 * (t & 1));
+      flip[t >> 1] |= ((a.rv.signs[i >> 5] >> (i & 31)) & 1u) << (16 * (t & 1) + 15);
+    }
     bool ok = true;
     while (ok) {
       if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
       const Item& in = ctl.items[it.i];
       struct {
-        int seq, head, row0, rows, q_start, split, chunks, keys[2];
-      } e = {in.seq, in.head, in.row0, in.rows, in.q_start, in.split, in.chunks, {in.key_end[0] - in.c0, in.key_end[1] - in.c0}};
+        int seq, head, row0, rows, q_start, split, chunks, keys, lane0;
+      } e = {in.seq,   in.head,   in.row0,                   in.rows,    in.q_start,
+             in.split, in.chunks, in.key_end[g] - in.c0, in.lane0[g]};
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
       it.next();
       if (e.seq < 0) break;
+      const int row = e.row0 + kTile * g + r - e.lane0;
+      const bool warp_rows = 32 * quarter >= e.lane0 && row - lane < e.rows, valid = warp_rows && row < e.rows;
+      const bool some = e.keys > 0, two = e.keys > kStep;
+      const uint32_t turn = nt & 1u;
+      float m = -INFINITY, l = 0.0f, fa = 0.0f, fb = 0.0f;
+      if (some) {
+        if (!wait(ctl.o_full[g], turn, ctl, err)) {
+          ok = false;
+          break;
+        }
+        ++nt;
+        tc_fence_after();
+        const float ma = ctl.m[turn][g][0][r], mb = two ? ctl.m[turn][g][1][r] : -INFINITY;
+        m = fmaxf(ma, mb);
+        const float wa = ma == -INFINITY ? 0.0f : ex2(ma - m), wb = mb == -INFINITY ? 0.0f : ex2(mb - m);
+        l = ctl.l[turn][g][0][r] * wa;
+        // 2^(eV - 126) / 64 takes the scales of V and of the levels back out
+        fa = wa * __int_as_float((ctl.ve[turn][g][0] - 5) << 23);
+        if (two) {
+          l += ctl.l[turn][g][1][r] * wb;
+          fb = wb * __int_as_float((ctl.ve[turn][g][1] - 5) << 23);
+        }
+      }
+      const bool part = e.chunks > 1;
+      if (!part) {
+        const float inv = l == 0.0f ? 0.0f : __fdividef(0.125f, l);
+        fa *= inv;
+        fb *= inv;
+      }
+      // 16 coordinates at a time: the chains joined, and butterflies of width 1..8
+      float* sums = reinterpret_cast<float*>(stage + lane * kSumPitch);
+      long long at = 0;
+      if (part) {
+        Span s;
+        s.q_start = e.q_start;
+        at = part_at(a, s, e.head, e.split, row);
+      }
+      float* const to = part ? a.part + at * 64 : sums;
+      if (warp_rows) {
 #pragma unroll 1
-      for (int g = 0; g < 2; ++g) {
-        const int row = e.row0 + kTile * g + r;
-        const bool valid = row < e.rows, warp_rows = row - lane < e.rows;
-        const int keys = g ? e.keys[1] : e.keys[0];
-        const bool some = keys > 0, two = keys > kStep;
-        const uint32_t turn = (g ? nt[1] : nt[0]) & 1u;
-        float m = -INFINITY, l = 0.0f, fa = 0.0f, fb = 0.0f;
-        if (some) {
-          if (!wait(ctl.o_full[g], turn, ctl, err)) {
-            ok = false;
-            break;
-          }
-          if (g) ++nt[1]; else ++nt[0];
-          tc_fence_after();
-          const float ma = ctl.m[turn][g][0][r], mb = two ? ctl.m[turn][g][1][r] : -INFINITY;
-          m = fmaxf(ma, mb);
-          const float wa = ma == -INFINITY ? 0.0f : ex2(ma - m), wb = mb == -INFINITY ? 0.0f : ex2(mb - m);
-          l = ctl.l[turn][g][0][r] * wa;
-          // 2^(eV - 126) / 64 takes the scales of V and of the levels back out
-          fa = wa * __int_as_float((ctl.ve[turn][g][0] - 5) << 23);
-          if (two) {
-            l += ctl.l[turn][g][1][r] * wb;
-            fb = wb * __int_as_float((ctl.ve[turn][g][1] - 5) << 23);
-          }
-        }
-        const bool part = e.chunks > 1;
-        if (!part) {
-          const float inv = l == 0.0f ? 0.0f : __fdividef(0.125f, l);
-          fa *= inv;
-          fb *= inv;
-        }
-        // 16 coordinates at a time: the chains joined, and butterflies of width 1..8
-        float* sums = reinterpret_cast<float*>(smem_raw + pad + kSumAt + r * kSumPitch);
-        const uint32_t t_o = t_lane + kOCol + 128u * g;
-        long long at = 0;
-        if (part) {
-          Span s;
-          s.q_start = e.q_start;
-          at = part_at(a, s, e.head, e.split, row);
-        }
-        if (warp_rows) {
-#pragma unroll 1
-          for (int h = 0; h < 4; ++h) {
-            uint32_t x[16], y[16];
-            if (some) tmem_ld16(t_o + 16u * h, x);
-            if (two) tmem_ld16(t_o + 64u + 16u * h, y);
-            tmem_ld_wait();
-            float o[16];
+        for (int h = 0; h < 4; ++h) {
+          uint32_t x[16], y[16];
+          tmem_ld16(t_o + 16u * h, x);
+          tmem_ld16(t_o + 64u + 16u * h, y);
+          tmem_ld_wait();
+          float o[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {  // a chain without a step has no O
-              o[i] = some ? __uint_as_float(x[i]) * fa : 0.0f;
-              if (two) o[i] = fmaf(__uint_as_float(y[i]), fb, o[i]);
-            }
-            if (part) {
-              if (valid) {
-                float4* dst = reinterpret_cast<float4*>(a.part + at * 64 + 16 * h);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-              }
-              continue;
-            }
+          for (int i = 0; i < 16; ++i)  // a chain without a step has no O
+            o[i] = fmaf(__uint_as_float(two ? y[i] : 0u), fb, __uint_as_float(some ? x[i] : 0u) * fa);
+          if (!part) {
 #pragma unroll
             for (int w = 1; w < 16; w <<= 1)
 #pragma unroll
@@ -904,68 +938,62 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
                   o[i] = u + v;
                   o[i + w] = u - v;
                 }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sums[16 * h + i] = o[i];
           }
-        }
-        if (some) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&ctl.o_free[g]));
-        }
-        if (part && valid) a.part_ml[at] = make_float2(m, l);
-        if (part || !warp_rows) continue;
-        // widths 16 and 32, signs and permutation; whole rows leave through shared memory
-        uint8_t* stage = smem_raw + pad + kOutAt + 32 * quarter * kOutPitch;
-        uint8_t* my = stage + lane * kOutPitch;
-#pragma unroll 1
-        for (int i0 = 0; i0 < 16; i0 += 4) {
-          float z[4][4];
-          uint32_t to[4][4];
+          float4* dst = reinterpret_cast<float4*>(to + 16 * h);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              z[i][k] = sums[i0 + i + 16 * k];
-              to[i][k] = ctl.turn_out[i0 + i + 16 * k];
-            }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = z[i][0] + z[i][1], q = z[i][0] - z[i][1], u = z[i][2] + z[i][3], v = z[i][2] - z[i][3];
-            z[i][0] = p + u, z[i][1] = q + v, z[i][2] = p - u, z[i][3] = q - v;
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<uint16_t*>(my + (to[i][k] & 0xffu)) = __bfloat16_as_ushort(
-                  __float2bfloat16_rn(__uint_as_float(__float_as_uint(z[i][k]) ^ (to[i][k] & 0x80000000u))));
+            if (!part || valid) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
-        __syncwarp();
-        const int tok = row / a.group, qh = e.head * a.group + row % a.group;
-        const unsigned long long mine =
-            (unsigned long long)((__nv_bfloat16*)a.out + (long long)(e.q_start + tok) * a.o_ld + (long long)qh * a.o_hs);
-        const int n_rows = min(32, e.rows - (row - lane));
-#pragma unroll 1
-        for (int i = 0; i < n_rows; i += 16) {  // eight lanes a row, 16 bytes each
-          uint8_t* dst[4];
-          uint4 x[4];
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int k = i + 4 * w + (lane >> 3);
-            dst[w] = (uint8_t*)__shfl_sync(0xffffffffu, mine, k);
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(stage + k * kOutPitch + 16 * (lane & 7));
-            x[w] = make_uint4(src[0], src[1], src[2], src[3]);
-          }
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            if (i + 4 * w + (lane >> 3) < n_rows) *reinterpret_cast<uint4*>(dst[w] + 16 * (lane & 7)) = x[w];
-        }
-        __syncwarp();
-        if (a.lse != nullptr && valid)
-          a.lse[(long long)(e.q_start + tok) * (a.pool.heads * a.group) + qh] =
-              l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       }
+      if (some) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.o_free[g]));
+      }
+      if (part && valid) a.part_ml[at] = make_float2(m, l);
+      if (part || !warp_rows) continue;
+      // widths 16 and 32, in place: four coordinates from each of the four 16s become bf16 over the first two of them
+#pragma unroll 1
+      for (int i = 0; i < 16; i += 4) {
+        float z[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 f = *reinterpret_cast<const float4*>(sums + i + 16 * k);
+          z[0][k] = f.x, z[1][k] = f.y, z[2][k] = f.z, z[3][k] = f.w;
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float p = z[w][0] + z[w][1], q = z[w][0] - z[w][1], u = z[w][2] + z[w][3], v = z[w][2] - z[w][3];
+          z[w][0] = p + u, z[w][1] = q + v, z[w][2] = p - u, z[w][3] = q - v;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint2*>(sums + i + 16 * k) = make_uint2(pack_bf16(z[0][k], z[1][k]), pack_bf16(z[2][k], z[3][k]));
+      }
+      __syncwarp();
+      // signs and permutation on the way out: eight lanes a row, which each have the same eight places in all rows
+      const int tok = row / a.group, qh = e.head * a.group + row % a.group;
+      const unsigned long long mine =
+          (unsigned long long)((__nv_bfloat16*)a.out + (long long)(e.q_start + tok) * a.o_ld + (long long)qh * a.o_hs);
+      const int n_rows = min(32, e.rows - (row - lane));
+#pragma unroll 2
+      for (int i = 0; i < n_rows; i += 4) {
+        const int k = i + (lane >> 3);
+        uint8_t* dst = (uint8_t*)__shfl_sync(0xffffffffu, mine, k);
+        const uint8_t* src = stage + k * kSumPitch;
+        uint32_t w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t x = *reinterpret_cast<const uint16_t*>(src + (from[t] & 0xffffu)),
+                         y = *reinterpret_cast<const uint16_t*>(src + (from[t] >> 16));
+          w[t] = (x | y << 16) ^ flip[t];
+        }
+        if (k < n_rows) *reinterpret_cast<uint4*>(dst + 16 * (lane & 7)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      __syncwarp();
+      if (a.lse != nullptr && valid)
+        a.lse[(long long)(e.q_start + tok) * (a.pool.heads * a.group) + qh] =
+            l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
     }
   }
 
@@ -989,8 +1017,13 @@ int launch_attend_tc(const Args& a, cudaStream_t st) {
     CC2_CUDA(cudaFuncSetAttribute(attend_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem + 1024));
     if (dev < 64) attr_done |= 1ull << dev;
   }
+  Turn turn;
+  for (int i = 0; i < 64; ++i) {
+    turn.place[i] = 4u * a.rk.perm[i];
+    turn.sign[i] = (a.rk.signs[i >> 5] >> (i & 31)) & 1u ? -1.0f : 1.0f;
+  }
   const unsigned q_blocks = (unsigned)(((long long)a.total_q * a.group + 127) / 128);
-  CC2_CUDA(launch_k(rotate_queries_kernel, dim3(q_blocks, (unsigned)a.pool.heads), kQThreads, 0, st, a, q_tiles));
+  CC2_CUDA(launch_k(rotate_queries_kernel, dim3(q_blocks, (unsigned)a.pool.heads), kQThreads, 0, st, a, turn, q_tiles));
   const unsigned grid = (unsigned)std::min<long long>(items, num_sms());
   CC2_CUDA(launch_k(attend_tc_kernel, grid, kThreads, kSmem + 1024, st, a, q_tiles, (int)items));
   CC2_CHECK_LAUNCH();
