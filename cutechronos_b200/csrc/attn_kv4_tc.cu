@@ -152,30 +152,16 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// Butterflies of a row of 64 in registers: width 1 within a pair of neighbours,
-// widths 2..32 two at a time.
-__device__ __forceinline__ void walsh(float* y) {
-  uint64_t p[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) p[i] = f2_pack(y[2 * i] + y[2 * i + 1], y[2 * i] - y[2 * i + 1]);
-  const uint64_t minus = f2_pack(-1.0f, -1.0f);
-#pragma unroll
-  for (int w = 1; w < 32; w <<= 1)
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (!(i & w)) {
-        const uint64_t a = p[i], b = p[i + w];
-        p[i] = f2_add(a, b);
-        p[i + w] = f2_fma(b, minus, a);
-      }
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f2_unpack(p[i], y[2 * i], y[2 * i + 1]);
-}
 // ------------------------------------------------------------------ queries --
-// A block rotates 128 rows of the call for one head, whatever sequences they
-// belong to: a thread a row, as in kv4_cache.cu.  Rows come in by four threads
-// each through shared memory and leave as 16-byte pieces of their tile.
-constexpr int kQThreads = 128, kQPitch = 65;
+// A block rotates 128 rows of the call for some heads, whatever sequences the
+// rows belong to.  The rotation is a product with a 64 x 64 matrix of +-1, which
+// mma.sync takes from a row's elements as they come from memory: a lane has four
+// neighbours of each 16, RoPE turns them in registers (its pairs, 32 apart, are
+// one lane's), and the matrix' rows are in the order that this gives.  In bf16,
+// as the elements and the next 8 bits of what RoPE leaves of them (2^-17 of an
+// element where the fp16 result keeps 2^-11); sums in fp32.  Finished rows leave
+// through shared memory as whole 128-byte lines.
+constexpr int kQThreads = 128;
 
 struct QueryRow {
   int seq, q_start;  // -1: no sequence has it
@@ -194,121 +180,161 @@ __device__ __forceinline__ QueryRow find_row(const Args& a, int tok, int lane) {
   return r;
 }
 
-__global__ void __launch_bounds__(kQThreads)
-rotate_queries_kernel(const __grid_constant__ Args a, const __grid_constant__ Turn turn, const long long q_tiles) {
+__device__ __forceinline__ void mma_pm1(float (&d)[4], const uint32_t (&x)[4], uint2 b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b.x), "r"(b.y));
+}
+
+__global__ void __launch_bounds__(kQThreads, 4)
+rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles, const int per) {
   pdl_launch_dependents();
   pdl_wait();
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.counter = 0;  // for the kernel after this one
-  __shared__ __align__(16) float rows[128 * kQPitch];
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int head = blockIdx.y, base = blockIdx.x * 128, all = a.total_q * a.group;
+  __shared__ __align__(16) uint8_t stage[128 * 128];
+  __shared__ uint2 matrix[4 * 8 * 32];  // [16 elements][8 coordinates][lane]
   __shared__ const __nv_bfloat16* row_at[128];
+  __shared__ long long row_to[128];  // row among the tiles of head 0; -1: none
   __shared__ int row_pos[128];
-  // this thread's row: a block's rows mostly belong to one sequence, the others follow it
-  const QueryRow at = find_row(a, base / a.group, lane);
-  const int row = base + tid;
-  const __nv_bfloat16* from = nullptr;
-  int pos = -1, in_seq = 0;
-  long long to = -1;
-  if (row < all) {
-    const int tok = row / a.group;
-    int seq = at.seq;
-    if (a.cu == nullptr) seq = tok / a.max_q;
-    else
-      while (seq + 1 < a.num_seqs && a.cu[seq + 1] <= tok) ++seq;
-    if (seq >= 0) {
-      const Span s = span_of(a, seq, 0, false);
-      in_seq = row - s.q_start * a.group;
-      if (in_seq < s.rows) {
-        from = (const __nv_bfloat16*)a.q + (long long)tok * a.q_ld + (long long)(head * a.group + row % a.group) * a.q_hs;
-        to = (long long)head * q_tiles + first_query_tile(a, seq, s.q_start) + in_seq / 128;
-        if (a.rotate) pos = s.len - s.n + (tok - s.q_start);
-        if (pos >= a.rope_len) {
-          if (a.rotate) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
-          pos = -1;
+  __shared__ uint8_t coord[64];  // of an element, its sign in bit 7
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int base = blockIdx.x * 128, all = a.total_q * a.group;
+  if (tid < 64) {
+    const uint32_t i = a.rk.inv[tid];
+    coord[tid] = (uint8_t)(i | ((a.rk.signs[i >> 5] >> (i & 31)) & 1u) << 7);
+  }
+  {
+    // this thread's row: a block's rows mostly belong to one sequence, the others follow it
+    const QueryRow at = find_row(a, base / a.group, lane);
+    const int row = base + tid;
+    const __nv_bfloat16* from = nullptr;
+    int pos = -1;
+    long long to = -1;
+    if (row < all) {
+      const int tok = row / a.group;
+      int seq = at.seq;
+      if (a.cu == nullptr) seq = tok / a.max_q;
+      else
+        while (seq + 1 < a.num_seqs && a.cu[seq + 1] <= tok) ++seq;
+      if (seq >= 0) {
+        const Span s = span_of(a, seq, 0, false);
+        const int in_seq = row - s.q_start * a.group;
+        if (in_seq < s.rows) {
+          from = (const __nv_bfloat16*)a.q + (long long)tok * a.q_ld + (long long)(row % a.group) * a.q_hs;
+          to = first_query_tile(a, seq, s.q_start) * 128 + in_seq;
+          if (a.rotate) pos = s.len - s.n + (tok - s.q_start);
+          if (pos >= a.rope_len) {
+            if (a.rotate) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+            pos = -1;
+          }
         }
       }
     }
-  }
-  row_at[tid] = from;
-  row_pos[tid] = pos;
-  __syncthreads();
-  const int c = tid & 3;
-  uint4 lo[4], hi[4];
-#pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const __nv_bfloat16* q = row_at[it * 32 + (tid >> 2)];
-    lo[it] = hi[it] = make_uint4(0, 0, 0, 0);
-    if (q != nullptr) {
-      lo[it] = *reinterpret_cast<const uint4*>(q + 8 * c);
-      hi[it] = *reinterpret_cast<const uint4*>(q + 8 * c + 32);
-    }
-  }
-#pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int r = it * 32 + (tid >> 2), p = row_pos[r];
-    float x[16];
-    const uint32_t w[8] = {lo[it].x, lo[it].y, lo[it].z, lo[it].w, hi[it].x, hi[it].y, hi[it].z, hi[it].w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[2 * j] = __uint_as_float(w[j] << 16);
-      x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    }
-    if (p >= 0) {
-      const float4* cs = reinterpret_cast<const float4*>(a.rope + (long long)p * 32 + 8 * c);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 f = cs[j];
-        const float p0 = x[2 * j], q0 = x[8 + 2 * j], p1 = x[2 * j + 1], q1 = x[9 + 2 * j];
-        x[2 * j] = p0 * f.x - q0 * f.y;
-        x[8 + 2 * j] = q0 * f.x + p0 * f.y;
-        x[2 * j + 1] = p1 * f.z - q1 * f.w;
-        x[9 + 2 * j] = q1 * f.z + p1 * f.w;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      rows[r * kQPitch + 8 * c + j] = x[j];
-      rows[r * kQPitch + 32 + 8 * c + j] = x[8 + j];
-    }
+    row_at[tid] = from;
+    row_to[tid] = to;
+    row_pos[tid] = pos;
   }
   __syncthreads();
-  float y[64];
+#pragma unroll 2
+  for (int k = tid; k < 4 * 8 * 32; k += kQThreads) {
+    const int n = 8 * ((k >> 5) & 7) + ((k & 31) >> 2), t = k >> 8, col = 32 * (t >> 1) + 8 * (k & 3) + 4 * (t & 1);
+    uint32_t v[4];
 #pragma unroll
-  for (int i = 0; i < 64; ++i) {
-    y[i] = turn.sign[i] * *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(rows + tid * kQPitch) + turn.place[i]);
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t i = coord[col + j];
+      v[j] = 0x3f80u | ((__popc(n & i & 63u) ^ (i >> 7)) & 1u) << 15;  // +-1
+    }
+    matrix[k] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
   }
-  walsh(y);
-  float top = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 64; ++i) top = fmaxf(top, fabsf(y[i]));
+  __syncthreads();
+  const int c = lane & 3;
   const float by = 0.125f * a.qscale;
-  const int e = min(max((int)(__float_as_uint(top * fabsf(by)) >> 23), 30), 254);
-  const float up = by * __int_as_float((261 - e) << 23);  // 2^(134 - e): the row below 2^8
-  const int r = in_seq & 127;
-  // a warp's rows go out as whole lines (a thread's 16-byte pieces of its own row would touch 32 lines each time):
-  // through the warp's part of `rows`, 144 bytes a row, pieces exchanged within 8 rows as the tensor core reads them
-  __syncwarp();
-  uint8_t* stage = reinterpret_cast<uint8_t*>(rows + (tid - lane) * kQPitch);
+  const int head0 = blockIdx.y * per, head1 = min(head0 + per, a.pool.heads);
+#pragma unroll 1
+  for (int mt = 0; mt < 2; ++mt) {
+    const int first = 32 * warp + 16 * mt + (lane >> 2);  // the lane's rows: this one and the eighth after it
+    float4 cs[2][4];  // [half][elements 8c + 2j, 8c + 2j + 1]: cosine, sine; of all heads
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    uint4 w;
-    w.x = pack_half(y[8 * c] * up, y[8 * c + 1] * up);
-    w.y = pack_half(y[8 * c + 2] * up, y[8 * c + 3] * up);
-    w.z = pack_half(y[8 * c + 4] * up, y[8 * c + 5] * up);
-    w.w = pack_half(y[8 * c + 6] * up, y[8 * c + 7] * up);
-    *reinterpret_cast<uint4*>(stage + lane * 144 + ((c ^ (r & 7)) << 4)) = w;
-  }
-  if (to >= 0) const_cast<float*>(a.q_scale)[to * 128 + r] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64
-  const unsigned long long mine =
-      to < 0 ? 0ull : (unsigned long long)(const_cast<uint8_t*>(a.qt) + to * kTileBytes + r * 128);
-  __syncwarp();
+    for (int half = 0; half < 2; ++half) {
+      const int p = row_pos[first + 8 * half];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int k = 4 * i + (lane >> 3);
-    uint8_t* dst = (uint8_t*)__shfl_sync(0xffffffffu, mine, k);
-    const uint4 w = *reinterpret_cast<const uint4*>(stage + k * 144 + 16 * (lane & 7));
-    if (dst != nullptr) *reinterpret_cast<uint4*>(dst + 16 * (lane & 7)) = w;
+      for (int j = 0; j < 4; ++j)
+        cs[half][j] = p >= 0 ? *reinterpret_cast<const float4*>(a.rope + (long long)p * 32 + 8 * c + 2 * j)
+                             : make_float4(1.0f, 0.0f, 1.0f, 0.0f);
+    }
+#pragma unroll 1
+    for (int head = head0; head < head1; ++head) {
+      uint32_t hi[4][4], lo[4][4];  // [elements][row + 8 * half, elements 0, 1 / 2, 3]
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const __nv_bfloat16* q = row_at[first + 8 * half];
+        uint4 u = make_uint4(0, 0, 0, 0), v = u;
+        if (q != nullptr) {
+          q += (long long)(head * a.group) * a.q_hs + 8 * c;
+          u = *reinterpret_cast<const uint4*>(q);
+          v = *reinterpret_cast<const uint4*>(q + 32);
+        }
+        hi[0][half] = u.x, hi[0][half + 2] = u.y, hi[1][half] = u.z, hi[1][half + 2] = u.w;
+        hi[2][half] = v.x, hi[2][half + 2] = v.y, hi[3][half] = v.z, hi[3][half + 2] = v.w;
+        if (a.rotate) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int t = j >> 1, i = half + 2 * (j & 1);
+            const float4 f = cs[half][j];
+            const uint32_t pw = hi[t][i], qw = hi[t + 2][i];
+            const float p0 = __uint_as_float(pw << 16), p1 = __uint_as_float(pw & 0xffff0000u);
+            const float q0 = __uint_as_float(qw << 16), q1 = __uint_as_float(qw & 0xffff0000u);
+            const float x0 = p0 * f.x - q0 * f.y, y0 = q0 * f.x + p0 * f.y;
+            const float x1 = p1 * f.z - q1 * f.w, y1 = q1 * f.z + p1 * f.w;
+            const uint32_t x = pack_bf16(x0, x1), y = pack_bf16(y0, y1);
+            hi[t][i] = x;
+            hi[t + 2][i] = y;
+            lo[t][i] = pack_bf16(x0 - __uint_as_float(x << 16), x1 - __uint_as_float(x & 0xffff0000u));
+            lo[t + 2][i] = pack_bf16(y0 - __uint_as_float(y << 16), y1 - __uint_as_float(y & 0xffff0000u));
+          }
+        }
+      }
+      float y[8][4];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const uint2 b = matrix[(8 * t + n) * 32 + lane];
+          if (a.rotate) mma_pm1(y[n], lo[t], b);
+          mma_pm1(y[n], hi[t], b);
+        }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float top = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) top = max3(top, fabsf(y[n][2 * half]), fabsf(y[n][2 * half + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(__float_as_uint(top * fabsf(by)) >> 23), 30), 254);
+        const float up = by * __int_as_float((261 - e) << 23);  // 2^(134 - e): the row below 2^8
+        const long long to = row_to[first + 8 * half];
+        // the 16-byte pieces exchanged within 8 rows of a tile as the tensor core reads them
+        uint8_t* out = stage + (first + 8 * half) * 128 + 4 * c;
+        const int r7 = (int)to & 7;
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+          *reinterpret_cast<uint32_t*>(out + ((n ^ r7) << 4)) = pack_half(y[n][2 * half] * up, y[n][2 * half + 1] * up);
+        if (to >= 0 && c == 0)  // 2^(e - 134) / 64
+          const_cast<float*>(a.q_scale)[head * q_tiles * 128 + to] = __int_as_float((e - 13) << 23);
+      }
+      __syncwarp();
+      uint8_t* const tiles = const_cast<uint8_t*>(a.qt) + head * q_tiles * kTileBytes + 16 * (lane & 7);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = 32 * warp + 16 * mt + 4 * i + (lane >> 3);
+        const long long to = row_to[k];
+        if (to >= 0) *reinterpret_cast<uint4*>(tiles + to * 128) = *reinterpret_cast<const uint4*>(stage + k * 128 + 16 * (lane & 7));
+      }
+      __syncwarp();
+    }
   }
 }
 
@@ -1017,13 +1043,11 @@ int launch_attend_tc(const Args& a, cudaStream_t st) {
     CC2_CUDA(cudaFuncSetAttribute(attend_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem + 1024));
     if (dev < 64) attr_done |= 1ull << dev;
   }
-  Turn turn;
-  for (int i = 0; i < 64; ++i) {
-    turn.place[i] = 4u * a.rk.perm[i];
-    turn.sign[i] = (a.rk.signs[i >> 5] >> (i & 31)) & 1u ? -1.0f : 1.0f;
-  }
   const unsigned q_blocks = (unsigned)(((long long)a.total_q * a.group + 127) / 128);
-  CC2_CUDA(launch_k(rotate_queries_kernel, dim3(q_blocks, (unsigned)a.pool.heads), kQThreads, 0, st, a, turn, q_tiles));
+  // heads a block: as many as leave one round of blocks
+  const int per = (int)std::min<long long>(a.pool.heads, ((long long)q_blocks * a.pool.heads + 4 * num_sms() - 1) / (4 * num_sms()));
+  CC2_CUDA(launch_k(rotate_queries_kernel, dim3(q_blocks, (unsigned)((a.pool.heads + per - 1) / per)), kQThreads, 0, st, a,
+                    q_tiles, per));
   const unsigned grid = (unsigned)std::min<long long>(items, num_sms());
   CC2_CUDA(launch_k(attend_tc_kernel, grid, kThreads, kSmem + 1024, st, a, q_tiles, (int)items));
   CC2_CHECK_LAUNCH();
