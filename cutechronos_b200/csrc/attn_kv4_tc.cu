@@ -263,18 +263,26 @@ rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles, c
         cs[half][j] = p >= 0 ? *reinterpret_cast<const float4*>(a.rope + (long long)p * 32 + 8 * c + 2 * j)
                              : make_float4(1.0f, 0.0f, 1.0f, 0.0f);
     }
+    uint4 next[2][2];  // the next head's elements
+    auto fetch = [&](int head) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const __nv_bfloat16* q = row_at[first + 8 * half];
+        next[half][0] = next[half][1] = make_uint4(0, 0, 0, 0);
+        if (q != nullptr && head < head1) {
+          q += (long long)(head * a.group) * a.q_hs + 8 * c;
+          next[half][0] = *reinterpret_cast<const uint4*>(q);
+          next[half][1] = *reinterpret_cast<const uint4*>(q + 32);
+        }
+      }
+    };
+    fetch(head0);
 #pragma unroll 1
     for (int head = head0; head < head1; ++head) {
       uint32_t hi[4][4], lo[4][4];  // [elements][row + 8 * half, elements 0, 1 / 2, 3]
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const __nv_bfloat16* q = row_at[first + 8 * half];
-        uint4 u = make_uint4(0, 0, 0, 0), v = u;
-        if (q != nullptr) {
-          q += (long long)(head * a.group) * a.q_hs + 8 * c;
-          u = *reinterpret_cast<const uint4*>(q);
-          v = *reinterpret_cast<const uint4*>(q + 32);
-        }
+        const uint4 u = next[half][0], v = next[half][1];
         hi[0][half] = u.x, hi[0][half + 2] = u.y, hi[1][half] = u.z, hi[1][half + 2] = u.w;
         hi[2][half] = v.x, hi[2][half + 2] = v.y, hi[3][half] = v.z, hi[3][half + 2] = v.w;
         if (a.rotate) {
@@ -295,6 +303,7 @@ rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles, c
           }
         }
       }
+      fetch(head + 1);
       float y[8][4];
 #pragma unroll
       for (int n = 0; n < 8; ++n) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.0f;
