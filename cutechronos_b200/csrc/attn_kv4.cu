@@ -23,9 +23,15 @@
 // 256 pairs in shared memory that every lane has its own bank's copy of, so no
 // lookup waits for another: one byte permute makes the address of two values
 // (the code byte above the lane's place, hence 256 bytes an entry) and one load
-// brings them.  One block an SM, for one table.  Byte permutes of the levels' bytes took 1.6 (K) and 2.1 (V)
-// operations a value on the half-rate integer pipe and were what bound the kernel
-// (208 us instead of see below for the 484 MB of 64 sequences of up to 16384 tokens).
+// brings them.  One block an SM, for one table.  Byte permutes of the levels' bytes
+// took 1.6 (K) and 2.1 (V) operations a value on the half-rate integer pipe, which
+// was 73% busy and bound the kernel.
+// Measured, one token for each of 64 sequences of up to 16384 tokens, 12 heads
+// (484 MB of cache): 146 us, 3.3 TB/s; 207 us with the byte permutes; 192 us with
+// a fixed chunk of keys a block instead of the call's work cut evenly over teams
+// that stay.  A stage of 64 keys takes a warp some 815 instructions; issue slots
+// are 63% used, the load/store pipe 58% and the integer pipe 51%, with the
+// 16 warps an SM that the table and the rings leave room for.
 // What must not leave the type's range is scaled by powers of two, which are
 // exact: a row of Q to below 2^8, P n_v to below 2^14 against the largest norm
 // met so far.
@@ -62,7 +68,12 @@ using namespace tcx;
 
 constexpr int kStageKeys = 64;
 constexpr int kStageBytes = kStageKeys / kBlockTokens * kBlockBytes;  // 4352
-constexpr int kTcMoreThan = 32;  // bf16 rows of a sequence and head from which the tcgen05 kernel takes over
+// bf16 rows of a sequence and head above which the tcgen05 kernel takes over.  It
+// costs the same for 17 rows as for 128; this one costs a pass over the keys for
+// each 32.  This one / tcgen05, us, 8 heads, 16 sequences of 8192 tokens: 72 / 123
+// with 32 rows, 106 / 128 with 40, 115 / 131 with 64; 64 sequences of 1024: 79 / 70
+// with 20, 90 / 70 with 32, 138 / 72 with 40.
+constexpr int kTcMoreThan = 32;
 constexpr int kQPitch = 72;  // halves
 constexpr int kOPitch = 66;  // floats
 
@@ -699,12 +710,17 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
   const int rows = std::max(1, max_q * (q_heads / pool.heads));
   p = Plan{};
   p.tc = dtype == CC2_BF16 && rows > kTcMoreThan;
+  // As few columns of 8 rows as hold the rows: with 16 sequences of 8192 tokens and 8 heads, one / two / four columns
+  // take 35 / 43 / 61 us for 4 rows, 56 / 47 / 66 for 12, 92 / 72 / 73 for 32 (there four spare half the passes over
+  // the keys' bytes).  fp32 splits need the registers of four.
   p.nb = rows <= 8 ? 1 : rows <= 16 || dtype == CC2_F32 ? 2 : 4;
   p.tile_rows = p.tc ? kTcRows : 8 * p.nb;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const long long tiles = (long long)num_seqs * pool.heads * p.row_tiles;
   if (p.tc) {
-    // blocks take items as they get to them: about four an SM even them out; a chunk's own cost is some 1000 keys
+    // Blocks take items as they get to them: about four an SM even them out; a chunk's own cost is some 1000 keys.
+    // One / two / four / eight an SM: 168 / 123 / 113 / 119 us for 64 tokens of 2 sequences of 65536, 8 heads;
+    // 229 / 185 / 172 / 186 us for 256 tokens of 4 of 32768; 299 / 305 / 310 / 311 us where there are items enough.
     const long long want = (4LL * num_sms() + tiles - 1) / tiles;
     const int splits = (int)std::min<long long>(std::max(1, (max_len + 1023) / 1024), std::max<long long>(1, want));
     p.chunk = ((std::max(1, max_len) + splits - 1) / splits + 255) / 256 * 256;
@@ -778,7 +794,9 @@ template <typename T>
 int join(const Args& a, const Plan& p, cudaStream_t st) {
   if (!p.joined) return CC2_OK;
   const long long rows = (long long)a.total_q * a.group * a.pool.heads;
-  // where there are fewer rows than warps on the card, four share one: a row then has many parts
+  // Where there are fewer rows than warps on the card, four share one: a row then has many parts.  Whole calls with
+  // four / one a row: 35.0 / 37.1 us with 128 rows, 113 / 121 us with 1024 in 8 chunks, 51 / 49 us with 2048,
+  // 51 / 43 us with 4096, 178 / 145 us with 16384.
   const bool four = rows <= 16LL * num_sms();
   const unsigned grid = (unsigned)(four ? rows : (rows + 3) / 4);
   if (p.tc) {
