@@ -96,7 +96,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kUnits = 64;   // (token, head) pairs a block handles: a thread for each K and each V
-constexpr int kPitch = 65;
+constexpr int kInPitch = 65, kOutPitch = 69;  // words of a row: append, read (its halves 4 words apart)
 
 struct Places {
   const int32_t* seq;
@@ -148,19 +148,23 @@ template <> struct Raw<__nv_bfloat16> {
     }
   }
 };
-template <typename T> __device__ __forceinline__ void store8(T* p, const float* x);
-template <> __device__ __forceinline__ void store8<float>(float* p, const float* x) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+// Thread c of 8: its eighth of a row (halves 4 words apart) to memory.
+__device__ __forceinline__ void store_part(float* p, const float* row, int c) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const float* x = row + 36 * half + 4 * c;
+    reinterpret_cast<float4*>(p)[8 * half + c] = make_float4(x[0], x[1], x[2], x[3]);
+  }
 }
-template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const float* x) {
+__device__ __forceinline__ void store_part(__nv_bfloat16* p, const float* row, int c) {
+  const float* x = row + 8 * c + (c & 4);
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
     w[i] = *reinterpret_cast<uint32_t*>(&h);
   }
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  reinterpret_cast<uint4*>(p)[c] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Butterflies of width 1, 2, ..., 32 over 64 registers, each sum and difference rounded once: width 1 within pairs of
@@ -191,23 +195,29 @@ struct Unit {
   int slot;          // place in the block of 16; bit 8: masked
 };
 
-// A block's 64 units, neighbours in (token, head) order.
+// A block's 64 units: 16 neighbouring tokens of each of 4 heads (the next 16
+// tokens' where the heads run out).  Their rows in shared memory are 4 t + h: a
+// warp that brings 8 rows in or out has one or two tokens' (one line of RoPE
+// factors for 4 of them); the owners, lane = token, have 16 neighbours of a head,
+// whose codes are 512 bytes in one piece.
 struct Units {
-  int t0, h0, heads, last;  // last: the last unit that there is
-  __device__ __forceinline__ Units(int tokens, int heads_) : heads(heads_) {
-    const long long u0 = (long long)blockIdx.x * kUnits;
-    t0 = (int)(u0 / heads);
-    h0 = (int)(u0 % heads);
-    last = (int)min((long long)tokens * heads - u0, (long long)kUnits) - 1;
-  }
-  // token and head of unit r; false past the end (then the last one's)
+  int tokens, heads;
+  // of row r; false past the end (then the last token's)
   __device__ __forceinline__ bool find(int r, int& t, int& h) const {
-    const unsigned x = (unsigned)(h0 + min(r, last)), dt = x / (unsigned)heads;
-    h = (int)(x - dt * (unsigned)heads);
-    t = t0 + (int)dt;
-    return r <= last;
+    const unsigned q = blockIdx.x * 4u + ((unsigned)r & 3u), run = q / (unsigned)heads;
+    h = (int)(q - run * (unsigned)heads);
+    t = (int)run * 16 + (r >> 2);
+    const bool is = t < tokens;
+    t = min(t, tokens - 1);
+    return is;
   }
+  static __device__ __forceinline__ int row_of(int tid) { return 4 * (tid & 15) + ((tid >> 4) & 3); }
 };
+// Place of a row of floats: the second 32 rows two words on, which keeps the
+// owners' accesses (rows 4 apart and two heads) free of bank conflicts at a pitch
+// that is odd.
+template <int kPitch> __device__ __forceinline__ int row_at(int row) { return row * kPitch + 2 * (row >> 5); }
+template <int kPitch> constexpr int kRowsWords = 2 * kUnits * kPitch + 8;
 
 // An owner's row: at constant places, times constant signs.
 __device__ __forceinline__ void take_row(const float* row, const Turn& turn, float (&y)[64]) {
@@ -223,7 +233,7 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn tu
               const T* __restrict__ v, long long v_ld, long long v_hs, int tokens, Places at,
               const uint8_t* __restrict__ mask, const float2* __restrict__ rope, int rope_len, int* __restrict__ err) {
   pdl_launch_dependents();
-  __shared__ __align__(16) float rows[2 * kUnits * kPitch];
+  __shared__ __align__(16) float rows[kRowsWords<kInPitch>];
   __shared__ float norm[2 * kUnits];
   __shared__ Cells::Cell cells[64];
   __shared__ Unit units[kUnits];
@@ -231,7 +241,7 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn tu
   const int tid = threadIdx.x;
   if (tid < 64) cells[tid] = table.of[tid];
   pdl_wait();
-  const Units my(tokens, pool.heads);
+  const Units my{tokens, pool.heads};
 
   // four threads bring a vector in: thread c its values 8c .. 8c+7 and 32 + 8c ..
   const int c = tid & 3;
@@ -298,7 +308,7 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn tu
 #pragma unroll
         for (int j = 0; j < o; ++j) s[j] = __fadd_rn(s[j], s[j + o]);
       }
-      float* row = rows + (is_v * kUnits + r) * kPitch + 8 * c;
+      float* row = rows + row_at<kInPitch>(is_v * kUnits + r) + 8 * c;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         row[j] = a[j];
@@ -310,13 +320,14 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn tu
   __syncthreads();
 
   const int is_v = tid >= kUnits;  // whole warps
-  const Unit& u = units[tid & (kUnits - 1)];
+  const int mine = is_v * kUnits + Units::row_of(tid);
+  const Unit& u = units[mine & (kUnits - 1)];
   if (u.block < 0) return;
   float y[64];
-  if (is_v) take_row(rows + tid * kPitch, turn_v, y);  // two copies, each with its own constants
-  else take_row(rows + tid * kPitch, turn_k, y);
+  if (is_v) take_row(rows + row_at<kInPitch>(mine), turn_v, y);  // two copies, each with its own constants
+  else take_row(rows + row_at<kInPitch>(mine), turn_k, y);
   walsh(y);
-  const float n = norm[tid];
+  const float n = norm[mine];
   const float n8 = __fmul_rn(n, 8.0f);
   const float fine = n8 > 0.0f ? __fdividef(511.0f, n8) : 0.0f;  // its error is within the cells' room
   const uint8_t* entries = reinterpret_cast<const uint8_t*>(cells);
@@ -352,7 +363,7 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn
             const float4 levels_lo, const float4 levels_hi, T* __restrict__ k_out, T* __restrict__ v_out, int tokens,
             Places at, int* __restrict__ err) {
   pdl_launch_dependents();
-  __shared__ __align__(16) float rows[2 * kUnits * kPitch];
+  __shared__ __align__(16) float rows[kRowsWords<kOutPitch>];
   __shared__ __align__(16) float level[8];
   const int tid = threadIdx.x;
   if (tid == 0) {
@@ -361,12 +372,12 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn
   }
   pdl_wait();
   __syncthreads();
-  const Units my(tokens, pool.heads);
+  const Units my{tokens, pool.heads};
   {
     const bool is_v = tid >= kUnits;
     int off = 0, t, h;
     long long at_block = -1;
-    if (my.find(tid & (kUnits - 1), t, h) && (is_v ? v_out : k_out) != nullptr)
+    if (my.find(Units::row_of(tid), t, h) && (is_v ? v_out : k_out) != nullptr)
       at_block = place(pool, at, t, h, 0x7fffffff, &off, err);
     float f = 0.0f;
     float y[64];
@@ -389,7 +400,7 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn
       }
       walsh(y);
     }
-    uint8_t* row = reinterpret_cast<uint8_t*>(rows + tid * kPitch);
+    uint8_t* row = reinterpret_cast<uint8_t*>(rows + row_at<kOutPitch>(is_v * kUnits + Units::row_of(tid)));
     if (is_v) {
 #pragma unroll
       for (int i = 0; i < 64; ++i)
@@ -401,26 +412,19 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn
     }
   }
   __syncthreads();
-  const int c = tid & 3;
+  // eight threads a row: whole lines
+  const int c = tid & 7;
 #pragma unroll
   for (int is_v = 0; is_v < 2; ++is_v) {
     T* out = is_v ? v_out : k_out;
     if (out == nullptr) continue;
 #pragma unroll
-    for (int it = 0; it < kUnits * 4 / kThreads; ++it) {
-      const int r = it * (kThreads / 4) + (tid >> 2);
+    for (int it = 0; it < kUnits * 8 / kThreads; ++it) {
+      const int r = it * (kThreads / 8) + (tid >> 3);
       int t, h;
       if (!my.find(r, t, h)) continue;
-      const float* row = rows + (is_v * kUnits + r) * kPitch + 8 * c;
-      float a[8], b[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        a[j] = row[j];
-        b[j] = row[32 + j];
-      }
-      T* to = out + ((long long)t * pool.heads + h) * 64 + 8 * c;
-      store8(to, a);
-      store8(to + 32, b);
+      const float* row = rows + row_at<kOutPitch>(is_v * kUnits + r);
+      store_part(out + ((long long)t * pool.heads + h) * 64, row, c);
     }
   }
 }
@@ -438,7 +442,7 @@ bool rows_ok(int dtype, const void* p, int64_t ld, int64_t hs) {
 }
 
 int grid_of(int T, int heads, int* grid) {
-  const long long blocks = ((long long)T * heads + kUnits - 1) / kUnits;
+  const long long blocks = (((long long)T + 15) / 16 * heads + 3) / 4;
   CC2_REQUIRE(blocks <= 0x1fffffffLL, "kv4: too many tokens for one call");
   *grid = (int)blocks;
   return CC2_OK;
@@ -507,6 +511,10 @@ int launch_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_
   Turn turn_k, turn_v;
   CC2_TRY(make_turn(cache->key, "kv4_read", turn_k));
   CC2_TRY(make_turn(cache->value, "kv4_read", turn_v));
+  for (int i = 0; i < 64; ++i) {  // the second half of a row is 4 words on
+    turn_k.place[i] += turn_k.place[i] >= 128 ? 16u : 0u;
+    turn_v.place[i] += turn_v.place[i] >= 128 ? 16u : 0u;
+  }
   const float* lv = cache->levels;
   const float4 lo = make_float4(lv[0], lv[1], lv[2], lv[3]), hi = make_float4(lv[4], lv[5], lv[6], lv[7]);
   const Places at{seq, pos, table, table_ld, num_seqs};
