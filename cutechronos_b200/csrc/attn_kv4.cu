@@ -8,7 +8,7 @@
 //
 // Rows are the queries of one sequence that share a head of keys: row r is
 // query token r / group, head r % group.  A unit of work is one head of keys of
-// one sequence, up to 8 NB rows and a chunk of the keys; persistent blocks walk
+// one sequence, up to 4, 8, 16 or 32 rows and a chunk of the keys; persistent blocks walk
 // the units, one for each of their teams of warps; a team's warps take 64-key
 // stages of its unit in turn, each with a ring of its own that bulk copies fill,
 // and an online softmax of its own, joined at the end of the unit while the next
@@ -16,7 +16,7 @@
 //   S^T (16 keys x 8 rows) = K (the A operand, decoded in registers) . Q^T
 //   O^T (16 coordinates x 8 rows) += V^T (A, decoded) . P^T
 // Keys and coordinates as the long axis of the product: one token's query
-// fills 1 of 8 columns and not 1 of 16 rows.  P^T comes from S^T by one matrix
+// fills 2 of 8 columns (its two fp16 parts) and not 2 of 16 rows.  P^T comes from S^T by one matrix
 // move a register pair.
 // Decoding: a byte of codes is an fp16 pair (K: neighbouring coordinates; V: one
 // coordinate of two tokens, their words zipped first), looked up in a table of
@@ -35,11 +35,13 @@
 // What must not leave the type's range is scaled by powers of two, which are
 // exact: a row of Q to below 2^8, P n_v to below 2^14 against the largest norm
 // met so far.
-// Rounding: Q and P n_v to fp16 (2^-12 of each, next to the output's bf16 with
-// 2^-9), levels to fp16.  fp32 calls split all three into two fp16 parts and
-// sum three products, which leaves about 2^-22.
+// Rounding: P n_v to fp16 (2^-12 of each, next to the output's bf16 with 2^-9),
+// the levels to fp16 after a common factor that moves all of them close to its
+// values, Q to one or two fp16 parts (split_q).  fp32 calls split all three into
+// two parts and sum three products, which leaves about 2^-22.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "kv4_attn.cuh"
 
@@ -49,10 +51,40 @@ int attention_error_word(int** p);
 
 namespace kv4 {
 
+// fp16 keeps the levels to 2^-12 of each at best, the same error in every key.
+// One factor for all of them, taken out again exactly where it does not matter,
+// moves them: of 64 in an octave the one that leaves the least, weighted by how
+// much of a vector's length a level holds (coordinates are nearly normal with
+// variance 1 / 64).  Lloyd-Max levels: 2.4e-4 of a level without, 0.9e-4 with it.
+float level_scale(const float (&c)[8]) {
+  float weight[8], best = INFINITY, scale = 64.0f;
+  for (int i = 0; i < 8; ++i) {
+    const float width = i < 7 ? c[i + 1] - c[i] : c[i] - c[i - 1];
+    weight[i] = width * std::exp(-32.0f * c[i] * c[i]);
+  }
+  for (int k = 0; k < 64; ++k) {
+    const float f = 64.0f + (float)k;
+    float sum = 0.0f;
+    for (int i = 0; i < 8; ++i) {
+      const float x = f * c[i];
+      uint32_t u;
+      memcpy(&u, &x, sizeof u);
+      u = (u + 0xfffu + ((u >> 13) & 1u)) & ~0x1fffu;  // 11 bits
+      float h;
+      memcpy(&h, &u, sizeof h);
+      sum += weight[i] * (h - x) * (h - x);
+    }
+    sum /= f * f;
+    if (sum < best) best = sum, scale = f;
+  }
+  return scale;
+}
+
 Levels make_levels(const cc2_kv4_cache& cache) {
   Levels r{};
+  r.scale = level_scale(cache.levels);
   for (int i = 0; i < 8; ++i) {
-    const float c = 64.0f * cache.levels[i];
+    const float c = r.scale * cache.levels[i];
     const __half h = __float2half_rn(c);
     r.value[i] = __half_as_ushort(h);
     r.rest[i] = __half_as_ushort(__float2half_rn(c - __half2float(h)));
@@ -104,15 +136,20 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   return v;
 }
 // Teams of a block and their warps: what registers and shared memory leave room for.
-template <int NB, bool F32> constexpr int teams_of() { return NB == 2 && !F32 ? 3 : 2; }
-template <int NB, bool F32> constexpr int warps_of() { return NB == 1 && !F32 ? 8 : 4; }
+template <int R, bool F32> constexpr int teams_of() { return R == 16 && !F32 ? 3 : 2; }
+// Whether Q is held as two fp16 parts.  One part's rounding, the same for every key, is most of what a long context
+// costs in precision (131072 keys, scores of deviation 2: 0.9e-3 of the output next to its own rounding's 1.7e-3, 0.4e-3
+// with both).  Up to 4 rows the second part takes columns that would be empty; as products of their own they cost 5%
+// with 8 rows and 10% with 16, and would 17% with 32, which keeps one like the tcgen05 kernel.
+template <int R, bool F32> constexpr bool split_q() { return R <= 16 || F32; }
+template <int R, bool F32> constexpr int warps_of() { return R <= 8 && !F32 ? 8 : 4; }
 
-template <int NB, bool F32>
+template <int R, bool F32>
 struct Shared {
-  static constexpr int kTeams = teams_of<NB, F32>(), kWarps = warps_of<NB, F32>(), kRows = 8 * NB;
+  static constexpr int kTeams = teams_of<R, F32>(), kWarps = warps_of<R, F32>(), kRows = R;
   struct Team {
     alignas(128) uint8_t ring[kWarps][2][kStageBytes];
-    alignas(16) __half q[F32 ? 2 : 1][kRows][kQPitch];
+    alignas(16) __half q[split_q<R, F32>() ? 2 : 1][kRows][kQPitch];  // and what its rounding leaves
     float rs[kRows];
     float m[kWarps][kRows], l[kWarps][kRows];
     uint64_t full[kWarps][2];
@@ -125,7 +162,7 @@ struct Shared {
   static_assert(kRows * kOPitch * 4 <= 2 * kStageBytes, "a warp's sums fit its ring");
 };
 // Whether a warp's sums leave one slot of its ring free.
-template <int NB> constexpr bool sums_in_a_slot() { return 8 * NB * kOPitch * 4 <= kStageBytes; }
+template <int R> constexpr bool sums_in_a_slot() { return R * kOPitch * 4 <= kStageBytes; }
 
 template <bool kBf16> __device__ __forceinline__ float norm_of(uint32_t bits) { return norm_value((uint16_t)bits, kBf16); }
 
@@ -197,11 +234,15 @@ struct Walk {
   }
 };
 
-template <int NB, bool F32, bool NormBf16>
-__global__ void __launch_bounds__(32 * warps_of<NB, F32>() * teams_of<NB, F32>(), 1)
+// R rows a tile: 4 (each in two columns of the products), or 8, 16, 32 in as many columns.
+template <int R, bool F32, bool NormBf16>
+__global__ void __launch_bounds__(32 * warps_of<R, F32>() * teams_of<R, F32>(), 1)
 attend_kernel(const __grid_constant__ Args a) {
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
-  using S = Shared<NB, F32>;
+  using S = Shared<R, F32>;
+  constexpr bool kPaired = R == 4;
+  constexpr int NB = kPaired ? 1 : R / 8, kPer = kPaired ? 1 : 2;  // blocks of 8 columns, rows of a lane in one
+  constexpr bool kSplit = !kPaired && split_q<R, F32>();           // Q's second part by products of its own
   constexpr int kRows = S::kRows, kWarps = S::kWarps;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   S& all = *reinterpret_cast<S*>(smem_raw);
@@ -305,7 +346,7 @@ attend_kernel(const __grid_constant__ Args a) {
       const int row = s.row0 + r;
       if (row >= s.rows) {  // a column of zeros
 #pragma unroll
-        for (int p = 0; p < (F32 ? 2 : 1); ++p) sm.q[p][r][lane] = sm.q[p][r][lane + 32] = __float2half_rn(0.0f);
+        for (int p = 0; p < (split_q<R, F32>() ? 2 : 1); ++p) sm.q[p][r][lane] = sm.q[p][r][lane + 32] = __float2half_rn(0.0f);
         if (lane == 0) sm.rs[r] = 1.0f;
         continue;
       }
@@ -327,8 +368,8 @@ attend_kernel(const __grid_constant__ Args a) {
       float y0 = flip(spread_get(x0, x1, all.turns.k_perm[lane]), a.rk.signs, 0, lane);
       float y1 = flip(spread_get(x0, x1, all.turns.k_perm[lane + 32]), a.rk.signs, 1, lane);
       spread_walsh(y0, y1, lane);
-      y0 *= 0.125f * a.qscale;
-      y1 *= 0.125f * a.qscale;
+      y0 *= a.qscale;
+      y1 *= a.qscale;
       const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(y0), fabsf(y1))));
       const int e = min(max((int)(top >> 23), 30), 254);
       const float up = __int_as_float((261 - e) << 23);  // 2^(134 - e)
@@ -337,29 +378,30 @@ attend_kernel(const __grid_constant__ Args a) {
       const __half g0 = __float2half_rn(y0), g1 = __float2half_rn(y1);
       sm.q[0][r][lane] = g0;
       sm.q[0][r][lane + 32] = g1;
-      if (F32) {
-        sm.q[F32 ? 1 : 0][r][lane] = __float2half_rn(y0 - __half2float(g0));
-        sm.q[F32 ? 1 : 0][r][lane + 32] = __float2half_rn(y1 - __half2float(g1));
+      if (split_q<R, F32>()) {
+        sm.q[split_q<R, F32>() ? 1 : 0][r][lane] = __float2half_rn(y0 - __half2float(g0));
+        sm.q[split_q<R, F32>() ? 1 : 0][r][lane + 32] = __float2half_rn(y1 - __half2float(g1));
       }
       if (lane == 0) sm.rs[r] = __int_as_float((e - 13) << 23);  // 2^(e - 134) / 64: undoes both scalings
     }
     meet(true);
 
-    uint32_t qf[NB][F32 ? 16 : 8];
+    uint32_t qf[NB][kSplit ? 16 : 8];
     float rs[NB][2];
     int limit[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
-      for (int p = 0; p < (F32 ? 2 : 1); ++p) {
-        const uint4* src = reinterpret_cast<const uint4*>(&sm.q[p][8 * b + g][16 * t]);
+      for (int p = 0; p < (kSplit ? 2 : 1); ++p) {  // a paired row's parts are neighbouring columns
+        const __half* column = kPaired ? sm.q[kPaired ? g & 1 : 0][g >> 1] : sm.q[p][8 * b + g];
+        const uint4* src = reinterpret_cast<const uint4*>(column + 16 * t);
         const uint4 x = src[0], y = src[1];
         uint32_t* d = &qf[b][8 * p];
         d[0] = x.x, d[1] = x.y, d[2] = x.z, d[3] = x.w, d[4] = y.x, d[5] = y.y, d[6] = y.z, d[7] = y.w;
       }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = 8 * b + 2 * t + c;
+      for (int c = 0; c < kPer; ++c) {
+        const int r = 8 * b + kPer * t + c;
         rs[b][c] = sm.rs[r];
         limit[b][c] = a.causal ? min(s.len - s.n + (s.row0 + r) / a.group + 1, s.len) : s.len;
       }
@@ -406,8 +448,8 @@ attend_kernel(const __grid_constant__ Args a) {
               if (F32) {
                 const uint32_t e[4] = {ra[2 * p], rb[2 * p], ra[2 * p + 1], rb[2 * p + 1]};
                 mma(x[j][b], e, qf[b][k], qf[b][k + 1]);
-                mma(x[j][b], f, qf[b][F32 ? 8 + k : k], qf[b][F32 ? 9 + k : k + 1]);
               }
+              if (kSplit) mma(x[j][b], f, qf[b][kSplit ? 8 + k : k], qf[b][kSplit ? 9 + k : k]);
               mma(x[j][b], f, qf[b][k], qf[b][k + 1]);
             }
           }
@@ -423,8 +465,9 @@ attend_kernel(const __grid_constant__ Args a) {
 #pragma unroll
           for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kPer; ++i) {
               float& v = x[j][b][2 * c + i];
+              if (kPaired) v += x[j][b][2 * c + 1];
               v *= nk;
               if (!seen || (kEdge && key0 + 16 * j + krow + 8 * c >= limit[b][i])) v = -INFINITY;
             }
@@ -439,7 +482,7 @@ attend_kernel(const __grid_constant__ Args a) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kPer; ++c) {
           float v = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 4; ++j) v = max3(v, x[j][b][c], x[j][b][c + 2]);
@@ -451,7 +494,7 @@ attend_kernel(const __grid_constant__ Args a) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < kPer; ++c) {
             float v = mx[b][c];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -478,18 +521,29 @@ attend_kernel(const __grid_constant__ Args a) {
         const uint64_t n0 = f2_pack(nv[j][0] * vs, nv[j][0] * vs), n1 = f2_pack(nv[j][1] * vs, nv[j][1] * vs);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const uint64_t r2 = f2_pack(rs[b][0], rs[b][1]), g2 = f2_pack(neg[b][0], neg[b][1]);
           float p[4];
+          if (kPaired) {  // the odd columns' stay zero
+            p[1] = p[3] = 0.0f;
+            f2_unpack(f2_fma(f2_pack(x[j][b][0], x[j][b][2]), f2_pack(rs[b][0], rs[b][0]), f2_pack(neg[b][0], neg[b][0])), p[0], p[2]);
+            p[0] = ex2(p[0]);
+            p[2] = ex2(p[2]);
+            l[b][0] += p[0] + p[2];
+          } else {
+            const uint64_t r2 = f2_pack(rs[b][0], rs[b][1]), g2 = f2_pack(neg[b][0], neg[b][1]);
 #pragma unroll
-          for (int c = 0; c < 4; c += 2) {
-            f2_unpack(f2_fma(f2_pack(x[j][b][c], x[j][b][c + 1]), r2, g2), p[c], p[c + 1]);
-            p[c] = ex2(p[c]);
-            p[c + 1] = ex2(p[c + 1]);
+            for (int c = 0; c < 4; c += 2) {
+              f2_unpack(f2_fma(f2_pack(x[j][b][c], x[j][b][c + 1]), r2, g2), p[c], p[c + 1]);
+              p[c] = ex2(p[c]);
+              p[c + 1] = ex2(p[c + 1]);
+            }
+            f2_unpack(f2_add(f2_add(f2_pack(l[b][0], l[b][1]), f2_pack(p[0], p[1])), f2_pack(p[2], p[3])), l[b][0], l[b][1]);
           }
-          f2_unpack(f2_add(f2_add(f2_pack(l[b][0], l[b][1]), f2_pack(p[0], p[1])), f2_pack(p[2], p[3])), l[b][0], l[b][1]);
           if (kEdge) {  // a key that a row does not see adds nothing, whatever its norm
 #pragma unroll
-            for (int c = 0; c < 4; ++c) p[c] = x[j][b][c] == -INFINITY ? 0.0f : p[c] * (c < 2 ? nv[j][0] : nv[j][1]) * vs;
+            for (int c = 0; c < 4; c += 3 - kPer) p[c] = x[j][b][c] == -INFINITY ? 0.0f : p[c] * (c < 2 ? nv[j][0] : nv[j][1]) * vs;
+          } else if (kPaired) {
+            p[0] *= nv[j][0] * vs;
+            p[2] *= nv[j][1] * vs;
           } else {
             f2_unpack(f2_mul(f2_pack(p[0], p[1]), n0), p[0], p[1]);
             f2_unpack(f2_mul(f2_pack(p[2], p[3]), n1), p[2], p[3]);
@@ -549,17 +603,17 @@ attend_kernel(const __grid_constant__ Args a) {
     // the next unit's first stage sets out before this one is joined
     ahead = 0;
     more = next(coming);
-    if (sums_in_a_slot<NB>() && more && !broken && coming.stages > 0) issue(coming, 0, n), ahead = 1;
-    float* mine_sums = reinterpret_cast<float*>(sm.ring[warp][sums_in_a_slot<NB>() ? (n + 1u) & 1u : 0]);
+    if (sums_in_a_slot<R>() && more && !broken && coming.stages > 0) issue(coming, 0, n), ahead = 1;
+    float* mine_sums = reinterpret_cast<float*>(sm.ring[warp][sums_in_a_slot<R>() ? (n + 1u) & 1u : 0]);
     const float down = __int_as_float((ve - 11) << 23);  // 2^(ve - 132) / 64
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < kPer; ++c) {
         float v = l[b][c];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        const int r = 8 * b + 2 * t + c;
+        const int r = 8 * b + kPer * t + c;
         if (g == 0) {
           sm.m[warp][r] = m[b][c] * rs[b][c];
           sm.l[warp][r] = v;
@@ -691,7 +745,7 @@ join_kernel(const __grid_constant__ Args a) {
 struct Plan {
   bool tc;  // attn_kv4_tc.cu's kernel
   bool joined;
-  int nb, row_tiles, tile_rows;
+  int row_tiles, tile_rows;
   int chunk, splits;               // tcgen05
   int round_keys, blocks, teams;   // else
   long long tiles;
@@ -710,11 +764,10 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
   const int rows = std::max(1, max_q * (q_heads / pool.heads));
   p = Plan{};
   p.tc = dtype == CC2_BF16 && rows > kTcMoreThan;
-  // As few columns of 8 rows as hold the rows: with 16 sequences of 8192 tokens and 8 heads, one / two / four columns
-  // take 35 / 43 / 61 us for 4 rows, 56 / 47 / 66 for 12, 92 / 72 / 73 for 32 (there four spare half the passes over
-  // the keys' bytes).  fp32 splits need the registers of four.
-  p.nb = rows <= 8 ? 1 : rows <= 16 || dtype == CC2_F32 ? 2 : 4;
-  p.tile_rows = p.tc ? kTcRows : 8 * p.nb;
+  // As few columns as hold the rows: with 16 sequences of 8192 tokens and 8 heads, one / two / four blocks of 8 take
+  // 35 / 43 / 61 us for 4 rows, 56 / 47 / 66 for 12, 92 / 72 / 73 for 32 (there four spare half the passes over the
+  // keys' bytes); a block with 4 rows in column pairs and one with 8 35 / 39.  fp32 splits need the registers of four.
+  p.tile_rows = p.tc ? kTcRows : dtype == CC2_F32 ? (rows <= 8 ? 8 : 16) : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const long long tiles = (long long)num_seqs * pool.heads * p.row_tiles;
   if (p.tc) {
@@ -734,10 +787,11 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
     p.scale_bytes = (size_t)p.tiles * 128 * sizeof(float) + 128;  // and the items' counter
   } else {
     const bool f32 = dtype == CC2_F32;
-    const int warps = p.nb == 1 && !f32 ? warps_of<1, false>() : 4, a_block = p.nb == 2 && !f32 ? teams_of<2, false>() : 2;
-    static_assert(warps_of<2, false>() == 4 && warps_of<4, false>() == 4 && warps_of<1, true>() == 4 &&
-                      warps_of<2, true>() == 4 && teams_of<1, false>() == 2 && teams_of<4, false>() == 2 &&
-                      teams_of<1, true>() == 2 && teams_of<2, true>() == 2,
+    const int warps = p.tile_rows <= 8 && !f32 ? warps_of<4, false>() : 4, a_block = p.tile_rows == 16 && !f32 ? teams_of<16, false>() : 2;
+    static_assert(warps_of<8, false>() == warps_of<4, false>() && warps_of<16, false>() == 4 && warps_of<32, false>() == 4 &&
+                      warps_of<8, true>() == 4 && warps_of<16, true>() == 4 && teams_of<4, false>() == 2 &&
+                      teams_of<8, false>() == 2 && teams_of<32, false>() == 2 && teams_of<8, true>() == 2 &&
+                      teams_of<16, true>() == 2,
                   "as assumed above");
     p.round_keys = warps * kStageKeys;
     // no more blocks than there are rounds
@@ -770,24 +824,24 @@ int wait_word(int** p) {
   return CC2_OK;
 }
 
-template <int NB, bool F32, bool NormBf16>
+template <int R, bool F32, bool NormBf16>
 int launch(const Args& a, const Plan& p, cudaStream_t st) {
-  const size_t smem = sizeof(Shared<NB, F32>);
+  const size_t smem = sizeof(Shared<R, F32>);
   static unsigned long long attr_done = 0;  // one bit per device
   int dev = 0;
   CC2_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !((attr_done >> dev) & 1ull)) {
-    CC2_CUDA(cudaFuncSetAttribute(attend_kernel<NB, F32, NormBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CC2_CUDA(cudaFuncSetAttribute(attend_kernel<R, F32, NormBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (dev < 64) attr_done |= 1ull << dev;
   }
-  CC2_CUDA(launch_k(attend_kernel<NB, F32, NormBf16>, (unsigned)p.blocks, 32 * teams_of<NB, F32>() * warps_of<NB, F32>(),
+  CC2_CUDA(launch_k(attend_kernel<R, F32, NormBf16>, (unsigned)p.blocks, 32 * teams_of<R, F32>() * warps_of<R, F32>(),
                     smem, st, a));
   CC2_CHECK_LAUNCH();
   return CC2_OK;
 }
-template <int NB, bool F32>
+template <int R, bool F32>
 int launch(const Args& a, const Plan& p, cudaStream_t st) {
-  return a.pool.norm_bf16 ? launch<NB, F32, true>(a, p, st) : launch<NB, F32, false>(a, p, st);
+  return a.pool.norm_bf16 ? launch<R, F32, true>(a, p, st) : launch<R, F32, false>(a, p, st);
 }
 
 template <typename T>
@@ -884,7 +938,6 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   a.round_keys = p.round_keys;
   a.causal = causal != 0;
   a.rotate = rotate_q != 0;
-  a.qscale = scale * 1.4426950408889634f;
   const cc2_kv4_quant* quant[2] = {&cache->key, &cache->value};
   Rotation* rotation[2] = {&a.rk, &a.rv};
   for (int k = 0; k < 2; ++k) {
@@ -894,9 +947,12 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
     for (int i = 0; i < 64; ++i) r.inv[r.perm[i] = quant[k]->perm[i] & 63] = (uint8_t)i;
   }
   a.levels = make_levels(*cache);
+  a.back = 8.0f / a.levels.scale;
+  a.qscale = scale * 1.4426950408889634f * a.back;
   if (p.tc) CC2_TRY(launch_attend_tc(a, st));
-  else if (dtype == CC2_F32) CC2_TRY(p.nb == 1 ? (launch<1, true>(a, p, st)) : (launch<2, true>(a, p, st)));
-  else CC2_TRY(p.nb == 1 ? (launch<1, false>(a, p, st)) : p.nb == 2 ? (launch<2, false>(a, p, st)) : (launch<4, false>(a, p, st)));
+  else if (dtype == CC2_F32) CC2_TRY(p.tile_rows == 8 ? (launch<8, true>(a, p, st)) : (launch<16, true>(a, p, st)));
+  else if (p.tile_rows <= 8) CC2_TRY(p.tile_rows == 4 ? (launch<4, false>(a, p, st)) : (launch<8, false>(a, p, st)));
+  else CC2_TRY(p.tile_rows == 16 ? (launch<16, false>(a, p, st)) : (launch<32, false>(a, p, st)));
   return dtype == CC2_F32 ? join<float>(a, p, st) : join<__nv_bfloat16>(a, p, st);
 }
 

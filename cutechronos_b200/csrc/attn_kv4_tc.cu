@@ -261,7 +261,7 @@ rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles, c
   }
   __syncthreads();
   const int c = lane & 3;
-  const float by = 0.125f * a.qscale;
+  const float by = a.qscale;
   const int head0 = blockIdx.y * per, head1 = min(head0 + per, a.pool.heads);
 #pragma unroll 1
   for (int mt = 0; mt < 2; ++mt) {
@@ -951,7 +951,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
       }
       const bool part = e.chunks > 1;
       if (!part) {
-        const float inv = l == 0.0f ? 0.0f : __fdividef(0.125f, l);
+        const float inv = l == 0.0f ? 0.0f : __fdividef(a.back, l);
         fa *= inv;
         fb *= inv;
       }

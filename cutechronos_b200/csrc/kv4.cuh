@@ -53,12 +53,13 @@ struct Cells {
   } of[64];
 };
 
-// The levels as the fp16 decoders take them: 64 c_i split into its fp16 value
-// and, for fp32 calls, what that leaves over.  The factor 64 keeps the rest of
-// the split out of fp16's subnormal range; it is exact and taken out again at
-// the end.  `lo` and `hi` are the low and the high bytes of the eight fp16
+// The levels as the fp16 decoders take them: f c_i split into its fp16 value
+// and, for fp32 calls, what that leaves over.  The factor f (64 .. 127) keeps the
+// rest of the split out of fp16's subnormal range, and the values close to fp16's;
+// it is taken out again from the queries and at the end.  `lo` and `hi` are the low and the high bytes of the eight fp16
 // values, for byte permutes.
 struct Levels {
+  float scale;  // f
   uint16_t value[8], rest[8];
   uint32_t lo[2], hi[2];
 };

@@ -53,7 +53,8 @@ struct Args {
   int chunk, splits, row_tiles, tile_rows;
   int teams, round_keys;  // else: teams of warps on the card, keys that one takes in a round of its warps
   int causal, rotate;
-  float qscale;  // scale * log2(e)
+  float qscale;  // scale * log2(e) / 8 * 64 / f: of a rotated query (f: the levels' factor)
+  float back;    // 64 / f / 8: of a rotated sum
   Rotation rk, rv;
   Levels levels;
 };
@@ -163,8 +164,8 @@ __device__ __forceinline__ void finish_row(const Args& a, const Turns& turns, co
                                            float l, int lane) {
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   spread_walsh(o0, o1, lane);
-  o0 = flip(o0 * (0.125f * inv), a.rv.signs, 0, lane);
-  o1 = flip(o1 * (0.125f * inv), a.rv.signs, 1, lane);
+  o0 = flip(o0 * (a.back * inv), a.rv.signs, 0, lane);
+  o1 = flip(o1 * (a.back * inv), a.rv.signs, 1, lane);
   const float x0 = spread_get(o0, o1, turns.v_inv[lane]);
   const float x1 = spread_get(o0, o1, turns.v_inv[lane + 32]);
   const int tok = s.q_start + row / a.group, qh = head * a.group + row % a.group;
