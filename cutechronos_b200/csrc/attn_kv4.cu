@@ -27,7 +27,7 @@
 // took 1.6 (K) and 2.1 (V) operations a value on the half-rate integer pipe, which
 // was 73% busy and bound the kernel.
 // Measured, one token for each of 64 sequences of up to 16384 tokens, 12 heads
-// (484 MB of cache): 146 us, 3.3 TB/s; 207 us with the byte permutes; 192 us with
+// (484 MB of cache): 145 us, 3.3 TB/s; 207 us with the byte permutes; 192 us with
 // a fixed chunk of keys a block instead of the call's work cut evenly over teams
 // that stay.  A stage of 64 keys takes a warp some 815 instructions; issue slots
 // are 63% used, the load/store pipe 58% and the integer pipe 51%, with the
@@ -53,7 +53,7 @@ namespace kv4 {
 
 // fp16 keeps the levels to 2^-12 of each at best, the same error in every key.
 // One factor for all of them, taken out again exactly where it does not matter,
-// moves them: of 64 in an octave the one that leaves the least, weighted by how
+// moves them: of 32 in an octave the one that leaves the least, weighted by how
 // much of a vector's length a level holds (coordinates are nearly normal with
 // variance 1 / 64).  Lloyd-Max levels: 2.4e-4 of a level without, 0.9e-4 with it.
 float level_scale(const float (&c)[8]) {
@@ -62,7 +62,7 @@ float level_scale(const float (&c)[8]) {
     const float width = i < 7 ? c[i + 1] - c[i] : c[i] - c[i - 1];
     weight[i] = width * std::exp(-32.0f * c[i] * c[i]);
   }
-  for (int k = 0; k < 64; ++k) {
+  for (int k = 0; k < 64; k += 2) {
     const float f = 64.0f + (float)k;
     float sum = 0.0f;
     for (int i = 0; i < 8; ++i) {
