@@ -58,18 +58,24 @@ def _quant(p: TurboQuantParams, which: str) -> tuple[nat.KV4Quant, np.ndarray, n
 
 
 _PER = {torch.bfloat16: 7, torch.float32: 3}  # elements of 16 bytes, less one
+_BYTES = (torch.bool, torch.uint8)
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(i).cuda_stream in a fraction of its time
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    rows, heads, last = t.stride()
-    return last == 1 and not (rows | heads) & _PER[t.dtype] and not t.data_ptr() & 15
+def _place(t: torch.Tensor, per: int) -> tuple[int, int, int] | None:
+    """Address of t (rows, heads, 64), elements from row to row and from head to head, as the kernels take them: last
+    axis dense, rows and heads on 16-byte boundaries (``per`` + 1 elements).  None where it does not lie so."""
+    (rows, heads, last), at = t.stride(), t.data_ptr()
+    return None if last != 1 or (rows | heads) & per or at & 15 else (at, rows, heads)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t (rows, heads, 64) as the kernels read it: last axis dense, rows and heads on 16-byte boundaries (copied where
-    they are not)."""
-    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
+def _rows(t: torch.Tensor, per: int) -> tuple[torch.Tensor, tuple[int, int, int]]:
+    """t, copied where the kernels cannot read it as it is, and where it lies."""
+    at = _place(t, per)
+    if at is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        at = _place(t, per)
+    return t, at
 
 
 class PagedKV4Cache:
@@ -183,11 +189,12 @@ class PagedKV4Cache:
         if token_mask is not None:
             if token_mask.shape != seq.shape or token_mask.device != self.device:
                 raise ValueError("token_mask must have one entry for each token, on the cache's device")
-            mask = token_mask.view(torch.uint8) if token_mask.dtype == torch.bool else token_mask
-            mask = (mask if mask.dtype == torch.uint8 else (mask != 0).view(torch.uint8)).contiguous()
-        k, v = _rows(k), _rows(v)
-        self._call(self._lib.cc2_kv4_append, "cc2_kv4_append", code, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                   v.stride(0), v.stride(1), n, seq.data_ptr(), pos.data_ptr(),
+            mask = token_mask if token_mask.dtype in _BYTES else token_mask != 0
+            if not mask.is_contiguous():
+                mask = mask.contiguous()
+        per = _PER[k.dtype]
+        (k, k_at), (v, v_at) = _rows(k, per), _rows(v, per)
+        self._call(self._lib.cc2_kv4_append, "cc2_kv4_append", code, *k_at, *v_at, n, seq.data_ptr(), pos.data_ptr(),
                    None if mask is None else mask.data_ptr(), table.data_ptr(), ld, seqs)
 
     def read(self, seq_ids: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor, *,
@@ -242,12 +249,17 @@ class PagedKV4Cache:
             raise ValueError("max_q and max_len must not be negative")
         if rotate_q and self.rope is None:
             raise ValueError("the cache was made without a rotation (rope_theta None)")
-        q = _rows(q)
+        per = _PER[q.dtype]
+        q, q_at = _rows(q, per)
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif (out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not _aligned(out)
-              or any(n > 1 and st < DIM for n, st in zip(out.shape[:2], out.stride()))):
-            raise ValueError("out must have q's shape, type and device, its rows apart, dense and on 16-byte boundaries")
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
+            out_at = (out.data_ptr(), heads * DIM, DIM)
+        else:
+            out_at = None
+            if out.shape == q.shape and out.dtype == q.dtype and out.device == self.device:
+                out_at = _place(out, per)
+            if out_at is None or any(n > 1 and st < DIM for n, st in zip(out.shape[:2], out_at[1:])):
+                raise ValueError("out must have q's shape, type and device, its rows apart, dense and on 16-byte boundaries")
         lse = torch.empty((total, heads), dtype=torch.float32, device=self.device) if return_lse else None
         sizes = (code, heads, seqs, total, max_q, max_len)
         if self._plan[0] != sizes:
@@ -257,8 +269,8 @@ class PagedKV4Cache:
             self._plan = (sizes, nbytes.value)
         need = self._plan[1]
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._call(self._lib.cc2_kv4_attention, "cc2_kv4_attention", code, q.data_ptr(), q.stride(0), q.stride(1),
-                   out.data_ptr(), out.stride(0), out.stride(1), heads, seqs, total, cu, max_q, lens.data_ptr(), max_len,
+        self._call(self._lib.cc2_kv4_attention, "cc2_kv4_attention", code, *q_at, *out_at, heads, seqs, total, cu,
+                   max_q, lens.data_ptr(), max_len,
                    table.data_ptr(), ld, causal, scale, rotate_q, None if lse is None else lse.data_ptr(),
                    None if ws is None else ws.data_ptr(), need)
         return (out, lse) if return_lse else out
