@@ -309,23 +309,25 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn tu
       float s[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] = __fadd_rn(__fmul_rn(a[j], a[j]), __fmul_rn(b[j], b[j]));
+      // each thread keeps half of the sums at either step, j and j + 4 together
+      const bool up = (c & 2) != 0, odd = (c & 1) != 0;
+      float h[4];  // j = 0, 1, 4, 5 or 2, 3, 6, 7
 #pragma unroll
-      for (int o = 2; o > 0; o >>= 1) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = __fadd_rn(s[j], __shfl_xor_sync(0xffffffffu, s[j], o));
+      for (int i = 0; i < 4; ++i) {
+        const int j = (i & 1) + 2 * (i & 2);
+        h[i] = __fadd_rn(up ? s[j + 2] : s[j], __shfl_xor_sync(0xffffffffu, up ? s[j] : s[j + 2], 2));
       }
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) {
-#pragma unroll
-        for (int j = 0; j < o; ++j) s[j] = __fadd_rn(s[j], s[j + o]);
-      }
+      float n2 = __fadd_rn(__fadd_rn(odd ? h[1] : h[0], __shfl_xor_sync(0xffffffffu, odd ? h[0] : h[1], 1)),
+                           __fadd_rn(odd ? h[3] : h[2], __shfl_xor_sync(0xffffffffu, odd ? h[2] : h[3], 1)));
+      n2 = __fadd_rn(n2, __shfl_xor_sync(0xffffffffu, n2, 2));
+      n2 = __fadd_rn(n2, __shfl_xor_sync(0xffffffffu, n2, 1));
       float* row = rows + row_at<kInPitch>(is_v * kUnits + r) + 8 * c;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         row[j] = a[j];
         row[32 + j] = b[j];
       }
-      if (c == 0) norm[is_v * kUnits + r] = __fsqrt_rn(s[0]);
+      if (c == 0) norm[is_v * kUnits + r] = __fsqrt_rn(n2);
     }
   }
   __syncthreads();
