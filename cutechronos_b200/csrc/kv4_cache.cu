@@ -377,11 +377,14 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn
             Places at, int* __restrict__ err) {
   pdl_launch_dependents();
   __shared__ __align__(16) float rows[kRowsWords<kOutPitch>];
-  __shared__ __align__(16) float level[8];
+  __shared__ __align__(16) float level[16];  // of a code, sign and magnitude
   const int tid = threadIdx.x;
   if (tid == 0) {
-    reinterpret_cast<float4*>(level)[0] = levels_lo;
-    reinterpret_cast<float4*>(level)[1] = levels_hi;
+    float4* to = reinterpret_cast<float4*>(level);
+    to[0] = levels_lo;
+    to[1] = levels_hi;
+    to[2] = make_float4(-levels_lo.x, -levels_lo.y, -levels_lo.z, -levels_lo.w);
+    to[3] = make_float4(-levels_hi.x, -levels_hi.y, -levels_hi.z, -levels_hi.w);
   }
   pdl_wait();
   __syncthreads();
@@ -407,9 +410,8 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn
       for (int i = 0; i < 64; ++i) {
         const uint32_t w = word[i >> 3];
         const int p = i & 7;
-        const uint32_t sel = (p ? w >> (4 * p - 2) : w << 2) & 28u;  // a level's byte offset
-        const float x = *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(level) + sel);
-        y[i] = __uint_as_float(__float_as_uint(x) ^ ((w << (31 - sign_bit(p))) & 0x80000000u));
+        const uint32_t sel = (p ? w >> (4 * p - 2) : w << 2) & 60u;  // a level's byte offset
+        y[i] = *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(level) + sel);
       }
       walsh(y);
     }
