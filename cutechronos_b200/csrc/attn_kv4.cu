@@ -100,12 +100,18 @@ using namespace tcx;
 
 constexpr int kStageKeys = 64;
 constexpr int kStageBytes = kStageKeys / kBlockTokens * kBlockBytes;  // 4352
-// bf16 rows of a sequence and head above which the tcgen05 kernel takes over.  It
-// costs the same for 17 rows as for 128; this one costs a pass over the keys for
-// each 32.  This one / tcgen05, us, 8 heads, 16 sequences of 8192 tokens: 72 / 123
-// with 32 rows, 106 / 128 with 40, 115 / 131 with 64; 64 sequences of 1024: 79 / 70
-// with 20, 90 / 70 with 32, 138 / 72 with 40.
-constexpr int kTcMoreThan = 32;
+// Whether a bf16 call is the tcgen05 kernel's.  It costs the same for 17 rows of a
+// sequence and head as for 128; this one costs a pass over the keys for each 32
+// rows, but less for a key and more for a sequence.  This one / tcgen05, us, 8 heads:
+//   20 to 24 rows, 256 sequences of 1024 tokens 237 / 203, of 1500 271 / 274,
+//   64 sequences of 512 62 / 47, of 2048 102 / 117, 16 of 8192 72 / 123;
+//   32 rows, 256 sequences of 256 tokens 129 / 90, 64 of 1024 90 / 70, 32 of 4096 79 / 117;
+//   40 rows, 64 sequences of 2048 tokens 165 / 127, 32 of 4096 121 / 121, 16 of 8192 106 / 128;
+//   64 rows, 64 sequences of 2048 tokens 183 / 138, 32 of 4096 136 / 127, 1 of 32768 52 / 43;
+//   16 rows, 256 sequences of 512 tokens 130 / 129, 64 of 1024 55 / 67.
+bool for_tcgen05(int dtype, int rows, int max_len) {
+  return dtype == CC2_BF16 && (rows > 32 || (rows > 16 && max_len <= 1024));
+}
 constexpr int kQPitch = 72;  // halves
 constexpr int kOPitch = 66;  // floats
 
@@ -763,7 +769,7 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
               std::max(max_q, total_q));
   const int rows = std::max(1, max_q * (q_heads / pool.heads));
   p = Plan{};
-  p.tc = dtype == CC2_BF16 && rows > kTcMoreThan;
+  p.tc = for_tcgen05(dtype, rows, max_len);
   // As few columns as hold the rows: with 16 sequences of 8192 tokens and 8 heads, one / two / four blocks of 8 take
   // 35 / 43 / 61 us for 4 rows, 56 / 47 / 66 for 12, 92 / 72 / 73 for 32 (there four spare half the passes over the
   // keys' bytes); a block with 4 rows in column pairs and one with 8 35 / 39.  fp32 splits need the registers of four.

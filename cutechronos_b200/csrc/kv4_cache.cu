@@ -19,14 +19,14 @@
 //    in one piece, and rows come in and go out as whole lines: with the 64 units
 //    in (token, head) order each owner's 32 bytes were a line of their own;
 //  - places in the cache, pointers and positions are worked out once a vector.
-// Measured, 131072 tokens of 8 heads, bf16: append 171 us (340 MB, 2.0 TB/s),
-// read 103 us (3.3 TB/s); read of 24 sequences of 4001 entries as fp32 55 us
-// (4.7 TB/s).  Append uses 79% of the shared-memory pipe's cycles (an owner's 64
-// loads, the 64 stores before them, 64 table lookups of which several meet in a
-// bank, the shuffles of the norm) and 66% of the issue slots; read 63% and 71%;
-// registers (80) and rows leave room for 24 warps an SM.  Tables of single words
-// (half the bank conflicts, one load more) took 174 us, 16 copies of the table
-// 206, three comparisons in place of the table 260.
+// Measured, 131072 tokens of 8 heads, bf16: append 166 us (340 MB, 2.0 TB/s),
+// read 96 us (3.5 TB/s); read of 24 sequences of up to 8192 entries as fp32 53 us
+// (4.9 TB/s).  Append uses 77% of the shared-memory pipe's cycles (an owner's 64
+// loads, the 64 stores before them, 64 table lookups of which some meet in a
+// bank) and 67% of the issue slots; read 68% and 69%; registers (80) and rows
+// leave room for 24 warps an SM.  At an earlier state (171 us) tables of single
+// words (fewer bank conflicts, one load more) took 174 us; 16 copies of the table
+// took 206 and three comparisons in place of the table 260.
 #include <algorithm>
 #include <cmath>
 

@@ -670,3 +670,13 @@ def test_rounding_of_a_long_context(group, new):
     want, *_ = oracle_attention(cache, params, q, [20000], table, [0, new], True, 0.5, False)
     own = (want.to(torch.bfloat16).double() - want).norm()
     assert (got - want).norm() <= 1.12 * own
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("norm", ["float16", "bfloat16"])
+def test_17_to_32_rows_of_long_sequences(norm, causal):
+    """Beside the same rows of short sequences, which another kernel takes."""
+    new = [13, 16, 9, 0, 1, 15]
+    run_case([1500, 1100, 64, 5, 1, 1030], new, 2, 2, 32, norm, causal=causal, mask_every=7)
+    run_case([500, 1000, 64, 5, 1, 530], new, 2, 2, 32, norm, causal=causal, mask_every=7)
