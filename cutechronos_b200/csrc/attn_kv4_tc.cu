@@ -175,21 +175,13 @@ __device__ __forceinline__ bool elect_one() {
 // through shared memory as whole 128-byte lines.
 constexpr int kQThreads = 128;
 
-struct QueryRow {
-  int seq, q_start;  // -1: no sequence has it
-};
-__device__ __forceinline__ QueryRow find_row(const Args& a, int tok, int lane) {
-  QueryRow r;
-  if (a.cu == nullptr) {
-    r.seq = tok / a.max_q;
-    r.q_start = r.seq * a.max_q;
-    return r;
-  }
-  r.seq = -1;  // the last sequence that starts at or before the token
+// The last sequence that starts at or before the token; -1: none does.
+__device__ __forceinline__ int find_seq(const Args& a, int tok, int lane) {
+  if (a.cu == nullptr) return tok / a.max_q;
+  int seq = -1;
   for (int i = lane; i - lane < a.num_seqs; i += 32)
-    r.seq += __popc(__ballot_sync(0xffffffffu, i < a.num_seqs && a.cu[i] <= tok));
-  r.q_start = r.seq >= 0 ? a.cu[r.seq] : 0;
-  return r;
+    seq += __popc(__ballot_sync(0xffffffffu, i < a.num_seqs && a.cu[i] <= tok));
+  return seq;
 }
 
 __device__ __forceinline__ void mma_pm1(float (&d)[4], const uint32_t (&x)[4], uint2 b) {
@@ -218,14 +210,14 @@ rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles, c
   }
   {
     // this thread's row: a block's rows mostly belong to one sequence, the others follow it
-    const QueryRow at = find_row(a, base / a.group, lane);
+    const int near = find_seq(a, base / a.group, lane);
     const int row = base + tid;
     const __nv_bfloat16* from = nullptr;
     int pos = -1;
     long long to = -1;
     if (row < all) {
       const int tok = row / a.group;
-      int seq = at.seq;
+      int seq = near;
       if (a.cu == nullptr) seq = tok / a.max_q;
       else
         while (seq + 1 < a.num_seqs && a.cu[seq + 1] <= tok) ++seq;
