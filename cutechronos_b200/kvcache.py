@@ -109,6 +109,7 @@ class PagedKV4Cache:
             raise RuntimeError("cutechronos_b200 kernels take CUDA tensors only (no CPU path)")
         self.pages = torch.zeros(num_pages, nbytes.value, dtype=torch.uint8, device=device)
         self.device = self.pages.device
+        self._at = self.pages.get_device()
         self.num_pages, self.num_heads, self.page_size = num_pages, num_heads, page_size
         self.rope = rope_rows(max_positions, rope_theta, self.device) if rope_theta is not None else None
         self._c = nat.KV4Cache(self.pages.data_ptr(), num_pages, page_size, num_heads, NORMS[key.norm_dtype],
@@ -123,7 +124,7 @@ class PagedKV4Cache:
     # Plain code on purpose: a single-token step's kernels take about as long as these checks.
     def _call(self, fn, what: str, *args) -> None:
         """fn(cache, *args, stream) on the cache's device and the caller's current stream."""
-        i = self.device.index
+        i = self._at
         if torch._C._cuda_getDevice() == i:
             status = fn(self._ref, *args, _raw_stream(i))
         else:
@@ -133,7 +134,7 @@ class PagedKV4Cache:
             nat.check(status, what)
 
     def _index(self, t: torch.Tensor, what: str, dim: int = 1) -> torch.Tensor:
-        if t.device != self.device:
+        if t.get_device() != self._at:
             raise RuntimeError(f"{what} must be on {self.device}, got {t.device}")
         if t.dim() != dim:
             raise ValueError(f"{what} must have {dim} axis(es), got shape {tuple(t.shape)}")
@@ -144,7 +145,7 @@ class PagedKV4Cache:
         return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
 
     def _values(self, t: torch.Tensor, what: str) -> int:
-        if t.device != self.device:
+        if t.get_device() != self._at:
             raise RuntimeError(f"{what} must be on {self.device}, got {t.device} (no CPU path)")
         if t.dim() != 3 or t.shape[2] != DIM:
             raise ValueError(f"{what} must be (tokens, heads, {DIM}), got {tuple(t.shape)}")
