@@ -1057,7 +1057,8 @@ int launch_attend_tc(const Args& a, cudaStream_t st) {
     if (dev < 64) attr_done |= 1ull << dev;
   }
   const unsigned q_blocks = (unsigned)(((long long)a.total_q * a.group + 127) / 128);
-  // heads a block: as many as leave one round of blocks
+  // Heads a block: as many as leave one round of blocks.  1 / 2 / 3 / 6 / 12 of 12 heads with 408576 rows (6 leave one
+  // round): 182 / 170 / 170 / 167 / 174 us for the whole call.
   const int per = (int)std::min<long long>(a.pool.heads, ((long long)q_blocks * a.pool.heads + 4 * num_sms() - 1) / (4 * num_sms()));
   CC2_CUDA(launch_k(rotate_queries_kernel, dim3(q_blocks, (unsigned)((a.pool.heads + per - 1) / per)), kQThreads, 0, st, a,
                     q_tiles, per));
