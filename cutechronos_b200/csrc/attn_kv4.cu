@@ -185,9 +185,9 @@ struct Walk {
   long long unit;
   bool whole;
 
-  __device__ __forceinline__ void load(const Args& a, int lane, long long cost0, long long units0) {
+  __device__ __forceinline__ void load(const Args& a, int lane, long long cost0, long long units0, bool report = false) {
     mine = SeqCost{0, 0, 0, 0};
-    if (window + lane < a.num_seqs) mine = cost_of(a, window + lane);
+    if (window + lane < a.num_seqs) mine = cost_of(a, window + lane, report);
     long long c = mine.cost, u = mine.units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -203,10 +203,10 @@ struct Walk {
     long long total = 0;
     if (a.num_seqs <= 32) {
       window = 0;
-      load(a, lane, 0, 0);
+      load(a, lane, 0, 0, team == 0);  // what is out of range shows here: a sequence may have no unit
       total = window_end;
     } else {
-      for (int i = lane; i < a.num_seqs; i += 32) total += cost_of(a, i).cost;
+      for (int i = lane; i < a.num_seqs; i += 32) total += cost_of(a, i, team == 0).cost;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
       window = 0;
@@ -325,7 +325,7 @@ attend_kernel(const __grid_constant__ Args a) {
   walk.start(a, team_at, lane);
   auto next = [&](Unit& u) {
     if (!walk.next(a, lane)) return false;
-    u.s = span_of(a, walk.seq, walk.tile, warp == 0 && walk.head == 0 && walk.tile == 0 && walk.r0 == 0);
+    u.s = span_of(a, walk.seq, walk.tile, false);
     u.seq = walk.seq;
     u.head = walk.head;
     u.c0 = walk.r0 * (kWarps * kStageKeys);
@@ -648,6 +648,10 @@ attend_kernel(const __grid_constant__ Args a) {
         finish_row<T>(a, all.turns, s, u.head, s.row0 + r, o0, o1, top, sum, lane);
       } else {
         const long long at = u.piece * kRows + r;
+        if (at >= a.parts) {  // sequences that overlap have more units than rows make
+          if (lane == 0) atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+          continue;
+        }
         a.part[at * 64 + lane] = o0;
         a.part[at * 64 + lane + 32] = o1;
         if (lane == 0) a.part_ml[at] = make_float2(top, sum);
@@ -692,7 +696,7 @@ join_kernel(const __grid_constant__ Args a) {
   const int q0 = a.cu == nullptr ? seq * a.max_q : a.cu[seq];
   const int row = (tok - q0) * a.group + call_row % a.group;
   const Span s = span_of(a, seq, row / a.tile_rows, false);
-  if (row >= s.rows) return;
+  if (row < 0 || row >= s.rows) return;
   int chunks = chunks_of(a, s);
   long long first = part_at(a, s, head, 0, row), step = (long long)a.pool.heads * rows;
   if (kPieces) {
@@ -714,6 +718,7 @@ join_kernel(const __grid_constant__ Args a) {
     chunks = team_of(total, at + c.rounds - 1, a.teams) - t0 + 1;
     first = (units + k + t0) * a.tile_rows + row % a.tile_rows;
     step = a.tile_rows;
+    if (first + (chunks - 1) * step >= a.parts) return;  // as where they are written
   }
   if (chunks <= 1) return;
   float top = -INFINITY;
@@ -941,6 +946,7 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   a.row_tiles = p.row_tiles;
   a.tile_rows = p.tile_rows;
   a.teams = p.teams;
+  a.parts = (long long)(p.part_bytes / (64 * sizeof(float)));
   a.round_keys = p.round_keys;
   a.causal = causal != 0;
   a.rotate = rotate_q != 0;

@@ -224,7 +224,7 @@ rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles, c
       if (seq >= 0) {
         const Span s = span_of(a, seq, 0, false);
         const int in_seq = row - s.q_start * a.group;
-        if (in_seq < s.rows) {
+        if (in_seq >= 0 && in_seq < s.rows) {  // a cu_q that falls may find a sequence that starts after the token
           from = (const __nv_bfloat16*)a.q + (long long)tok * a.q_ld + (long long)(row % a.group) * a.q_hs;
           to = first_query_tile(a, seq, s.q_start) * 128 + in_seq;
           if (a.rotate) pos = s.len - s.n + (tok - s.q_start);

@@ -43,6 +43,7 @@ struct Args {
   const float2* rope;
   float* part;       // tcgen05: [split][head][row of the call][64], else [piece][row][64]: a part's sums, rotated
   float2* part_ml;   // the same places: maximum (log2) and sum of exponentials
+  long long parts;   // else: the places there are
   const uint8_t* qt;  // rotated queries as fp16 tiles (attn_kv4_tc.cu) and their rows' scales
   const float* q_scale;
   int* counter;       // items that the tcgen05 kernel's blocks have taken
@@ -131,8 +132,8 @@ struct SeqCost {
   int rounds;      // of a unit's keys
   long long units, cost;
 };
-__device__ __forceinline__ SeqCost cost_of(const Args& a, int seq) {
-  const Span s = span_of(a, seq, 0, false);
+__device__ __forceinline__ SeqCost cost_of(const Args& a, int seq, bool report = false) {
+  const Span s = span_of(a, seq, 0, report);
   SeqCost c;
   c.tiles = (s.rows + a.tile_rows - 1) / a.tile_rows;
   c.rounds = max((s.len + a.round_keys - 1) / a.round_keys, 1);

@@ -680,3 +680,33 @@ def test_17_to_32_rows_of_long_sequences(norm, causal):
     new = [13, 16, 9, 0, 1, 15]
     run_case([1500, 1100, 64, 5, 1, 1030], new, 2, 2, 32, norm, causal=causal, mask_every=7)
     run_case([500, 1000, 64, 5, 1, 530], new, 2, 2, 32, norm, causal=causal, mask_every=7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [3, 60])
+def test_row_bounds_that_fall_or_overlap(rows, dtype):
+    """cu_q is device data that a call cannot check before it launches: bounds that fall, run past the rows or name the
+    same rows for many sequences leave unspecified rows, nothing else; a call after them is right."""
+    n = 12
+    cache, params, table, _ = filled([700] * n, 2, dtype=dtype)
+    lens = torch.full((n,), 700, dtype=torch.int32).cuda()
+    total = n * rows
+    q = torch.randn(total, 4, D, generator=torch.Generator().manual_seed(9)).to(dtype).cuda()
+    pages = cache.pages.clone()
+    good = torch.arange(0, total + 1, rows, dtype=torch.int32)
+    args = dict(max_q=total, scale=0.125, rotate_q=True)
+    want = cache.attention(q, lens, table.cuda(), cu_q=good.cuda(), **args)
+    falling = good.clone()
+    falling[0], falling[3], falling[7] = total // 2, 0, total + 50
+    again = torch.tensor([0, total] * (n // 2) + [0], dtype=torch.int32)
+    backwards = good.flip(0).contiguous()
+    for cu in (falling, again, backwards, torch.full_like(good, -7), torch.full_like(good, 2**31 - 1)):
+        out = torch.empty(total + 64, 4, D, dtype=dtype, device="cuda").fill_(7)
+        cache.attention(q, lens, table.cuda(), cu_q=cu.cuda(), out=out[32:-32], **args)
+        assert (out[:32] == 7).all() and (out[-32:] == 7).all()
+        with pytest.raises(nat.NativeError, match="out of range"):
+            cache.check()
+        assert torch.equal(cache.pages, pages)
+        assert torch.equal(cache.attention(q, lens, table.cuda(), cu_q=good.cuda(), **args), want)
+        cache.check()
