@@ -93,9 +93,10 @@ size_t gemm_f32_splitk_floats();
 int read_kv4_error(int clear, int* value);
 int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs, const void* v,
                       int64_t v_ld, int64_t v_hs, int T, const int32_t* seq, const int32_t* pos, const uint8_t* mask,
-                      const int32_t* table, int table_ld, int num_seqs, cudaStream_t st);
+                      const int32_t* table, int table_ld, int table_cols, int num_seqs, cudaStream_t st);
 int launch_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_out, int T, const int32_t* seq,
-                    const int32_t* pos, const int32_t* table, int table_ld, int num_seqs, cudaStream_t st);
+                    const int32_t* pos, const int32_t* table, int table_ld, int table_cols, int num_seqs,
+                    cudaStream_t st);
 int kv4_attention_workspace(const cc2_kv4_cache* cache, int dtype, int q_heads, int num_seqs, int total_q, int max_q,
                             int max_len, size_t* bytes);
 int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, int64_t q_ld, int64_t q_hs, void* out,
@@ -977,15 +978,29 @@ int cc2_model_set_kv_quant(cc2_model* m, int layer, const cc2_kvq* key, const cc
 int cc2_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs, const void* v,
                    int64_t v_ld, int64_t v_hs, int T, const int32_t* seq, const int32_t* pos,
                    const uint8_t* token_mask, const int32_t* block_table, int table_ld, int num_seqs, void* stream) {
+  return cc2_kv4_append_cols(cache, dtype, k, k_ld, k_hs, v, v_ld, v_hs, T, seq, pos, token_mask, block_table, table_ld,
+                             table_ld, num_seqs, stream);
+}
+
+int cc2_kv4_append_cols(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs, const void* v,
+                        int64_t v_ld, int64_t v_hs, int T, const int32_t* seq, const int32_t* pos,
+                        const uint8_t* token_mask, const int32_t* block_table, int table_ld, int table_cols,
+                        int num_seqs, void* stream) {
   clear_error();
   return launch_kv4_append(cache, dtype, k, k_ld, k_hs, v, v_ld, v_hs, T, seq, pos, token_mask, block_table, table_ld,
-                           num_seqs, (cudaStream_t)stream);
+                           table_cols, num_seqs, (cudaStream_t)stream);
 }
 
 int cc2_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_out, int T, const int32_t* seq,
                  const int32_t* pos, const int32_t* block_table, int table_ld, int num_seqs, void* stream) {
+  return cc2_kv4_read_cols(cache, dtype, k_out, v_out, T, seq, pos, block_table, table_ld, table_ld, num_seqs, stream);
+}
+
+int cc2_kv4_read_cols(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_out, int T, const int32_t* seq,
+                      const int32_t* pos, const int32_t* block_table, int table_ld, int table_cols, int num_seqs,
+                      void* stream) {
   clear_error();
-  return launch_kv4_read(cache, dtype, k_out, v_out, T, seq, pos, block_table, table_ld, num_seqs,
+  return launch_kv4_read(cache, dtype, k_out, v_out, T, seq, pos, block_table, table_ld, table_cols, num_seqs,
                          (cudaStream_t)stream);
 }
 

@@ -113,7 +113,7 @@ struct Places {
   const int32_t* seq;
   const int32_t* pos;
   const int32_t* table;
-  int table_ld, num_seqs;
+  int table_ld, table_cols, num_seqs;  // elements from row to row, entries of a row
 };
 
 // Byte offset of the block of token t's head, -1 for a token to skip.
@@ -122,7 +122,7 @@ __device__ __forceinline__ long long place(const Pool& pool, const Places& at, i
   const int s = at.seq[t], pos = at.pos[t];
   if (s < 0 || pos < 0) return -1;
   const int pg = pos >> pool.page_shift;
-  if (s >= at.num_seqs || pg >= at.table_ld || pos >= pos_limit) {
+  if (s >= at.num_seqs || pg >= at.table_cols || pos >= pos_limit) {
     atomicOr(err, (int)DEV_ERR_CACHE_RANGE);
     return -1;
   }
@@ -445,9 +445,10 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn
 }
 
 int check_places(const char* what, int T, const int32_t* seq, const int32_t* pos, const int32_t* table, int table_ld,
-                 int num_seqs) {
+                 int table_cols, int num_seqs) {
   CC2_REQUIRE(T >= 0 && seq && pos && table, "%s: null sequences, positions or block table", what);
-  CC2_REQUIRE(table_ld > 0 && num_seqs > 0, "%s: empty block table", what);
+  CC2_REQUIRE(table_cols > 0 && num_seqs > 0, "%s: empty block table", what);
+  CC2_REQUIRE(table_cols <= table_ld, "%s: block table of %d columns with rows %d apart", what, table_cols, table_ld);
   return CC2_OK;
 }
 
@@ -477,13 +478,13 @@ int read_kv4_error(int clear, int* value) {
 
 int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs, const void* v,
                       int64_t v_ld, int64_t v_hs, int T, const int32_t* seq, const int32_t* pos, const uint8_t* mask,
-                      const int32_t* table, int table_ld, int num_seqs, cudaStream_t st) {
+                      const int32_t* table, int table_ld, int table_cols, int num_seqs, cudaStream_t st) {
   using namespace kv4;
   Pool pool;
   CC2_TRY(check_cache(cache, "kv4_append", pool));
   CC2_REQUIRE(dtype == CC2_BF16 || dtype == CC2_F32, "kv4_append: unsupported dtype %d", dtype);
   if (T == 0) return CC2_OK;
-  CC2_TRY(check_places("kv4_append", T, seq, pos, table, table_ld, num_seqs));
+  CC2_TRY(check_places("kv4_append", T, seq, pos, table, table_ld, table_cols, num_seqs));
   CC2_REQUIRE(k && v, "kv4_append: null keys or values");
   CC2_REQUIRE(rows_ok(dtype, k, k_ld, k_hs) && rows_ok(dtype, v, v_ld, v_hs),
               "kv4_append: keys and values must start on 16 bytes, as must their strides");
@@ -495,7 +496,7 @@ int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int6
   CC2_TRY(make_turn(cache->key, "kv4_append", turn_k));
   CC2_TRY(make_turn(cache->value, "kv4_append", turn_v));
   CC2_TRY(make_cells(*cache, "kv4_append", cells));
-  const Places at{seq, pos, table, table_ld, num_seqs};
+  const Places at{seq, pos, table, table_ld, table_cols, num_seqs};
   const float2* rope = (const float2*)cache->rope_cs;
 #define CC2_APPEND(TT, ROPE)                                                                                        \
   CC2_CUDA(launch_k(append_kernel<TT, ROPE>, grid, kThreads, 0, st, pool, turn_k, turn_v, cells, (const TT*)k, (long long)k_ld,    \
@@ -512,13 +513,14 @@ int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int6
 }
 
 int launch_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_out, int T, const int32_t* seq,
-                    const int32_t* pos, const int32_t* table, int table_ld, int num_seqs, cudaStream_t st) {
+                    const int32_t* pos, const int32_t* table, int table_ld, int table_cols, int num_seqs,
+                    cudaStream_t st) {
   using namespace kv4;
   Pool pool;
   CC2_TRY(check_cache(cache, "kv4_read", pool));
   CC2_REQUIRE(dtype == CC2_BF16 || dtype == CC2_F32, "kv4_read: unsupported dtype %d", dtype);
   if (T == 0 || (!k_out && !v_out)) return CC2_OK;
-  CC2_TRY(check_places("kv4_read", T, seq, pos, table, table_ld, num_seqs));
+  CC2_TRY(check_places("kv4_read", T, seq, pos, table, table_ld, table_cols, num_seqs));
   CC2_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15u) == 0, "kv4_read: outputs must be 16-byte aligned");
   int grid = 0, *err = nullptr;
   CC2_TRY(grid_of(T, pool.heads, &grid));
@@ -532,7 +534,7 @@ int launch_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_
   }
   const float* lv = cache->levels;
   const float4 lo = make_float4(lv[0], lv[1], lv[2], lv[3]), hi = make_float4(lv[4], lv[5], lv[6], lv[7]);
-  const Places at{seq, pos, table, table_ld, num_seqs};
+  const Places at{seq, pos, table, table_ld, table_cols, num_seqs};
   if (dtype == CC2_BF16) {
     CC2_CUDA(launch_k(read_kernel<__nv_bfloat16>, grid, kThreads, 0, st, pool, turn_k, turn_v, lo, hi,
                       (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, T, at, err));

@@ -185,7 +185,7 @@ class PagedKV4Cache:
             raise ValueError(f"k and v must both be (tokens, {self.num_heads}, {DIM}) of one type, got "
                              f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
         seq, pos, n = self._places(seq_ids, positions, k.shape[0])
-        table, seqs, _, ld = self._table(block_table)
+        table, seqs, cols, ld = self._table(block_table)
         mask = None
         if token_mask is not None:
             if token_mask.shape != seq.shape or token_mask.device != self.device:
@@ -195,8 +195,8 @@ class PagedKV4Cache:
                 mask = mask.contiguous()
         per = _PER[k.dtype]
         (k, k_at), (v, v_at) = _rows(k, per), _rows(v, per)
-        self._call(self._lib.cc2_kv4_append, "cc2_kv4_append", code, *k_at, *v_at, n, seq.data_ptr(), pos.data_ptr(),
-                   None if mask is None else mask.data_ptr(), table.data_ptr(), ld, seqs)
+        self._call(self._lib.cc2_kv4_append_cols, "cc2_kv4_append", code, *k_at, *v_at, n, seq.data_ptr(), pos.data_ptr(),
+                   None if mask is None else mask.data_ptr(), table.data_ptr(), ld, cols, seqs)
 
     def read(self, seq_ids: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor, *,
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
@@ -206,11 +206,11 @@ class PagedKV4Cache:
         if code is None:
             raise TypeError(f"dtype {dtype} not supported (bfloat16 / float32)")
         seq, pos, n = self._places(seq_ids, positions, None)
-        table, seqs, _, ld = self._table(block_table)
+        table, seqs, cols, ld = self._table(block_table)
         k = torch.empty((n, self.num_heads, DIM), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        self._call(self._lib.cc2_kv4_read, "cc2_kv4_read", code, k.data_ptr(), v.data_ptr(), n, seq.data_ptr(),
-                   pos.data_ptr(), table.data_ptr(), ld, seqs)
+        self._call(self._lib.cc2_kv4_read_cols, "cc2_kv4_read", code, k.data_ptr(), v.data_ptr(), n, seq.data_ptr(),
+                   pos.data_ptr(), table.data_ptr(), ld, cols, seqs)
         return k, v
 
     def attention(self, q: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, *,

@@ -438,7 +438,9 @@ typedef struct {
 /* A cache (host struct, read by each call; the caller owns the memory it
  * points to).  Token `pos` of sequence s lies in page
  * block_table[s * table_ld + pos / page_size], a page holds page_size tokens
- * of all heads. */
+ * of all heads.  A table has table_ld entries a row; where it is a part of a
+ * wider one, the calls that end in _cols take its own columns beside table_ld,
+ * and attention's max_len must not pass them. */
 typedef struct {
   void* pages;            /* (dev) num_pages * cc2_kv4_page_bytes, 16-byte aligned */
   int num_pages;
@@ -467,6 +469,11 @@ CC2_API int cc2_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k,
                            const void* v, int64_t v_ld, int64_t v_hs, int T, const int32_t* seq,
                            const int32_t* pos, const uint8_t* token_mask, const int32_t* block_table,
                            int table_ld, int num_seqs, void* stream);
+/* The same for a block table of table_cols <= table_ld entries a row. */
+CC2_API int cc2_kv4_append_cols(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs,
+                                const void* v, int64_t v_ld, int64_t v_hs, int T, const int32_t* seq,
+                                const int32_t* pos, const uint8_t* token_mask, const int32_t* block_table,
+                                int table_ld, int table_cols, int num_seqs, void* stream);
 
 /* What T entries of the cache stand for, as dense rows k_out, v_out (dev,
  * dtype, (T, heads, 64); either may be NULL): keys as they were rotated.
@@ -474,6 +481,9 @@ CC2_API int cc2_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k,
 CC2_API int cc2_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_out, int T,
                          const int32_t* seq, const int32_t* pos, const int32_t* block_table, int table_ld,
                          int num_seqs, void* stream);
+CC2_API int cc2_kv4_read_cols(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_out, int T,
+                              const int32_t* seq, const int32_t* pos, const int32_t* block_table, int table_ld,
+                              int table_cols, int num_seqs, void* stream);
 
 /* Attention of total_q query rows over the cache.
  *   q, out     (dev, dtype) row i, head h at i * ld + h * hs (64 consecutive

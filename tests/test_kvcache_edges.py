@@ -1,0 +1,81 @@
+"""Edges of the paged 4-bit K/V cache: what lies beside a call's operands, values at the ends of their range, and the
+errors that calls leave for :meth:`PagedKV4Cache.check`."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+from cutechronos_b200 import _native as nat
+from test_kvcache import D, make
+
+I32 = dict(device="cuda", dtype=torch.int32)
+
+
+# ------------------------------------------------------------------ a block table within a wider one --
+def test_calls_are_bounded_by_a_tables_columns():
+    """What append and read hand to the library for a table of three columns within one of six: rows 6 apart, 3 long."""
+    from cutechronos_b200.kvcache import PagedKV4Cache
+
+    class Recorded(PagedKV4Cache):
+        def __init__(self):
+            self._at, self.device, self.num_heads, self.page_size = -1, torch.device("cpu"), 2, 16
+            self._lib = nat.load()
+
+        def _call(self, fn, what, *args):
+            self.last = args
+
+    cache = Recorded()
+    big = torch.arange(18, dtype=torch.int32).view(3, 6)
+    k = torch.zeros(5, 2, D)
+    seq, pos = torch.zeros(5, dtype=torch.int32), torch.arange(5, dtype=torch.int32)
+    for table, ld in ((big[:, 3:6], 6), (big[:1, 3:6], 3), (big[:, 3:6].clone(), 3), (big[:1, 3:6].expand(3, 3), 3)):
+        cache.append(k, k, seq, pos, table)
+        assert cache.last[-3:] == (ld, 3, table.shape[0])
+        cache.read(seq, pos, table)
+        assert cache.last[-3:] == (ld, 3, table.shape[0])
+
+
+def test_table_columns_are_checked():
+    lib = nat.load()
+    c = nat.KV4Cache(pages=1 << 20, num_pages=4, page_size=64, heads=2)
+    r = C.byref(c)
+    for ld, cols in ((4, 5), (4, 0), (0, 0), (4, -1)):
+        assert lib.cc2_kv4_append_cols(r, 1, 1 << 20, 128, 64, 1 << 20, 128, 64, 1, 64, 64, None, 64, ld, cols, 1, None) == -1
+        assert b"block table" in lib.cc2_last_error()
+        assert lib.cc2_kv4_read_cols(r, 1, 1 << 20, 1 << 20, 1, 64, 64, 64, ld, cols, 1, None) == -1
+        assert b"block table" in lib.cc2_last_error()
+
+
+@pytest.mark.gpu
+def test_positions_past_a_sliced_tables_columns():
+    """They are skipped and reported: neither the next row's pages nor what lies past the table is touched."""
+    cache, _ = make(18, 2, 16, max_positions=400)
+    big = torch.arange(18, **I32).view(3, 6)
+    table = big[:, 3:6]
+    g = torch.Generator().manual_seed(1)
+    k = torch.randn(1, 2, D, generator=g).cuda()
+    before = cache.pages.clone()
+    for s in range(3):
+        for p in (48, 63, 95, 399):
+            seq, pos = torch.tensor([s], **I32), torch.tensor([p], **I32)
+            cache.append(k, k, seq, pos, table)
+            with pytest.raises(nat.NativeError, match="out of range"):
+                cache.check()
+            assert torch.equal(before, cache.pages)
+            assert all((t == 0).all() for t in cache.read(seq, pos, table))
+            with pytest.raises(nat.NativeError, match="out of range"):
+                cache.check()
+    # what lies in the columns goes where a table of its own would put it
+    own, _ = make(18, 2, 16, max_positions=400)
+    seq = torch.arange(3, **I32).repeat_interleave(48)
+    pos = torch.arange(48, **I32).repeat(3)
+    k, v = (torch.randn(144, 2, D, generator=g).cuda() for _ in range(2))
+    cache.append(k, v, seq, pos, table)
+    own.append(k, v, seq, pos, table.contiguous())
+    assert torch.equal(cache.pages, own.pages) and not torch.equal(cache.pages, before)
+    for a, b in zip(cache.read(seq, pos, table), own.read(seq, pos, table.contiguous())):
+        assert torch.equal(a, b)
+    cache.check()
