@@ -59,6 +59,7 @@ int check_cache(const cc2_kv4_cache* c, const char* what, Pool& pool) {
   CC2_TRY(cc2_kv4_page_bytes(c->page_size, c->heads, &bytes));
   CC2_REQUIRE(c->norm_dtype == 0 || c->norm_dtype == 1, "%s: norm_dtype must be 0 (float16) or 1 (bfloat16)", what);
   CC2_REQUIRE(c->rope_cs == nullptr || c->rope_len > 0, "%s: rope_len must be positive", what);
+  CC2_REQUIRE(((uintptr_t)c->rope_cs & 15u) == 0, "%s: rope_cs must be 16-byte aligned", what);
   pool.pages = (uint8_t*)c->pages;
   pool.page_bytes = (long long)bytes;
   pool.head_bytes = c->page_size / kBlockTokens * kBlockBytes;

@@ -447,7 +447,7 @@ typedef struct {
   int page_size;          /* 16, 32, 64, 128 or 256 tokens */
   int heads;              /* key / value heads, 64 values each */
   int norm_dtype;         /* 0 float16, 1 bfloat16 */
-  const float* rope_cs;   /* (dev) float2 (cos, sin) [rope_len][32], or NULL: keys are not rotated */
+  const float* rope_cs;   /* (dev) float2 (cos, sin) [rope_len][32], 16-byte aligned, or NULL: keys are not rotated */
   int rope_len;
   float levels[8];        /* magnitudes, ascending; the negative half mirrors them */
   float bounds[7];        /* between them, ascending from above 0, more than 1/60 apart */

@@ -79,3 +79,14 @@ def test_positions_past_a_sliced_tables_columns():
     for a, b in zip(cache.read(seq, pos, table), own.read(seq, pos, table.contiguous())):
         assert torch.equal(a, b)
     cache.check()
+
+
+def test_rotation_table_must_be_aligned():
+    """The kernels read it 16 bytes at a time."""
+    lib = nat.load()
+    n = C.c_size_t()
+    c = nat.KV4Cache(pages=1 << 20, num_pages=4, page_size=64, heads=2, rope_cs=(1 << 20) + 8, rope_len=16)
+    assert lib.cc2_kv4_attention_workspace_bytes(C.byref(c), 1, 2, 1, 1, 1, 64, C.byref(n)) == -1
+    assert b"rope_cs must be 16-byte aligned" in lib.cc2_last_error()
+    c.rope_cs = 1 << 20
+    assert lib.cc2_kv4_attention_workspace_bytes(C.byref(c), 1, 2, 1, 1, 1, 64, C.byref(n)) == 0
