@@ -775,7 +775,9 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         kv.next();
         if (j >= steps) continue;
         const int key0 = c0 + j * kStep;
-        const float sc = rs * __int_as_float((ex.x + 1) << 23);  // rs 2^(eK - 126)
+        // rs 2^(eK - 126).  Both are least where there is nothing to scale, a row of zeros over keys of zero norm or all
+        // masked; their product would be 0 then and 0 * -inf, a hidden score, NaN.  At 2^-100 scores are 0 all the same.
+        const float sc = fmaxf(rs * __int_as_float((ex.x + 1) << 23), 0x1p-100f);
         const bool clean = key0 + kStep <= clear && (note.seen[0] & note.seen[1]) == 0xffffffffu &&
                            (note.poison[0] | note.poison[1]) == 0;
         const int cols = min(keys - j * kStep, kStep);

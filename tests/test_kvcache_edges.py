@@ -4,12 +4,13 @@ errors that calls leave for :meth:`PagedKV4Cache.check`."""
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import pytest
 import torch
 
 from cutechronos_b200 import _native as nat
-from test_kvcache import D, make
+from test_kvcache import D, allowed, make, oracle_attention
 
 I32 = dict(device="cuda", dtype=torch.int32)
 
@@ -90,3 +91,52 @@ def test_rotation_table_must_be_aligned():
     assert b"rope_cs must be 16-byte aligned" in lib.cc2_last_error()
     c.rope_cs = 1 << 20
     assert lib.cc2_kv4_attention_workspace_bytes(C.byref(c), 1, 2, 1, 1, 1, 64, C.byref(n)) == 0
+
+
+# -------------------------------------------------------------------- scores and values at their ends --
+def against_oracle(cache, params, table, q, lens, new, scale, sway=None, causal=True):
+    """Output and log-sum-exp of a call next to the 64-bit ones, within ``allowed``; as a whole the rounding is random."""
+    f32 = q.dtype == torch.float32
+    out, lse = cache.attention(q.cuda(), torch.tensor(lens, **I32), table.cuda(), scale=scale, causal=causal, return_lse=True)
+    want, wlse, most, weight = oracle_attention(cache, params, q, lens, table, [i * new for i in range(len(lens) + 1)],
+                                                causal, scale, False)
+    tol, ltol = allowed(want, most if sway is None else sway, weight, f32)
+    assert torch.isfinite(out).all()
+    err = (out.double().cpu() - want).norm(dim=-1)
+    assert (err <= tol).all(), (err / tol).max()
+    assert err.norm() <= want.norm() * (2.0 ** -17 if f32 else 2.0 ** -8)
+    empty, lse = wlse == -math.inf, lse.double().cpu()
+    assert torch.equal(lse == -math.inf, empty) and (out.cpu()[empty] == 0).all()
+    assert ((lse - wlse).abs()[~empty] <= ltol[~empty]).all()
+    cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 20, 40, 200])
+@pytest.mark.parametrize("zero", ["queries", "scale", "all"])
+@pytest.mark.parametrize("what", ["masked", "keys", "masked and keys", "all masked"])
+def test_scores_of_zero_beside_blocks_of_masked_or_zero_keys(what, zero, new, dtype):
+    """Rows of zeros, a scale of zero, or both, over blocks of 128 keys that are all masked, of zero norm, or both: the
+    mean of the values that a row sees, and nothing where it sees none."""
+    n = 400
+    cache, params = make(8, 2, 64, theta=None)
+    g = torch.Generator().manual_seed(31)
+    k, v = (torch.randn(n, 2, D, generator=g) for _ in range(2))
+    q = torch.randn(new, 4, D, generator=g)
+    at = torch.arange(n, dtype=torch.int32)
+    mask = torch.ones(n, dtype=torch.bool)
+    if "masked" in what:
+        mask[:256] = False  # two whole blocks, and their rows' only keys
+    if what == "all masked":
+        mask[:] = False
+    if "keys" in what:
+        k[200:] = 0.0       # the rest of a block, a whole one and a last one of 16 keys
+    if zero != "scale":
+        q[::2] = 0.0
+    if zero == "all":
+        q[:] = 0.0
+    table = torch.tensor([[5, 1, 0, 7, 2, 6, 3]], dtype=torch.int32)
+    cache.append(k.to(dtype).cuda(), v.to(dtype).cuda(), torch.zeros(n, **I32), at.cuda(), table.cuda(),
+                 token_mask=mask.cuda())
+    against_oracle(cache, params, table, q.to(dtype), [n], new, 0.0 if zero == "scale" else 0.125)
