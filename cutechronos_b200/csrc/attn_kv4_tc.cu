@@ -21,17 +21,22 @@
 // maximum, sum and O of its own.  One warp alone leaves its scheduler idle most
 // of the time (each of the steps waits for the one before it); four warps a
 // scheduler, none of which waits for another, fill it.
-// Exponents: K^ of a block is scaled by 2^-eK with eK from its largest norm,
-// which goes into the scores' factor; V^ by 2^-eV, which goes into P's exponent
-// against the largest eV so far.  Neither costs an operation a score.
+// Exponents: K^ of a block is scaled by 2^(8 - eK) with eK from its largest norm
+// (norms below 2^8, products with the levels below 2^15), which goes into the
+// scores' factor; V^ by 2^(8 - eV), which goes into P's exponent.  A row's
+// running maximum is that of score + eV of the score's block, so what P and V^
+// have as fp16 is measured against the largest P V of the blocks so far and not
+// against the largest V: P = 2^(x + eV - m + 7), up to 2^15.  Neither costs an
+// operation a score.  fp16 keeps its 11 bits down to 2^-22 of a block's largest
+// norm and of a row's largest P 2^eV.
 // A masked key's column is -inf and its V^ zero.  A K or V that is not finite
 // is zero too and instead marks the rows that see it (their sum becomes NaN), so
 // that it cannot reach the others through 0 * NaN.
 // Every wait is bounded (about 2 s): on expiry all roles leave their loops,
 // copies and MMAs in flight are waited for, TMEM is freed, the kernel returns.
 // Measured: 2048, 1450 and 853 tokens against 16384, 11603 and 6822 keys, 4
-// heads on each of 8, causal, 726 us, 594 TFLOP/s of the scores' and values'
-// products; 256 series of 133 tokens, 12 heads, 167 us (40 of them the first
+// heads on each of 8, causal, 723 us, 597 TFLOP/s of the scores' and values'
+// products; 256 series of 133 tokens, 12 heads, 164 us (40 of them the first
 // kernel).  What bounds it: issue slots are 65% used, the exponentials' unit 60%,
 // and a step's chain of waits does not fill the rest; a third of the instructions
 // are the decoders', two thirds the softmax'.  Computing part of the exponentials
@@ -63,7 +68,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr int kStep = 64;                       // keys of a step of the softmax
 // TMEM columns of tile g, chain c: S (and P over it) at 128 g + 64 c, O at 256 + 128 g + 64 c
 constexpr uint32_t kSCol = 0, kOCol = 256;
-constexpr float kRescaleLog2 = 8.0f;
+constexpr float kRescaleLog2 = 8.0f, kLiftLog2 = 7.0f;  // P up to 2^(8 + 7)
 
 __device__ __forceinline__ uint32_t idesc_f16(int M, int N, bool b_mn_major) {
   return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
@@ -99,9 +104,8 @@ struct Control {
   uint64_t s_full[2][2], p_full[2][2];  // [tile][chain]
   Item items[kItems];
   alignas(16) Note notes[kKvStages][2];
-  int2 exps[kKvStages];                 // eK, eV
+  alignas(16) float4 exps[kKvStages];   // 2^(eK - 134), eV - 126, 2^(119 - eV)
   float m[2][2][2][128], l[2][2][2][128];  // [turn][tile][chain][row]
-  int ve[2][2][2];
   uint32_t top[2][4];
   uint32_t tmem;
   int abort_flag;
@@ -680,7 +684,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         if (lane == 0) ctl.top[flip][w] = tk | tv << 16;
         ok = barrier_and(1, 128, ok);
         if (!ok) break;
-        uint32_t ek = 20, ev = 20;
+        uint32_t ek = 20, ev = 40;  // 2^-86: a row's sum, in units of 2^-eV, stays far inside fp32
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t t = ctl.top[flip][i];
@@ -691,11 +695,13 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         if (lane == 0) {
           ctl.notes[kv.i][w >> 1].seen[w & 1] = sb;
           ctl.notes[kv.i][w >> 1].poison[w & 1] = pb;
-          if (w == 0) ctl.exps[kv.i] = make_int2((int)ek, (int)ev);
+          if (w == 0)
+            ctl.exps[kv.i] = make_float4(__int_as_float(((int)ek - 7) << 23), (float)((int)ev - 126),
+                                         __int_as_float((246 - (int)ev) << 23), 0.0f);
         }
-        // norms below 1: 2^(126 - e)
-        const __half2 hk = __float2half2_rn(nk * __int_as_float((253 - (int)ek) << 23));
-        const __half2 hv = __float2half2_rn(nv * __int_as_float((253 - (int)ev) << 23));
+        // norms below 2^8: 2^(134 - e)
+        const __half2 hk = __float2half2_rn(nk * __int_as_float((261 - (int)ek) << 23));
+        const __half2 hv = __float2half2_rn(nv * __int_as_float((261 - (int)ev) << 23));
         const uint32_t dst = smem + kKvAt + kv.i * 2 * kTileBytes + k * 128;
         // warps past the last key's group of 16 have nothing that an MMA reads
         const bool used = 32 * w < c1 - (c0 + j * kTile);
@@ -759,8 +765,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
       it.next();
       if (seq < 0) break;
       const float rs = valid ? *q_scale : 0.0f;
-      float m = -INFINITY, l = 0.0f;
-      int ve = 20;
+      float m = -INFINITY, l = 0.0f;  // largest score + eV, sum of 2^(score - m)
       for (int t = 0; t < all; ++t) {
         // the decoders' notes on the block, then the scores
         if (!wait(ctl.kv_full[kv.i], kv.phase, ctl, err)) {
@@ -769,15 +774,15 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         }
         const int j = 2 * t + c;
         const Note note = ctl.notes[kv.i][c];
-        const int2 ex = ctl.exps[kv.i];
+        const float4 ex = ctl.exps[kv.i];
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctl.kv_empty[kv.i]));
         kv.next();
         if (j >= steps) continue;
         const int key0 = c0 + j * kStep;
-        // rs 2^(eK - 126).  Both are least where there is nothing to scale, a row of zeros over keys of zero norm or all
+        // rs 2^(eK - 134).  Both are least where there is nothing to scale, a row of zeros over keys of zero norm or all
         // masked; their product would be 0 then and 0 * -inf, a hidden score, NaN.  At 2^-100 scores are 0 all the same.
-        const float sc = fmaxf(rs * __int_as_float((ex.x + 1) << 23), 0x1p-100f);
+        const float sc = fmaxf(rs * ex.x, 0x1p-100f);
         const bool clean = key0 + kStep <= clear && (note.seen[0] & note.seen[1]) == 0xffffffffu &&
                            (note.poison[0] | note.poison[1]) == 0;
         const int cols = min(keys - j * kStep, kStep);
@@ -824,21 +829,15 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
               b3 = max3(b3, __uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
             }
           }
-          const float bm = fmaxf(max3(b0, b1, b2), b3) * sc;
+          const float bm = fmaf(fmaxf(max3(b0, b1, b2), b3), sc, ex.y);
           if (bm > m + kRescaleLog2 || (m == -INFINITY && bm > m)) {
             scale = m == -INFINITY ? 0.0f : ex2(m - bm);
             l *= scale;
             m = bm;
             rescale = true;
           }
-          if (ex.y > ve) {
-            scale *= __int_as_float((127 - min(ex.y - ve, 126)) << 23);
-            ve = ex.y;
-            rescale = true;
-          }
-          // P = 2^(x - m) times 2^(eV - largest eV), the latter taken back out of the row's sum
-          const float dv = (float)max(ex.y - ve, -60);
-          const float off = (m == -INFINITY ? 0.0f : -m) + dv;
+          // P = 2^(x + eV - m + 7), of which the row's sum takes 2^(eV + 7) back out
+          const float off = ex.y + kLiftLog2 - (m == -INFINITY ? 0.0f : m);
           const uint64_t sc2 = f2_pack(sc, sc), off2 = f2_pack(off, off);
           uint64_t la = f2_pack(0.0f, 0.0f), lb = la;
 #pragma unroll
@@ -861,7 +860,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
           }
           float l0, l1;
           f2_unpack(f2_add(la, lb), l0, l1);
-          l += (l0 + l1) * __int_as_float((127 - (int)dv) << 23);
+          l += (l0 + l1) * ex.z;
         }
         if (t > 0 && __any_sync(0xffffffffu, rescale)) {  // S_j's completion said that O stands still
 #pragma unroll 1
@@ -882,7 +881,6 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
           const int turn = (int)(nt & 1u);
           ctl.m[turn][g][c][r] = m;
           ctl.l[turn][g][c][r] = l;
-          if (at == 0) ctl.ve[turn][g][c] = ve;
         }
         tmem_st_wait();
         tc_fence_before();
@@ -936,11 +934,11 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         m = fmaxf(ma, mb);
         const float wa = ma == -INFINITY ? 0.0f : ex2(ma - m), wb = mb == -INFINITY ? 0.0f : ex2(mb - m);
         l = ctl.l[turn][g][0][r] * wa;
-        // 2^(eV - 126) / 64 takes the scales of V and of the levels back out
-        fa = wa * __int_as_float((ctl.ve[turn][g][0] - 5) << 23);
+        // 2^-7, 2^-8 and 1 / 64 take the scales of P, V and the levels back out
+        fa = wa * 0x1p-21f;
         if (two) {
           l += ctl.l[turn][g][1][r] * wb;
-          fb = wb * __int_as_float((ctl.ve[turn][g][1] - 5) << 23);
+          fb = wb * 0x1p-21f;
         }
       }
       const bool part = e.chunks > 1;

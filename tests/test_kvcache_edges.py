@@ -140,3 +140,29 @@ def test_scores_of_zero_beside_blocks_of_masked_or_zero_keys(what, zero, new, dt
     cache.append(k.to(dtype).cuda(), v.to(dtype).cuda(), torch.zeros(n, **I32), at.cuda(), table.cuda(),
                  token_mask=mask.cuda())
     against_oracle(cache, params, table, q.to(dtype), [n], new, 0.0 if zero == "scale" else 0.125)
+
+
+def spread_case(spread, where, new, dtype):
+    """300 keys of norm about 1, of values of norm 2^(15 - spread), but for one of norm 2^15 that has no weight (a key far
+    against the queries' common direction) or that only the last row could see."""
+    n, at = 300, {"first block": 3, "second block": 200, "last": 299}[where]
+    cache, params = make(6, 1, 64, theta=None)
+    g = torch.Generator().manual_seed(41)
+    unit = lambda t: t / t.norm(dim=-1, keepdim=True)  # noqa: E731
+    u = unit(torch.randn(D, generator=g))
+    k, v = unit(torch.randn(n, 1, D, generator=g)), unit(torch.randn(n, 1, D, generator=g)) * 2.0 ** (15 - spread)
+    k[at], v[at] = -60 * u, v[at] * 2.0 ** spread
+    q = (unit(torch.randn(new, 2, D, generator=g)) + 2 * u).to(dtype)
+    table = torch.tensor([[4, 1, 0, 5, 2]], dtype=torch.int32)
+    cache.append(k.to(dtype).cuda(), v.to(dtype).cuda(), torch.zeros(n, **I32), torch.arange(n, **I32), table.cuda())
+    # the one key's weight is under 2^-60: its score may be off by what it likes
+    sway = q.double().norm(dim=-1) * 1.2
+    against_oracle(cache, params, table, q, [n], new, 1.0, sway)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["first block", "second block", "last"])
+@pytest.mark.parametrize("new", [1, 7, 12, 20, 140])
+@pytest.mark.parametrize("spread", [0, 10, 13, 16, 18, 20])
+def test_one_value_far_larger_than_those_that_count(spread, new, where):
+    spread_case(spread, where, new, torch.bfloat16)
