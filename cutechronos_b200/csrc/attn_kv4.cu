@@ -34,7 +34,11 @@
 // 16 warps an SM that the table and the rings leave room for.
 // What must not leave the type's range is scaled by powers of two, which are
 // exact: a row of Q to below 2^8, P n_v to below 2^14 against the largest norm
-// met so far.
+// met so far; in fp32 calls against the row's largest P n_v itself, so that two
+// fp16 parts keep 2^-22 of it whatever the norms beside it (against the largest
+// norm a row was off by 6e-5 where that was 2^16 above those that counted; the
+// row's own costs 3 to 4%: 64 sequences of 4096 tokens, 8 heads, 2 rows a head
+// 94 us for 91).
 // Rounding: P n_v to fp16 (2^-12 of each, next to the output's bf16 with 2^-9),
 // the levels to fp16 after a common factor that moves all of them close to its
 // values, Q to one or two fp16 parts (split_q).  fp32 calls split all three into
@@ -416,10 +420,12 @@ attend_kernel(const __grid_constant__ Args a) {
     const int clear = a.causal ? s.len - s.n + s.row0 / a.group + 1 : s.len;
 
     float m[NB][2], lift[NB][2], neg[NB][2], l[NB][2], acc[4][NB][4];
+    int pe[NB][2];  // fp32: exponent of the row's largest P n_v
   #pragma unroll
     for (int b = 0; b < NB; ++b) {
       m[b][0] = m[b][1] = lift[b][0] = lift[b][1] = -INFINITY;
       neg[b][0] = neg[b][1] = 0.0f;
+      pe[b][0] = pe[b][1] = 20;
       l[b][0] = l[b][1] = 0.0f;
   #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i][b][0] = acc[i][b][1] = acc[i][b][2] = acc[i][b][3] = 0.0f;
@@ -482,13 +488,15 @@ attend_kernel(const __grid_constant__ Args a) {
 
       // The running maximum moves only when a score is more than 2^8 above it, the
       // largest norm when a larger one comes; then the sums so far follow.
-      const int ve_new = max(ve, (int)(__reduce_max_sync(0xffffffffu, top) >> 23));
+      const int ve_new = F32 ? ve : max(ve, (int)(__reduce_max_sync(0xffffffffu, top) >> 23));
       float mx[NB][2];
+      float drop[NB][2];  // fp32: log2 of what the maximum's move takes the sums down by
       bool moved = ve_new != ve;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int c = 0; c < kPer; ++c) {
+          drop[b][c] = 0.0f;
           float v = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 4; ++j) v = max3(v, x[j][b][c], x[j][b][c + 2]);
@@ -505,11 +513,13 @@ attend_kernel(const __grid_constant__ Args a) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
             v = fmaxf(m[b][c], v);
-            const float f = m[b][c] == -INFINITY ? 0.0f : ex2((m[b][c] - v) * rs[b][c]);
+            drop[b][c] = m[b][c] == -INFINITY ? -INFINITY : (m[b][c] - v) * rs[b][c];
+            const float f = ex2(drop[b][c]);
             m[b][c] = v;
             neg[b][c] = v == -INFINITY ? 0.0f : -v * rs[b][c];
             lift[b][c] = v + 8.0f / rs[b][c];  // -inf until a key is seen
             l[b][c] *= f;
+            if (F32) continue;  // its sums follow below
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               acc[k][b][c] *= f * fv;
@@ -517,6 +527,62 @@ attend_kernel(const __grid_constant__ Args a) {
             }
           }
         ve = ve_new;
+      }
+      float up[NB][2];  // fp32: 2^(140 - pe)
+      if (F32) {
+        // Scores become P n_v.  The exponent that a row's have moves when one passes 2^15 by it or its maximum moved; then
+        // the sums so far follow.
+        bool other = moved;
+        float most[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          most[b][0] = most[b][1] = 0.0f;
+          const uint64_t r2 = f2_pack(rs[b][0], rs[b][1]), g2 = f2_pack(neg[b][0], neg[b][1]);
+          uint64_t l2 = f2_pack(l[b][0], l[b][1]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float& v0 = x[j][b][2 * i];
+              float& v1 = x[j][b][2 * i + 1];
+              float p0, p1;
+              f2_unpack(f2_fma(f2_pack(v0, v1), r2, g2), p0, p1);
+              const uint64_t p2 = f2_pack(ex2(p0), ex2(p1));
+              l2 = f2_add(l2, p2);
+              f2_unpack(f2_mul(p2, f2_pack(nv[j][i], nv[j][i])), p0, p1);
+              v0 = kEdge && v0 == -INFINITY ? 0.0f : p0;  // a key that a row does not see adds nothing
+              v1 = kEdge && v1 == -INFINITY ? 0.0f : p1;
+              most[b][0] = fmaxf(most[b][0], v0);
+              most[b][1] = fmaxf(most[b][1], v1);
+            }
+          f2_unpack(l2, l[b][0], l[b][1]);
+          other = other || (int)(__float_as_uint(most[b][0]) >> 23) > pe[b][0] + 1 ||
+                  (int)(__float_as_uint(most[b][1]) >> 23) > pe[b][1] + 1;
+        }
+        if (__any_sync(0xffffffffu, other)) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) {
+              float v = most[b][c];
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+              const bool none = drop[b][c] == -INFINITY;
+              const int e = max(none ? 20 : max(20, pe[b][c] + (int)ceilf(fmaxf(drop[b][c], -300.0f))),
+                                (int)(__float_as_uint(v) >> 23));
+              const float fit = none ? 0.0f : ex2(drop[b][c] + (float)(pe[b][c] - e));
+              pe[b][c] = e;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                acc[k][b][c] *= fit;
+                acc[k][b][c + 2] *= fit;
+              }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int c = 0; c < kPer; ++c) up[b][c] = __int_as_float((267 - pe[b][c]) << 23);
       }
       const float vs = __int_as_float((259 - ve) << 23);  // 2^(132 - ve): norms below 2^6, P n_v below 2^14
 
@@ -528,7 +594,11 @@ attend_kernel(const __grid_constant__ Args a) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           float p[4];
-          if (kPaired) {  // the odd columns' stay zero
+          if (F32) {
+            const uint64_t u2 = f2_pack(up[b][0], up[b][1]);
+            f2_unpack(f2_mul(f2_pack(x[j][b][0], x[j][b][1]), u2), p[0], p[1]);
+            f2_unpack(f2_mul(f2_pack(x[j][b][2], x[j][b][3]), u2), p[2], p[3]);
+          } else if (kPaired) {  // the odd columns' stay zero
             p[1] = p[3] = 0.0f;
             f2_unpack(f2_fma(f2_pack(x[j][b][0], x[j][b][2]), f2_pack(rs[b][0], rs[b][0]), f2_pack(neg[b][0], neg[b][0])), p[0], p[2]);
             p[0] = ex2(p[0]);
@@ -544,7 +614,8 @@ attend_kernel(const __grid_constant__ Args a) {
             }
             f2_unpack(f2_add(f2_add(f2_pack(l[b][0], l[b][1]), f2_pack(p[0], p[1])), f2_pack(p[2], p[3])), l[b][0], l[b][1]);
           }
-          if (kEdge) {  // a key that a row does not see adds nothing, whatever its norm
+          if (F32) {
+          } else if (kEdge) {  // a key that a row does not see adds nothing, whatever its norm
 #pragma unroll
             for (int c = 0; c < 4; c += 3 - kPer) p[c] = x[j][b][c] == -INFINITY ? 0.0f : p[c] * (c < 2 ? nv[j][0] : nv[j][1]) * vs;
           } else if (kPaired) {
@@ -611,11 +682,11 @@ attend_kernel(const __grid_constant__ Args a) {
     more = next(coming);
     if (sums_in_a_slot<R>() && more && !broken && coming.stages > 0) issue(coming, 0, n), ahead = 1;
     float* mine_sums = reinterpret_cast<float*>(sm.ring[warp][sums_in_a_slot<R>() ? (n + 1u) & 1u : 0]);
-    const float down = __int_as_float((ve - 11) << 23);  // 2^(ve - 132) / 64
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int c = 0; c < kPer; ++c) {
+        const float down = __int_as_float((F32 ? pe[b][c] - 19 : ve - 11) << 23);  // 2^(ve - 132) / 64, 2^(pe - 140) / 64
         float v = l[b][c];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

@@ -166,3 +166,11 @@ def spread_case(spread, where, new, dtype):
 @pytest.mark.parametrize("spread", [0, 10, 13, 16, 18, 20])
 def test_one_value_far_larger_than_those_that_count(spread, new, where):
     spread_case(spread, where, new, torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["first block", "second block", "last"])
+@pytest.mark.parametrize("new", [1, 3, 7, 140])
+@pytest.mark.parametrize("spread", [0, 10, 13, 16, 18, 20])
+def test_one_value_far_larger_than_those_that_count_fp32(spread, new, where):
+    spread_case(spread, where, new, torch.float32)
