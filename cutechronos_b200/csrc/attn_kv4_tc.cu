@@ -29,14 +29,15 @@
 // against the largest V: P = 2^(x + eV - m + 7), up to 2^15.  Neither costs an
 // operation a score.  fp16 keeps its 11 bits down to 2^-22 of a block's largest
 // norm and of a row's largest P 2^eV.
-// A masked key's column is -inf and its V^ zero.  A K or V that is not finite
-// is zero too and instead marks the rows that see it (their sum becomes NaN), so
-// that it cannot reach the others through 0 * NaN.
+// A masked key's column is -inf and its V^ zero.  A K that is not finite makes
+// its column of scores NaN, which is hidden like others.  A V that is not finite
+// is zero, so that it cannot reach through 0 * NaN the rows that do not see it;
+// those that do are marked, by the sign of their sum of weights, for the output.
 // Every wait is bounded (about 2 s): on expiry all roles leave their loops,
 // copies and MMAs in flight are waited for, TMEM is freed, the kernel returns.
 // Measured: 2048, 1450 and 853 tokens against 16384, 11603 and 6822 keys, 4
-// heads on each of 8, causal, 723 us, 597 TFLOP/s of the scores' and values'
-// products; 256 series of 133 tokens, 12 heads, 164 us (40 of them the first
+// heads on each of 8, causal, 724 us, 596 TFLOP/s of the scores' and values'
+// products; 256 series of 133 tokens, 12 heads, 167 us (40 of them the first
 // kernel).  What bounds it: issue slots are 65% used, the exponentials' unit 60%,
 // and a step's chain of waits does not fill the rest; a third of the instructions
 // are the decoders', two thirds the softmax'.  Computing part of the exponentials
@@ -93,7 +94,7 @@ struct Item {
 
 struct Note {  // on half a block of keys: bit k of the words is key k
   uint32_t seen[2];    // the key counts
-  uint32_t poison[2];  // its K or V is not finite
+  uint32_t poison[2];  // its V is not finite
 };
 
 struct Control {
@@ -674,12 +675,12 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(nbits) : "r"(src + kNorms + (k & 15) * 4));
         }
         const bool seen = !(nbits & 0x8000u) && c0 + j * kTile + k < c1;
-        float nk = seen ? norm_value((uint16_t)nbits, a.pool.norm_bf16) : 0.0f;
+        const float nk = seen ? norm_value((uint16_t)nbits, a.pool.norm_bf16) : 0.0f;
         float nv = seen ? norm_value((uint16_t)(nbits >> 16), a.pool.norm_bf16) : 0.0f;
-        const bool bad = !(nv <= 3.402823466e38f && nk <= 3.402823466e38f);
-        if (bad) nk = nv = 0.0f;
+        const bool bad = !(nv <= 3.402823466e38f);
+        if (bad) nv = 0.0f;
         const uint32_t sb = __ballot_sync(0xffffffffu, seen), pb = __ballot_sync(0xffffffffu, bad);
-        const uint32_t tk = __reduce_max_sync(0xffffffffu, __float_as_uint(nk)) >> 23;
+        const uint32_t tk = __reduce_max_sync(0xffffffffu, nk <= 3.402823466e38f ? __float_as_uint(nk) : 0u) >> 23;
         const uint32_t tv = __reduce_max_sync(0xffffffffu, __float_as_uint(nv)) >> 23;
         if (lane == 0) ctl.top[flip][w] = tk | tv << 16;
         ok = barrier_and(1, 128, ok);
@@ -766,6 +767,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
       if (seq < 0) break;
       const float rs = valid ? *q_scale : 0.0f;
       float m = -INFINITY, l = 0.0f;  // largest score + eV, sum of 2^(score - m)
+      bool lost = false;              // the row sees a V that is not finite
       for (int t = 0; t < all; ++t) {
         // the decoders' notes on the block, then the scores
         if (!wait(ctl.kv_full[kv.i], kv.phase, ctl, err)) {
@@ -802,7 +804,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               vis[h] = visible(note.seen[h], limit - key0 - 32 * h);
-              if (note.poison[h] & vis[h]) l = __int_as_float(0x7fffffff);
+              lost = lost || (note.poison[h] & vis[h]) != 0;
             }
 #pragma unroll 1
             for (int i = 0; i < (two ? 4 : 2); ++i) {
@@ -880,7 +882,7 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
           }
           const int turn = (int)(nt & 1u);
           ctl.m[turn][g][c][r] = m;
-          ctl.l[turn][g][c][r] = l;
+          ctl.l[turn][g][c][r] = lost ? -l : l;
         }
         tmem_st_wait();
         tc_fence_before();
@@ -933,13 +935,11 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
         const float ma = ctl.m[turn][g][0][r], mb = two ? ctl.m[turn][g][1][r] : -INFINITY;
         m = fmaxf(ma, mb);
         const float wa = ma == -INFINITY ? 0.0f : ex2(ma - m), wb = mb == -INFINITY ? 0.0f : ex2(mb - m);
-        l = ctl.l[turn][g][0][r] * wa;
-        // 2^-7, 2^-8 and 1 / 64 take the scales of P, V and the levels back out
-        fa = wa * 0x1p-21f;
-        if (two) {
-          l += ctl.l[turn][g][1][r] * wb;
-          fb = wb * 0x1p-21f;
-        }
+        const float la = ctl.l[turn][g][0][r], lb = two ? ctl.l[turn][g][1][r] : 0.0f;
+        l = fabsf(la) * wa + fabsf(lb) * wb;
+        // 2^-7, 2^-8 and 1 / 64 take the scales of P, V and the levels back out; a sum below 0 says that O is lost
+        fa = la < 0.0f || lb < 0.0f ? __int_as_float(0x7fffffff) : wa * 0x1p-21f;
+        fb = wb * 0x1p-21f;
       }
       const bool part = e.chunks > 1;
       if (!part) {

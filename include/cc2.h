@@ -500,7 +500,8 @@ CC2_API int cc2_kv4_read_cols(const cc2_kv4_cache* cache, int dtype, void* k_out
  *   lse        (dev, float32 (total_q, q_heads)) natural logarithm of each
  *              row's sum of exponentials, or NULL
  * Masked tokens are not seen; a row that sees nothing gives 0 and a
- * log-sum-exp of -inf.  A length or page out of range raises
+ * log-sum-exp of -inf.  A value that is not finite makes the rows that see it
+ * NaN, a key their log-sum-exp too.  A length or page out of range raises
  * CC2_DEV_CACHE_RANGE; that sequence's rows are then unspecified.
  * Sums are fp32.  bf16 calls take the levels and a key's weight times its V
  * norm as fp16: 11 bits while the V norm is at least 2^-20 of the largest one

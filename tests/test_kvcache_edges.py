@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from cutechronos_b200 import _native as nat
-from test_kvcache import D, allowed, make, oracle_attention
+from test_kvcache import D, allowed, filled, make, oracle_attention
 
 I32 = dict(device="cuda", dtype=torch.int32)
 
@@ -174,3 +174,32 @@ def test_one_value_far_larger_than_those_that_count(spread, new, where):
 @pytest.mark.parametrize("spread", [0, 10, 13, 16, 18, 20])
 def test_one_value_far_larger_than_those_that_count_fp32(spread, new, where):
     spread_case(spread, where, new, torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 9, 25, 140])
+@pytest.mark.parametrize("bad", ["value", "key", "both"])
+def test_not_finite_keys_and_values_reach_the_rows_that_see_them(bad, new, dtype):
+    """A visible value that is not finite makes the rows that see it NaN and leaves their log-sum-exp, which has no value
+    in it; a key makes both NaN.  Rows that do not see it stay what the clean cache gives, to within both roundings."""
+    n = 200
+    cache, params, table, (k, v, seq, pos, _) = filled([n], 2, dtype=dtype, theta=None)
+    q = torch.randn(new, 2, D, generator=torch.Generator().manual_seed(4)).to(dtype)
+    want, wlse, sway, weight = oracle_attention(cache, params, q, [n], table, [0, new], True, 0.125, False)
+    tol, ltol = allowed(want, sway, weight, dtype == torch.float32)
+    if bad != "key":
+        v[198, 0, 3], v[198, 1, 60] = float("nan"), float("-inf")
+    if bad != "value":
+        k[198, 0, 3], k[198, 1, 60] = float("inf"), float("nan")
+    cache.append(k.cuda(), v.cuda(), seq.cuda(), pos.cuda(), table.cuda())
+    out, lse = (t.double().cpu() for t in cache.attention(q.cuda(), torch.tensor([n], **I32), table.cuda(), scale=0.125,
+                                                          return_lse=True))
+    late = n - new + torch.arange(new) >= 198
+    assert torch.isnan(out[late]).all()
+    assert ((out - want).norm(dim=-1) <= tol)[~late].all()
+    near = (lse - wlse).abs() <= ltol
+    if bad == "value":
+        assert near.all()
+    else:
+        assert torch.isnan(lse[late]).all() and near[~late].all()
