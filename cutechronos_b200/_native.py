@@ -12,10 +12,11 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libcc2_b200.so"
 
 CC2_F32, CC2_BF16 = 0, 1
+DEV_CACHE_RANGE, DEV_FORWARD, DEV_CACHE = 8, 7, 24  # bits of cc2_device_status: CC2_DEV_*
 EPI_ROWSCALE, EPI_BIAS, EPI_RELU, EPI_RESID, EPI_SSQ, EPI_SPECIAL, EPI_ROPE, EPI_LO = 1, 2, 4, 8, 16, 32, 64, 128
 
 EXPORTED = (
-    "cc2_last_error", "cc2_version", "cc2_device_status", "cc2_model_pack_bytes", "cc2_model_create",
+    "cc2_last_error", "cc2_version", "cc2_device_status", "cc2_device_status_of", "cc2_model_pack_bytes", "cc2_model_create",
     "cc2_model_destroy", "cc2_group_layout", "cc2_forward_workspace_bytes", "cc2_forward",
     "cc2_preprocess", "cc2_gemm", "cc2_rmsnorm_rows", "cc2_attention", "cc2_output_transform",
     "cc2_profile_begin", "cc2_profile_read", "cc2_set_gemm_variant", "cc2_forward_noalloc",
@@ -106,6 +107,7 @@ def load(path: Path | str | None = None) -> C.CDLL:
     lib.cc2_last_error.restype = C.c_char_p
     lib.cc2_version.restype = C.c_char_p
     lib.cc2_device_status.argtypes = [i]
+    lib.cc2_device_status_of.argtypes = [i, i]
     lib.cc2_model_pack_bytes.argtypes = [C.POINTER(Config), i, C.POINTER(sz)]
     lib.cc2_model_create.argtypes = [C.POINTER(Config), i, C.POINTER(Weights), v, sz, v, C.POINTER(v)]
     lib.cc2_model_destroy.argtypes = [v]

@@ -51,8 +51,6 @@
 
 namespace cc2 {
 
-int attention_error_word(int** p);
-
 namespace kv4 {
 
 // fp16 keeps the levels to 2^-12 of each at best, the same error in every key.
@@ -892,20 +890,6 @@ int plan(const Pool& pool, int dtype, int q_heads, int num_seqs, int total_q, in
   return CC2_OK;
 }
 
-// The attention kernels' error word, looked up once a device.
-int wait_word(int** p) {
-  static int* at[64] = {};
-  int dev = 0;
-  CC2_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && at[dev] != nullptr) {
-    *p = at[dev];
-    return CC2_OK;
-  }
-  CC2_TRY(attention_error_word(p));
-  if (dev < 64) at[dev] = *p;
-  return CC2_OK;
-}
-
 template <int R, bool F32, bool NormBf16>
 int launch(const Args& a, const Plan& p, cudaStream_t st) {
   const size_t smem = sizeof(Shared<R, F32>);
@@ -1003,8 +987,8 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   a.part_ml = (float2*)((char*)a.part + p.part_bytes);
   a.counter = (int*)((char*)a.part_ml + p.ml_bytes);
   a.q_scale = (float*)((char*)a.counter + 128);
-  CC2_TRY(wait_word(&a.wait_err));
-  CC2_TRY(error_word(&a.range_err));
+  CC2_TRY(error_words(&a.range_err));
+  a.wait_err = a.range_err + 1;
   a.table_ld = table_ld;
   a.rope_len = cache->rope_len;
   a.max_len = max_len;

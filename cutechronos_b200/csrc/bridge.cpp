@@ -532,8 +532,8 @@ void predict(Session& s, const float* context, int context_length, int H, float*
   cuda_check(cudaStreamSynchronize(s.stream), "cudaStreamSynchronize");
   const auto t1 = std::chrono::steady_clock::now();
   // a kernel whose bounded wait ran out returns early with incomplete outputs
-  const int dev_status = cc2_device_status(1);
-  if (dev_status < 0) cc2_check(dev_status, "cc2_device_status");
+  const int dev_status = cc2_device_status_of(CC2_DEV_FORWARD, 1);
+  if (dev_status < 0) cc2_check(dev_status, "cc2_device_status_of");
   if (dev_status != 0)
     throw BridgeError(fmt("a kernel of the forward gave up waiting (device status %d); no forecast returned",
                           dev_status));

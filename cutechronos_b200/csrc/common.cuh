@@ -60,6 +60,7 @@ enum : int {
   DEV_ERR_ATTN_TIMEOUT = 2,
   DEV_ERR_LAYER_TIMEOUT = 4,  // grid barrier of the layer-persistent forward
   DEV_ERR_CACHE_RANGE = 8,    // 4-bit cache: sequence, position, page or length out of range
+  DEV_ERR_CACHE_TIMEOUT = 16,
 };
 // Read (and optionally clear) the device error words of the current device.
 int read_device_error(int clear, int* value);

@@ -465,14 +465,17 @@ extern "C" {
 const char* cc2_last_error(void) { return t_error.c_str(); }
 const char* cc2_version(void) { return "cc2-b200 0.1 (sm_100a)"; }
 
-int cc2_device_status(int clear) {
+int cc2_device_status(int clear) { return cc2_device_status_of(CC2_DEV_FORWARD | CC2_DEV_CACHE, clear); }
+
+int cc2_device_status_of(int whose, int clear) {
   clear_error();
   CC2_CUDA(cudaDeviceSynchronize());
-  int v = 0, a = 0;
-  CC2_TRY(read_device_error(clear, &v));
-  CC2_TRY(read_attention_error(clear, &a));
-  int r = 0;
-  CC2_TRY(read_kv4_error(clear, &r));
+  int v = 0, a = 0, r = 0;
+  if (whose & CC2_DEV_FORWARD) {
+    CC2_TRY(read_device_error(clear, &v));
+    CC2_TRY(read_attention_error(clear, &a));
+  }
+  if (whose & CC2_DEV_CACHE) CC2_TRY(read_kv4_error(clear, &r));
   return v | (a ? DEV_ERR_ATTN_TIMEOUT : 0) | r;
 }
 

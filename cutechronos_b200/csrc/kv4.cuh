@@ -112,8 +112,8 @@ __device__ __forceinline__ void zip(uint32_t a, uint32_t b, uint32_t& u, uint32_
 int check_cache(const cc2_kv4_cache* c, const char* what, Pool& pool);
 int make_turn(const cc2_kv4_quant& q, const char* what, Turn& t);
 Levels make_levels(const cc2_kv4_cache& c);
-// Device error word of the cache's kernels (DEV_ERR_CACHE_RANGE).
-int error_word(int** p);
+// Device error words of the cache's kernels: DEV_ERR_CACHE_RANGE, and one for waits that ran out.
+int error_words(int** p);
 
 }  // namespace kv4
 }  // namespace cc2

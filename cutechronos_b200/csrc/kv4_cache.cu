@@ -36,10 +36,10 @@
 namespace cc2 {
 namespace kv4 {
 
-__device__ int g_kv4_error = 0;
+__device__ int g_kv4_error[2] = {0, 0};  // DEV_ERR_CACHE_RANGE; not 0: a wait ran out
 
-int error_word(int** p) {
-  static int* at[64] = {};  // per device: the word's address does not change
+int error_words(int** p) {
+  static int* at[64] = {};  // per device: the words' address does not change
   int dev = 0;
   CC2_CUDA(cudaGetDevice(&dev));
   if (dev < 64 && at[dev] != nullptr) {
@@ -469,10 +469,12 @@ int grid_of(int T, int heads, int* grid) {
 }  // namespace kv4
 
 int read_kv4_error(int clear, int* value) {
-  CC2_CUDA(cudaMemcpyFromSymbol(value, kv4::g_kv4_error, sizeof(int)));
+  int words[2];
+  CC2_CUDA(cudaMemcpyFromSymbol(words, kv4::g_kv4_error, sizeof words));
+  *value = words[0] | (words[1] ? DEV_ERR_CACHE_TIMEOUT : 0);
   if (clear) {
-    int z = 0;
-    CC2_CUDA(cudaMemcpyToSymbol(kv4::g_kv4_error, &z, sizeof(int)));
+    const int z[2] = {0, 0};
+    CC2_CUDA(cudaMemcpyToSymbol(kv4::g_kv4_error, z, sizeof z));
   }
   return CC2_OK;
 }
@@ -491,7 +493,7 @@ int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int6
               "kv4_append: keys and values must start on 16 bytes, as must their strides");
   int grid = 0, *err = nullptr;
   CC2_TRY(grid_of(T, pool.heads, &grid));
-  CC2_TRY(error_word(&err));
+  CC2_TRY(error_words(&err));
   Turn turn_k, turn_v;
   Cells cells;
   CC2_TRY(make_turn(cache->key, "kv4_append", turn_k));
@@ -525,7 +527,7 @@ int launch_kv4_read(const cc2_kv4_cache* cache, int dtype, void* k_out, void* v_
   CC2_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15u) == 0, "kv4_read: outputs must be 16-byte aligned");
   int grid = 0, *err = nullptr;
   CC2_TRY(grid_of(T, pool.heads, &grid));
-  CC2_TRY(error_word(&err));
+  CC2_TRY(error_words(&err));
   Turn turn_k, turn_v;
   CC2_TRY(make_turn(cache->key, "kv4_read", turn_k));
   CC2_TRY(make_turn(cache->value, "kv4_read", turn_v));

@@ -7,8 +7,8 @@ keys to their positions on the way (rotate-half, like the model's attention), an
 rotates a query into the codes' frame and the result back out, never the cache.
 
 Every method enqueues work on the current stream of the cache's device and returns; lengths, positions and tables stay on
-the device.  A sequence, position, page or length out of range sets bit 8 of ``cc2_device_status`` (see
-:meth:`PagedKV4Cache.check`).
+the device.  A sequence, position, page or length out of range sets a bit of the library's device status, which stands
+until :meth:`PagedKV4Cache.check` reads it.
 """
 
 from __future__ import annotations
@@ -23,7 +23,7 @@ from .turboquant import TurboQuantParams
 
 DIM = 64
 NORMS = {"float16": 0, "bfloat16": 1}
-DEV_CACHE_RANGE = 8
+DEV_CACHE_RANGE = nat.DEV_CACHE_RANGE
 _CODES = {torch.bfloat16: nat.CC2_BF16, torch.float32: nat.CC2_F32}
 
 
@@ -277,11 +277,14 @@ class PagedKV4Cache:
         return (out, lse) if return_lse else out
 
     def check(self) -> None:
-        """Wait for the device and raise if a kernel of this library reported an error: for the cache, a sequence,
-        position, page or length out of range."""
+        """Wait for the device and raise if a cache call on it reported an error since the last check: a sequence,
+        position, page or length out of range, or a kernel that gave up waiting.  A forward's errors are its own (see
+        :meth:`CuteChronos2Model.set_device_checks`)."""
         with torch.cuda.device(self.device):
-            status = self._lib.cc2_device_status(1)
+            status = self._lib.cc2_device_status_of(nat.DEV_CACHE, 1)
+        if status < 0:
+            nat.check(status, "cc2_device_status_of")
         if status:
             raise nat.NativeError(f"device status {status}" + (
                 ": a sequence, position, page or length of a cache call was out of range"
-                if status > 0 and status & DEV_CACHE_RANGE else ""))
+                if status & DEV_CACHE_RANGE else ": a kernel of a cache call gave up waiting, its outputs are incomplete"))

@@ -329,9 +329,9 @@ class CuteChronos2Model(nn.Module):
         if not getattr(self, "_device_checks", False) or torch.cuda.is_current_stream_capturing():
             return
         with torch.cuda.device(dev):
-            st = nat.load().cc2_device_status(1)
+            st = nat.load().cc2_device_status_of(nat.DEV_FORWARD, 1)
         if st < 0:
-            nat.check(st, "cc2_device_status")
+            nat.check(st, "cc2_device_status_of")
         if st:
             raise nat.NativeError(f"a kernel of the forward gave up waiting (device status {st}); "
                                   "its outputs are incomplete")

@@ -59,17 +59,23 @@ enum {
 CC2_API const char* cc2_last_error(void);
 /* Library version string. */
 CC2_API const char* cc2_version(void);
-/* Device-side error word written by bounded waits inside kernels (0 = none,
+/* Device-side error words written by bounded waits inside kernels (0 = none,
  * else CC2_DEV_* bits); synchronises the current device.  clear != 0 resets
- * it.  A kernel whose wait ran out returns early and leaves its outputs
+ * them.  A kernel whose wait ran out returns early and leaves its outputs
  * incomplete while the launching call has already returned CC2_OK, so callers
  * that need to know poll this after synchronising (the native bridge and
  * CuteChronos2Model.set_device_checks(True) do). */
 enum {
   CC2_DEV_GEMM_TIMEOUT = 1, CC2_DEV_ATTN_TIMEOUT = 2, CC2_DEV_LAYER_TIMEOUT = 4,
-  CC2_DEV_CACHE_RANGE = 8  /* a 4-bit cache call met a sequence, position, page or length out of range */
+  CC2_DEV_CACHE_RANGE = 8, /* a 4-bit cache call met a sequence, position, page or length out of range */
+  CC2_DEV_CACHE_TIMEOUT = 16, /* a wait of the 4-bit cache's attention ran out */
+  CC2_DEV_FORWARD = 7,     /* the bits of the forward and its parts */
+  CC2_DEV_CACHE = 24       /* the bits of the 4-bit cache's calls */
 };
 CC2_API int cc2_device_status(int clear);
+/* The same for the bits of one side, whose = CC2_DEV_FORWARD or CC2_DEV_CACHE:
+ * the other side's are neither reported nor reset. */
+CC2_API int cc2_device_status_of(int whose, int clear);
 
 /* ------------------------------------------------------------------------ */
 /* Model configuration: mirror of CuteChronos2Config (model.py:59-91).       */

@@ -203,3 +203,85 @@ def test_not_finite_keys_and_values_reach_the_rows_that_see_them(bad, new, dtype
         assert near.all()
     else:
         assert torch.isnan(lse[late]).all() and near[~late].all()
+
+
+# ------------------------------------------------------------------------ whose error a status bit is --
+def out_of_range(cache):
+    """An append to a place that the cache does not have."""
+    k = torch.zeros(1, cache.num_heads, D, device="cuda")
+    cache.append(k, k, torch.zeros(1, **I32), torch.full((1,), 10**6, **I32), torch.zeros(1, 1, **I32))
+
+
+@pytest.mark.gpu
+def test_a_cache_error_is_not_the_forwards():
+    """A checked forward succeeds beside a cache call that was out of range, and leaves the report of it to the cache."""
+    from conftest import small_config
+    from cutechronos_b200.model import CuteChronos2Model
+    from cutechronos_b200.workloads import seeded_init_
+    model = seeded_init_(CuteChronos2Model(small_config()), seed=1).to("cuda").eval().set_device_checks(True)
+    x = torch.randn(2, 300, generator=torch.Generator().manual_seed(2)).cuda()
+    want = model(x, num_output_patches=2).clone()
+    cache, _ = make(2, 2, 16)
+    cache.check()
+    out_of_range(cache)
+    assert torch.equal(want, model(x, num_output_patches=2))
+    with pytest.raises(nat.NativeError, match="out of range"):
+        cache.check()
+    cache.check()
+
+
+@pytest.mark.gpu
+def test_a_cache_error_is_not_the_bridges(tmp_path):
+    from conftest import small_config, write_checkpoint
+    from cutechronos_b200.foreign import NativeBridge
+    from cutechronos_b200.model import CuteChronos2Model
+    from cutechronos_b200.workloads import seeded_init_
+    write_checkpoint(seeded_init_(CuteChronos2Model(small_config()), seed=5), tmp_path)
+    bridge = NativeBridge(nat.load())
+    x = torch.randn(300, generator=torch.Generator().manual_seed(2)).tolist()
+    h = bridge.init_pipeline(str(tmp_path))
+    try:
+        want, _ = bridge.predict_median(h, x, 16)
+        cache, _ = make(2, 2, 16)
+        out_of_range(cache)
+        got, _ = bridge.predict_median(h, x, 16)
+    finally:
+        bridge.destroy_pipeline(h)
+    assert want == got
+    with pytest.raises(nat.NativeError, match="out of range"):
+        cache.check()
+    cache.check()
+
+
+@pytest.mark.gpu
+def test_a_forwards_timeout_is_not_the_caches():
+    """The hook that withholds a load, as in the failure path's own test: the GEMM gives up after its bounded wait."""
+    from cutechronos_b200 import kernels
+    lib = nat.load()
+    x, w = torch.randn(64, 768, device="cuda").to(torch.bfloat16), torch.randn(512, 768, device="cuda").to(torch.bfloat16)
+    torch.cuda.synchronize()
+    assert lib.cc2_device_status(1) == 0
+    cache, _ = make(2, 2, 16)
+    nat.check(lib.cc2_test_starve_gemm(1), "cc2_test_starve_gemm")
+    try:
+        kernels.linear(x, w)
+        torch.cuda.synchronize()
+        cache.check()
+        assert lib.cc2_device_status(1) == 1
+    finally:
+        nat.check(lib.cc2_test_starve_gemm(0), "cc2_test_starve_gemm")
+        lib.cc2_device_status(1)
+
+
+@pytest.mark.gpu
+def test_each_side_reads_and_resets_its_own_bits():
+    lib = nat.load()
+    cache, _ = make(2, 2, 16)
+    assert lib.cc2_device_status(1) == 0
+    out_of_range(cache)
+    assert lib.cc2_device_status_of(nat.DEV_FORWARD, 1) == 0
+    assert lib.cc2_device_status_of(nat.DEV_CACHE, 0) == nat.DEV_CACHE_RANGE
+    assert lib.cc2_device_status(0) == nat.DEV_CACHE_RANGE
+    assert lib.cc2_device_status(1) == nat.DEV_CACHE_RANGE
+    assert lib.cc2_device_status(0) == 0
+    cache.check()
