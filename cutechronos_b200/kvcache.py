@@ -141,7 +141,7 @@ class PagedKV4Cache:
         if t.dtype != torch.int32:
             if t.dtype != torch.int64:
                 raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
-            t = t.to(torch.int32)
+            t = t.clamp(-2**31, 2**31 - 1).to(torch.int32)  # out of range stays out of range
         return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
 
     def _values(self, t: torch.Tensor, what: str) -> int:

@@ -285,3 +285,39 @@ def test_each_side_reads_and_resets_its_own_bits():
     assert lib.cc2_device_status(1) == nat.DEV_CACHE_RANGE
     assert lib.cc2_device_status(0) == 0
     cache.check()
+
+
+# ------------------------------------------------------------------------------------ 64-bit indexes --
+@pytest.mark.gpu
+def test_64_bit_indexes_do_not_wrap():
+    """An index that 32 bits would turn into a valid one is out of range, or, where it is negative, skips."""
+    cache, _ = make(4, 2, 16, max_positions=64)
+    I64 = dict(device="cuda", dtype=torch.int64)
+    table = torch.tensor([[0, 1, 2, 3]], **I64)
+    zero, at = torch.zeros(1, **I64), torch.tensor([5], **I64)
+    k = torch.randn(1, 2, D, device="cuda")
+    before = cache.pages.clone()
+
+    def reported(yes=True):
+        if yes:
+            with pytest.raises(nat.NativeError, match="out of range"):
+                cache.check()
+        cache.check()
+
+    for seq, pos, tab, bad in ((zero, at + 2**32, table, True), (zero + 2**32, at, table, True), (zero, at, table + 2**32, True),
+                               (zero, at - 2**63, table, False), (zero - 2**40, at, table, False), (zero, at, table - 2**32, True)):
+        cache.append(k, k, seq, pos, tab)
+        reported(bad)
+        assert torch.equal(before, cache.pages)
+        assert all((t == 0).all() for t in cache.read(seq, pos, tab))
+        reported(bad)
+    cache.append(k, k, zero, at, table)
+    assert not torch.equal(before, cache.pages)
+    q = torch.randn(1, 2, D, device="cuda")
+    want = cache.attention(q, torch.tensor([6], **I64), table)
+    reported(False)
+    cache.attention(q, torch.tensor([6 + 2**32], **I64), table)
+    reported()
+    cache.attention(q, torch.tensor([6], **I64), table, cu_q=torch.tensor([2**32, 2**32 + 1], **I64))
+    reported()
+    assert torch.equal(want, cache.attention(q, torch.tensor([6], **I32), table.int()))
