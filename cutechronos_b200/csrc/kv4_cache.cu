@@ -343,6 +343,10 @@ append_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn tu
   walsh(y);
   const float n = norm[mine];
   const float n8 = __fmul_rn(n, 8.0f);
+  if (n8 > 0.0f && n8 < 0x1p-50f) {  // squares may have lost bits below fp32's range: a |y| above 8n would leave the cells
+#pragma unroll
+    for (int i = 0; i < 64; ++i) y[i] = fminf(fmaxf(y[i], -n8), n8);
+  }
   const float fine = n8 > 0.0f ? __fdividef(511.0f, n8) : 0.0f;  // its error is within the cells' room
   const uint8_t* entries = reinterpret_cast<const uint8_t*>(cells);
   uint32_t word[8];

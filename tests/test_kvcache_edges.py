@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from cutechronos_b200 import _native as nat
-from test_kvcache import D, allowed, filled, make, oracle_attention
+from test_kvcache import D, allowed, filled, make, oracle_attention, tables, unpack, walsh
 
 I32 = dict(device="cuda", dtype=torch.int32)
 
@@ -321,3 +321,21 @@ def test_64_bit_indexes_do_not_wrap():
     cache.attention(q, torch.tensor([6], **I64), table, cu_q=torch.tensor([2**32, 2**32 + 1], **I64))
     reported()
     assert torch.equal(want, cache.attention(q, torch.tensor([6], **I32), table.int()))
+
+
+# ----------------------------------------------------------------------------------------- tiny vectors --
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [3e-23, 4.4e-23, 6e-23, 1e-22, 1e-20, 1e-15])
+def test_codes_of_vectors_whose_squares_underflow(size):
+    """All of a vector's weight on one rotated coordinate: |y| = 8n passes every bound however the squares of fp32 round."""
+    cache, params = make(1, 1, 16, norm="bfloat16", theta=None)
+    _, _, signs, perm = tables(params[1])
+    x = torch.zeros(4, 1, D)
+    row = (walsh()[[0, 5, 38, 63]] * signs).float() * size
+    x[:, 0, perm] = row
+    x[2:] *= -1
+    cache.append(x.cuda(), x.cuda(), torch.zeros(4, **I32), torch.arange(4, **I32), torch.zeros(1, 1, **I32))
+    mag, sign, norm, _ = unpack(cache, 1)
+    for i, j in enumerate((0, 5, 38, 63)):
+        assert mag[0, i, 0, j] == 7 and sign[0, i, 0, j] == (1 if i < 2 else -1)
+    assert (norm[0, :4, 0] > 0).all()
