@@ -263,12 +263,13 @@ class PagedKV4Cache:
                 raise ValueError("out must have q's shape, type and device, its rows apart, dense and on 16-byte boundaries")
         lse = torch.empty((total, heads), dtype=torch.float32, device=self.device) if return_lse else None
         sizes = (code, heads, seqs, total, max_q, max_len)
-        if self._plan[0] != sizes:
+        plan = self._plan  # another thread's call may leave its own at any time
+        if plan[0] != sizes:
             nbytes = C.c_size_t()
             self._call(lambda ref, *a: self._lib.cc2_kv4_attention_workspace_bytes(ref, *a[:-1]),
                        "cc2_kv4_attention_workspace_bytes", *sizes, C.byref(nbytes))
-            self._plan = (sizes, nbytes.value)
-        need = self._plan[1]
+            self._plan = plan = (sizes, nbytes.value)
+        need = plan[1]
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._call(self._lib.cc2_kv4_attention, "cc2_kv4_attention", code, *q_at, *out_at, heads, seqs, total, cu,
                    max_q, lens.data_ptr(), max_len,

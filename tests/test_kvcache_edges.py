@@ -339,3 +339,31 @@ def test_codes_of_vectors_whose_squares_underflow(size):
     for i, j in enumerate((0, 5, 38, 63)):
         assert mag[0, i, 0, j] == 7 and sign[0, i, 0, j] == (1 if i < 2 else -1)
     assert (norm[0, :4, 0] > 0).all()
+
+
+# -------------------------------------------------------------------------------- calls of two threads --
+@pytest.mark.gpu
+def test_a_call_keeps_the_plan_it_found():
+    """Between a call's look at the cache's plan and its use, another thread's call may have left its own."""
+    from cutechronos_b200.kvcache import PagedKV4Cache
+
+    class Raced(PagedKV4Cache):
+        @property
+        def _plan(self):
+            found, self.plan = self.plan, ((), 0)  # the other call's, which takes no workspace
+            return found
+
+        @_plan.setter
+        def _plan(self, plan):
+            self.plan = self.known = plan
+
+    cache = Raced(64, 2, rope_theta=None)
+    table = torch.arange(64, **I32).view(1, 64)
+    k = torch.randn(3000, 2, D, device="cuda")
+    cache.append(k, k, torch.zeros(3000, **I32), torch.arange(3000, **I32), table)
+    q, lens = torch.randn(1, 2, D, device="cuda"), torch.tensor([3000], **I32)
+    want = cache.attention(q, lens, table)
+    assert cache.known[1] > 0
+    cache.plan = cache.known
+    assert torch.equal(want, cache.attention(q, lens, table))
+    cache.check()
