@@ -325,6 +325,7 @@ attend_kernel(const __grid_constant__ Args a) {
   Walk walk;
   const int team_at = (int)blockIdx.x * S::kTeams + team;
   walk.start(a, team_at, lane);
+  if (a.fill) fill_rows<T>(a, blockIdx.x * blockDim.x + tid, gridDim.x * blockDim.x);
   auto next = [&](Unit& u) {
     if (!walk.next(a, lane)) return false;
     u.s = span_of(a, walk.seq, walk.tile, false);
@@ -952,14 +953,17 @@ int kv4_attention_workspace(const cc2_kv4_cache* cache, int dtype, int q_heads, 
 int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, int64_t q_ld, int64_t q_hs, void* out,
                          int64_t o_ld, int64_t o_hs, int q_heads, int num_seqs, int total_q, const int32_t* cu_q,
                          int max_q, const int32_t* seq_lens, int max_len, const int32_t* table, int table_ld,
-                         int causal, float scale, int rotate_q, float* lse, void* ws, size_t ws_bytes,
+                         int causal, float scale, int rotate_q, int fill, float* lse, void* ws, size_t ws_bytes,
                          cudaStream_t st) {
   using namespace kv4;
   Args a{};
   CC2_TRY(check_cache(cache, "kv4_attention", a.pool));
   Plan p;
   CC2_TRY(plan(a.pool, dtype, q_heads, num_seqs, total_q, max_q, max_len, p));
-  if (total_q == 0 || max_q == 0) return CC2_OK;
+  CC2_REQUIRE((fill & ~3) == 0, "kv4_attention: bad fill %d", fill);
+  if (cu_q == nullptr) fill = 0;  // every row has a sequence
+  if (lse == nullptr) fill &= 1;
+  if (total_q == 0 || (max_q == 0 && fill == 0)) return CC2_OK;
   CC2_REQUIRE(q && out && seq_lens && table && table_ld > 0, "kv4_attention: null operand");
   CC2_REQUIRE(cu_q != nullptr || (long long)num_seqs * max_q == total_q,
               "kv4_attention: without cu_q the rows must be num_seqs * max_q, got %d", total_q);
@@ -1005,6 +1009,7 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   a.round_keys = p.round_keys;
   a.causal = causal != 0;
   a.rotate = rotate_q != 0;
+  a.fill = fill;
   const cc2_kv4_quant* quant[2] = {&cache->key, &cache->value};
   Rotation* rotation[2] = {&a.rk, &a.rv};
   for (int k = 0; k < 2; ++k) {

@@ -196,6 +196,18 @@ __device__ __forceinline__ void mma_pm1(float (&d)[4], const uint32_t (&x)[4], u
       : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b.x), "r"(b.y));
 }
 
+// A row of no sequence, of some heads.  Not inlined: the kernel's registers are full, and such rows are few.
+__device__ __noinline__ void fill_row(const Args& a, int row, int head0, int head1) {
+  const int heads = a.pool.heads * a.group, tok = row / a.group;
+  for (int head = head0; head < head1; ++head) {
+    const int qh = head * a.group + row % a.group;
+    uint4* const out = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (long long)tok * a.o_ld + (long long)qh * a.o_hs);
+    if (a.fill & 1)
+      for (int i = 0; i < 8; ++i) out[i] = make_uint4(0, 0, 0, 0);
+    if (a.fill & 2) a.lse[(long long)tok * heads + qh] = -INFINITY;
+  }
+}
+
 __global__ void __launch_bounds__(kQThreads, 4)
 rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles, const int per) {
   pdl_launch_dependents();
@@ -240,6 +252,7 @@ rotate_queries_kernel(const __grid_constant__ Args a, const long long q_tiles, c
         }
       }
     }
+    if (a.fill && row < all && from == nullptr) fill_row(a, row, blockIdx.y * per, min((int)(blockIdx.y + 1) * per, a.pool.heads));
     row_at[tid] = from;
     row_to[tid] = to;
     row_pos[tid] = pos;

@@ -102,7 +102,7 @@ int kv4_attention_workspace(const cc2_kv4_cache* cache, int dtype, int q_heads, 
 int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, int64_t q_ld, int64_t q_hs, void* out,
                          int64_t o_ld, int64_t o_hs, int q_heads, int num_seqs, int total_q, const int32_t* cu_q,
                          int max_q, const int32_t* seq_lens, int max_len, const int32_t* table, int table_ld,
-                         int causal, float scale, int rotate_q, float* lse, void* ws, size_t ws_bytes,
+                         int causal, float scale, int rotate_q, int fill, float* lse, void* ws, size_t ws_bytes,
                          cudaStream_t st);
 int launch_kv_quant(int dtype, void* qkv, int ld, int rows, int q_col, int k_col, int v_col, int heads,
                     const cc2_kvq* key, const cc2_kvq* value, const float* rope_cs, int rope_period, float* stats,
@@ -1018,9 +1018,19 @@ int cc2_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, int6
                       int max_q, const int32_t* seq_lens, int max_len, const int32_t* block_table, int table_ld,
                       int causal, float scale, int rotate_q, float* lse, void* workspace, size_t workspace_bytes,
                       void* stream) {
+  return cc2_kv4_attention_fill(cache, dtype, q, q_ld, q_hs, out, o_ld, o_hs, q_heads, num_seqs, total_q, cu_q, max_q,
+                                seq_lens, max_len, block_table, table_ld, causal, scale, rotate_q, 0, lse, workspace,
+                                workspace_bytes, stream);
+}
+
+int cc2_kv4_attention_fill(const cc2_kv4_cache* cache, int dtype, const void* q, int64_t q_ld, int64_t q_hs, void* out,
+                           int64_t o_ld, int64_t o_hs, int q_heads, int num_seqs, int total_q, const int32_t* cu_q,
+                           int max_q, const int32_t* seq_lens, int max_len, const int32_t* block_table, int table_ld,
+                           int causal, float scale, int rotate_q, int fill, float* lse, void* workspace,
+                           size_t workspace_bytes, void* stream) {
   clear_error();
   return launch_kv4_attention(cache, dtype, q, q_ld, q_hs, out, o_ld, o_hs, q_heads, num_seqs, total_q, cu_q, max_q,
-                              seq_lens, max_len, block_table, table_ld, causal, scale, rotate_q, lse, workspace,
+                              seq_lens, max_len, block_table, table_ld, causal, scale, rotate_q, fill, lse, workspace,
                               workspace_bytes, (cudaStream_t)stream);
 }
 

@@ -54,6 +54,7 @@ struct Args {
   int chunk, splits, row_tiles, tile_rows;
   int teams, round_keys;  // else: teams of warps on the card, keys that one takes in a round of its warps
   int causal, rotate;
+  int fill;      // rows of no sequence: 1 in out, 2 in lse
   float qscale;  // scale * log2(e) / 8 * 64 / f: of a rotated query (f: the levels' factor)
   float back;    // 64 / f / 8: of a rotated sum
   Rotation rk, rv;
@@ -118,6 +119,22 @@ __device__ __forceinline__ Span span_of(const Args& a, int seq, int row_tile, bo
   const int last = (min(s.row0 + a.tile_rows, s.rows) - 1) / a.group;  // the tile's last query token
   s.keys = a.causal ? min(max(s.len - s.n + last + 1, 0), s.len) : s.len;
   return s;
+}
+
+// Rows that no sequence has, before the first one's and from the end of the
+// last one's on: 0, and -inf as log-sum-exp.  Thread `id` of `threads`; a call's
+// rows times heads times 64 fit 31 bits.
+template <typename T>
+__device__ __forceinline__ void fill_rows(const Args& a, unsigned id, unsigned threads) {
+  constexpr unsigned kParts = 64 * sizeof(T) / 16;
+  const unsigned head = min(max(a.cu[0], 0), a.total_q), tail = min(max(a.cu[a.num_seqs], (int)head), a.total_q);
+  const unsigned heads = a.pool.heads * a.group, parts = (head + a.total_q - tail) * heads * kParts;
+  for (unsigned i = id; i < parts; i += threads) {
+    const unsigned row = i / kParts, at = row / heads, tok = at < head ? at : at - head + tail, h = row - at * heads;
+    if (a.fill & 1)
+      reinterpret_cast<uint4*>((T*)a.out + (long long)tok * a.o_ld + (long long)h * a.o_hs)[i % kParts] = make_uint4(0, 0, 0, 0);
+    if ((a.fill & 2) && i % kParts == 0) a.lse[(long long)tok * heads + h] = -INFINITY;
+  }
 }
 
 // The work of a call without tcgen05, as one line of rounds: sequence after

@@ -224,7 +224,8 @@ class PagedKV4Cache:
         ``causal`` lets a row see the entries up to its own.  Query head h reads key head h // (query heads / heads).
         ``scale`` multiplies the scores (1, as in the model's attention); ``rotate_q`` rotates the queries to their
         positions.  ``max_len`` bounds seq_lens (default: what the block table has room for); a tighter bound splits the
-        work better.  A row that sees no token gives 0.  With ``return_lse`` also the (tokens, query heads) float32
+        work better.  A row that sees no token gives 0, as does one of no sequence (before ``cu_q[0]``, from ``cu_q[-1]`` on),
+        which in an ``out`` of the caller's is left alone.  With ``return_lse`` also the (tokens, query heads) float32
         logarithm of each row's sum of exponentials (-inf for such a row), to join it with attention over other keys."""
         code = self._values(q, "q")
         lens = self._index(seq_lens, "seq_lens")
@@ -252,7 +253,9 @@ class PagedKV4Cache:
             raise ValueError("the cache was made without a rotation (rope_theta None)")
         per = _PER[q.dtype]
         q, q_at = _rows(q, per)
+        fill = 2 if return_lse else 0  # what this call allocates is written whole
         if out is None:
+            fill |= 1
             out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
             out_at = (out.data_ptr(), heads * DIM, DIM)
         else:
@@ -271,9 +274,9 @@ class PagedKV4Cache:
             self._plan = plan = (sizes, nbytes.value)
         need = plan[1]
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._call(self._lib.cc2_kv4_attention, "cc2_kv4_attention", code, *q_at, *out_at, heads, seqs, total, cu,
+        self._call(self._lib.cc2_kv4_attention_fill, "cc2_kv4_attention", code, *q_at, *out_at, heads, seqs, total, cu,
                    max_q, lens.data_ptr(), max_len,
-                   table.data_ptr(), ld, causal, scale, rotate_q, None if lse is None else lse.data_ptr(),
+                   table.data_ptr(), ld, causal, scale, rotate_q, fill, None if lse is None else lse.data_ptr(),
                    None if ws is None else ws.data_ptr(), need)
         return (out, lse) if return_lse else out
 

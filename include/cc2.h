@@ -523,6 +523,14 @@ CC2_API int cc2_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void*
                               const int32_t* cu_q, int max_q, const int32_t* seq_lens, int max_len,
                               const int32_t* block_table, int table_ld, int causal, float scale, int rotate_q,
                               float* lse, void* workspace, size_t workspace_bytes, void* stream);
+/* The same for outputs that hold nothing yet.  Rows of no sequence (before
+ * cu_q[0], from cu_q[num_seqs] on) are not written by the call above; here
+ * they become 0 in out (fill & 1) and -inf in lse (fill & 2). */
+CC2_API int cc2_kv4_attention_fill(const cc2_kv4_cache* cache, int dtype, const void* q, int64_t q_ld, int64_t q_hs,
+                                   void* out, int64_t o_ld, int64_t o_hs, int q_heads, int num_seqs, int total_q,
+                                   const int32_t* cu_q, int max_q, const int32_t* seq_lens, int max_len,
+                                   const int32_t* block_table, int table_ld, int causal, float scale, int rotate_q,
+                                   int fill, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Pipeline steps on the device (pipeline.py:221-322, 24-58).                 */

@@ -367,3 +367,35 @@ def test_a_call_keeps_the_plan_it_found():
     cache.plan = cache.known
     assert torch.equal(want, cache.attention(q, lens, table))
     cache.check()
+
+
+# ------------------------------------------------------------------------- rows that no sequence has --
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 5, 24, 150])
+def test_rows_of_no_sequence(new, dtype):
+    """Rows before cu_q's first entry and from its last on (a batch padded to a fixed size): 0 and -inf in a new output,
+    left alone in one that the caller gives."""
+    cache, _, table, _ = filled([300, 90, 700], 2, dtype=dtype)
+    lens, tab = torch.tensor([300, 90, 700], **I32), table.cuda()
+    total = 3 * new + 37
+    q = torch.randn(total, 6, D, generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+    want, wlse = cache.attention(q[7:7 + 3 * new], lens, tab, scale=0.125, return_lse=True)
+    cu = torch.tensor([7, 7 + new, 7 + 2 * new, 7 + 3 * new], **I32)
+    args = dict(cu_q=cu, max_q=new, scale=0.125, return_lse=True)
+    for fill in (7.0, float("nan")):
+        stale = [torch.full_like(q, fill), torch.full((total, 6), fill, device="cuda")]
+        del stale  # what a new output may be cut from
+        out, lse = cache.attention(q, lens, tab, **args)
+        assert torch.equal(out[7:7 + 3 * new], want) and torch.equal(lse[7:7 + 3 * new], wlse)
+        for part in (slice(0, 7), slice(7 + 3 * new, None)):
+            assert (out[part] == 0).all() and (lse[part] == -math.inf).all()
+        room = torch.full_like(q, fill)
+        got, lse = cache.attention(q, lens, tab, out=room, **args)
+        assert torch.equal(got[7:7 + 3 * new], out[7:7 + 3 * new])
+        for part in (slice(0, 7), slice(7 + 3 * new, None)):
+            assert torch.equal(got[part].isnan(), room[part].isnan()) and (math.isnan(fill) or (got[part] == fill).all())
+            assert (lse[part] == -math.inf).all()
+    none, lse = cache.attention(q, lens, tab, cu_q=torch.full((4,), 9, **I32), max_q=0, return_lse=True)
+    assert (none == 0).all() and (lse == -math.inf).all()
+    cache.check()
