@@ -107,18 +107,29 @@ class PagedKV4Cache:
         device = torch.device(device)
         if device.type != "cuda":
             raise RuntimeError("cutechronos_b200 kernels take CUDA tensors only (no CPU path)")
-        self.pages = torch.zeros(num_pages, nbytes.value, dtype=torch.uint8, device=device)
-        self.device = self.pages.device
-        self._at = self.pages.get_device()
+        self._pages = torch.zeros(num_pages, nbytes.value, dtype=torch.uint8, device=device)
+        self.device = self._pages.device
+        self._at = self._pages.get_device()
         self.num_pages, self.num_heads, self.page_size = num_pages, num_heads, page_size
-        self.rope = rope_rows(max_positions, rope_theta, self.device) if rope_theta is not None else None
-        self._c = nat.KV4Cache(self.pages.data_ptr(), num_pages, page_size, num_heads, NORMS[key.norm_dtype],
-                               self.rope.data_ptr() if self.rope is not None else None,
-                               max_positions if self.rope is not None else 0, (C.c_float * 8)(*levels),
+        self._rope = rope_rows(max_positions, rope_theta, self.device) if rope_theta is not None else None
+        self._c = nat.KV4Cache(self._pages.data_ptr(), num_pages, page_size, num_heads, NORMS[key.norm_dtype],
+                               self._rope.data_ptr() if self._rope is not None else None,
+                               max_positions if self._rope is not None else 0, (C.c_float * 8)(*levels),
                                (C.c_float * 7)(*bounds), kq, vq)
         self._ref = C.byref(self._c)
         self._lib = lib
         self._plan = (None, 0)  # sizes of the last attention call, bytes of its workspace
+
+    # The library holds these two by address: their contents may be written, they cannot be replaced.
+    @property
+    def pages(self) -> torch.Tensor:
+        """The storage: uint8, (num_pages, bytes of a page)."""
+        return self._pages
+
+    @property
+    def rope(self) -> torch.Tensor | None:
+        """(max_positions, 32, 2) float32 (cos, sin) that keys and queries are rotated by; None without a rotation."""
+        return self._rope
 
     # -- arguments ---------------------------------------------------------------------------
     # Plain code on purpose: a single-token step's kernels take about as long as these checks.
@@ -249,7 +260,7 @@ class PagedKV4Cache:
         max_len = room if max_len is None or max_len > room else int(max_len)
         if max_q < 0 or max_len < 0:
             raise ValueError("max_q and max_len must not be negative")
-        if rotate_q and self.rope is None:
+        if rotate_q and self._rope is None:
             raise ValueError("the cache was made without a rotation (rope_theta None)")
         per = _PER[q.dtype]
         q, q_at = _rows(q, per)

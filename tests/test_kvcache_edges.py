@@ -399,3 +399,19 @@ def test_rows_of_no_sequence(new, dtype):
     none, lse = cache.attention(q, lens, tab, cu_q=torch.full((4,), 9, **I32), max_q=0, return_lse=True)
     assert (none == 0).all() and (lse == -math.inf).all()
     cache.check()
+
+
+@pytest.mark.gpu
+def test_storage_is_written_not_replaced():
+    """Calls go to the memory that the cache was made with: another tensor in its place would be passed over in silence."""
+    cache, params = make(2, 2, 16)
+    for name in ("pages", "rope"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name).clone())
+    other, _ = make(2, 2, 16)
+    k = torch.randn(16, 2, D, device="cuda")
+    at = torch.zeros(16, **I32), torch.arange(16, **I32), torch.ones(1, 1, **I32)
+    other.append(k, k, *at)
+    cache.pages.copy_(other.pages)
+    for a, b in zip(cache.read(*at), other.read(*at)):
+        assert torch.equal(a, b) and (a != 0).any()
