@@ -128,10 +128,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t pack_half(float a, float b) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
 __device__ __forceinline__ float2 unpack_half(uint32_t x) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
@@ -420,13 +416,13 @@ attend_kernel(const __grid_constant__ Args a) {
 
     float m[NB][2], lift[NB][2], neg[NB][2], l[NB][2], acc[4][NB][4];
     int pe[NB][2];  // fp32: exponent of the row's largest P n_v
-  #pragma unroll
+#pragma unroll
     for (int b = 0; b < NB; ++b) {
       m[b][0] = m[b][1] = lift[b][0] = lift[b][1] = -INFINITY;
       neg[b][0] = neg[b][1] = 0.0f;
       pe[b][0] = pe[b][1] = 20;
       l[b][0] = l[b][1] = 0.0f;
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 4; ++i) acc[i][b][0] = acc[i][b][1] = acc[i][b][2] = acc[i][b][3] = 0.0f;
     }
     int ve = 20;  // exponent of the largest V norm met
@@ -931,11 +927,6 @@ int join(const Args& a, const Plan& p, cudaStream_t st) {
   return CC2_OK;
 }
 
-bool row_aligned(int dtype, const void* p, int64_t ld, int64_t hs) {
-  const int64_t e = dtype == CC2_BF16 ? 8 : 4;
-  return ((uintptr_t)p & 15u) == 0 && ld % e == 0 && hs % e == 0;
-}
-
 }  // namespace
 }  // namespace kv4
 
@@ -967,7 +958,7 @@ int launch_kv4_attention(const cc2_kv4_cache* cache, int dtype, const void* q, i
   CC2_REQUIRE(q && out && seq_lens && table && table_ld > 0, "kv4_attention: null operand");
   CC2_REQUIRE(cu_q != nullptr || (long long)num_seqs * max_q == total_q,
               "kv4_attention: without cu_q the rows must be num_seqs * max_q, got %d", total_q);
-  CC2_REQUIRE(row_aligned(dtype, q, q_ld, q_hs) && row_aligned(dtype, out, o_ld, o_hs),
+  CC2_REQUIRE(rows_ok(dtype, q, q_ld, q_hs) && rows_ok(dtype, out, o_ld, o_hs),
               "kv4_attention: rows must start on 16 bytes, as must their strides");
   CC2_REQUIRE(!rotate_q || cache->rope_cs, "kv4_attention: the cache has no table to rotate queries with");
   CC2_REQUIRE(std::isfinite(scale), "kv4_attention: scale must be finite");

@@ -74,10 +74,6 @@ constexpr float kRescaleLog2 = 8.0f, kLiftLog2 = 7.0f;  // P up to 2^(8 + 7)
 __device__ __forceinline__ uint32_t idesc_f16(int M, int N, bool b_mn_major) {
   return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ uint32_t pack_half(float a, float b) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -411,257 +407,255 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
   const uint32_t tmem = ctl.tmem;
 
   if (warp < kSoftmaxWarp) {
-    
-  if (warp == 0) {
-    // ---------------- loader ----------------
-    Ring<kItems> it;
-    Ring<kRawStages> raw;
-    long long n_items = 0, n_raw = 0;
-    const int mask = (1 << a.pool.page_shift) - 1;
-    const int run = min((mask + 1) / kBlockTokens, 8);  // blocks of 16 keys a copy brings
-    bool ok = true;
-    // Items are taken as blocks get to them (their costs differ by the rows' and
-    // sequences' lengths): a few at a time where there are many, since many of
-    // them may turn out to have no rows or no keys.
-    const int batch = min(max(total_items / (8 * (int)gridDim.x), 1), 32);
-    while (ok) {
-      int base = 0;
-      if (lane == 0) base = atomicAdd(a.counter, batch);
-      base = __shfl_sync(0xffffffffu, base, 0);
-      const bool any_left = base < total_items;
-      const int mine = lane < batch ? base + lane : total_items;  // each lane looks at one item
-      Item d;
-      d.seq = -1;
-      if (mine < total_items) {
-        unsigned idx = (unsigned)mine;
-        const int tile = a.row_tiles - 1 - (int)(idx % a.row_tiles);  // causal rows with the most keys first
-        idx /= a.row_tiles;
-        d.split = (int)(idx % a.splits);
-        idx /= a.splits;
-        d.head = (int)(idx % a.pool.heads);
-        const int seq = (int)(idx / a.pool.heads);
-        const Span s = span_of(a, seq, tile, d.split == 0 && d.head == 0 && tile == 0);
-        d.chunks = chunks_of(a, s);
-        if (s.row0 < s.rows && d.split < max(d.chunks, 1)) {
-          d.seq = seq;
-          d.row0 = s.row0;
-          d.rows = s.rows;
-          d.q_start = s.q_start;
-          d.n = s.n;
-          d.len = s.len;
-          d.c0 = d.split * a.chunk;
-          d.c1 = min(s.keys, d.c0 + a.chunk);
-          for (int g = 0; g < 2; ++g) {
-            const int first = s.row0 + kTile * g, last = min(first + kTile, s.rows) - 1;
-            int end = first < s.rows ? (a.causal ? min(s.len - s.n + last / a.group + 1, s.len) : s.len) : 0;
-            end = min(end, d.c1);
-            d.key_end[g] = end;
-            d.blocks[g] = end > d.c0 ? (end - d.c0 + kTile - 1) / kTile : 0;
+    if (warp == 0) {
+      // ---------------- loader ----------------
+      Ring<kItems> it;
+      Ring<kRawStages> raw;
+      long long n_items = 0, n_raw = 0;
+      const int mask = (1 << a.pool.page_shift) - 1;
+      const int run = min((mask + 1) / kBlockTokens, 8);  // blocks of 16 keys a copy brings
+      bool ok = true;
+      // Items are taken as blocks get to them (their costs differ by the rows' and
+      // sequences' lengths): a few at a time where there are many, since many of
+      // them may turn out to have no rows or no keys.
+      const int batch = min(max(total_items / (8 * (int)gridDim.x), 1), 32);
+      while (ok) {
+        int base = 0;
+        if (lane == 0) base = atomicAdd(a.counter, batch);
+        base = __shfl_sync(0xffffffffu, base, 0);
+        const bool any_left = base < total_items;
+        const int mine = lane < batch ? base + lane : total_items;  // each lane looks at one item
+        Item d;
+        d.seq = -1;
+        if (mine < total_items) {
+          unsigned idx = (unsigned)mine;
+          const int tile = a.row_tiles - 1 - (int)(idx % a.row_tiles);  // causal rows with the most keys first
+          idx /= a.row_tiles;
+          d.split = (int)(idx % a.splits);
+          idx /= a.splits;
+          d.head = (int)(idx % a.pool.heads);
+          const int seq = (int)(idx / a.pool.heads);
+          const Span s = span_of(a, seq, tile, d.split == 0 && d.head == 0 && tile == 0);
+          d.chunks = chunks_of(a, s);
+          if (s.row0 < s.rows && d.split < max(d.chunks, 1)) {
+            d.seq = seq;
+            d.row0 = s.row0;
+            d.rows = s.rows;
+            d.q_start = s.q_start;
+            d.n = s.n;
+            d.len = s.len;
+            d.c0 = d.split * a.chunk;
+            d.c1 = min(s.keys, d.c0 + a.chunk);
+            for (int g = 0; g < 2; ++g) {
+              const int first = s.row0 + kTile * g, last = min(first + kTile, s.rows) - 1;
+              int end = first < s.rows ? (a.causal ? min(s.len - s.n + last / a.group + 1, s.len) : s.len) : 0;
+              end = min(end, d.c1);
+              d.key_end[g] = end;
+              d.blocks[g] = end > d.c0 ? (end - d.c0 + kTile - 1) / kTile : 0;
+            }
+            d.q_tile = (long long)d.head * q_tiles + first_query_tile(a, seq, s.q_start) + s.row0 / kTile;
           }
-          d.q_tile = (long long)d.head * q_tiles + first_query_tile(a, seq, s.q_start) + s.row0 / kTile;
         }
-      }
-      unsigned live = __ballot_sync(0xffffffffu, d.seq >= 0);
-      while (ok && (live != 0 || !any_left)) {
-        const int src = live != 0 ? __ffs(live) - 1 : 0;
-        live &= live - 1;
-        if (n_items >= kItems && !wait(ctl.item_empty[it.i], it.phase ^ 1u, ctl, err)) {
-          ok = false;
-          break;
-        }
-        if (lane == src) {
-          // A scheduler has one quarter of the lanes of both tiles: a tile that leaves quarters unused starts in
-          // another one each time, so that short tiles do not all fall to the first.
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const int used = (min(d.rows - d.row0 - kTile * g, kTile) + 31) / 32, n = (int)n_items;
-            d.lane0[g] = used > 3 ? 0 : used == 3 ? 32 * (n & 1) : used == 2 ? 64 * (n & 1) : 32 * (n & 3);
-          }
-          ctl.items[it.i] = d;
-          if (!any_left) ctl.items[it.i].seq = -1;
-        }
-        __syncwarp();
-        const Item& e = ctl.items[it.i];
-        const int seq = e.seq, c0 = e.c0, c1 = e.c1, head = e.head, nb = max(e.blocks[0], e.blocks[1]);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ctl.item_full[it.i]));
-        it.next();
-        ++n_items;
-        if (seq < 0) {
-          ok = false;
-          break;
-        }
-        const int* table = a.table + (long long)seq * a.table_ld;
-        const int first = lane * run;  // this lane's first block of 16 keys
-        int page = -1;
-        if (nb > 0 && lane < 8 && c0 + first * kBlockTokens < c1 && first < 8)
-          page = table[(c0 + first * kBlockTokens) >> a.pool.page_shift];
-        for (int j = 0; j < nb && ok; ++j) {
-          const int key0 = c0 + j * kTile;
-          const int n = min((c1 - key0 + kBlockTokens - 1) / kBlockTokens, 8);
-          if (n_raw >= kRawStages && !wait(ctl.raw_empty[raw.i], raw.phase ^ 1u, ctl, err)) {
+        unsigned live = __ballot_sync(0xffffffffu, d.seq >= 0);
+        while (ok && (live != 0 || !any_left)) {
+          const int src = live != 0 ? __ffs(live) - 1 : 0;
+          live &= live - 1;
+          if (n_items >= kItems && !wait(ctl.item_empty[it.i], it.phase ^ 1u, ctl, err)) {
             ok = false;
             break;
           }
-          const uint32_t bar = smem_u32(&ctl.raw_full[raw.i]);
-          if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)n * kBlockBytes);
-          __syncwarp();
-          if (lane < 8 && first < n) {
-            if ((unsigned)page >= (unsigned)a.pool.num_pages) {
-              atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
-              page = 0;
+          if (lane == src) {
+            // A scheduler has one quarter of the lanes of both tiles: a tile that leaves quarters unused starts in
+            // another one each time, so that short tiles do not all fall to the first.
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int used = (min(d.rows - d.row0 - kTile * g, kTile) + 31) / 32, n = (int)n_items;
+              d.lane0[g] = used > 3 ? 0 : used == 3 ? 32 * (n & 1) : used == 2 ? 64 * (n & 1) : 32 * (n & 3);
             }
-            bulk_load(smem + kRawAt + raw.i * kRawBytes + first * kBlockBytes,
-                      a.pool.pages + block_offset(a.pool, page, head, (key0 + first * kBlockTokens) & mask),
-                      (uint32_t)min(run, n - first) * kBlockBytes, bar);
+            ctl.items[it.i] = d;
+            if (!any_left) ctl.items[it.i].seq = -1;
           }
-          const int next = key0 + kTile + first * kBlockTokens;  // the next block's page, ahead of its copy
-          if (j + 1 < nb && lane < 8 && first < 8 && next < c1) page = table[next >> a.pool.page_shift];
-          raw.next();
-          ++n_raw;
-        }
-      }
-      if (!any_left) break;
-    }
-    // no copy may still be landing in shared memory when the block exits
-    if (lane == 0) {
-      const unsigned long long t0 = globaltimer_ns();
-      for (int k = 0; k < kRawStages && k < n_raw; ++k) {
-        const long long at = n_raw - 1 - k;
-        while (!mbar_try(smem_u32(&ctl.raw_full[at % kRawStages]), (uint32_t)(at / kRawStages) & 1u) &&
-               globaltimer_ns() - t0 < kWaitLimitNs) {
-        }
-      }
-    }
-    __syncwarp();
-  } else if (warp == 3) {
-    // ---------------- query loader ----------------
-    Ring<kItems> it;
-    uint32_t nq[2] = {0, 0};
-    bool ok = true;
-    while (ok) {
-      if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
-      const Item& e = ctl.items[it.i];
-      const int seq = e.seq, rows = e.rows - e.row0, blocks[2] = {e.blocks[0], e.blocks[1]},
-                lane0[2] = {e.lane0[0], e.lane0[1]};
-      const long long q_tile = e.q_tile;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
-      it.next();
-      if (seq < 0) break;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (blocks[g] == 0 || !ok) continue;
-        if (nq[g] > 0) ok = wait(ctl.q_empty[g], (nq[g] - 1) & 1u, ctl, err);
-        if (!ok) break;
-        if (lane == 0) {  // the tile's rows, in groups of 8
-          const uint32_t bytes = (uint32_t)min((rows - kTile * g + 7) / 8, kTile / 8) * 1024u;
-          mbar_arrive_expect_tx(smem_u32(&ctl.q_full[g]), bytes);
-          bulk_load(smem + kQAt + g * kTileBytes + lane0[g] * 128, a.qt + (q_tile + g) * kTileBytes, bytes, smem_u32(&ctl.q_full[g]));
-        }
-        __syncwarp();
-        ++nq[g];
-      }
-    }
-    if (lane == 0) {  // as above
-      const unsigned long long t0 = globaltimer_ns();
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (nq[g] > 0)
-          while (!mbar_try(smem_u32(&ctl.q_full[g]), (nq[g] - 1) & 1u) && globaltimer_ns() - t0 < kWaitLimitNs) {
+          __syncwarp();
+          const Item& e = ctl.items[it.i];
+          const int seq = e.seq, c0 = e.c0, c1 = e.c1, head = e.head, nb = max(e.blocks[0], e.blocks[1]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ctl.item_full[it.i]));
+          it.next();
+          ++n_items;
+          if (seq < 0) {
+            ok = false;
+            break;
           }
-    }
-    __syncwarp();
-  } else if (warp < 3) {
-    // ---------------- MMA issuer of tile g ----------------
-    // The warp stays converged and what it branches on is broadcast, so that
-    // descriptors stay in uniform registers; one elected lane issues.  The tensor
-    // core runs its products in order: S_{j+2} may follow P_j V_j, whose P it
-    // overwrites, at once, and its completion says that P_j V_j is done too.
-    const int g = warp - 1;
-    Ring<kItems> it;
-    Ring<kKvStages> kv_s, kv_p;  // stage of the next S, of the next P V
-    uint32_t nt = 0, np0 = 0, np1 = 0;  // items with keys, steps of the two chains
-    const uint32_t t_s = tmem + kSCol + 128u * g, t_o = tmem + kOCol + 128u * g;
-    const uint64_t dq = sw128_desc(smem + kQAt + g * kTileBytes), dk0 = sw128_desc(smem + kKvAt),
-                   dv0 = sw128_desc(smem + kKvAt + kTileBytes);
-    const uint32_t id_o = idesc_f16(128, 64, true);
-    constexpr uint64_t kStage = 2 * kTileBytes >> 4, kHalf = kTileBytes / 2 >> 4;  // descriptor steps
-    bool ok = true;
-    while (ok) {
-      if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
-      const Item& e = ctl.items[it.i];
-      const int seq = __shfl_sync(0xffffffffu, e.seq, 0), blocks = __shfl_sync(0xffffffffu, e.blocks[g], 0),
-                keys = __shfl_sync(0xffffffffu, e.key_end[g] - e.c0, 0),
-                all = __shfl_sync(0xffffffffu, max(e.blocks[0], e.blocks[1]), 0);
-      if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
-      __syncwarp();
-      it.next();
-      if (seq < 0) break;
-      const int steps = blocks > 0 ? (keys + kStep - 1) / kStep : 0;
-      if (steps > 0) ok = wait(ctl.q_full[g], nt & 1u, ctl, err);
-      for (int j = -2; j < steps && ok; ++j) {  // P_j V_j, then S_{j+2}
-        if (j >= 0) {
-          const int n = min((keys - j * kStep + 15) >> 4, kStep / 16);
-          const uint32_t c = j & 1, parity = (c ? np1++ : np0++) & 1u;
-          const uint64_t dv = dv0 + kv_p.i * kStage + c * kHalf;
-          const bool last = j == steps - 1, done = c == 1 || last;
-          // the first product of an item waits until the item before has been read out
-          ok = (j > 0 || nt == 0 || wait(ctl.o_free[g], (nt - 1) & 1u, ctl, err)) &&
-               wait(ctl.p_full[g][c], parity, ctl, err);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t tp = t_s + 64u * c, to = t_o + 64u * c, acc = j > 1 ? 1u : 0u;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (k < n) mma_bf16_ts(to, tp + 8u * k, dv + 128u * k, id_o, k > 0 ? 1u : acc);
-            if (done) mma_commit(smem_u32(&ctl.kv_empty[kv_p.i]));
-            if (last) {
-              mma_commit(smem_u32(&ctl.o_full[g]));
-              mbar_arrive(smem_u32(&ctl.o_full[g]));  // hands on the maxima and sums that came with P
+          const int* table = a.table + (long long)seq * a.table_ld;
+          const int first = lane * run;  // this lane's first block of 16 keys
+          int page = -1;
+          if (nb > 0 && lane < 8 && c0 + first * kBlockTokens < c1 && first < 8)
+            page = table[(c0 + first * kBlockTokens) >> a.pool.page_shift];
+          for (int j = 0; j < nb && ok; ++j) {
+            const int key0 = c0 + j * kTile;
+            const int n = min((c1 - key0 + kBlockTokens - 1) / kBlockTokens, 8);
+            if (n_raw >= kRawStages && !wait(ctl.raw_empty[raw.i], raw.phase ^ 1u, ctl, err)) {
+              ok = false;
+              break;
             }
+            const uint32_t bar = smem_u32(&ctl.raw_full[raw.i]);
+            if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)n * kBlockBytes);
+            __syncwarp();
+            if (lane < 8 && first < n) {
+              if ((unsigned)page >= (unsigned)a.pool.num_pages) {
+                atomicOr(a.range_err, (int)DEV_ERR_CACHE_RANGE);
+                page = 0;
+              }
+              bulk_load(smem + kRawAt + raw.i * kRawBytes + first * kBlockBytes,
+                        a.pool.pages + block_offset(a.pool, page, head, (key0 + first * kBlockTokens) & mask),
+                        (uint32_t)min(run, n - first) * kBlockBytes, bar);
+            }
+            const int next = key0 + kTile + first * kBlockTokens;  // the next block's page, ahead of its copy
+            if (j + 1 < nb && lane < 8 && first < 8 && next < c1) page = table[next >> a.pool.page_shift];
+            raw.next();
+            ++n_raw;
           }
-          __syncwarp();
-          if (done) kv_p.next();
         }
-        const int i = j + 2;
-        if (i < steps) {
-          const uint32_t id = idesc_f16(128, min((keys - i * kStep + 15) & ~15, kStep), false), c = i & 1;
-          if (c == 0) ok = wait(ctl.kv_full[kv_s.i], kv_s.phase, ctl, err);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t dk = dk0 + kv_s.i * kStage + c * kHalf;
-          const bool last = i == steps - 1;
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_bf16(t_s + 64u * c, dq + 2u * k, dk + 2u * k, id, k > 0);
-            mma_commit(smem_u32(&ctl.s_full[g][c]));
-            if (last) mma_commit(smem_u32(&ctl.q_empty[g]));
+        if (!any_left) break;
+      }
+      // no copy may still be landing in shared memory when the block exits
+      if (lane == 0) {
+        const unsigned long long t0 = globaltimer_ns();
+        for (int k = 0; k < kRawStages && k < n_raw; ++k) {
+          const long long at = n_raw - 1 - k;
+          while (!mbar_try(smem_u32(&ctl.raw_full[at % kRawStages]), (uint32_t)(at / kRawStages) & 1u) &&
+                 globaltimer_ns() - t0 < kWaitLimitNs) {
           }
-          __syncwarp();
-          if (c == 1 || last) kv_s.next();
         }
       }
-      if (steps > 0) ++nt;
-      for (int j = blocks; j < all && ok; ++j) {  // blocks that only the other tile's rows see
-        ok = wait(ctl.kv_full[kv_p.i], kv_p.phase, ctl, err);
-        if (ok && lane == 0) mbar_arrive(smem_u32(&ctl.kv_empty[kv_p.i]));
+      __syncwarp();
+    } else if (warp == 3) {
+      // ---------------- query loader ----------------
+      Ring<kItems> it;
+      uint32_t nq[2] = {0, 0};
+      bool ok = true;
+      while (ok) {
+        if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
+        const Item& e = ctl.items[it.i];
+        const int seq = e.seq, rows = e.rows - e.row0, blocks[2] = {e.blocks[0], e.blocks[1]},
+                  lane0[2] = {e.lane0[0], e.lane0[1]};
+        const long long q_tile = e.q_tile;
         __syncwarp();
-        kv_p.next();
-        kv_s.next();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
+        it.next();
+        if (seq < 0) break;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (blocks[g] == 0 || !ok) continue;
+          if (nq[g] > 0) ok = wait(ctl.q_empty[g], (nq[g] - 1) & 1u, ctl, err);
+          if (!ok) break;
+          if (lane == 0) {  // the tile's rows, in groups of 8
+            const uint32_t bytes = (uint32_t)min((rows - kTile * g + 7) / 8, kTile / 8) * 1024u;
+            mbar_arrive_expect_tx(smem_u32(&ctl.q_full[g]), bytes);
+            bulk_load(smem + kQAt + g * kTileBytes + lane0[g] * 128, a.qt + (q_tile + g) * kTileBytes, bytes, smem_u32(&ctl.q_full[g]));
+          }
+          __syncwarp();
+          ++nq[g];
+        }
       }
-    }
-    if (nt > 0 && elect_one()) {  // every MMA has completed before TMEM is released
-      mma_commit(smem_u32(&ctl.mma_done[g]));
-      const unsigned long long t0 = globaltimer_ns();
-      while (!mbar_try(smem_u32(&ctl.mma_done[g]), 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
+      if (lane == 0) {  // as above
+        const unsigned long long t0 = globaltimer_ns();
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (nq[g] > 0)
+            while (!mbar_try(smem_u32(&ctl.q_full[g]), (nq[g] - 1) & 1u) && globaltimer_ns() - t0 < kWaitLimitNs) {
+            }
       }
+      __syncwarp();
+    } else if (warp < 3) {
+      // ---------------- MMA issuer of tile g ----------------
+      // The warp stays converged and what it branches on is broadcast, so that
+      // descriptors stay in uniform registers; one elected lane issues.  The tensor
+      // core runs its products in order: S_{j+2} may follow P_j V_j, whose P it
+      // overwrites, at once, and its completion says that P_j V_j is done too.
+      const int g = warp - 1;
+      Ring<kItems> it;
+      Ring<kKvStages> kv_s, kv_p;  // stage of the next S, of the next P V
+      uint32_t nt = 0, np0 = 0, np1 = 0;  // items with keys, steps of the two chains
+      const uint32_t t_s = tmem + kSCol + 128u * g, t_o = tmem + kOCol + 128u * g;
+      const uint64_t dq = sw128_desc(smem + kQAt + g * kTileBytes), dk0 = sw128_desc(smem + kKvAt),
+                     dv0 = sw128_desc(smem + kKvAt + kTileBytes);
+      const uint32_t id_o = idesc_f16(128, 64, true);
+      constexpr uint64_t kStage = 2 * kTileBytes >> 4, kHalf = kTileBytes / 2 >> 4;  // descriptor steps
+      bool ok = true;
+      while (ok) {
+        if (!wait(ctl.item_full[it.i], it.phase, ctl, err)) break;
+        const Item& e = ctl.items[it.i];
+        const int seq = __shfl_sync(0xffffffffu, e.seq, 0), blocks = __shfl_sync(0xffffffffu, e.blocks[g], 0),
+                  keys = __shfl_sync(0xffffffffu, e.key_end[g] - e.c0, 0),
+                  all = __shfl_sync(0xffffffffu, max(e.blocks[0], e.blocks[1]), 0);
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[it.i]));
+        __syncwarp();
+        it.next();
+        if (seq < 0) break;
+        const int steps = blocks > 0 ? (keys + kStep - 1) / kStep : 0;
+        if (steps > 0) ok = wait(ctl.q_full[g], nt & 1u, ctl, err);
+        for (int j = -2; j < steps && ok; ++j) {  // P_j V_j, then S_{j+2}
+          if (j >= 0) {
+            const int n = min((keys - j * kStep + 15) >> 4, kStep / 16);
+            const uint32_t c = j & 1, parity = (c ? np1++ : np0++) & 1u;
+            const uint64_t dv = dv0 + kv_p.i * kStage + c * kHalf;
+            const bool last = j == steps - 1, done = c == 1 || last;
+            // the first product of an item waits until the item before has been read out
+            ok = (j > 0 || nt == 0 || wait(ctl.o_free[g], (nt - 1) & 1u, ctl, err)) &&
+                 wait(ctl.p_full[g][c], parity, ctl, err);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t tp = t_s + 64u * c, to = t_o + 64u * c, acc = j > 1 ? 1u : 0u;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < n) mma_bf16_ts(to, tp + 8u * k, dv + 128u * k, id_o, k > 0 ? 1u : acc);
+              if (done) mma_commit(smem_u32(&ctl.kv_empty[kv_p.i]));
+              if (last) {
+                mma_commit(smem_u32(&ctl.o_full[g]));
+                mbar_arrive(smem_u32(&ctl.o_full[g]));  // hands on the maxima and sums that came with P
+              }
+            }
+            __syncwarp();
+            if (done) kv_p.next();
+          }
+          const int i = j + 2;
+          if (i < steps) {
+            const uint32_t id = idesc_f16(128, min((keys - i * kStep + 15) & ~15, kStep), false), c = i & 1;
+            if (c == 0) ok = wait(ctl.kv_full[kv_s.i], kv_s.phase, ctl, err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t dk = dk0 + kv_s.i * kStage + c * kHalf;
+            const bool last = i == steps - 1;
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_bf16(t_s + 64u * c, dq + 2u * k, dk + 2u * k, id, k > 0);
+              mma_commit(smem_u32(&ctl.s_full[g][c]));
+              if (last) mma_commit(smem_u32(&ctl.q_empty[g]));
+            }
+            __syncwarp();
+            if (c == 1 || last) kv_s.next();
+          }
+        }
+        if (steps > 0) ++nt;
+        for (int j = blocks; j < all && ok; ++j) {  // blocks that only the other tile's rows see
+          ok = wait(ctl.kv_full[kv_p.i], kv_p.phase, ctl, err);
+          if (ok && lane == 0) mbar_arrive(smem_u32(&ctl.kv_empty[kv_p.i]));
+          __syncwarp();
+          kv_p.next();
+          kv_s.next();
+        }
+      }
+      if (nt > 0 && elect_one()) {  // every MMA has completed before TMEM is released
+        mma_commit(smem_u32(&ctl.mma_done[g]));
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try(smem_u32(&ctl.mma_done[g]), 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
+        }
+      }
+      __syncwarp();
     }
-    __syncwarp();
-  }
   } else if (warp >= kDecodeWarp && warp < kOutWarp) {
-    
     // ---------------- decoders ----------------
     Ring<kItems> it;
     Ring<kRawStages> raw;
@@ -753,7 +747,6 @@ attend_tc_kernel(const __grid_constant__ Args a, const long long q_tiles, const 
       }
     }
   } else if (warp < kDecodeWarp) {
-    
     // ---------------- softmax: chain c of tile g ----------------
     const int g = (warp - kSoftmaxWarp) >> 3, c = ((warp - kSoftmaxWarp) >> 2) & 1, quarter = warp & 3,
               r = 32 * quarter + lane;

@@ -109,6 +109,11 @@ __device__ __forceinline__ void zip(uint32_t a, uint32_t b, uint32_t& u, uint32_
 }
 
 // --- host side --------------------------------------------------------------
+// Whether rows and heads start on 16 bytes.
+inline bool rows_ok(int dtype, const void* p, int64_t ld, int64_t hs) {
+  const int64_t e = dtype == CC2_BF16 ? 8 : 4;  // elements of 16 bytes
+  return ((uintptr_t)p & 15u) == 0 && ld % e == 0 && hs % e == 0;
+}
 int check_cache(const cc2_kv4_cache* c, const char* what, Pool& pool);
 int make_turn(const cc2_kv4_quant& q, const char* what, Turn& t);
 Levels make_levels(const cc2_kv4_cache& c);

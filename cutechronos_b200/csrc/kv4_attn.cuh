@@ -66,6 +66,10 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                "l"((uint64_t)__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
                : "memory");
 }
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
 __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));

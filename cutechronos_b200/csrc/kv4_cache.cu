@@ -457,11 +457,6 @@ int check_places(const char* what, int T, const int32_t* seq, const int32_t* pos
   return CC2_OK;
 }
 
-bool rows_ok(int dtype, const void* p, int64_t ld, int64_t hs) {
-  const int64_t e = dtype == CC2_BF16 ? 8 : 4;  // elements of 16 bytes
-  return ((uintptr_t)p & 15u) == 0 && ld % e == 0 && hs % e == 0;
-}
-
 int grid_of(int T, int heads, int* grid) {
   const long long blocks = (((long long)T + 15) / 16 * heads + 3) / 4;
   CC2_REQUIRE(blocks <= 0x1fffffffLL, "kv4: too many tokens for one call");
