@@ -24,7 +24,7 @@ EXPORTED = (
     "cc2_set_attention_trace", "cc2_set_gemm_trace", "cc2_kv_quant", "cc2_model_set_kv_quant",
     "cc2_set_launch_overlap", "cc2_test_starve_gemm", "cc2_group_attention_tc", "cc2_set_layer_chain",
     "cc2_test_starve_layer_barrier", "cc2_set_layer_trace", "cc2_kv4_page_bytes", "cc2_kv4_append", "cc2_kv4_read",
-    "cc2_kv4_append_cols", "cc2_kv4_read_cols", "cc2_kv4_attention_fill",
+    "cc2_kv4_append_cols", "cc2_kv4_read_cols", "cc2_kv4_attention_fill", "cc2_kv4_index32",
     "cc2_kv4_attention_workspace_bytes", "cc2_kv4_attention",
 )
 KIND_NAMES = {1: "preprocess", 2: "gemm_tc", 3: "attn_time", 4: "attn_group", 5: "rmsnorm", 6: "output_transform",
@@ -140,6 +140,7 @@ def load(path: Path | str | None = None) -> C.CDLL:
     lib.cc2_kv4_read_cols.argtypes = [kv4, i, v, v, i, v, v, v, i, i, i, v]
     lib.cc2_kv4_attention_workspace_bytes.argtypes = [kv4, i, i, i, i, i, i, C.POINTER(sz)]
     lib.cc2_kv4_attention.argtypes = [kv4, i, v, i64, i64, v, i64, i64, i, i, i, v, i, v, i, v, i, i, f, i, v, v, sz, v]
+    lib.cc2_kv4_index32.argtypes = [v, i64, i64, i, i, v, v]
     lib.cc2_kv4_attention_fill.argtypes = [kv4, i, v, i64, i64, v, i64, i64, i, i, i, v, i, v, i, v, i, i, f, i, i, v, v, sz, v]
     lib.cc2_forward_noalloc.argtypes = [v, v, v, i, i, i, v, v, v, v, v]
     lib.cc2_profile_read.argtypes = [v, v, v, v, i, C.POINTER(i)]

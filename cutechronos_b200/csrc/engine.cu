@@ -91,6 +91,7 @@ int set_chain_starve(int on);
 int set_chain_trace(void* buf);
 size_t gemm_f32_splitk_floats();
 int read_kv4_error(int clear, int* value);
+int launch_kv4_index32(const int64_t* in, int64_t ld, int64_t inc, int rows, int cols, int32_t* out, cudaStream_t st);
 int launch_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs, const void* v,
                       int64_t v_ld, int64_t v_hs, int T, const int32_t* seq, const int32_t* pos, const uint8_t* mask,
                       const int32_t* table, int table_ld, int table_cols, int num_seqs, cudaStream_t st);
@@ -976,6 +977,11 @@ int cc2_model_set_kv_quant(cc2_model* m, int layer, const cc2_kvq* key, const cc
   q.stats = stats;
   m->kvq[layer] = q;
   return CC2_OK;
+}
+
+int cc2_kv4_index32(const int64_t* in, int64_t ld, int64_t inc, int rows, int cols, int32_t* out, void* stream) {
+  clear_error();
+  return launch_kv4_index32(in, ld, inc, rows, cols, out, (cudaStream_t)stream);
 }
 
 int cc2_kv4_append(const cc2_kv4_cache* cache, int dtype, const void* k, int64_t k_ld, int64_t k_hs, const void* v,

@@ -449,6 +449,17 @@ read_kernel(const __grid_constant__ Pool pool, const __grid_constant__ Turn turn
   }
 }
 
+// 64-bit indexes to 32 bits, what does not fit to the nearest that does.
+__global__ void __launch_bounds__(256)
+index32_kernel(const int64_t* __restrict__ in, long long ld, long long inc, unsigned cols, unsigned n, int32_t* __restrict__ out) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= n) return;
+  const int64_t v = in[(long long)(i / cols) * ld + (long long)(i % cols) * inc];
+  out[i] = (int32_t)max(min((long long)v, 0x7fffffffLL), -0x80000000LL);
+}
+
 int check_places(const char* what, int T, const int32_t* seq, const int32_t* pos, const int32_t* table, int table_ld,
                  int table_cols, int num_seqs) {
   CC2_REQUIRE(T >= 0 && seq && pos && table, "%s: null sequences, positions or block table", what);
@@ -475,6 +486,16 @@ int read_kv4_error(int clear, int* value) {
     const int z[2] = {0, 0};
     CC2_CUDA(cudaMemcpyToSymbol(kv4::g_kv4_error, z, sizeof z));
   }
+  return CC2_OK;
+}
+
+int launch_kv4_index32(const int64_t* in, int64_t ld, int64_t inc, int rows, int cols, int32_t* out, cudaStream_t st) {
+  CC2_REQUIRE(rows >= 0 && cols >= 0 && (long long)rows * cols <= 0x7fffffffLL, "kv4_index32: bad size %d x %d", rows, cols);
+  const unsigned n = (unsigned)rows * (unsigned)cols;
+  if (n == 0) return CC2_OK;
+  CC2_REQUIRE(in && out, "kv4_index32: null operand");
+  CC2_CUDA(launch_k(kv4::index32_kernel, (n + 255u) / 256u, 256, 0, st, in, (long long)ld, (long long)inc, (unsigned)cols, n, out));
+  CC2_CHECK_LAUNCH();
   return CC2_OK;
 }
 

@@ -152,8 +152,22 @@ class PagedKV4Cache:
         if t.dtype != torch.int32:
             if t.dtype != torch.int64:
                 raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
-            t = t.clamp(-2**31, 2**31 - 1).to(torch.int32)  # out of range stays out of range
+            return self._narrow(t)
         return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
+
+    def _narrow(self, t: torch.Tensor) -> torch.Tensor:
+        """t in 32 bits; what does not fit stays out of range."""
+        i, shape, stride = self._at, t.shape, t.stride()
+        out = torch.empty(shape, dtype=torch.int32, device=self.device)
+        args = t.data_ptr(), stride[0], stride[-1], shape[0] if len(shape) > 1 else 1, shape[-1], out.data_ptr()
+        if torch._C._cuda_getDevice() == i:
+            status = self._lib.cc2_kv4_index32(*args, _raw_stream(i))
+        else:
+            with torch.cuda.device(i):
+                status = self._lib.cc2_kv4_index32(*args, _raw_stream(i))
+        if status:
+            nat.check(status, "cc2_kv4_index32")
+        return out
 
     def _values(self, t: torch.Tensor, what: str) -> int:
         if t.get_device() != self._at:

@@ -463,6 +463,12 @@ typedef struct {
 /* Bytes of one page. */
 CC2_API int cc2_kv4_page_bytes(int page_size, int heads, size_t* bytes);
 
+/* 64-bit indexes (dev; entry (r, c) at r * ld + c * inc) as the calls below take
+ * them: out (dev, (rows, cols)), what does not fit 32 bits as the nearest that
+ * does, so that it stays out of range. */
+CC2_API int cc2_kv4_index32(const int64_t* in, int64_t ld, int64_t inc, int rows, int cols, int32_t* out,
+                            void* stream);
+
 /* Append T tokens: k and v (dev, dtype; token t's head h at t * ld + h * hs,
  * 64 consecutive elements, 16-byte aligned), seq and pos (dev, int32, T):
  * token t becomes entry pos[t] of sequence seq[t].  k is rotated to its

@@ -323,6 +323,24 @@ def test_64_bit_indexes_do_not_wrap():
     assert torch.equal(want, cache.attention(q, torch.tensor([6], **I32), table.int()))
 
 
+@pytest.mark.gpu
+def test_64_bit_indexes_of_any_strides():
+    cache, _, table, (_, _, seq, pos, _) = filled([300, 90, 700], 2)
+    tab = table.cuda()
+    ref = cache.read(seq.cuda(), pos.cuda(), tab)
+    wide = torch.full((3, 2 * table.shape[1] + 3), 2**40, dtype=torch.int64, device="cuda")
+    wide[:, 1:-2:2] = tab
+    pair = torch.stack([seq, pos], 1).long().cuda()
+    for t in (tab.long(), wide[:, 1:-2:2], tab.long().t().contiguous().t()):
+        for a, b in zip(ref, cache.read(pair[:, 0], pair[:, 1], t)):
+            assert torch.equal(a, b)
+    one = torch.zeros(1, dtype=torch.int64, device="cuda").expand(300)
+    for a, b in zip(ref, cache.read(one, torch.arange(300, device="cuda"), tab[:1].long().expand(2, -1))):
+        assert torch.equal(a[:300], b)
+    assert cache.read(one[:0], one[:0], tab.long())[0].shape == (0, 2, D)
+    cache.check()
+
+
 # ----------------------------------------------------------------------------------------- tiny vectors --
 @pytest.mark.gpu
 @pytest.mark.parametrize("size", [3e-23, 4.4e-23, 6e-23, 1e-22, 1e-20, 1e-15])
