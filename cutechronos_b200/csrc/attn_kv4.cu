@@ -30,8 +30,9 @@
 // (484 MB of cache): 145 us, 3.3 TB/s; 207 us with the byte permutes; 192 us with
 // a fixed chunk of keys a block instead of the call's work cut evenly over teams
 // that stay.  A stage of 64 keys takes a warp some 815 instructions; issue slots
-// are 63% used, the load/store pipe 58% and the integer pipe 51%, with the
-// 16 warps an SM that the table and the rings leave room for.
+// are 63% used, the load/store pipe 58% and the integer pipe 51%, with 16 warps
+// an SM: at 128 registers they fill the register file.  Of the table's 64 KB
+// bf16 calls use every other 128 bytes, fp32 calls all.
 // What must not leave the type's range is scaled by powers of two, which are
 // exact: a row of Q to below 2^8, P n_v to below 2^14 against the largest norm
 // met so far; in fp32 calls against the row's largest P n_v itself, so that two
@@ -39,7 +40,9 @@
 // norm a row was off by 6e-5 where that was 2^16 above those that counted; the
 // row's own costs 3 to 4%: 64 sequences of 4096 tokens, 8 heads, 2 rows a head
 // 94 us for 91).
-// Rounding: P n_v to fp16 (2^-12 of each, next to the output's bf16 with 2^-9),
+// Rounding: P n_v to fp16 (2^-12 of each, next to the output's bf16 with 2^-9;
+// from 2^-20 of the largest norm met on, below it a bit less for each power of
+// two),
 // the levels to fp16 after a common factor that moves all of them close to its
 // values, Q to one or two fp16 parts (split_q).  fp32 calls split all three into
 // two parts and sum three products, which leaves about 2^-22.
@@ -50,7 +53,6 @@
 #include "kv4_attn.cuh"
 
 namespace cc2 {
-
 namespace kv4 {
 
 // fp16 keeps the levels to 2^-12 of each at best, the same error in every key.

@@ -37,7 +37,7 @@
 // copies and MMAs in flight are waited for, TMEM is freed, the kernel returns.
 // Measured: 2048, 1450 and 853 tokens against 16384, 11603 and 6822 keys, 4
 // heads on each of 8, causal, 724 us, 596 TFLOP/s of the scores' and values'
-// products; 256 series of 133 tokens, 12 heads, 167 us (40 of them the first
+// products; 256 series of 133 tokens, 12 heads, 168 us (40 of them the first
 // kernel).  What bounds it: issue slots are 65% used, the exponentials' unit 60%,
 // and a step's chain of waits does not fill the rest; a third of the instructions
 // are the decoders', two thirds the softmax'.  Computing part of the exponentials

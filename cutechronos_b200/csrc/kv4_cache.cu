@@ -19,7 +19,7 @@
 //    in one piece, and rows come in and go out as whole lines: with the 64 units
 //    in (token, head) order each owner's 32 bytes were a line of their own;
 //  - places in the cache, pointers and positions are worked out once a vector.
-// Measured, 131072 tokens of 8 heads, bf16: append 166 us (340 MB, 2.0 TB/s),
+// Measured, 131072 tokens of 8 heads, bf16: append 165 us (340 MB, 2.1 TB/s),
 // read 96 us (3.5 TB/s); read of 55760 entries of 24 sequences as fp32 53 us
 // (4.9 TB/s).  Append uses 77% of the shared-memory pipe's cycles (an owner's 64
 // loads, the 64 stores before them, 64 table lookups of which some meet in a

@@ -7,7 +7,8 @@ keys to their positions on the way (rotate-half, like the model's attention), an
 rotates a query into the codes' frame and the result back out, never the cache.
 
 Every method enqueues work on the current stream of the cache's device and returns; lengths, positions and tables stay on
-the device.  A sequence, position, page or length out of range sets a bit of the library's device status, which stands
+the device (int32; int64 is converted first, a launch an operand).  There is no gradient: what a call returns is detached,
+like all of this library's kernels'.  A sequence, position, page or length out of range sets a bit of the library's device status, which stands
 until :meth:`PagedKV4Cache.check` reads it.
 """
 
@@ -245,13 +246,15 @@ class PagedKV4Cache:
         """Attention of q (tokens, query heads, 64; bfloat16 or float32) over the cache -> the same shape and type.
 
         ``seq_lens`` counts each sequence's cached tokens, the queries' own among them.  Sequence s has the rows
-        ``cu_q[s] : cu_q[s + 1]`` (at most ``max_q``; default: one equal share each), standing at its last positions;
+        ``cu_q[s] : cu_q[s + 1]``, at most ``max_q`` (with ``cu_q`` the default is all rows of the call, and the kernel is
+        chosen for that many: give the real bound), or without ``cu_q`` one equal share each, standing at its last positions;
         ``causal`` lets a row see the entries up to its own.  Query head h reads key head h // (query heads / heads).
         ``scale`` multiplies the scores (1, as in the model's attention); ``rotate_q`` rotates the queries to their
         positions.  ``max_len`` bounds seq_lens (default: what the block table has room for); a tighter bound splits the
         work better.  A row that sees no token gives 0, as does one of no sequence (before ``cu_q[0]``, from ``cu_q[-1]`` on),
         which in an ``out`` of the caller's is left alone.  With ``return_lse`` also the (tokens, query heads) float32
-        logarithm of each row's sum of exponentials (-inf for such a row), to join it with attention over other keys."""
+        logarithm of each row's sum of exponentials (-inf for such a row), to join it with attention over other keys.
+        bfloat16 calls keep 11 bits of a value whose norm is at least 2^-20 of the sequence's largest."""
         code = self._values(q, "q")
         lens = self._index(seq_lens, "seq_lens")
         table, rows, cols, ld = self._table(block_table)

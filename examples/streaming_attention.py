@@ -1,9 +1,14 @@
 """Series that keep growing: time attention of one encoder layer over a 4-bit K/V cache.
 
-Each series' past patches are embedded and their keys and values appended to a paged cache once; every new patch then
-costs one token: its projections, one append, one attention over everything cached.  The layer's weights are the
-model's; attention is causal, so that what is cached never changes (the model's own forward lets patches see later ones,
-and recomputes them).  Prints what the cache takes next to bf16 and how far its attention is from dense attention over
+Each series' past patches have their keys and values appended to a paged cache once; every new patch then costs one
+token: its projections, one append, one attention over everything cached.  The layer's weights are the model's; attention
+is causal, so that one layer's cached keys do not depend on later patches (the model's own forward lets patches see later
+ones, and recomputes them).
+
+The series stand in for a stream: all patches are embedded at the start, the later ones too.  The model's embedding scales
+a series by its mean and deviation and counts its time encoding from the end, and both move with every new value.  A stream
+has to fix them (the past's, say) or to encode and append anew; with those that change under it, what is cached goes out of
+date.  Prints what the cache takes next to bf16 and how far its attention is from dense attention over
 unquantised keys and values.
 
     python examples/streaming_attention.py [--series 16] [--context 4096] [--steps 32]

@@ -434,7 +434,7 @@ CC2_API int cc2_model_set_kv_quant(cc2_model* m, int layer, const cc2_kvq* key, 
  * n is the square root of the squares added in halves (32 + 32, 16 + 16, ...)
  * in fp32, y the fp32 butterflies of width 1, 2, ..., 32: a cache's content
  * does not depend on how a call was split.  A finite n above fp16's largest
- * value is held as that value, one that is not finite as NaN (the vector
+ * value is held as that value (65536 as bfloat16), one that is not finite as NaN (the vector
  * reads back as NaN). */
 typedef struct {
   uint64_t signs;      /* bit i: signs_i = -1 */
