@@ -254,7 +254,8 @@ class PagedKV4Cache:
         work better.  A row that sees no token gives 0, as does one of no sequence (before ``cu_q[0]``, from ``cu_q[-1]`` on),
         which in an ``out`` of the caller's is left alone.  With ``return_lse`` also the (tokens, query heads) float32
         logarithm of each row's sum of exponentials (-inf for such a row), to join it with attention over other keys.
-        bfloat16 calls keep 11 bits of a value whose norm is at least 2^-20 of the sequence's largest."""
+        bfloat16 calls keep 11 bits of a weight times its value's norm down to 2^-20 of the row's largest weight times the
+        sequence's largest norm."""
         code = self._values(q, "q")
         lens = self._index(seq_lens, "seq_lens")
         table, rows, cols, ld = self._table(block_table)

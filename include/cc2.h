@@ -516,9 +516,10 @@ CC2_API int cc2_kv4_read_cols(const cc2_kv4_cache* cache, int dtype, void* k_out
  * NaN, a key their log-sum-exp too.  A length or page out of range raises
  * CC2_DEV_CACHE_RANGE; that sequence's rows are then unspecified.
  * Sums are fp32.  bf16 calls take the levels and a key's weight times its V
- * norm as fp16: 11 bits while the V norm is at least 2^-20 of the largest one
- * among the sequence's keys, whatever that one's weight; one bit fewer for
- * each power of two below.  fp32 calls take them as two fp16 parts against the
+ * norm as fp16: 11 bits while that product is at least 2^-20 of the row's
+ * largest weight times the largest V norm among the sequence's keys, whatever
+ * that one's weight; one bit fewer for each power of two below, so that none
+ * is left under 2^-31.  fp32 calls take them as two fp16 parts against the
  * row's largest such product: about 2^-22 of it.
  * workspace (dev, 16-byte aligned) >= cc2_kv4_attention_workspace_bytes, which
  * may be 0. */
